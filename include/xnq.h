@@ -328,12 +328,64 @@ int xnq_rope_attn_decode(const float *qkv, const float *cos_table, const float *
                          void *v_cache, float *out, int64_t batch, int heads, int kv_heads, int head_dim, int64_t max_seq,
                          void *workspace, size_t ws_bytes, void *stream);
 
+/* ---- a KV cache held in GGUF blocks (no counterpart in the reference, whose caches hold the model's own type) ------------------------
+ * Keys and values as Q4_0 or Q8_0 blocks of 32 along head_dim (codes and an f16 scale: 72 or 136 bytes a row of 128, against 256 in bf16).
+ * head_dim 64 or 128. The memory is the caller's: num_pages pages of xnq_kv_page_bytes, 16-byte aligned; their layout is the library's own.
+ * A new buffer has to be zeroed once. page_table NULL: sequence b is page b (max_seq <= page_size); else it holds, in device memory, the page of
+ * positions i * page_size .. of sequence b at [b * table_stride + i]; an entry outside [0, num_pages) has no page (nothing is stored there, such
+ * positions read as zeros and are not attended to, a status bit is set when they are asked for). page_size: a multiple of 32.
+ * Positions: `pos` (device memory, pos_stride 1: one for each sequence, 0: one for all) is that of the first of `seq` tokens of every sequence.
+ * A token at a negative position is none: it is not stored, and as a query it sees nothing. One past max_seq is not stored and sets a status bit. */
+typedef struct xnq_kv_cache {
+  int ggml_dtype; /* XNQ_Q4_0 or XNQ_Q8_0 */
+  int kv_heads, head_dim;
+  int64_t page_size, num_pages;
+  void *pages;
+  const int32_t *page_table;
+  int64_t table_stride;
+  int64_t max_seq; /* positions a sequence may have */
+} xnq_kv_cache;
+/* A [batch, seq, heads, head_dim] tensor in device memory, XNQ_F32 / XNQ_F16 / XNQ_BF16, strides in elements. head_dim is contiguous, every row
+ * 16-byte aligned. */
+typedef struct xnq_rows {
+  void *data;
+  int dtype;
+  int64_t stride_b, stride_s, stride_h;
+} xnq_rows;
+/* Rotary embedding (rotate-half) at the tokens' positions: f32 tables [table_rows, head_dim / 2]. heads > 0: q (k's type) is rotated into q_out
+ * (any float type) as well; a query outside the tables gives zeros. */
+typedef struct xnq_kv_rope {
+  const float *cos_table, *sin_table;
+  int64_t table_rows;
+  int heads;
+  xnq_rows q, q_out;
+} xnq_kv_rope;
+size_t xnq_kv_page_bytes(int ggml_dtype, int kv_heads, int head_dim, int64_t page_size); /* 0: not a cache this library serves */
+/* k and v [batch, seq, kv_heads, head_dim] of one type into the cache. k is rotated first with `rope` (may be NULL), in f32. The codes and scales are
+ * those of BlockQ4_0 / BlockQ8_0::from_float (k_quants.rs:235-270, 636-661) on the f32 values, bit for bit. */
+int xnq_kv_store(const xnq_kv_cache *cache, const xnq_rows *k, const xnq_rows *v, int64_t batch, int64_t seq, const long long *pos, int pos_stride,
+                 const xnq_kv_rope *rope, void *stream);
+/* What n positions of every sequence stand for: k_out, v_out [batch, kv_heads, n, head_dim] contiguous, 16-byte aligned. They start at start_dev
+ * (device memory, start_stride as pos_stride) or, where that is NULL, at `start`. f32 results are exact. */
+int xnq_kv_load(const xnq_kv_cache *cache, int64_t batch, const long long *start_dev, int start_stride, int64_t start, int64_t n, int out_dtype, void *k_out,
+                void *v_out, void *stream);
+/* out[b, i, h] = softmax over the positions j that query i sees of (scale q k_j), times v_j; heads / kv_heads query heads share a KV head. Query i
+ * of sequence b is at p = pos[b] + i and sees j <= p (causal) or j < pos[b] + seq, and with a window > 0 only j > p - window. One that sees nothing gives
+ * zeros (lse -inf). q and out [batch, seq, heads, head_dim] have one type; lse (may be NULL): f32 [batch, seq, heads], the natural logarithm of the sum of
+ * exponentials. f32 queries: products and sums to f32 accuracy. f16 / bf16: the softmax weights are rounded to 16 bits before they meet v.
+ * workspace: xnq_kv_attend_workspace_bytes, 16-byte aligned, zeroed once after it was allocated; one call at a time may use it. */
+size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim);
+int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
+                  int pos_stride, float scale, int causal, int64_t window, void *workspace, size_t ws_bytes, void *stream);
+
 /* Sticky device-side status bits of this library's kernels on the current device (0 = healthy).
  * Bits 0-7, one-row ring kernel: bit 0 a consumer's bounded mbarrier wait expired, bit 1 a producer's, bit 2 a
  * self-check refused an access. Bits 8-15: the same for the fp16 tensor-core kernel. Bits 16-23, integer
  * tensor-core kernel: a wait of the producer (16), a converter (17), the MMA issuer (18), a drain warp (19)
  * expired. Bits 24-25: a decode position outside [0, max_seq) reached xnq_rope_kv_store (24) or
- * xnq_attn_decode (25); bit 26: xnq_embed_rows met a token outside the table. Synchronizes the device.
+ * xnq_attn_decode (25); bit 26: xnq_embed_rows met a token outside the table.
+ * Bits 27-29, the quantized KV cache: 27 a position past it was to be stored or read back, 28 attended to, 29 a page table's entry was no page.
+ * Synchronizes the device.
  * No counterpart in the reference (its kernels never wait on anything). */
 int xnq_device_status(unsigned int *bits);
 /* When bit 2 of the status is set, a kernel's self-check refused an out-of-range copy or store

@@ -89,6 +89,13 @@ def lib() -> ctypes.CDLL:
     L.xnq_rope_kv_store_prompt.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, ci, ci, ci, i64, vp]
     L.xnq_add_square.argtypes = [vp, vp, vp, i64, vp]
     L.xnq_norm_scale.argtypes = [vp, vp, vp, fp, vp, i64, i64, vp]
+    L.xnq_kv_page_bytes.argtypes = [ci, ci, ci, i64]
+    L.xnq_kv_page_bytes.restype = sz
+    L.xnq_kv_store.argtypes = [vp, vp, vp, i64, i64, vp, ci, vp, vp]
+    L.xnq_kv_load.argtypes = [vp, i64, vp, ci, i64, i64, ci, vp, vp, vp]
+    L.xnq_kv_attend_workspace_bytes.argtypes = [i64, i64, ci, ci, ci]
+    L.xnq_kv_attend_workspace_bytes.restype = sz
+    L.xnq_kv_attend.argtypes = [vp, vp, vp, vp, i64, i64, ci, vp, ci, fp, ci, i64, vp, sz, vp]
     L.xnq_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint)]
     L.xnq_device_check_record.argtypes = [ctypes.POINTER(ctypes.c_ulonglong)]
     L.xnq_set_option.argtypes = [ctypes.c_char_p, ci]

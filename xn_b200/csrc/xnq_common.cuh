@@ -339,6 +339,11 @@ int launch_imma(const WeightView &w, const void *x, int x_dtype, int64_t m, int6
 int imma_init(int device);
 int imma_status(unsigned int *bits);
 int decoder_ops_init();
+// xnq_kv_store.cu, xnq_kv_attend.cu: status bits 27 and up
+int kv_store_status(unsigned int *bits);
+int kv_store_init();
+int kv_attend_status(unsigned int *bits);
+int kv_attend_init(int device);
 int decoder_status(unsigned int *bits); // 1 rope/store, 2 attention: a position outside [0, max_seq)
 // Activation OPERAND image (XNQ_ACT_OPERAND): up to 64 rows quantized to Q8_K and laid out as the integer tensor-core kernel reads them,
 // so that a producer (add+RMSNorm, SwiGLU) can write them directly and the matmul needs no activation kernel of its own:
