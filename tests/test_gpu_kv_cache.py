@@ -59,8 +59,19 @@ def _pos(*p):
 
 
 def _held(O, fmt, x):
-    """What the oracle's blocks of the f32 rows stand for."""
+    """What the blocks of the f32 rows stand for: Q4_0 the oracle's, Q8_0 with its scale formed by a product with 1 / 127."""
     a = x.float().cpu().numpy()
+    if fmt == "q8_0":
+        blocks = a.reshape(-1, 32)
+        d = np.abs(blocks).max(1, keepdims=True) * (np.float32(1) / np.float32(127))
+        with np.errstate(divide="ignore"):
+            y = blocks * np.where(d != 0, np.float32(1) / d, np.float32(0))
+        code = np.sign(y) * np.floor(np.abs(y).astype(np.float64) + 0.5)
+        held = (code.astype(np.float32) * d.astype(np.float16).astype(np.float32)).reshape(a.shape)
+        near = O.to_float(8, O.from_float(8, a), a.size).reshape(a.shape)   # the file's quantizer: a last bit of the scale, a code at a tie
+        assert np.all(np.abs(held - near) <= np.repeat(np.abs(blocks).max(1), 32).reshape(a.shape) * (1 / 127 + 2.0 ** -11))
+        assert np.mean(held != near) < 0.02
+        return torch.from_numpy(held).to(DEV)
     return torch.from_numpy(O.to_float(int(_fmt(fmt)), O.from_float(int(_fmt(fmt)), a), a.size).reshape(a.shape)).to(DEV)
 
 
@@ -344,6 +355,17 @@ def test_positions_past_the_cache_and_missing_pages_are_reported():
         else:                                                 # queries before position 32 see nothing
             _check(got[:1, S - 32:], want[:1, S - 32:], tol, "no page")
             assert not got[0, :S - 32].any()
+
+
+def test_calls_of_any_shape_share_a_workspace():
+    """A call with few rows writes its parts where a call with many rows must not look for its tickets."""
+    B, KV, hd, L = 1, 8, 128, 4096
+    c = _filled("q4_0", B, KV, L, hd)
+    few, many = (_rand(S, B, S, 32, hd).to(DEV) for S in (1, 300))
+    first = _pos(L - 1), _pos(L - 300)
+    want = [c.attend(q, p) for q, p in zip((many, few), first[::-1])]
+    for _ in range(3):
+        assert torch.equal(c.attend(few, first[0]), want[1]) and torch.equal(c.attend(many, first[1]), want[0])
 
 
 def test_strided_queries_results_and_graphs():

@@ -1,99 +1,726 @@
 // Attention over the quantized KV cache.
+//
+// ---- few query rows (a decode step, drafts) and f32 queries: kv_attend_split_kernel ----
+//
+//   s[j, r] = scale sum_blocks d_k[j, blk] (sum_i c_k[j, i] q[r, i] - z sum_i q[r, i])          z: the code of zero, 8 or 128
+//   o[r, :] = sum_j p[j, r] d_v[j, blk] (c_v[j, :] - z) / sum_j p[j, r]                          p = 2^(s log2 e - reference)
+//
+// The codes are whole numbers and go to the tensor cores as they are, one matrix instruction (m16n8k16, f32 sums) for 16 positions (S) or 16 dims
+// (O) by 8 query rows; scales meet the f32 sums (keys) or the weights (values). Bound by the cache's bytes, if unpacking stays cheap: a tile's 32
+// positions are 4608 bytes, which an SM gets in 200 cycles. So no code is converted: masked out of its word, a nibble or byte in the low ten
+// bits of a half is the f16 SUBNORMAL c 2^-24 (bits 4..7: 16 c 2^-24, the 16 undone in q or in the result), exact in the product; one shift and four masks a
+// word of eight 4-bit codes. The -z term comes from the sums' start value (S) or from one product of the weights with ones (O).
+//
+// The rows of a KV head's query heads (and of a few tokens) are the 8 NT columns of a tile; a wider group takes several row tiles. The work is the
+// flattened list of (sequence, KV head, row tile, tile of 32 positions), cut into equal runs, one a CTA, so that ragged batches balance. The four
+// warps of a CTA take its tiles in turn, each with a ring of stages filled by cp.async and a running maximum and sum of its own; they meet in shared memory
+// where the run leaves an item. An item that is cut goes through records in the workspace: its last CTA to arrive adds them, in the order of the
+// parts, whoever came first.
+//
+// f32 queries (SPLIT): q and the weights are taken apart into two f16 each (22 bits), and the values' codes have their zero taken off first (with few
+// weights above the others the two sums in O would cancel); 16-bit queries: q is exact in f16 after a power of two a row, the weights are rounded to f16.
+// Ranges: p is held within 2^12 (rescaled when a maximum grows by more than 2^4), the values' scales are brought near one by a power of two a warp.
+#include <algorithm>
 #include <cmath>
 
 #include "xnq_kv_cache.cuh"
+#include "xnq_quantize_act.cuh"
 
 namespace xnq {
 namespace {
 
 __device__ unsigned int g_kv_attend_status;
 
+constexpr int SPLIT_WARPS = 4, SPLIT_STAGES = 3;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
 struct AttendArgs {
   KvView c;
   KvRows q, out;
   float *lse; // [batch, seq, heads], or null
-  long long batch, seq;
-  int heads, pos_stride, causal;
+  long long batch, seq, window;
+  int heads, group, dtype, pos_stride, causal; // group: query heads of a KV head
   const long long *pos;
   float scale;
-  long long window;
+  // split kernel
+  int row_tiles, min_tiles;
+  unsigned int *tickets; // [batch * kv_heads * row_tiles], zero between calls
+  float *records;        // [grid][2] of RECORD_STRIDE floats
 };
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void from_float(float *p, float v) { *p = v; }
-__device__ __forceinline__ void from_float(__half *p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void from_float(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
-
-// One warp per query row; a lane holds one dim of every block of 32.
-template <int BITS, int HD, typename T>
-__global__ void __launch_bounds__(128) kv_attend_rows_kernel(AttendArgs a) {
-  using L = KvTile<BITS, HD>;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= a.batch * a.seq * a.heads) return;
-  const long long bs = row / a.heads, b = bs / a.seq, s = bs - b * a.seq;
-  const int h = (int)(row - bs * a.heads), kvh = h / (a.heads / a.c.kv_heads);
-  const long long first = a.pos[b * a.pos_stride], p = first + s;
-  long long hi = a.causal ? p : first + a.seq - 1, lo = a.window ? p - a.window + 1 : 0;
-  if (lo < 0) lo = 0;
-  if (hi >= a.c.max_seq) {
-    hi = a.c.max_seq - 1;
-    if (lane == 0) atomicOr(&g_kv_attend_status, KV_PAST_ATTEND);
-  }
-  if (p < 0) hi = -1;
-  float q[L::NB], acc[L::NB], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < L::NB; i++) {
-    q[i] = to_float(static_cast<const T *>(a.q.p)[b * a.q.sb + s * a.q.ss + h * a.q.sh + i * 32 + lane]) * a.scale;
-    acc[i] = 0.f;
-  }
-  for (long long j = lo; j <= hi; j++) {
-    const uint8_t *tile = kv_tile_at(a.c, (int)b, kvh, (int)(j / KV_TILE), L::BYTES);
-    if (!tile) {
-      if (lane == 0) atomicOr(&g_kv_attend_status, KV_NO_PAGE);
-      continue;
-    }
-    const int r = (int)(j % KV_TILE);
-    float d = 0.f;
-#pragma unroll
-    for (int i = 0; i < L::NB; i++) {
-      const float sc = __half2float(*reinterpret_cast<const __half *>(tile + L::k_scale(r, i)));
-      int code;
-      if (BITS == 4) code = *reinterpret_cast<const uint32_t *>(tile + L::k_word(r, lane / 8, i)) >> (4 * (lane & 7)) & 15;
-      else code = *reinterpret_cast<const uint32_t *>(tile + L::k_word(r, lane / 8, 2 * i + (lane & 7) / 4)) >> (8 * (lane & 3)) & 255;
-      d += q[i] * (sc * (float)(code - L::ZERO));
-    }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    const float mn = fmaxf(m, d), corr = m == -INFINITY ? 0.f : expf(m - mn), w = expf(d - mn);
-    l = l * corr + w;
-    m = mn;
-#pragma unroll
-    for (int i = 0; i < L::NB; i++) {
-      const float sc = __half2float(*reinterpret_cast<const __half *>(tile + L::v_scale(r / 2, i) + 2 * (r & 1)));
-      int code;
-      if (BITS == 4) code = *reinterpret_cast<const uint32_t *>(tile + L::v_word(r / 2, lane / 4, i)) >> (16 * (r & 1) + 4 * (lane & 3)) & 15;
-      else code = *reinterpret_cast<const uint32_t *>(tile + L::v_word(r / 2, lane / 4, 2 * i + (lane & 3) / 2)) >> (16 * (r & 1) + 8 * (lane & 1)) & 255;
-      acc[i] = acc[i] * corr + w * (sc * (float)(code - L::ZERO));
-    }
-  }
-  T *o = static_cast<T *>(a.out.p) + b * a.out.sb + s * a.out.ss + h * a.out.sh;
-#pragma unroll
-  for (int i = 0; i < L::NB; i++) from_float(o + i * 32 + lane, l > 0.f ? acc[i] / l : 0.f);
-  if (a.lse && lane == 0) a.lse[row] = l > 0.f ? m + logf(l) : -INFINITY;
+// What sequence b's queries see, as tiles [first, first + count).
+struct Span {
+  int first, count;
+  long long pos;
+};
+__device__ __forceinline__ Span span_of(const AttendArgs &a, int b) {
+  Span s;
+  s.pos = a.pos[(long long)b * a.pos_stride];
+  const long long hi = min(s.pos + a.seq - 1, a.c.max_seq - 1), p0 = max(s.pos, 0ll), lo = a.window ? max(p0 - a.window + 1, 0ll) : 0ll;
+  s.first = (int)(min(lo, a.c.max_seq) / KV_TILE);
+  s.count = hi < lo ? 0 : (int)(hi / KV_TILE) - s.first + 1;
+  return s;
+}
+// positions [lo, hi] that the query at token s of a sequence at `pos` sees
+__device__ __forceinline__ void seen_by(const AttendArgs &a, long long pos, long long s, int &lo, int &hi) {
+  const long long p = pos + s;
+  const long long h = p < 0 ? -1 : min(a.causal ? p : pos + a.seq - 1, a.c.max_seq - 1);
+  const long long l = a.window ? max(p - a.window + 1, 0ll) : 0ll;
+  hi = (int)h, lo = (int)min(l, a.c.max_seq);
 }
 
-template <int BITS, int HD, typename T>
-int run_attend(const AttendArgs &a, cudaStream_t s) {
-  const long long blocks = (a.batch * a.seq * a.heads + 3) / 4;
-  if (blocks > INT32_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: too many rows");
-  XNQ_CUDA(launch_pdl(kv_attend_rows_kernel<BITS, HD, T>, dim3((unsigned)blocks), dim3(128), 0, s, a));
+__device__ __forceinline__ void load8_any(const void *p, int dtype, long long at, float (&v)[8]) {
+  if (dtype == XNQ_F32) load8(static_cast<const float *>(p) + at, v);
+  else if (dtype == XNQ_F16) load8(static_cast<const __half *>(p) + at, v);
+  else load8(static_cast<const __nv_bfloat16 *>(p) + at, v);
+}
+__device__ __forceinline__ void store_any(void *p, int dtype, long long at, float v) {
+  if (dtype == XNQ_F32) static_cast<float *>(p)[at] = v;
+  else if (dtype == XNQ_F16) static_cast<__half *>(p)[at] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) { // of 16-bit values: lane (g, t) gives row g's columns 2 t, 2 t + 1 and gets column g's rows
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2 *>(&v); }
+__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t *>(&v); }
+__device__ __forceinline__ float exp2_approx(float x) { // 2^x within 2 ulp
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// d = {a & mask} of the four registers of an operand: words w0 and w1 (rows g and g + 8 of K; positions 2 t and 2 t + 8 of V)
+template <int BITS>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) { // the i-th of a word's pairs (16 bits apart), as subnormals; 4 bits: times 16 where i is odd
+  if (BITS == 4) return (i & 2 ? w >> 8 : w) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+  return (i & 1 ? w >> 8 : w) & 0x00ff00ffu;
+}
+template <int BITS>
+__device__ __forceinline__ uint32_t signed_pair(uint32_t w, int i) { // the same pair as the whole numbers that it stands for
+  if (BITS == 4) {
+    const uint32_t m = code_pair<4>(w, i) | 0x64006400u; // 1024 + c, or 1024 + 16 c
+    return as_u32(i & 1 ? __hfma2(as_half2(m), __float2half2_rn(0.0625f), __float2half2_rn(-72.f)) : __hsub2(as_half2(m), __float2half2_rn(1032.f)));
+  }
+  return as_u32(__hsub2(as_half2(code_pair<8>(w, i) | 0x64006400u), __float2half2_rn(1152.f)));
+}
+
+template <int HD, int NT>
+struct SplitShape {
+  static constexpr int R = 8 * NT;        // query rows of an item
+  static constexpr int COL = HD + 4;      // floats from row to row of the accumulators in shared memory
+  static constexpr int MERGE = SPLIT_WARPS * R * (COL + 2) * 4; // bytes
+};
+
+// Parts of items in the workspace, two places a CTA: references [R], sums [R], accumulators [R][HD]. The tickets lie behind all places, at one
+// offset whatever the shape of the call: they are zero between calls and no other call's parts may fall on them.
+constexpr int MAX_SPLIT_GRID = 148 * 4, RECORD_STRIDE = 16 * (128 + 2);
+constexpr size_t RECORDS_BYTES = (size_t)MAX_SPLIT_GRID * 2 * RECORD_STRIDE * 4;
+
+// A tile's copy into shared memory by one warp; null: zeros.
+template <int BYTES>
+__device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t *src, const uint8_t *some, int lane) {
+  const uint32_t n = src ? 16u : 0u;
+  const uint8_t *s = src ? src : some;
+#pragma unroll
+  for (int i = 0; i < (BYTES / 16 + 31) / 32; i++) {
+    const int ch = i * 32 + lane;
+    if (BYTES / 16 % 32 == 0 || ch < BYTES / 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + ch * 16), "l"(s + ch * 16), "r"(n) : "memory");
+  }
+}
+
+template <int BITS, int HD, int NT, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const AttendArgs a) {
+  using L = KvTile<BITS, HD>;
+  using P = SplitShape<HD, NT>;
+  constexpr int NB = L::NB, W = L::W, R = P::R;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_sum[SPLIT_WARPS];
+  __shared__ long long s_before;
+  __shared__ int s_b, s_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float *const merge = reinterpret_cast<float *>(smem + SPLIT_WARPS * SPLIT_STAGES * L::BYTES);
+  float *const s_m = merge, *const s_l = merge + SPLIT_WARPS * R, *const s_acc = merge + 2 * SPLIT_WARPS * R;
+  uint8_t *const ring = smem + warp * SPLIT_STAGES * L::BYTES;
+  const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- this CTA's run of the flattened list: [t0, t1) of `total` tiles ----
+  const int per_seq = a.c.kv_heads * a.row_tiles; // items of a sequence, all of its count of tiles
+  const int batch = (int)a.batch;
+  long long mine = 0;
+  for (int b = threadIdx.x; b < batch; b += SPLIT_WARPS * 32) mine += span_of(a, b).count;
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) s_sum[warp] = mine;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < SPLIT_WARPS; w++) total += s_sum[w];
+  total *= per_seq;
+  const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)a.min_tiles);
+  const long long t0 = blockIdx.x * share, t1 = min(total, t0 + share);
+
+  // sequences that see nothing: rows of zeros
+  for (int b = blockIdx.x; b < batch; b += gridDim.x) {
+    const Span sp = span_of(a, b);
+    if (threadIdx.x == 0 && sp.pos + a.seq > a.c.max_seq) atomicOr(&g_kv_attend_status, KV_PAST_ATTEND);
+    if (sp.count) continue;
+    for (long long i = threadIdx.x; i < a.seq * a.heads * HD; i += SPLIT_WARPS * 32) {
+      const long long row = i / HD, s = row / a.heads;
+      const int h = (int)(row - s * a.heads), d = (int)(i - row * HD);
+      store_any(a.out.p, a.dtype, b * a.out.sb + s * a.out.ss + h * a.out.sh + d, 0.f);
+      if (a.lse && d == 0) a.lse[(b * a.seq + s) * a.heads + h] = -INFINITY;
+    }
+  }
+  if (t0 >= t1) return;
+  // the sequence of tile t0: a scan of the counts, 32 at a time, by the first warp
+  if (warp == 0) {
+    long long before = 0;
+    int found = -1;
+    for (int base = 0; base < batch && found < 0; base += 32) {
+      const long long n = base + lane < batch ? (long long)span_of(a, base + lane).count * per_seq : 0;
+      long long inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      const unsigned here = __ballot_sync(0xffffffffu, before + inc > t0);
+      if (here) {
+        const int f = __ffs(here) - 1;
+        found = base + f;
+        before += __shfl_sync(0xffffffffu, inc - n, f);
+      } else before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) s_b = found, s_before = before;
+  }
+  __syncthreads();
+  int b = s_b;
+  long long item0 = s_before; // first tile of the item at hand in the flattened list
+  Span sp = span_of(a, b);
+  int item = (int)((t0 - item0) / sp.count); // of the sequence: (KV head, row tile)
+  item0 += (long long)item * sp.count;
+
+  for (long long at = t0; at < t1;) {
+    while (item == per_seq || sp.count == 0) { // on to the next sequence that has tiles
+      item = 0;
+      if (++b >= batch) return; // (only where pos changes under the kernel)
+      sp = span_of(a, b);
+    }
+    const int kvh = item / a.row_tiles, rt = item - kvh * a.row_tiles;
+    const int ta = (int)(at - item0), tb = (int)min((long long)sp.count, t1 - item0); // tiles [ta, tb) of the item are this CTA's
+    const int rows = (int)min((long long)R, a.seq * a.group - (long long)rt * R);
+
+    // ---- start the ring: this warp's tiles are ta + warp, + 4, ...; lane i looks up the page of the i-th of a batch of 32 ----
+    const int n_tiles = tb - ta > warp ? (tb - ta - warp + SPLIT_WARPS - 1) / SPLIT_WARPS : 0;
+    const uint8_t *ahead = nullptr; // lane i's tile
+    unsigned gone = 0;              // bit s: the tile in stage s has no page
+    auto issue = [&](int i) {
+      if (i < n_tiles) {
+        if ((i & 31) == 0) {
+          const int mine_i = i + lane;
+          ahead = mine_i < n_tiles ? kv_tile_at(a.c, b, kvh, sp.first + ta + warp + mine_i * SPLIT_WARPS, L::BYTES) : nullptr;
+        }
+        const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ahead), i & 31));
+        const int stage = i % SPLIT_STAGES;
+        gone = (gone & ~(1u << stage)) | (src ? 0u : 1u << stage);
+        copy_tile<L::BYTES>(ring_addr + stage * L::BYTES, src, a.c.pages, lane);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < SPLIT_STAGES - 1; i++) issue(i);
+
+    // ---- the query rows as operands ----
+    uint32_t qh[NT][NB][4], ql[SPLIT ? NT : 1][SPLIT ? NB : 1][4]; // [.. ][b][2 step + register]
+    float start[NT][NB][2], factor[NT][2]; // of columns 2 t, 2 t + 1
+    int lo[NT][2], hi[NT][2], lo_all = 0, hi_all = INT32_MAX, hi_any = -1, lo_any = INT32_MAX;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      const int r = n * 8 + g; // this lane's row as an operand's column
+      const long long row = (long long)rt * R + r, s = row / a.group;
+      const int h = kvh * a.group + (int)(row - s * a.group);
+      float v[NB][8], top = 0.f;
+#pragma unroll
+      for (int bl = 0; bl < NB; bl++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[bl][i] = 0.f;
+        if (r < rows) load8_any(a.q.p, a.dtype, b * a.q.sb + s * a.q.ss + h * a.q.sh + bl * 32 + t * 8, v[bl]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[bl][i]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int e = top > 0.f && top < INFINITY ? 13 - ilogbf(top) : 0; // the largest |q| to [2^13, 2^14)
+      e = max(-100, min(100, e));
+      const float up = ldexpf(1.f, e);
+      float sum[NB];
+#pragma unroll
+      for (int bl = 0; bl < NB; bl++) {
+        float hi_v[8], lo_v[8];
+        sum[bl] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float x = v[bl][i] * up;
+          hi_v[i] = __half2float(__float2half_rn(x));
+          lo_v[i] = SPLIT ? __half2float(__float2half_rn(x - hi_v[i])) : 0.f;
+          sum[bl] += hi_v[i] + lo_v[i];
+        }
+        sum[bl] += __shfl_xor_sync(0xffffffffu, sum[bl], 1);
+        sum[bl] += __shfl_xor_sync(0xffffffffu, sum[bl], 2);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { // pair i of a word: dims i and i + 4 (4 bits, the odd ones 16 times too large), or of word i / 2 bytes i % 2 and i % 2 + 2
+          const int x = BITS == 4 ? i : (i >> 1) * 4 + (i & 1), y = BITS == 4 ? i + 4 : x + 2;
+          const float down = BITS == 4 && (i & 1) ? 0.0625f : 1.f;
+          qh[n][bl][i] = pack_half2(hi_v[x] * down, hi_v[y] * down);
+          if (SPLIT) ql[n][bl][i] = pack_half2(lo_v[x] * down, lo_v[y] * down);
+        }
+      }
+      int l0, h0;
+      seen_by(a, sp.pos, s, l0, h0);
+      if (r >= rows) l0 = 0, h0 = INT32_MAX; // no row: its weights are thrown away
+      else hi_any = max(hi_any, h0), lo_any = min(lo_any, l0);
+      lo_all = max(lo_all, l0), hi_all = min(hi_all, h0);
+      const float f = ldexpf(a.scale * LOG2E, 24 - e);
+#pragma unroll
+      for (int c = 0; c < 2; c++) { // from the lane that holds row 2 t + c
+        const int from = (2 * t + c) * 4;
+#pragma unroll
+        for (int bl = 0; bl < NB; bl++) start[n][bl][c] = __shfl_sync(0xffffffffu, sum[bl], from) * (-(float)L::ZERO / 16777216.f);
+        factor[n][c] = __shfl_sync(0xffffffffu, f, from);
+        lo[n][c] = __shfl_sync(0xffffffffu, l0, from), hi[n][c] = __shfl_sync(0xffffffffu, h0, from);
+      }
+    }
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) {
+      lo_all = max(lo_all, __shfl_xor_sync(0xffffffffu, lo_all, o)), hi_all = min(hi_all, __shfl_xor_sync(0xffffffffu, hi_all, o));
+      lo_any = min(lo_any, __shfl_xor_sync(0xffffffffu, lo_any, o)), hi_any = max(hi_any, __shfl_xor_sync(0xffffffffu, hi_any, o));
+    }
+
+    // ---- this warp's tiles ----
+    float acc[NT][2 * NB][4], zsum[SPLIT ? 1 : NT][4], m[NT][2], ref[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int i = 0; i < 2 * NB; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[n][i][c] = 0.f;
+      if (!SPLIT)
+#pragma unroll
+        for (int c = 0; c < 4; c++) zsum[n][c] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY, ref[n][0] = ref[n][1] = 0.f, l[n][0] = l[n][1] = 0.f;
+    }
+    int k = 0;                 // the values' scales are taken times 2^k
+    bool k_set = false;
+    float d_most = 0.f;        // more than this: another k
+    for (int i = 0; i < n_tiles; i++) {
+      issue(i + SPLIT_STAGES - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(SPLIT_STAGES - 1) : "memory");
+      __syncwarp();
+      const int stage = i % SPLIT_STAGES;
+      const uint8_t *tile = ring + stage * L::BYTES;
+      const int j0 = (sp.first + ta + warp + i * SPLIT_WARPS) * KV_TILE;
+      const bool masked = j0 < lo_all || j0 + KV_TILE - 1 > hi_all;
+      if ((gone >> stage) & 1) { // no page: not attended to
+        if (lane == 0) atomicOr(&g_kv_attend_status, KV_NO_PAGE);
+        __syncwarp();
+        continue;
+      }
+      if (j0 > hi_any || j0 + KV_TILE - 1 < lo_any) { // (other row tiles of the sequence see it)
+        __syncwarp();
+        continue;
+      }
+      // scores: registers [group of 16][n][c]; c 0, 1: position g, 2, 3: g + 8 of the group; columns 2 t + (c & 1)
+      float s[2][NT][4];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        uint32_t w[2][W];
+        uint32_t dk[2][NB / 2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int row = u * 16 + e * 8 + g;
+          if (W == 2) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(tile + L::k_word(row, t, 0));
+            w[e][0] = x.x, w[e][1] = x.y;
+          } else {
+#pragma unroll
+            for (int q4 = 0; q4 < W; q4 += 4) {
+              const uint4 x = *reinterpret_cast<const uint4 *>(tile + L::k_word(row, t, q4));
+              w[e][q4] = x.x, w[e][q4 + 1] = x.y, w[e][q4 + 2] = x.z, w[e][q4 + 3] = x.w;
+            }
+          }
+#pragma unroll
+          for (int q2 = 0; q2 < NB / 2; q2++) dk[e][q2] = *reinterpret_cast<const uint32_t *>(tile + L::k_scale(row, 2 * q2));
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) s[u][n][c] = 0.f;
+#pragma unroll
+        for (int bl = 0; bl < NB; bl++) {
+          const float d0 = bl & 1 ? __high2float(as_half2(dk[0][bl / 2])) : __low2float(as_half2(dk[0][bl / 2]));
+          const float d1 = bl & 1 ? __high2float(as_half2(dk[1][bl / 2])) : __low2float(as_half2(dk[1][bl / 2]));
+          uint32_t op[2][4];
+#pragma unroll
+          for (int step = 0; step < 2; step++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const uint32_t x = BITS == 4 ? w[e][bl] : w[e][2 * bl + step];
+              op[step][e] = code_pair<BITS>(x, BITS == 4 ? 2 * step : 0), op[step][e + 2] = code_pair<BITS>(x, BITS == 4 ? 2 * step + 1 : 1);
+            }
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            float d[4] = {start[n][bl][0], start[n][bl][1], start[n][bl][0], start[n][bl][1]};
+            mma(d, op[0], qh[n][bl][0], qh[n][bl][1], d);
+            mma(d, op[1], qh[n][bl][2], qh[n][bl][3], d);
+            if (SPLIT) {
+              mma(d, op[0], ql[SPLIT ? n : 0][SPLIT ? bl : 0][0], ql[SPLIT ? n : 0][SPLIT ? bl : 0][1], d);
+              mma(d, op[1], ql[SPLIT ? n : 0][SPLIT ? bl : 0][2], ql[SPLIT ? n : 0][SPLIT ? bl : 0][3], d);
+            }
+            s[u][n][0] += d0 * d[0], s[u][n][1] += d0 * d[1], s[u][n][2] += d1 * d[2], s[u][n][3] += d1 * d[3];
+          }
+        }
+      }
+      // the values' scales: half2 of a pair of positions [group][pair t or t + 4][block]
+      uint32_t dv[2][2][NB];
+      __half2 d_top = __float2half2_rn(0.f);
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int pair = u * 8 + e * 4 + t;
+          if (NB == 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(tile + L::v_scale(pair, 0));
+            dv[u][e][0] = x.x, dv[u][e][1] = x.y, dv[u][e][NB - 2] = x.z, dv[u][e][NB - 1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(tile + L::v_scale(pair, 0));
+            dv[u][e][0] = x.x, dv[u][e][1] = x.y;
+          }
+          if (masked) { // what no row sees may be anything
+            const int j = j0 + 2 * pair;
+            const uint32_t keep = (j >= lo_any && j <= hi_any ? 0xffffu : 0u) | (j + 1 >= lo_any && j + 1 <= hi_any ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int bl = 0; bl < NB; bl++) dv[u][e][bl] &= keep;
+          }
+#pragma unroll
+          for (int bl = 0; bl < NB; bl++) d_top = __hmax2(d_top, __habs2(as_half2(dv[u][e][bl])));
+        }
+      const float d_max = fmaxf(__low2float(d_top), __high2float(d_top));
+      if (__any_sync(0xffffffffu, d_max > d_most || !k_set)) {
+        float top = d_max;
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // scales of up to 2^-6 .. 4 are taken as they are
+        const int e = top > 0.f && top < INFINITY ? ilogbf(top) : 0, k_new = e > 1 || e < -6 ? -e : 0;
+        if (top > 0.f) {
+          const float by = k_set ? ldexpf(1.f, k_new - k) : 0.f;
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int x = 0; x < 2 * NB; x++)
+#pragma unroll
+              for (int c = 0; c < 4; c++) acc[n][x][c] *= by;
+            if (!SPLIT)
+#pragma unroll
+              for (int c = 0; c < 4; c++) zsum[n][c] *= by;
+          }
+          k = k_new, k_set = true, d_most = ldexpf(4.f, -k);
+        }
+      }
+      if (k != 0) {
+        const __half2 by = __float2half2_rn(ldexpf(1.f, min(k, 15))), by2 = __float2half2_rn(ldexpf(1.f, max(k - 15, 0))); // 2^24 is past f16
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int bl = 0; bl < NB; bl++) dv[u][e][bl] = as_u32(__hmul2(__hmul2(as_half2(dv[u][e][bl]), by), by2));
+      }
+      // softmax
+      bool grew = false;
+      float top[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            s[u][n][c] *= factor[n][c & 1];
+            if (masked) {
+              const int j = j0 + u * 16 + (c >> 1) * 8 + g;
+              if (j < lo[n][c & 1] || j > hi[n][c & 1]) s[u][n][c] = -INFINITY;
+            }
+          }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float x = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
+#pragma unroll
+          for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+          top[n][c] = fmaxf(m[n][c], x);
+          grew |= top[n][c] > ref[n][c] + 12.f || (m[n][c] == -INFINITY && top[n][c] != -INFINITY); // the reference lies 8 below a maximum
+        }
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const float r2 = top[n][c] == -INFINITY ? 0.f : top[n][c] - 8.f;
+            const float by = m[n][c] == -INFINITY ? 0.f : exp2_approx(ref[n][c] - r2);
+            m[n][c] = top[n][c], ref[n][c] = r2, l[n][c] *= by;
+#pragma unroll
+            for (int x = 0; x < 2 * NB; x++) acc[n][x][c] *= by, acc[n][x][c + 2] *= by;
+            if (!SPLIT) zsum[SPLIT ? 0 : n][c] *= by, zsum[SPLIT ? 0 : n][c + 2] *= by;
+          }
+      }
+      uint32_t ph[2][NT][2], pl[2][SPLIT ? NT : 1][2]; // weights of positions (2 t, 2 t + 1), (+ 8) of the group, query row g
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float p0 = exp2_approx(s[u][n][2 * e] - ref[n][0]), p1 = exp2_approx(s[u][n][2 * e + 1] - ref[n][1]);
+            l[n][0] += p0, l[n][1] += p1;
+            const uint32_t h2 = pack_half2(p0, p1);
+            ph[u][n][e] = transpose8x8(h2);
+            if (SPLIT) pl[u][SPLIT ? n : 0][e] = transpose8x8(pack_half2(p0 - __low2float(as_half2(h2)), p1 - __high2float(as_half2(h2))));
+          }
+      // values
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        uint32_t w[2][W];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int pair = u * 8 + e * 4 + t;
+          if (W == 2) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(tile + L::v_word(pair, g, 0));
+            w[e][0] = x.x, w[e][1] = x.y;
+          } else {
+#pragma unroll
+            for (int q4 = 0; q4 < W; q4 += 4) {
+              const uint4 x = *reinterpret_cast<const uint4 *>(tile + L::v_word(pair, g, q4));
+              w[e][q4] = x.x, w[e][q4 + 1] = x.y, w[e][q4 + 2] = x.z, w[e][q4 + 3] = x.w;
+            }
+          }
+        }
+#pragma unroll
+        for (int bl = 0; bl < NB; bl++) {
+          uint32_t op[2][4]; // dims 4 g (rows 0..7) and 4 g + 1 (rows 8..15) of the block, then 4 g + 2 and 4 g + 3
+#pragma unroll
+          for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const uint32_t x = BITS == 4 ? w[e][bl] : w[e][2 * bl + half];
+              const int i0 = BITS == 4 ? 2 * half : 0;
+              op[half][2 * e] = SPLIT ? signed_pair<BITS>(x, i0) : code_pair<BITS>(x, i0);
+              op[half][2 * e + 1] = SPLIT ? signed_pair<BITS>(x, i0 + 1) : code_pair<BITS>(x, i0 + 1);
+            }
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            uint32_t bh[2], bl2[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const __half2 ph2 = as_half2(ph[u][n][e]), d2 = as_half2(dv[u][e][bl]);
+              if (!SPLIT) {
+                bh[e] = as_u32(__hmul2(ph2, d2));
+                if (masked) bh[e] &= __hne2_mask(ph2, __float2half2_rn(0.f)); // a scale that another row sees may be infinite
+              } else {
+                const __half2 pl2 = as_half2(pl[u][SPLIT ? n : 0][e]);
+                const float p0 = __low2float(ph2) + __low2float(pl2), p1 = __high2float(ph2) + __high2float(pl2);
+                float x0 = p0 * __low2float(d2), x1 = p1 * __high2float(d2);
+                if (masked) x0 = p0 == 0.f ? 0.f : x0, x1 = p1 == 0.f ? 0.f : x1;
+                bh[e] = pack_half2(x0, x1);
+                bl2[e] = pack_half2(x0 - __low2float(as_half2(bh[e])), x1 - __high2float(as_half2(bh[e])));
+              }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              mma(acc[n][2 * bl + half], op[half], bh[0], bh[1], acc[n][2 * bl + half]);
+              if (SPLIT) mma(acc[n][2 * bl + half], op[half], bl2[0], bl2[1], acc[n][2 * bl + half]);
+            }
+            if (!SPLIT) { // row bl of one more product: the block's sum of weights
+              const uint32_t one = g == bl ? 0x3c003c00u : 0u;
+              const uint32_t ones[4] = {one, 0u, one, 0u};
+              mma(zsum[SPLIT ? 0 : n], ones, bh[0], bh[1], zsum[SPLIT ? 0 : n]);
+            }
+          }
+        }
+      }
+      __syncwarp(); // the stage is free
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+
+    // ---- the warps meet ----
+    __syncthreads(); // (of the item before, everything has been read)
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const int col = n * 8 + 2 * t + c;
+        float sum = l[n][c];
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (g == 0) s_m[warp * R + col] = m[n][c] == -INFINITY ? -INFINITY : ref[n][c], s_l[warp * R + col] = sum;
+        const float down = ldexpf(1.f, -k);
+#pragma unroll
+        for (int bl = 0; bl < NB; bl++) {
+          float4 v;
+          const float *x = acc[n][2 * bl], *y = acc[n][2 * bl + 1];
+          if (SPLIT) v = make_float4(x[c] * down, x[c + 2] * down, y[c] * down, y[c + 2] * down);
+          else { // codes came as c 2^-24, those of the odd dims 16 times as much with 4 bits
+            const float z = __shfl_sync(0xffffffffu, zsum[SPLIT ? 0 : n][c], bl * 4 + t) * (float)L::ZERO, one = 16777216.f, odd = BITS == 4 ? 1048576.f : 16777216.f;
+            v = make_float4((x[c] * one - z) * down, (x[c + 2] * odd - z) * down, (y[c] * one - z) * down, (y[c + 2] * odd - z) * down);
+          }
+          *reinterpret_cast<float4 *>(s_acc + (warp * R + col) * P::COL + bl * 32 + g * 4) = v;
+        }
+      }
+    __syncthreads();
+    const bool whole = ta == 0 && tb == sp.count;
+    const long long c_first = item0 / share, c_last = (item0 + sp.count - 1) / share; // the CTAs that hold parts of the item
+    const long long seq_item = (long long)b * per_seq + item;
+    auto put = [&](int r, int d, float m_all, float l_all, float v) { // a finished value
+      const long long row = (long long)rt * R + r, s = row / a.group;
+      const int h = kvh * a.group + (int)(row - s * a.group);
+      store_any(a.out.p, a.dtype, b * a.out.sb + s * a.out.ss + h * a.out.sh + d, l_all > 0.f ? v / l_all : 0.f);
+      if (a.lse && d == 0) a.lse[((long long)b * a.seq + s) * a.heads + h] = l_all > 0.f ? (m_all + log2f(l_all)) * LN2 : -INFINITY;
+    };
+    float *const rec = a.records + (blockIdx.x * 2 + (ta == 0 ? 1 : 0)) * (long long)RECORD_STRIDE;
+    for (int i = threadIdx.x; i < rows * HD; i += SPLIT_WARPS * 32) {
+      const int r = i / HD, d = i - r * HD;
+      float m_all = -INFINITY, l_all = 0.f, v = 0.f;
+#pragma unroll
+      for (int w = 0; w < SPLIT_WARPS; w++) m_all = fmaxf(m_all, s_m[w * R + r]);
+#pragma unroll
+      for (int w = 0; w < SPLIT_WARPS; w++) {
+        const float mw = s_m[w * R + r];
+        const float by = mw == -INFINITY ? 0.f : exp2_approx(mw - m_all);
+        l_all += by * s_l[w * R + r];
+        if (mw != -INFINITY) v += by * s_acc[(w * R + r) * P::COL + d];
+      }
+      if (whole) put(r, d, m_all, l_all, v);
+      else {
+        if (d == 0) rec[r] = m_all, rec[R + r] = l_all;
+        rec[2 * R + i] = v;
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) s_last = atomicInc(a.tickets + seq_item, (unsigned)(c_last - c_first)) == (unsigned)(c_last - c_first);
+      __syncthreads();
+      if (s_last) { // all parts are there: added in an order of their places
+        __threadfence();
+        const float *const part0 = a.records + (c_first * 2 + 1) * RECORD_STRIDE, *const parts = a.records + (c_first + 1) * 2 * RECORD_STRIDE; // the first, the others
+        const int others = (int)(c_last - c_first);
+        for (int r = warp; r < rows; r += SPLIT_WARPS) {
+          float m_all = __ldcg(part0 + r), l_all = 0.f;
+          for (int c = lane; c < others; c += 32) m_all = fmaxf(m_all, __ldcg(parts + (long long)c * 2 * RECORD_STRIDE + r));
+#pragma unroll
+          for (int o = 16; o >= 1; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
+          auto add = [&](const float *p) {
+            const float mp = __ldcg(p + r);
+            if (mp != -INFINITY) l_all += exp2_approx(mp - m_all) * __ldcg(p + R + r);
+          };
+          if (lane == 0) add(part0);
+          for (int c = lane; c < others; c += 32) add(parts + (long long)c * 2 * RECORD_STRIDE);
+#pragma unroll
+          for (int o = 16; o >= 1; o >>= 1) l_all += __shfl_xor_sync(0xffffffffu, l_all, o);
+          if (lane == 0) s_m[r] = m_all, s_l[r] = l_all;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * (HD / 4); i += SPLIT_WARPS * 32) {
+          const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+          const float m_all = s_m[r], l_all = s_l[r];
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          auto add = [&](const float *p) {
+            const float mp = __ldcg(p + r);
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + 2 * R + 4 * i));
+            const float by = mp == -INFINITY ? 0.f : exp2_approx(mp - m_all);
+            if (by != 0.f) v.x += by * x.x, v.y += by * x.y, v.z += by * x.z, v.w += by * x.w;
+          };
+          add(part0);
+#pragma unroll 8
+          for (int c = 0; c < others; c++) add(parts + (long long)c * 2 * RECORD_STRIDE);
+          put(r, d, m_all, l_all, v.x), put(r, d + 1, m_all, l_all, v.y), put(r, d + 2, m_all, l_all, v.z), put(r, d + 3, m_all, l_all, v.w);
+        }
+      }
+    }
+    at = item0 + tb;
+    item0 += sp.count;
+    item++;
+  }
+}
+
+int g_sms[64]; // of the devices that xnq_init has seen
+
+template <int BITS, int HD, int NT, bool SPLIT>
+struct SplitLaunch {
+  static constexpr size_t smem() { return SPLIT_WARPS * SPLIT_STAGES * KvTile<BITS, HD>::BYTES + SplitShape<HD, NT>::MERGE; }
+  static inline int per_sm = 0;
+  static int init() {
+    XNQ_CUDA(cudaFuncSetAttribute(kv_attend_split_kernel<BITS, HD, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem()));
+    int n = 0;
+    XNQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attend_split_kernel<BITS, HD, NT, SPLIT>, SPLIT_WARPS * 32, smem()));
+    per_sm = std::max(1, std::min(n, 4));
+    return XNQ_OK;
+  }
+};
+// Query rows of a KV head to an item of the split kernel.
+int split_nt(int64_t rows) { return rows <= 8 ? 1 : 2; }
+size_t split_workspace(int64_t batch, int64_t seq, int heads, int kv_heads) {
+  const int64_t rows = seq * (heads / kv_heads), r = 8 * split_nt(rows);
+  return RECORDS_BYTES + (size_t)batch * kv_heads * ((rows + r - 1) / r) * 4;
+}
+
+template <int BITS, int HD, int NT, bool SPLIT>
+int run_split(AttendArgs a, void *workspace, int sms, cudaStream_t s) {
+  const int64_t rows = a.seq * a.group;
+  a.row_tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
+  a.min_tiles = SPLIT_WARPS;
+  a.records = static_cast<float *>(workspace);
+  a.tickets = reinterpret_cast<unsigned int *>(static_cast<uint8_t *>(workspace) + RECORDS_BYTES);
+  using Launch = SplitLaunch<BITS, HD, NT, SPLIT>;
+  // no more CTAs than the longest caches could fill
+  const int64_t most = a.batch * a.c.kv_heads * a.row_tiles * ((a.c.max_seq + KV_TILE - 1) / KV_TILE);
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(std::min(sms * Launch::per_sm, MAX_SPLIT_GRID), std::max<int64_t>((most + a.min_tiles - 1) / a.min_tiles, a.batch)));
+  XNQ_CUDA(launch_pdl(kv_attend_split_kernel<BITS, HD, NT, SPLIT>, dim3((unsigned)grid), dim3(SPLIT_WARPS * 32), Launch::smem(), s, a));
   count_launch();
   return XNQ_OK;
+}
+
+template <typename F>
+int for_each_split(F f) { // f<BITS, HD, NT, SPLIT>()
+  int rc = XNQ_OK;
+  auto one = [&](auto l) {
+    if (rc == XNQ_OK) rc = f(l);
+  };
+  one(SplitLaunch<4, 64, 1, false>{}), one(SplitLaunch<4, 64, 2, false>{}), one(SplitLaunch<4, 64, 1, true>{}), one(SplitLaunch<4, 64, 2, true>{});
+  one(SplitLaunch<4, 128, 1, false>{}), one(SplitLaunch<4, 128, 2, false>{}), one(SplitLaunch<4, 128, 1, true>{}), one(SplitLaunch<4, 128, 2, true>{});
+  one(SplitLaunch<8, 64, 1, false>{}), one(SplitLaunch<8, 64, 2, false>{}), one(SplitLaunch<8, 64, 1, true>{}), one(SplitLaunch<8, 64, 2, true>{});
+  one(SplitLaunch<8, 128, 1, false>{}), one(SplitLaunch<8, 128, 2, false>{}), one(SplitLaunch<8, 128, 1, true>{}), one(SplitLaunch<8, 128, 2, true>{});
+  return rc;
+}
+
+template <int BITS, int HD>
+int run_attend(const AttendArgs &a, void *workspace, int sms, cudaStream_t s) {
+  const bool one = split_nt(a.seq * a.group) == 1;
+  if (a.dtype == XNQ_F32) return one ? run_split<BITS, HD, 1, true>(a, workspace, sms, s) : run_split<BITS, HD, 2, true>(a, workspace, sms, s);
+  return one ? run_split<BITS, HD, 1, false>(a, workspace, sms, s) : run_split<BITS, HD, 2, false>(a, workspace, sms, s);
 }
 
 } // namespace
@@ -102,10 +729,11 @@ int kv_attend_status(unsigned int *bits) {
   XNQ_CUDA(cudaMemcpyFromSymbol(bits, g_kv_attend_status, sizeof(*bits)));
   return XNQ_OK;
 }
-int kv_attend_init(int) {
+int kv_attend_init(int device) {
   unsigned int zero = 0;
   XNQ_CUDA(cudaMemcpyToSymbol(g_kv_attend_status, &zero, sizeof(zero)));
-  return XNQ_OK;
+  if (device < 64) XNQ_CUDA(cudaDeviceGetAttribute(&g_sms[device], cudaDevAttrMultiProcessorCount, device));
+  return for_each_split([](auto l) { return decltype(l)::init(); });
 }
 
 } // namespace xnq
@@ -116,7 +744,7 @@ extern "C" {
 
 size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim) {
   if (batch <= 0 || seq <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
-  return 16;
+  return split_workspace(batch, seq, heads, kv_heads);
 }
 
 int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
@@ -128,16 +756,22 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
   if (!q || !out || !pos) return fail(XNQ_ERR_NULL, "kv_attend: NULL argument");
   if (seq < 0 || seq > INT32_MAX || heads < 1 || heads > 65535 || heads % cache->kv_heads || pos_stride < 0 || pos_stride > 1 || window < 0)
     return fail(XNQ_ERR_SHAPE, "kv_attend: seq %lld, heads %d over %d, pos_stride %d (0 or 1), window %lld", (long long)seq, heads, cache->kv_heads, pos_stride, (long long)window);
+  if (!std::isfinite(scale)) return fail(XNQ_ERR_SHAPE, "kv_attend: the scale is not a finite number");
   if (batch == 0 || seq == 0) return XNQ_OK;
   if ((rc = kv_rows("kv_attend", "q", q, &a.q)) != XNQ_OK || (rc = kv_rows("kv_attend", "out", out, &a.out)) != XNQ_OK) return rc;
   if (out->dtype != q->dtype) return fail(XNQ_ERR_DTYPE, "kv_attend: q has type %d, out %d", q->dtype, out->dtype);
-  if (!std::isfinite(scale)) return fail(XNQ_ERR_SHAPE, "kv_attend: the scale is not a finite number");
   const size_t need = xnq_kv_attend_workspace_bytes(batch, seq, heads, cache->kv_heads, cache->head_dim);
   if (!workspace || ws_bytes < need) return fail(XNQ_ERR_SIZE, "kv_attend: workspace has %zu bytes, needs %zu (zero it once after allocating)", ws_bytes, need);
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(XNQ_ERR_ALIGN, "kv_attend: the workspace must be 16-byte aligned");
-  a.lse = lse, a.batch = batch, a.seq = seq, a.heads = heads, a.pos_stride = pos_stride, a.causal = causal, a.pos = pos, a.scale = scale, a.window = window;
-  return kv_dispatch(kv_bits(cache->ggml_dtype), cache->head_dim, q->dtype,
-                     [&](auto f) { return run_attend<f.BITS, f.HD, typename decltype(f)::T>(a, static_cast<cudaStream_t>(stream)); });
+  int device = 0;
+  XNQ_CUDA(cudaGetDevice(&device));
+  const int sms = device < 64 ? g_sms[device] : 0;
+  if (!sms) return fail(XNQ_ERR_UNSUPPORTED, "kv_attend: xnq_init has not run for device %d", device);
+  a.lse = lse, a.batch = batch, a.seq = seq, a.heads = heads, a.group = heads / cache->kv_heads, a.dtype = q->dtype;
+  a.pos_stride = pos_stride, a.causal = causal, a.pos = pos, a.scale = scale, a.window = std::min<int64_t>(window, INT32_MAX);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (kv_bits(cache->ggml_dtype) == 4) return cache->head_dim == 64 ? run_attend<4, 64>(a, workspace, sms, s) : run_attend<4, 128>(a, workspace, sms, s);
+  return cache->head_dim == 64 ? run_attend<8, 64>(a, workspace, sms, s) : run_attend<8, 128>(a, workspace, sms, s);
 }
 
 } // extern "C"

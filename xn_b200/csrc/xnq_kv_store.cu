@@ -41,7 +41,9 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16 *p, const fl
 }
 
 // One block of 32 in four neighbouring lanes, 8 values each: the arithmetic of BlockQ4_0::from_float and BlockQ8_0::from_float
-// (k_quants.rs:235-270, 636-661), every operation rounded for itself. The codes come back unsigned: 4 bits, eight nibbles in lo; 8 bits, code + 128.
+// (k_quants.rs:235-270, 636-661), every operation rounded for itself, but for Q8_0's scale: max|x| times the f32 nearest 1 / 127, where the file's quantizer
+// divides by 127 (the two differ in the scale's last f32 bit, one f16 scale in some 4000 and one code at a tie). The codes come back unsigned: 4 bits, eight
+// nibbles in lo; 8 bits, code + 128.
 struct Codes8 {
   uint32_t lo, hi;
   __half d;
@@ -50,8 +52,18 @@ template <int BITS>
 __device__ __forceinline__ Codes8 quantize8(const float (&v)[8]) {
   Codes8 o;
   if (BITS == 8) {
-    const Quant8 q = quantize8_q8_0(v, 0);
-    o.lo = q.lo ^ 0x80808080u, o.hi = q.hi ^ 0x80808080u, o.d = __float2half_rn(q.d_unrounded);
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(v[i])); // a NaN is passed over
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const float d = __fmul_rn(amax, 1.0f / 127.0f), id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
+    int q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = round_away(__fmul_rn(v[i], id));
+    o.lo = pack_sat_i8(q[0], q[1], pack_sat_i8(q[2], q[3], 0u)) ^ 0x80808080u;
+    o.hi = pack_sat_i8(q[4], q[5], pack_sat_i8(q[6], q[7], 0u)) ^ 0x80808080u;
+    o.d = __float2half_rn(d);
     return o;
   }
   float amax = 0.f, mx = 0.f; // the first value of the largest magnitude; a NaN is passed over

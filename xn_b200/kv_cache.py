@@ -113,7 +113,7 @@ class QuantizedKVCache:
 
     def store(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor) -> None:
         """Quantize ``k`` and ``v`` ``[batch, seq, kv_heads, head_dim]`` (f32 / f16 / bf16, any strides) into positions ``pos ..``: the blocks that
-        ``BlockQ4_0`` / ``BlockQ8_0::from_float`` make of the f32 values (k_quants.rs:235-270, 636-661)."""
+        ``BlockQ4_0`` / ``BlockQ8_0::from_float`` make of the f32 values (k_quants.rs:235-270, 636-661), Q8_0's scale being ``max|x| * float32(1 / 127)``."""
         self._tokens("k", k, self.kv_heads), self._tokens("v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype is not v.dtype:
             raise ValueError(f"k is {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}")
