@@ -255,7 +255,7 @@ def test_attention(fmt, dt, B, S, H, KV, hd, L, page, first):
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("S,H,KV", [(1, 8, 2), (6, 8, 2), (150, 8, 2), (40, 3, 3)])
-@pytest.mark.parametrize("causal,window,scale", [(False, 0, None), (True, 1, None), (True, 33, 0.3), (False, 50, None), (True, 10000, -0.05)])
+@pytest.mark.parametrize("causal,window,scale", [(False, 0, None), (True, 1, None), (True, 33, 0.3), (False, 50, None), (True, 10000, -0.05), (True, 0, 0.0)])
 def test_masks_and_scales(dt, S, H, KV, causal, window, scale):
     B, L, hd = 3, 333, 128
     c = _filled("q4_0", B, KV, L, hd, 64)

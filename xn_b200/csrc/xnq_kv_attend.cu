@@ -17,8 +17,9 @@
 // where the run leaves an item. An item that is cut goes through records in the workspace: its last CTA to arrive adds them, in the order of the
 // parts, whoever came first.
 //
-// f32 queries (SPLIT): q and the weights are taken apart into two f16 each (22 bits), and the values' codes have their zero taken off first (with few
-// weights above the others the two sums in O would cancel); 16-bit queries: q is exact in f16 after a power of two a row, the weights are rounded to f16.
+// f32 queries (SPLIT): q and the weights are taken apart into two f16 each (22 bits), and the codes have their zero taken off first and are whole numbers in
+// f16: a subnormal operand's products are summed with the bits that a number of 2^-14 would have, some 2^-18 of the score (an output's error 3e-6 of its
+// norm with 4-bit codes; 5e-7 now, as much as f32 products), and with many weights the two sums in O would cancel. 16-bit queries: q is exact in f16 after a power of two a row, the weights are rounded to f16.
 // Ranges: p is held within 2^12 (rescaled when a maximum grows by more than 2^4), the values' scales are brought near one by a power of two a warp.
 #include <algorithm>
 #include <cmath>
@@ -43,7 +44,7 @@ struct AttendArgs {
   const long long *pos;
   float scale;
   // split kernel
-  int row_tiles, min_tiles;
+  int row_tiles;
   unsigned int *tickets; // [batch * kv_heads * row_tiles], zero between calls
   float *records;        // [grid][2] of RECORD_STRIDE floats
 };
@@ -80,10 +81,59 @@ __device__ __forceinline__ void store_any(void *p, int dtype, long long at, floa
   else static_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v);
 }
 
+template <int V> // 2 or 4 values
+__device__ __forceinline__ void load_vec(const float *p, float (&v)[V]) {
+  if (V == 4) {
+    const float4 x = *reinterpret_cast<const float4 *>(p);
+    v[0] = x.x, v[1] = x.y, v[V - 2] = x.z, v[V - 1] = x.w;
+  } else {
+    const float2 x = *reinterpret_cast<const float2 *>(p);
+    v[0] = x.x, v[1] = x.y;
+  }
+}
+template <int V>
+__device__ __forceinline__ void load_vec_cg(const float *p, float (&v)[V]) {
+  if (V == 4) {
+    const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
+    v[0] = x.x, v[1] = x.y, v[V - 2] = x.z, v[V - 1] = x.w;
+  } else {
+    const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
+    v[0] = x.x, v[1] = x.y;
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_vec(void *p, int dtype, long long at, const float (&v)[V]) {
+  if (dtype == XNQ_F32) {
+    float *q = static_cast<float *>(p) + at;
+    if (V == 4) *reinterpret_cast<float4 *>(q) = make_float4(v[0], v[1], v[V - 2], v[V - 1]);
+    else *reinterpret_cast<float2 *>(q) = make_float2(v[0], v[1]);
+    return;
+  }
+  uint32_t w[V / 2];
+#pragma unroll
+  for (int i = 0; i < V / 2; i++) {
+    if (dtype == XNQ_F16) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+  }
+  uint16_t *q = static_cast<uint16_t *>(p) + at;
+  if (V == 4) *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[V / 2 - 1]);
+  else *reinterpret_cast<uint32_t *>(q) = w[0];
+}
+
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { // d +=
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) { // of 16-bit values: lane (g, t) gives row g's columns 2 t, 2 t + 1 and gets column g's rows
   uint32_t d;
@@ -142,7 +192,7 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t *src, cons
 }
 
 template <int BITS, int HD, int NT, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_split_kernel(const AttendArgs a) {
   using L = KvTile<BITS, HD>;
   using P = SplitShape<HD, NT>;
   constexpr int NB = L::NB, W = L::W, R = P::R;
@@ -150,6 +200,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
   __shared__ long long s_sum[SPLIT_WARPS];
   __shared__ long long s_before;
   __shared__ int s_b, s_last;
+  __shared__ long long s_row[R], s_lse_row[R]; // where an item's rows go
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float *const merge = reinterpret_cast<float *>(smem + SPLIT_WARPS * SPLIT_STAGES * L::BYTES);
   float *const s_m = merge, *const s_l = merge + SPLIT_WARPS * R, *const s_acc = merge + 2 * SPLIT_WARPS * R;
@@ -161,8 +212,9 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
   // ---- this CTA's run of the flattened list: [t0, t1) of `total` tiles ----
   const int per_seq = a.c.kv_heads * a.row_tiles; // items of a sequence, all of its count of tiles
   const int batch = (int)a.batch;
-  long long mine = 0;
-  for (int b = threadIdx.x; b < batch; b += SPLIT_WARPS * 32) mine += span_of(a, b).count;
+  const int some = threadIdx.x < batch ? span_of(a, threadIdx.x).count : 0; // (most batches: the one look at the positions)
+  long long mine = some;
+  for (int b = threadIdx.x + SPLIT_WARPS * 32; b < batch; b += SPLIT_WARPS * 32) mine += span_of(a, b).count;
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) s_sum[warp] = mine;
@@ -171,7 +223,9 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
 #pragma unroll
   for (int w = 0; w < SPLIT_WARPS; w++) total += s_sum[w];
   total *= per_seq;
-  const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)a.min_tiles);
+  // Short items go to CTAs of their own: a run shorter than a tile a warp only where the items are shorter too.
+  const long long items = (long long)batch * per_seq, at_least = min((long long)SPLIT_WARPS, max(total / items, 1ll));
+  const long long share = max((total + gridDim.x - 1) / gridDim.x, at_least);
   const long long t0 = blockIdx.x * share, t1 = min(total, t0 + share);
 
   // sequences that see nothing: rows of zeros
@@ -187,31 +241,35 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
     }
   }
   if (t0 >= t1) return;
-  // the sequence of tile t0: a scan of the counts, 32 at a time, by the first warp
-  if (warp == 0) {
-    long long before = 0;
-    int found = -1;
-    for (int base = 0; base < batch && found < 0; base += 32) {
-      const long long n = base + lane < batch ? (long long)span_of(a, base + lane).count * per_seq : 0;
-      long long inc = n;
+  // the sequence of tile t0: a scan of the counts, a block of threads at a time
+  if (threadIdx.x == 0) s_b = batch;
+  long long before = 0;
+  for (int base = 0; base < batch; base += SPLIT_WARPS * 32) {
+    const long long n = (base == 0 ? (long long)some : base + (int)threadIdx.x < batch ? (long long)span_of(a, base + threadIdx.x).count : 0ll) * per_seq;
+    long long inc = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      const unsigned here = __ballot_sync(0xffffffffu, before + inc > t0);
-      if (here) {
-        const int f = __ffs(here) - 1;
-        found = base + f;
-        before += __shfl_sync(0xffffffffu, inc - n, f);
-      } else before += __shfl_sync(0xffffffffu, inc, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
     }
-    if (lane == 0) s_b = found, s_before = before;
+    __syncthreads(); // s_sum has been read
+    if (lane == 31) s_sum[warp] = inc;
+    __syncthreads();
+    long long here = before;
+#pragma unroll
+    for (int w = 0; w < SPLIT_WARPS; w++) {
+      if (w < warp) here += s_sum[w];
+      before += s_sum[w];
+    }
+    if (n && here + inc - n <= t0 && t0 < here + inc) s_b = base + threadIdx.x, s_before = here + inc - n; // one thread
+    if (before > t0) break;
   }
   __syncthreads();
   int b = s_b;
+  if (b >= batch) return; // (only where pos changes under the kernel)
   long long item0 = s_before; // first tile of the item at hand in the flattened list
   Span sp = span_of(a, b);
+  if (sp.count == 0) return; // (as above)
   int item = (int)((t0 - item0) / sp.count); // of the sequence: (KV head, row tile)
   item0 += (long long)item * sp.count;
 
@@ -247,13 +305,14 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
 
     // ---- the query rows as operands ----
     uint32_t qh[NT][NB][4], ql[SPLIT ? NT : 1][SPLIT ? NB : 1][4]; // [.. ][b][2 step + register]
-    float start[NT][NB][2], factor[NT][2]; // of columns 2 t, 2 t + 1
+    float start[SPLIT ? 1 : NT][SPLIT ? 1 : NB][4] = {}, factor[NT][2]; // of columns 2 t, 2 t + 1; start as the sums' registers are
     int lo[NT][2], hi[NT][2], lo_all = 0, hi_all = INT32_MAX, hi_any = -1, lo_any = INT32_MAX;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       const int r = n * 8 + g; // this lane's row as an operand's column
       const long long row = (long long)rt * R + r, s = row / a.group;
       const int h = kvh * a.group + (int)(row - s * a.group);
+      if (warp == 0 && t == 0) s_row[r] = b * a.out.sb + s * a.out.ss + h * a.out.sh, s_lse_row[r] = ((long long)b * a.seq + s) * a.heads + h;
       float v[NB][8], top = 0.f;
 #pragma unroll
       for (int bl = 0; bl < NB; bl++) {
@@ -267,7 +326,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       int e = top > 0.f && top < INFINITY ? 13 - ilogbf(top) : 0; // the largest |q| to [2^13, 2^14)
       e = max(-100, min(100, e));
-      const float up = ldexpf(1.f, e);
+      const float up = ldexpf(a.scale < 0.f ? -1.f : 1.f, e); // the scale's sign goes into q, so that the largest score is the largest sum
       float sum[NB];
 #pragma unroll
       for (int bl = 0; bl < NB; bl++) {
@@ -280,12 +339,14 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
           lo_v[i] = SPLIT ? __half2float(__float2half_rn(x - hi_v[i])) : 0.f;
           sum[bl] += hi_v[i] + lo_v[i];
         }
-        sum[bl] += __shfl_xor_sync(0xffffffffu, sum[bl], 1);
-        sum[bl] += __shfl_xor_sync(0xffffffffu, sum[bl], 2);
+        if (!SPLIT) {
+          sum[bl] += __shfl_xor_sync(0xffffffffu, sum[bl], 1);
+          sum[bl] += __shfl_xor_sync(0xffffffffu, sum[bl], 2);
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) { // pair i of a word: dims i and i + 4 (4 bits, the odd ones 16 times too large), or of word i / 2 bytes i % 2 and i % 2 + 2
           const int x = BITS == 4 ? i : (i >> 1) * 4 + (i & 1), y = BITS == 4 ? i + 4 : x + 2;
-          const float down = BITS == 4 && (i & 1) ? 0.0625f : 1.f;
+          const float down = !SPLIT && BITS == 4 && (i & 1) ? 0.0625f : 1.f;
           qh[n][bl][i] = pack_half2(hi_v[x] * down, hi_v[y] * down);
           if (SPLIT) ql[n][bl][i] = pack_half2(lo_v[x] * down, lo_v[y] * down);
         }
@@ -295,12 +356,14 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
       if (r >= rows) l0 = 0, h0 = INT32_MAX; // no row: its weights are thrown away
       else hi_any = max(hi_any, h0), lo_any = min(lo_any, l0);
       lo_all = max(lo_all, l0), hi_all = min(hi_all, h0);
-      const float f = ldexpf(a.scale * LOG2E, 24 - e);
+      const float f = ldexpf(fabsf(a.scale) * LOG2E, (SPLIT ? 0 : 24) - e);
 #pragma unroll
       for (int c = 0; c < 2; c++) { // from the lane that holds row 2 t + c
         const int from = (2 * t + c) * 4;
+        if (!SPLIT)
 #pragma unroll
-        for (int bl = 0; bl < NB; bl++) start[n][bl][c] = __shfl_sync(0xffffffffu, sum[bl], from) * (-(float)L::ZERO / 16777216.f);
+          for (int bl = 0; bl < NB; bl++)
+            start[SPLIT ? 0 : n][SPLIT ? 0 : bl][c] = start[SPLIT ? 0 : n][SPLIT ? 0 : bl][c + 2] = __shfl_sync(0xffffffffu, sum[bl], from) * (-(float)L::ZERO / 16777216.f);
         factor[n][c] = __shfl_sync(0xffffffffu, f, from);
         lo[n][c] = __shfl_sync(0xffffffffu, l0, from), hi[n][c] = __shfl_sync(0xffffffffu, h0, from);
       }
@@ -380,16 +443,17 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
 #pragma unroll
             for (int e = 0; e < 2; e++) {
               const uint32_t x = BITS == 4 ? w[e][bl] : w[e][2 * bl + step];
-              op[step][e] = code_pair<BITS>(x, BITS == 4 ? 2 * step : 0), op[step][e + 2] = code_pair<BITS>(x, BITS == 4 ? 2 * step + 1 : 1);
+              const int i0 = BITS == 4 ? 2 * step : 0;
+              op[step][e] = SPLIT ? signed_pair<BITS>(x, i0) : code_pair<BITS>(x, i0), op[step][e + 2] = SPLIT ? signed_pair<BITS>(x, i0 + 1) : code_pair<BITS>(x, i0 + 1);
             }
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            float d[4] = {start[n][bl][0], start[n][bl][1], start[n][bl][0], start[n][bl][1]};
-            mma(d, op[0], qh[n][bl][0], qh[n][bl][1], d);
-            mma(d, op[1], qh[n][bl][2], qh[n][bl][3], d);
+            float d[4];
+            mma(d, op[0], qh[n][bl][0], qh[n][bl][1], start[SPLIT ? 0 : n][SPLIT ? 0 : bl]);
+            mma(d, op[1], qh[n][bl][2], qh[n][bl][3]);
             if (SPLIT) {
-              mma(d, op[0], ql[SPLIT ? n : 0][SPLIT ? bl : 0][0], ql[SPLIT ? n : 0][SPLIT ? bl : 0][1], d);
-              mma(d, op[1], ql[SPLIT ? n : 0][SPLIT ? bl : 0][2], ql[SPLIT ? n : 0][SPLIT ? bl : 0][3], d);
+              mma(d, op[0], ql[SPLIT ? n : 0][SPLIT ? bl : 0][0], ql[SPLIT ? n : 0][SPLIT ? bl : 0][1]);
+              mma(d, op[1], ql[SPLIT ? n : 0][SPLIT ? bl : 0][2], ql[SPLIT ? n : 0][SPLIT ? bl : 0][3]);
             }
             s[u][n][0] += d0 * d[0], s[u][n][1] += d0 * d[1], s[u][n][2] += d1 * d[2], s[u][n][3] += d1 * d[3];
           }
@@ -410,15 +474,45 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
             const uint2 x = *reinterpret_cast<const uint2 *>(tile + L::v_scale(pair, 0));
             dv[u][e][0] = x.x, dv[u][e][1] = x.y;
           }
-          if (masked) { // what no row sees may be anything
-            const int j = j0 + 2 * pair;
+        }
+      if (masked) {
+        // What no row sees may be anything: zeros. What some row sees and another does not must not reach the other as 0 times infinity: such a scale is taken
+        // as zero, and the results of the rows that see it are made NaN.
+        unsigned bad = 0; // positions
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int in = u * 16 + e * 8 + 2 * t, j = j0 + in;
             const uint32_t keep = (j >= lo_any && j <= hi_any ? 0xffffu : 0u) | (j + 1 >= lo_any && j + 1 <= hi_any ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int bl = 0; bl < NB; bl++) dv[u][e][bl] &= keep;
+            for (int bl = 0; bl < NB; bl++) {
+              uint32_t x = dv[u][e][bl] & keep;
+              if ((x & 0x7c00u) == 0x7c00u) x &= 0xffff0000u, bad |= 1u << in;
+              if ((x & 0x7c000000u) == 0x7c000000u) x &= 0xffffu, bad |= 2u << in;
+              dv[u][e][bl] = x;
+            }
           }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        if (bad) {
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+              const int first = max(lo[n][c] - j0, 0), last = min(hi[n][c] - j0, 31);
+              if (first <= last && (bad >> first) << (31 - last + first)) {
+#pragma unroll
+                for (int x = 0; x < 2 * NB; x++) acc[n][x][c] = acc[n][x][c + 2] = NAN;
+              }
+            }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
 #pragma unroll
           for (int bl = 0; bl < NB; bl++) d_top = __hmax2(d_top, __habs2(as_half2(dv[u][e][bl])));
-        }
       const float d_max = fmaxf(__low2float(d_top), __high2float(d_top));
       if (__any_sync(0xffffffffu, d_max > d_most || !k_set)) {
         float top = d_max;
@@ -453,24 +547,25 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
       // softmax
       bool grew = false;
       float top[NT][2];
+      if (masked) {
 #pragma unroll
-      for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+          for (int u = 0; u < 2; u++)
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            s[u][n][c] *= factor[n][c & 1];
-            if (masked) {
+            for (int c = 0; c < 4; c++) {
               const int j = j0 + u * 16 + (c >> 1) * 8 + g;
               if (j < lo[n][c & 1] || j > hi[n][c & 1]) s[u][n][c] = -INFINITY;
             }
-          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           float x = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
 #pragma unroll
           for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-          top[n][c] = fmaxf(m[n][c], x);
+          top[n][c] = fmaxf(m[n][c], x == -INFINITY ? x : x * factor[n][c]);
           grew |= top[n][c] > ref[n][c] + 12.f || (m[n][c] == -INFINITY && top[n][c] != -INFINITY); // the reference lies 8 below a maximum
         }
       }
@@ -494,7 +589,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const float p0 = exp2_approx(s[u][n][2 * e] - ref[n][0]), p1 = exp2_approx(s[u][n][2 * e + 1] - ref[n][1]);
+            const float p0 = exp2_approx(fmaf(s[u][n][2 * e], factor[n][0], -ref[n][0])), p1 = exp2_approx(fmaf(s[u][n][2 * e + 1], factor[n][1], -ref[n][1]));
             l[n][0] += p0, l[n][1] += p1;
             const uint32_t h2 = pack_half2(p0, p1);
             ph[u][n][e] = transpose8x8(h2);
@@ -538,25 +633,23 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
               const __half2 ph2 = as_half2(ph[u][n][e]), d2 = as_half2(dv[u][e][bl]);
               if (!SPLIT) {
                 bh[e] = as_u32(__hmul2(ph2, d2));
-                if (masked) bh[e] &= __hne2_mask(ph2, __float2half2_rn(0.f)); // a scale that another row sees may be infinite
               } else {
                 const __half2 pl2 = as_half2(pl[u][SPLIT ? n : 0][e]);
                 const float p0 = __low2float(ph2) + __low2float(pl2), p1 = __high2float(ph2) + __high2float(pl2);
-                float x0 = p0 * __low2float(d2), x1 = p1 * __high2float(d2);
-                if (masked) x0 = p0 == 0.f ? 0.f : x0, x1 = p1 == 0.f ? 0.f : x1;
+                const float x0 = p0 * __low2float(d2), x1 = p1 * __high2float(d2);
                 bh[e] = pack_half2(x0, x1);
                 bl2[e] = pack_half2(x0 - __low2float(as_half2(bh[e])), x1 - __high2float(as_half2(bh[e])));
               }
             }
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-              mma(acc[n][2 * bl + half], op[half], bh[0], bh[1], acc[n][2 * bl + half]);
-              if (SPLIT) mma(acc[n][2 * bl + half], op[half], bl2[0], bl2[1], acc[n][2 * bl + half]);
+              mma(acc[n][2 * bl + half], op[half], bh[0], bh[1]);
+              if (SPLIT) mma(acc[n][2 * bl + half], op[half], bl2[0], bl2[1]);
             }
             if (!SPLIT) { // row bl of one more product: the block's sum of weights
               const uint32_t one = g == bl ? 0x3c003c00u : 0u;
               const uint32_t ones[4] = {one, 0u, one, 0u};
-              mma(zsum[SPLIT ? 0 : n], ones, bh[0], bh[1], zsum[SPLIT ? 0 : n]);
+              mma(zsum[SPLIT ? 0 : n], ones, bh[0], bh[1]);
             }
           }
         }
@@ -590,19 +683,19 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
         }
       }
     __syncthreads();
+    // A warp takes a row at a time, a lane HD / 32 neighbouring dims of it.
+    constexpr int V = HD / 32;
     const bool whole = ta == 0 && tb == sp.count;
-    const long long c_first = item0 / share, c_last = (item0 + sp.count - 1) / share; // the CTAs that hold parts of the item
-    const long long seq_item = (long long)b * per_seq + item;
-    auto put = [&](int r, int d, float m_all, float l_all, float v) { // a finished value
-      const long long row = (long long)rt * R + r, s = row / a.group;
-      const int h = kvh * a.group + (int)(row - s * a.group);
-      store_any(a.out.p, a.dtype, b * a.out.sb + s * a.out.ss + h * a.out.sh + d, l_all > 0.f ? v / l_all : 0.f);
-      if (a.lse && d == 0) a.lse[((long long)b * a.seq + s) * a.heads + h] = l_all > 0.f ? (m_all + log2f(l_all)) * LN2 : -INFINITY;
+    auto put = [&](int r, float m_all, float l_all, float (&v)[V]) { // a finished row
+      const float by = l_all > 0.f ? 1.f / l_all : l_all; // 0: nothing seen, zeros; NaN stays
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] *= by;
+      store_vec<V>(a.out.p, a.dtype, s_row[r] + lane * V, v);
+      if (a.lse && lane == 0) a.lse[s_lse_row[r]] = l_all > 0.f ? (m_all + log2f(l_all)) * LN2 : l_all == 0.f ? -INFINITY : l_all;
     };
     float *const rec = a.records + (blockIdx.x * 2 + (ta == 0 ? 1 : 0)) * (long long)RECORD_STRIDE;
-    for (int i = threadIdx.x; i < rows * HD; i += SPLIT_WARPS * 32) {
-      const int r = i / HD, d = i - r * HD;
-      float m_all = -INFINITY, l_all = 0.f, v = 0.f;
+    for (int r = warp; r < rows; r += SPLIT_WARPS) {
+      float m_all = -INFINITY, l_all = 0.f, v[V] = {};
 #pragma unroll
       for (int w = 0; w < SPLIT_WARPS; w++) m_all = fmaxf(m_all, s_m[w * R + r]);
 #pragma unroll
@@ -610,53 +703,58 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32) kv_attend_split_kernel(const
         const float mw = s_m[w * R + r];
         const float by = mw == -INFINITY ? 0.f : exp2_approx(mw - m_all);
         l_all += by * s_l[w * R + r];
-        if (mw != -INFINITY) v += by * s_acc[(w * R + r) * P::COL + d];
+        float x[V];
+        load_vec<V>(s_acc + (w * R + r) * P::COL + lane * V, x);
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] += by * x[i];
       }
-      if (whole) put(r, d, m_all, l_all, v);
+      if (whole) put(r, m_all, l_all, v);
       else {
-        if (d == 0) rec[r] = m_all, rec[R + r] = l_all;
-        rec[2 * R + i] = v;
+        if (lane == 0) rec[r] = m_all, rec[R + r] = l_all;
+        store_vec<V>(rec, XNQ_F32, 2 * R + r * HD + lane * V, v);
       }
     }
     if (!whole) {
-      __threadfence();
+      const long long c_first = item0 / share; // the CTAs that hold parts of the item: c_first .. c_first + others
+      const int others = (int)((item0 + sp.count - 1) / share - c_first);
       __syncthreads();
-      if (threadIdx.x == 0) s_last = atomicInc(a.tickets + seq_item, (unsigned)(c_last - c_first)) == (unsigned)(c_last - c_first);
-      __syncthreads();
-      if (s_last) { // all parts are there: added in an order of their places
+      if (threadIdx.x == 0) {
+        __threadfence(); // the CTA's parts, which the barrier has ordered before, become visible before the count does
+        s_last = atomicInc(a.tickets + (long long)b * per_seq + item, (unsigned)others) == (unsigned)others;
         __threadfence();
-        const float *const part0 = a.records + (c_first * 2 + 1) * RECORD_STRIDE, *const parts = a.records + (c_first + 1) * 2 * RECORD_STRIDE; // the first, the others
-        const int others = (int)(c_last - c_first);
+      }
+      __syncthreads();
+      if (s_last) { // all parts are there: added in the order of their places, PARTS in flight
+        constexpr int PARTS = 8;
+        const float *const part0 = a.records + (c_first * 2 + 1) * RECORD_STRIDE; // the first lies in its CTA's second place, the others in the first ones
         for (int r = warp; r < rows; r += SPLIT_WARPS) {
-          float m_all = __ldcg(part0 + r), l_all = 0.f;
-          for (int c = lane; c < others; c += 32) m_all = fmaxf(m_all, __ldcg(parts + (long long)c * 2 * RECORD_STRIDE + r));
+          float m_all = -INFINITY, l_all = 0.f, v[V] = {};
+          for (int c = 0; c <= others; c += PARTS) {
+            float mp[PARTS], lp[PARTS], x[PARTS][V], m_new = m_all;
 #pragma unroll
-          for (int o = 16; o >= 1; o >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
-          auto add = [&](const float *p) {
-            const float mp = __ldcg(p + r);
-            if (mp != -INFINITY) l_all += exp2_approx(mp - m_all) * __ldcg(p + R + r);
-          };
-          if (lane == 0) add(part0);
-          for (int c = lane; c < others; c += 32) add(parts + (long long)c * 2 * RECORD_STRIDE);
+            for (int i = 0; i < PARTS; i++) {
+              const float *p = part0 + (long long)(min(c + i, others) * 2 - (c + i ? 1 : 0)) * RECORD_STRIDE;
+              mp[i] = __ldcg(p + r), lp[i] = __ldcg(p + R + r);
+              load_vec_cg<V>(p + 2 * R + r * HD + lane * V, x[i]);
+            }
 #pragma unroll
-          for (int o = 16; o >= 1; o >>= 1) l_all += __shfl_xor_sync(0xffffffffu, l_all, o);
-          if (lane == 0) s_m[r] = m_all, s_l[r] = l_all;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < rows * (HD / 4); i += SPLIT_WARPS * 32) {
-          const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
-          const float m_all = s_m[r], l_all = s_l[r];
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          auto add = [&](const float *p) {
-            const float mp = __ldcg(p + r);
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + 2 * R + 4 * i));
-            const float by = mp == -INFINITY ? 0.f : exp2_approx(mp - m_all);
-            if (by != 0.f) v.x += by * x.x, v.y += by * x.y, v.z += by * x.z, v.w += by * x.w;
-          };
-          add(part0);
-#pragma unroll 8
-          for (int c = 0; c < others; c++) add(parts + (long long)c * 2 * RECORD_STRIDE);
-          put(r, d, m_all, l_all, v.x), put(r, d + 1, m_all, l_all, v.y), put(r, d + 2, m_all, l_all, v.z), put(r, d + 3, m_all, l_all, v.w);
+            for (int i = 0; i < PARTS; i++) m_new = fmaxf(m_new, mp[i]);
+            const float old = m_all == -INFINITY ? 0.f : exp2_approx(m_all - m_new);
+            l_all *= old;
+#pragma unroll
+            for (int k2 = 0; k2 < V; k2++) v[k2] *= old;
+#pragma unroll
+            for (int i = 0; i < PARTS; i++) {
+              const float by = c + i > others || mp[i] == -INFINITY ? 0.f : exp2_approx(mp[i] - m_new);
+              if (c + i <= others) {
+                l_all += by * lp[i];
+#pragma unroll
+                for (int k2 = 0; k2 < V; k2++) v[k2] += by * x[i][k2];
+              }
+            }
+            m_all = m_new;
+          }
+          put(r, m_all, l_all, v);
         }
       }
     }
@@ -691,13 +789,12 @@ template <int BITS, int HD, int NT, bool SPLIT>
 int run_split(AttendArgs a, void *workspace, int sms, cudaStream_t s) {
   const int64_t rows = a.seq * a.group;
   a.row_tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
-  a.min_tiles = SPLIT_WARPS;
   a.records = static_cast<float *>(workspace);
   a.tickets = reinterpret_cast<unsigned int *>(static_cast<uint8_t *>(workspace) + RECORDS_BYTES);
   using Launch = SplitLaunch<BITS, HD, NT, SPLIT>;
   // no more CTAs than the longest caches could fill
   const int64_t most = a.batch * a.c.kv_heads * a.row_tiles * ((a.c.max_seq + KV_TILE - 1) / KV_TILE);
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(std::min(sms * Launch::per_sm, MAX_SPLIT_GRID), std::max<int64_t>((most + a.min_tiles - 1) / a.min_tiles, a.batch)));
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(std::min(sms * Launch::per_sm, MAX_SPLIT_GRID), std::max<int64_t>(most, a.batch)));
   XNQ_CUDA(launch_pdl(kv_attend_split_kernel<BITS, HD, NT, SPLIT>, dim3((unsigned)grid), dim3(SPLIT_WARPS * 32), Launch::smem(), s, a));
   count_launch();
   return XNQ_OK;
@@ -768,7 +865,7 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
   const int sms = device < 64 ? g_sms[device] : 0;
   if (!sms) return fail(XNQ_ERR_UNSUPPORTED, "kv_attend: xnq_init has not run for device %d", device);
   a.lse = lse, a.batch = batch, a.seq = seq, a.heads = heads, a.group = heads / cache->kv_heads, a.dtype = q->dtype;
-  a.pos_stride = pos_stride, a.causal = causal, a.pos = pos, a.scale = scale, a.window = std::min<int64_t>(window, INT32_MAX);
+  a.pos_stride = pos_stride, a.causal = causal, a.pos = pos, a.scale = scale == 0.f ? 1e-30f : scale /* (a masked score is -inf times it) */, a.window = std::min<int64_t>(window, INT32_MAX);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (kv_bits(cache->ggml_dtype) == 4) return cache->head_dim == 64 ? run_attend<4, 64>(a, workspace, sms, s) : run_attend<4, 128>(a, workspace, sms, s);
   return cache->head_dim == 64 ? run_attend<8, 64>(a, workspace, sms, s) : run_attend<8, 128>(a, workspace, sms, s);
