@@ -112,7 +112,7 @@ def check(rc: int) -> None:
 
 
 def native():
-    """The torch side of a linear's call (``csrc/torch_linear.cpp``), bound to the library that :func:`lib` loaded."""
+    """The torch side of a linear's and of the quantized KV cache's calls (``csrc/torch_linear.cpp``, ``csrc/torch_kv_cache.cpp``), bound to the library that :func:`lib` loaded."""
     global _native
     if _native is None:
         import torch  # noqa: F401  (its libraries have to be loaded first)
@@ -122,6 +122,7 @@ def native():
             raise RuntimeError(f"xn_b200/_xnq_torch.so cannot be loaded ({e}). Build it with `python -m xn_b200.build`.") from e
         L = lib()
         address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
+        m.kv_bind(address(L.xnq_kv_store), address(L.xnq_kv_load), address(L.xnq_kv_attend), address(L.xnq_kv_attend_workspace_bytes), check)
         m.bind(address(L.xnq_matmul_t_bias), address(L.xnq_matvec), address(L.xnq_matmul_workspace_bytes), check)
         _native = m
     return _native

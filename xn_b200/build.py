@@ -59,9 +59,13 @@ def _torch_stamp() -> str:
     return f"torch {torch.__version__} {torch.version.git_version} python {sys.version}"
 
 
+def torch_sources() -> list[str]:
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.startswith("torch_") and f.endswith(".cpp"))
+
+
 def torch_module_is_stale() -> bool:
-    src = os.path.join(CSRC, "torch_linear.cpp")
-    if not os.path.exists(TORCH_MODULE) or os.path.getmtime(TORCH_MODULE) < os.path.getmtime(src):
+    deps = [*torch_sources(), *(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.startswith("torch_") and f.endswith(".h"))]
+    if not os.path.exists(TORCH_MODULE) or os.path.getmtime(TORCH_MODULE) < max(os.path.getmtime(p) for p in deps):
         return True
     try:
         with open(TORCH_STAMP) as f:
@@ -73,7 +77,7 @@ def torch_module_is_stale() -> bool:
 def build_torch_module(force: bool = False) -> str:
     if not force and not torch_module_is_stale():
         return TORCH_MODULE
-    src = os.path.join(CSRC, "torch_linear.cpp")
+    src = torch_sources()
     import sysconfig
 
     import torch
@@ -81,11 +85,11 @@ def build_torch_module(force: bool = False) -> str:
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     inc = [*include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(f"-I{p}" for p in inc), src, "-o", TORCH_MODULE, *(f"-L{p}" for p in library_paths()),
+           *(f"-I{p}" for p in inc), *src, "-o", TORCH_MODULE, *(f"-L{p}" for p in library_paths()),
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-ltorch"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"the host compiler failed on {src}:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"the host compiler failed on {' '.join(src)}:\n{r.stdout}\n{r.stderr}")
     os.makedirs(os.path.dirname(TORCH_STAMP), exist_ok=True)
     with open(TORCH_STAMP, "w") as f:
         f.write(_torch_stamp())

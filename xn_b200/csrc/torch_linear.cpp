@@ -5,26 +5,20 @@
 // ctypes, it took 10.5 us: some 25 attribute reads and comparisons, a tensor made through the dispatcher, twelve arguments converted one by one, and
 // the launch. Everything that is not ordinary returns None, and the Python code takes the call; nothing is kept from one call for the next but
 // scratch, by stream.
-#define PY_SSIZE_T_CLEAN
-#include <Python.h>
+#include "torch_common.h"
 
-#include <ATen/ATen.h>
-#include <ATen/EmptyTensor.h>
 #include <ATen/cuda/EmptyTensor.h>
-#include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/GradMode.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <mutex>
 
 namespace {
+
+using namespace xnq_torch;
 
 using MatmulFn = int (*)(const void *, const void *, int, int64_t, int64_t, const void *, void *, int, int64_t, void *, size_t, void *);
 using MatvecFn = int (*)(const void *, const void *, int, const void *, void *, int, void *);
@@ -64,11 +58,6 @@ Slab g_slabs[SLABS]; // they and the counts: under the interpreter's lock
 int g_num_slabs = 0;
 int64_t g_weights = 0;
 
-struct RelaxedCapture { // (a graph that another thread is capturing does not mind what this one allocates or frees)
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  RelaxedCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
-  ~RelaxedCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
-};
 // the slab of a stream of the current device, or null: the call takes a block of its own
 Slab *slab_for(c10::DeviceIndex device, cudaStream_t stream, size_t bytes) {
   if (bytes > SLAB) return nullptr;
@@ -104,23 +93,6 @@ size_t scratch_bytes(Weight *w, int64_t rows) {
   return w->ws_bytes;
 }
 
-int xnq_dtype(at::ScalarType t) { // F32 0, F16 1, BF16 30: the ggml ids
-  return t == at::kFloat ? 0 : (t == at::kHalf ? 1 : (t == at::kBFloat16 ? 30 : -1));
-}
-// an ordinary dense CUDA tensor: no subclass, no wrapper of a transform
-bool plain(PyObject *o) {
-  if (!THPVariable_CheckExact(o)) return false;
-  constexpr c10::DispatchKeySet allowed({c10::DispatchKey::CUDA, c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::AutocastCUDA});
-  const c10::DispatchKeySet ks = THPVariable_Unpack(o).key_set();
-  return (ks.raw_repr() & ~allowed.raw_repr()) == 0 && ks.has(c10::DispatchKey::CUDA);
-}
-// Something of torch looks at operators or replaces them: a function or dispatch mode, a transform of torch.func (whatever tensors it has wrapped), a tracer.
-bool observed() {
-  constexpr c10::DispatchKeySet ordinary({c10::DispatchKey::BackendSelect, c10::DispatchKey::ADInplaceOrView});
-  return (c10::impl::tls_local_dispatch_key_set().included_.raw_repr() & ~ordinary.raw_repr()) != 0 || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
-         at::impl::torch_function_mode_enabled();
-}
-
 PyObject *py_observed(PyObject *, PyObject *) { return PyBool_FromLong(observed()); }
 
 // linear(weight capsule, x, bias or None) -> y, or None where the general code has to take the call
@@ -154,8 +126,7 @@ PyObject *linear(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   }
   c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
   shape[dims - 1] = w->n;
-  // (what empty_cuda does behind its look for the device, which is the current one here)
-  at::Tensor y = at::Tensor(at::detail::empty_generic(shape, c10::cuda::CUDACachingAllocator::get(), c10::DispatchKeySet(c10::DispatchKey::CUDA), x.scalar_type(), std::nullopt));
+  at::Tensor y = empty_here(shape, x.scalar_type());
   void *const yp = y.mutable_data_ptr();
   const void *const xp = x.const_data_ptr();
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(w->device).stream();
@@ -218,12 +189,19 @@ PyObject *bind(PyObject *, PyObject *args) {
   Py_RETURN_NONE;
 }
 
+#define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(f)), METH_FASTCALL
 PyMethodDef methods[] = {
     {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(linear)), METH_FASTCALL, "linear(weight, x, bias) -> y or None"},
     {"workspace", workspace, METH_VARARGS, "workspace(weight, rows) -> scratch"},
     {"weight", weight, METH_VARARGS, "weight(handle, n, k, device index) -> capsule"},
     {"observed", py_observed, METH_NOARGS, "observed() -> whether a mode, a transform or a tracer looks at torch's operators"},
     {"bind", bind, METH_VARARGS, "bind(matmul, matvec, workspace_bytes, check)"},
+    {"kv_cache", kv_cache, METH_VARARGS, "kv_cache(address of an xnq_kv_cache, batch, device index) -> capsule"},
+    {"kv_bind", kv_bind, METH_VARARGS, "kv_bind(store, load, attend, workspace_bytes, check)"},
+    {"kv_store", FAST(kv_store), "kv_store(cache, k, v, pos) -> True or None"},
+    {"kv_rope_store", FAST(kv_rope_store), "kv_rope_store(cache, qkv, cos, sin, pos, heads, type or -1) -> q or None"},
+    {"kv_load", FAST(kv_load), "kv_load(cache, start, length, type) -> (k, v) or None"},
+    {"kv_attend", FAST(kv_attend), "kv_attend(cache, q, pos, causal, window, scale) -> out or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_xnq_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

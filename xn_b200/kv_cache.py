@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from .dtypes import GgmlDType
-from .quantized import _TORCH_TO_XNQ, _stream_ptr, init
+from .quantized import _TORCH_TO_XNQ, _XNQ_IDS, _stream_ptr, init
 
 PAGE_UNIT = 32  # positions of a tile: page sizes are multiples of it
 
@@ -92,6 +92,9 @@ class QuantizedKVCache:
         self._view = _Cache(int(self.dtype), kv_heads, head_dim, self.page_size, self.num_pages, self.pages.data_ptr(),
                             self.page_table.data_ptr() if paged else None, self.page_table.stride(0) if paged else 0, max_seq)
 
+        self._native = _lib.native()   # the ordinary call, in C++ (csrc/torch_kv_cache.cpp); what it hands back as None is taken here
+        self._handle = self._native.kv_cache(ctypes.addressof(self._view), batch, self.device.index)
+
     @property
     def nbytes(self) -> int:
         return self.pages.numel()
@@ -114,6 +117,8 @@ class QuantizedKVCache:
     def store(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor) -> None:
         """Quantize ``k`` and ``v`` ``[batch, seq, kv_heads, head_dim]`` (f32 / f16 / bf16, any strides) into positions ``pos ..``: the blocks that
         ``BlockQ4_0`` / ``BlockQ8_0::from_float`` make of the f32 values (k_quants.rs:235-270, 636-661), Q8_0's scale being ``max|x| * float32(1 / 127)``."""
+        if self._native.kv_store(self._handle, k, v, pos):
+            return
         self._tokens("k", k, self.kv_heads), self._tokens("v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype is not v.dtype:
             raise ValueError(f"k is {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}")
@@ -122,6 +127,10 @@ class QuantizedKVCache:
     def rope_store(self, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, heads: int, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """``qkv`` ``[batch, seq, (heads + 2 kv_heads) * head_dim]``, a fused projection's output: q and k rotated (rotate-half, f32 tables ``[rows, head_dim /
         2]``) at their positions, k and v stored. Returns q ``[batch, seq, heads, head_dim]`` as ``out_dtype`` (default: ``qkv``'s)."""
+        if out_dtype is None or out_dtype in _TORCH_TO_XNQ:
+            q = self._native.kv_rope_store(self._handle, qkv, cos, sin, pos, heads, -1 if out_dtype is None else _XNQ_IDS[out_dtype])
+            if q is not None:
+                return q
         hd, width = self.head_dim, (heads + 2 * self.kv_heads) * self.head_dim
         if heads < 1 or qkv.dim() != 3 or qkv.shape[2] != width:
             raise ValueError(f"rope_store: qkv is {tuple(qkv.shape)}; {heads} + 2 * {self.kv_heads} heads of {hd}")
@@ -151,6 +160,9 @@ class QuantizedKVCache:
         times code, in f32, rounded once. Positions that are not in the cache or have no page are zeros."""
         if dtype not in _TORCH_TO_XNQ or length < 0:
             raise ValueError(f"load: {length} positions as {dtype}")
+        both = self._native.kv_load(self._handle, start, length, _XNQ_IDS[dtype])
+        if both is not None:
+            return both
         k = torch.empty((self.batch, self.kv_heads, length, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         sp, stride = self._positions(start, "start") if isinstance(start, torch.Tensor) else (None, 0)
@@ -166,6 +178,10 @@ class QuantizedKVCache:
         Query ``i`` of a sequence is at ``p = pos + i`` and sees positions ``j <= p`` (``causal``) or ``j < pos + seq``, with a ``window`` only ``j > p - window``;
         one that sees nothing gives zeros. ``scale``: default ``head_dim ** -0.5``. ``out``: where the result goes (``q``'s shape and type, rows contiguous and
         16-byte aligned). ``lse``: float32 ``[batch, seq, heads]`` that receives the logarithm of the sum of exponentials (-inf: nothing seen)."""
+        if out is None and lse is None:
+            res = self._native.kv_attend(self._handle, q, pos, causal, window, self.head_dim ** -0.5 if scale is None else scale)
+            if res is not None:
+                return res
         self._tokens("q", q)
         heads, seq = q.shape[2], q.shape[1]
         if heads < 1 or heads % self.kv_heads:
