@@ -385,7 +385,8 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
  * tensor-core kernel: a wait of the producer (16), a converter (17), the MMA issuer (18), a drain warp (19)
  * expired. Bits 24-25: a decode position outside [0, max_seq) reached xnq_rope_kv_store (24) or
  * xnq_attn_decode (25); bit 26: xnq_embed_rows met a token outside the table.
- * Bits 27-29, the quantized KV cache: 27 a position past it was to be stored or read back, 28 attended to, 29 a page table's entry was no page.
+ * Bits 27-29, the quantized KV cache: 27 a position past it was to be stored or read back, 28 attended to, 29 a page table's entry was no page,
+ * 30 a wait inside the kernel for many query rows expired.
  * Synchronizes the device.
  * No counterpart in the reference (its kernels never wait on anything). */
 int xnq_device_status(unsigned int *bits);

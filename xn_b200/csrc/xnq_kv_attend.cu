@@ -24,7 +24,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "xnq_kv_cache.cuh"
+#include "xnq_kv_attend.cuh"
 #include "xnq_quantize_act.cuh"
 
 namespace xnq {
@@ -33,22 +33,6 @@ namespace {
 __device__ unsigned int g_kv_attend_status;
 
 constexpr int SPLIT_WARPS = 4, SPLIT_STAGES = 3;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-struct AttendArgs {
-  KvView c;
-  KvRows q, out;
-  float *lse; // [batch, seq, heads], or null
-  long long batch, seq, window;
-  int heads, group, dtype, pos_stride, causal; // group: query heads of a KV head
-  const long long *pos;
-  float scale;
-  // split kernel
-  int row_tiles;
-  unsigned int *tickets; // [batch * kv_heads * row_tiles], zero between calls
-  float *records;        // [grid][2] of RECORD_STRIDE floats
-};
-
 // What sequence b's queries see, as tiles [first, first + count).
 struct Span {
   int first, count;
@@ -62,14 +46,6 @@ __device__ __forceinline__ Span span_of(const AttendArgs &a, int b) {
   s.count = hi < lo ? 0 : (int)(hi / KV_TILE) - s.first + 1;
   return s;
 }
-// positions [lo, hi] that the query at token s of a sequence at `pos` sees
-__device__ __forceinline__ void seen_by(const AttendArgs &a, long long pos, long long s, int &lo, int &hi) {
-  const long long p = pos + s;
-  const long long h = p < 0 ? -1 : min(a.causal ? p : pos + a.seq - 1, a.c.max_seq - 1);
-  const long long l = a.window ? max(p - a.window + 1, 0ll) : 0ll;
-  hi = (int)h, lo = (int)min(l, a.c.max_seq);
-}
-
 __device__ __forceinline__ void load8_any(const void *p, int dtype, long long at, float (&v)[8]) {
   if (dtype == XNQ_F32) load8(static_cast<const float *>(p) + at, v);
   else if (dtype == XNQ_F16) load8(static_cast<const __half *>(p) + at, v);
@@ -140,32 +116,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) { // of 16-bit valu
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2 *>(&v); }
-__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t *>(&v); }
-__device__ __forceinline__ float exp2_approx(float x) { // 2^x within 2 ulp
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// d = {a & mask} of the four registers of an operand: words w0 and w1 (rows g and g + 8 of K; positions 2 t and 2 t + 8 of V)
-template <int BITS>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) { // the i-th of a word's pairs (16 bits apart), as subnormals; 4 bits: times 16 where i is odd
-  if (BITS == 4) return (i & 2 ? w >> 8 : w) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
-  return (i & 1 ? w >> 8 : w) & 0x00ff00ffu;
-}
-template <int BITS>
-__device__ __forceinline__ uint32_t signed_pair(uint32_t w, int i) { // the same pair as the whole numbers that it stands for
-  if (BITS == 4) {
-    const uint32_t m = code_pair<4>(w, i) | 0x64006400u; // 1024 + c, or 1024 + 16 c
-    return as_u32(i & 1 ? __hfma2(as_half2(m), __float2half2_rn(0.0625f), __float2half2_rn(-72.f)) : __hsub2(as_half2(m), __float2half2_rn(1032.f)));
-  }
-  return as_u32(__hsub2(as_half2(code_pair<8>(w, i) | 0x64006400u), __float2half2_rn(1152.f)));
-}
-
 template <int HD, int NT>
 struct SplitShape {
   static constexpr int R = 8 * NT;        // query rows of an item
@@ -173,8 +123,8 @@ struct SplitShape {
   static constexpr int MERGE = SPLIT_WARPS * R * (COL + 2) * 4; // bytes
 };
 
-// Parts of items in the workspace, two places a CTA: references [R], sums [R], accumulators [R][HD]. The tickets lie behind all places, at one
-// offset whatever the shape of the call: they are zero between calls and no other call's parts may fall on them.
+// Parts of items in the workspace, two places a CTA: references [R], sums [R], accumulators [R][HD]. A cut item's ticket is that of the CTA which holds its
+// first part.
 constexpr int MAX_SPLIT_GRID = 148 * 4, RECORD_STRIDE = 16 * (128 + 2);
 constexpr size_t RECORDS_BYTES = (size_t)MAX_SPLIT_GRID * 2 * RECORD_STRIDE * 4;
 
@@ -518,8 +468,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
         float top = d_max;
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // scales of up to 2^-6 .. 4 are taken as they are
-        const int e = top > 0.f && top < INFINITY ? ilogbf(top) : 0, k_new = e > 1 || e < -6 ? -e : 0;
+        const int k_new = scale_shift(top);
         if (top > 0.f) {
           const float by = k_set ? ldexpf(1.f, k_new - k) : 0.f;
 #pragma unroll
@@ -536,13 +485,12 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
         }
       }
       if (k != 0) {
-        const __half2 by = __float2half2_rn(ldexpf(1.f, min(k, 15))), by2 = __float2half2_rn(ldexpf(1.f, max(k - 15, 0))); // 2^24 is past f16
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
           for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int bl = 0; bl < NB; bl++) dv[u][e][bl] = as_u32(__hmul2(__hmul2(as_half2(dv[u][e][bl]), by), by2));
+            for (int bl = 0; bl < NB; bl++) dv[u][e][bl] = raise_pair(dv[u][e][bl], k);
       }
       // softmax
       bool grew = false;
@@ -720,7 +668,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
       __syncthreads();
       if (threadIdx.x == 0) {
         __threadfence(); // the CTA's parts, which the barrier has ordered before, become visible before the count does
-        s_last = atomicInc(a.tickets + (long long)b * per_seq + item, (unsigned)others) == (unsigned)others;
+        s_last = atomicInc(a.tickets + c_first, (unsigned)others) == (unsigned)others;
         __threadfence();
       }
       __syncthreads();
@@ -780,17 +728,13 @@ struct SplitLaunch {
 };
 // Query rows of a KV head to an item of the split kernel.
 int split_nt(int64_t rows) { return rows <= 8 ? 1 : 2; }
-size_t split_workspace(int64_t batch, int64_t seq, int heads, int kv_heads) {
-  const int64_t rows = seq * (heads / kv_heads), r = 8 * split_nt(rows);
-  return RECORDS_BYTES + (size_t)batch * kv_heads * ((rows + r - 1) / r) * 4;
-}
+// Rows from which the kernel for many rows takes 16-bit queries.
+constexpr int64_t PROMPT_ROWS = 64;
 
 template <int BITS, int HD, int NT, bool SPLIT>
-int run_split(AttendArgs a, void *workspace, int sms, cudaStream_t s) {
+int run_split(AttendArgs a, int sms, cudaStream_t s) {
   const int64_t rows = a.seq * a.group;
   a.row_tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
-  a.records = static_cast<float *>(workspace);
-  a.tickets = reinterpret_cast<unsigned int *>(static_cast<uint8_t *>(workspace) + RECORDS_BYTES);
   using Launch = SplitLaunch<BITS, HD, NT, SPLIT>;
   // no more CTAs than the longest caches could fill
   const int64_t most = a.batch * a.c.kv_heads * a.row_tiles * ((a.c.max_seq + KV_TILE - 1) / KV_TILE);
@@ -814,23 +758,27 @@ int for_each_split(F f) { // f<BITS, HD, NT, SPLIT>()
 }
 
 template <int BITS, int HD>
-int run_attend(const AttendArgs &a, void *workspace, int sms, cudaStream_t s) {
+int run_attend(const AttendArgs &a, int sms, cudaStream_t s) {
   const bool one = split_nt(a.seq * a.group) == 1;
-  if (a.dtype == XNQ_F32) return one ? run_split<BITS, HD, 1, true>(a, workspace, sms, s) : run_split<BITS, HD, 2, true>(a, workspace, sms, s);
-  return one ? run_split<BITS, HD, 1, false>(a, workspace, sms, s) : run_split<BITS, HD, 2, false>(a, workspace, sms, s);
+  if (a.dtype == XNQ_F32) return one ? run_split<BITS, HD, 1, true>(a, sms, s) : run_split<BITS, HD, 2, true>(a, sms, s);
+  return one ? run_split<BITS, HD, 1, false>(a, sms, s) : run_split<BITS, HD, 2, false>(a, sms, s);
 }
 
 } // namespace
 
 int kv_attend_status(unsigned int *bits) {
+  unsigned int prompt = 0;
   XNQ_CUDA(cudaMemcpyFromSymbol(bits, g_kv_attend_status, sizeof(*bits)));
-  return XNQ_OK;
+  const int rc = kv_prompt_status(&prompt);
+  *bits |= prompt;
+  return rc;
 }
 int kv_attend_init(int device) {
   unsigned int zero = 0;
   XNQ_CUDA(cudaMemcpyToSymbol(g_kv_attend_status, &zero, sizeof(zero)));
   if (device < 64) XNQ_CUDA(cudaDeviceGetAttribute(&g_sms[device], cudaDevAttrMultiProcessorCount, device));
-  return for_each_split([](auto l) { return decltype(l)::init(); });
+  const int rc = kv_prompt_init(device);
+  return rc != XNQ_OK ? rc : for_each_split([](auto l) { return decltype(l)::init(); });
 }
 
 } // namespace xnq
@@ -841,7 +789,8 @@ extern "C" {
 
 size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim) {
   if (batch <= 0 || seq <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
-  return split_workspace(batch, seq, heads, kv_heads);
+  // (for the kernel for many rows at its most: a part for every SM)
+  return KV_TICKET_BYTES + std::max(RECORDS_BYTES, seq * (heads / kv_heads) >= PROMPT_ROWS ? kv_prompt_parts_bytes(head_dim) : 0);
 }
 
 int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
@@ -866,9 +815,12 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
   if (!sms) return fail(XNQ_ERR_UNSUPPORTED, "kv_attend: xnq_init has not run for device %d", device);
   a.lse = lse, a.batch = batch, a.seq = seq, a.heads = heads, a.group = heads / cache->kv_heads, a.dtype = q->dtype;
   a.pos_stride = pos_stride, a.causal = causal, a.pos = pos, a.scale = scale == 0.f ? 1e-30f : scale /* (a masked score is -inf times it) */, a.window = std::min<int64_t>(window, INT32_MAX);
+  a.tickets = static_cast<unsigned int *>(workspace);
+  a.records = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + KV_TICKET_BYTES);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (kv_bits(cache->ggml_dtype) == 4) return cache->head_dim == 64 ? run_attend<4, 64>(a, workspace, sms, s) : run_attend<4, 128>(a, workspace, sms, s);
-  return cache->head_dim == 64 ? run_attend<8, 64>(a, workspace, sms, s) : run_attend<8, 128>(a, workspace, sms, s);
+  if (q->dtype != XNQ_F32 && seq * a.group >= PROMPT_ROWS) return launch_kv_prompt(a, kv_bits(cache->ggml_dtype), cache->head_dim, sms, s);
+  if (kv_bits(cache->ggml_dtype) == 4) return cache->head_dim == 64 ? run_attend<4, 64>(a, sms, s) : run_attend<4, 128>(a, sms, s);
+  return cache->head_dim == 64 ? run_attend<8, 64>(a, sms, s) : run_attend<8, 128>(a, sms, s);
 }
 
 } // extern "C"
