@@ -231,7 +231,8 @@ ATTEND = [  # B, S, H, KV, hd, L, page, first positions
     (1, 1, 1, 1, 128, 1, None, [0]), (1, 1, 32, 8, 128, 512, None, [511]), (1, 1, 4, 4, 64, 33, None, [32]), (2, 1, 8, 1, 128, 300, 64, [0, 299]),
     (16, 1, 32, 8, 128, 200, None, [199] * 16), (5, 1, 28, 4, 64, 1000, 32, [999, 31, 32, 500, -1]), (3, 5, 14, 2, 64, 400, None, [0, 395, 130]),
     (2, 9, 12, 12, 128, 90, 32, [-4, 81]), (2, 3, 40, 2, 128, 257, None, [100, 254]), (1, 17, 8, 8, 128, 50, None, [20]),
-    (2, 64, 8, 2, 128, 200, None, [0, 101]), (1, 128, 8, 2, 64, 300, 32, [172]), (1, 200, 16, 2, 128, 200, None, [0]), (2, 131, 6, 3, 128, 450, 64, [-31, 300])]
+    (2, 64, 8, 2, 128, 200, None, [0, 101]), (1, 128, 8, 2, 64, 300, 32, [172]), (1, 200, 16, 2, 128, 200, None, [0]), (2, 131, 6, 3, 128, 450, 64, [-31, 300]),
+    (4, 300, 32, 16, 128, 700, 64, [0, 400, 33, 399]), (3, 260, 64, 32, 64, 900, None, [640, 0, 7])]   # as many rows as take two tiles a CTA
 
 
 @pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])

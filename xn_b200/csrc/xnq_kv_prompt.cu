@@ -130,9 +130,13 @@ template <int BITS, int HD, int QT>
 struct PromptShape {
   using L = KvTile<BITS, HD>;
   static constexpr int OPERAND = 128 * HD * 2; // a tile of Q, K or V^T
-  static constexpr int Q0 = 0, K0 = QT * OPERAND, V0 = K0 + 2 * OPERAND, RAW0 = V0 + 2 * OPERAND;
+  static constexpr int V_STAGES = BITS == 8 && HD == 128 && QT == 2 ? 1 : 2; // (two would leave three raw tiles)
+  static constexpr int Q0 = 0, K0 = QT * OPERAND, V0 = K0 + 2 * OPERAND, RAW0 = V0 + V_STAGES * OPERAND;
   static constexpr int MOST = 227 * 1024 - 3072; // (1024 of them to start on 1024 bytes, the rest for what is static)
   static constexpr int SLOTS = (MOST - RAW0) / L::BYTES < 16 ? (MOST - RAW0) / L::BYTES : 16;
+  // A producer waits for its tile's scan and then not before the tile STEP_TILES further on, whose barrier must by then be in the phase before, not two
+  // before, which reads as complete: the tile that had the slot last lies no nearer than STEP_TILES.
+  static_assert(SLOTS >= STEP_TILES, "raw tiles");
   static constexpr int SMEM_USED = RAW0 + SLOTS * L::BYTES + 1024;
   static constexpr int SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024; // one CTA an SM: each takes all of the tensor memory
   static constexpr int RECORD = QT * 128 * (HD + 2); // floats of a part: references, sums, rows
@@ -261,12 +265,15 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     for (int j = 0; j < n; j++) {
       const int i = j * STEP_TILES + in_step, slot = i % P::SLOTS, stage = j & 1;
       if (!wait_for(raw_scanned + 8 * slot, (i / P::SLOTS) & 1, dead)) break;
-      if (j >= 2 && !wait_for(empty + 8 * stage, ((j >> 1) - 1) & 1, dead)) break;
+      const int v_stage = P::V_STAGES == 2 ? stage : 0;
+      if (is_v && P::V_STAGES == 1) {
+        if (j >= 1 && !wait_for(v_empty, (j - 1) & 1, dead)) break;
+      } else if (j >= 2 && !wait_for(empty + 8 * stage, ((j >> 1) - 1) & 1, dead)) break;
       const uint8_t *tile = smem + P::RAW0 + slot * L::BYTES;
       const int shift = is_v ? meta[j % META_STEPS][in_step].v_shift : meta[j % META_STEPS][in_step].k_shift;
       if (!is_v) {
         const uint32_t dst = base + P::K0 + stage * P::OPERAND + in_step * (KV_TILE * 128);
-#pragma unroll
+#pragma unroll 1
         for (int it = 0; it < 4; it++) {
           const int r = it * 8 + (lane & 7), t = (lane >> 3) ^ ((r >> 1) & 3), from = position_at(r);
           uint32_t w[W], d[NB / 2];
@@ -297,7 +304,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         }
       } else {
         const int pq = lane & 3, g = lane >> 2;
-        const uint32_t dst = base + P::V0 + stage * P::OPERAND + (in_step >> 1) * (HD * 128);
+        const uint32_t dst = base + P::V0 + v_stage * P::OPERAND + (in_step >> 1) * (HD * 128);
         uint32_t w[4][W], d[4][NB];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
@@ -338,7 +345,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       }
       fence_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(full + 8 * stage), mbar_arrive(raw_empty + 8 * slot);
+      if (lane == 0) mbar_arrive(full + 8 * (is_v ? v_stage : stage)), mbar_arrive(raw_empty + 8 * slot);
       __syncwarp();
     }
   } else if (warp == MMA) {
@@ -361,7 +368,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     }
     for (int j = 0; j < n && alive; j++) {
       const int stage = j & 1;
-      alive = wait_for(v_full + 8 * stage, (j >> 1) & 1, dead);
+      const int v_stage = P::V_STAGES == 2 ? stage : 0;
+      alive = wait_for(v_full + 8 * v_stage, (P::V_STAGES == 2 ? j >> 1 : j) & 1, dead);
       const bool more = j + 1 < n;
       if (alive && more) alive = wait_for(k_full + 8 * (stage ^ 1), ((j + 1) >> 1) & 1, dead);
 #pragma unroll
@@ -372,11 +380,11 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < BN / 16; ks++)
-            mma_ts(tmem + 256 + q * HD, tmem + q * 128 + ks * 8, operand(base + P::V0 + stage * P::OPERAND + (ks >> 2) * (HD * 128)) + (ks & 3) * 2, instruction(HD), j | ks ? 1u : 0u);
+            mma_ts(tmem + 256 + q * HD, tmem + q * 128 + ks * 8, operand(base + P::V0 + v_stage * P::OPERAND + (ks >> 2) * (HD * 128)) + (ks & 3) * 2, instruction(HD), j | ks ? 1u : 0u);
           if (more) scores(q, stage ^ 1);
           else commit(o_done + 8 * q);
           if (q == QT - 1) {
-            commit(v_empty + 8 * stage);
+            commit(v_empty + 8 * v_stage);
             if (more) commit(k_empty + 8 * (stage ^ 1));
           }
         }
@@ -442,7 +450,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       int hidden = 0, cut = 0; // bit c: tile c of the step is seen by no row of the warp; not by all
       float top = -INFINITY;
       int v_new = v_ref;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < STEP_TILES; c++) {
         const Meta mt = meta[j % META_STEPS][c];
         const int j0 = (t0 + j * STEP_TILES + c) * KV_TILE;
@@ -455,7 +463,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         uint32_t s[32];
         tmem_ld32(scores + c * 32, s);
         tmem_ld_wait();
-        float x = -INFINITY;
+        float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, x = -INFINITY;
         if ((cut >> c) & 1) {
 #pragma unroll
           for (int i = 0; i < 32; i++) {
@@ -468,7 +476,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; i++) x = fmaxf(x, __uint_as_float(s[i]));
+          for (int i = 0; i < 32; i += 2) y[(i >> 1) & 3] = fmaxf(y[(i >> 1) & 3], fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
+          x = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
           if (mt.bad) l = NAN;
         }
         top = fmaxf(top, x == -INFINITY ? x : x * (mt.k_shift ? ldexpf(f, -mt.k_shift) : f));
@@ -493,7 +502,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         }
         v_ref = v_new;
       }
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < STEP_TILES; c++) {
         uint32_t pk[16];
         if ((hidden >> c) & 1) {
