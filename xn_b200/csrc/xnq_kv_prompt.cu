@@ -1,16 +1,17 @@
 // Attention of many 16-bit query rows (prompts, pieces of them) over the quantized KV cache, on the 5th-generation tensor cores.
 //
-//   S[128 rows, 128 positions] = Q K^T      O[128 rows, head_dim] += P V      P = 2^(S f - reference), per row: running maximum, sum
+//   S[128 rows, 64 positions] = Q K^T      O[128 rows, head_dim] += P V      P = 2^(S f - reference), per row: a reference near the maximum, a sum
 //
 // A CTA has QT tiles of 128 query rows (the query heads of one KV head, token by token) and walks over the positions that any of them sees, 128 at a
-// step. Two row tiles take turns: while one's scores are in softmax the tensor core works on the other's. Warps have roles:
+// step, in two halves. Two row tiles take turns, and a tile's scores are in two buffers: the tensor core forms the next half's while this one's are in
+// softmax. Warps have roles:
 //   loader     one bulk copy (1-D, never multicast) a cache tile, into a ring of raw tiles
-//   scan       one look at a raw tile's scales: what no row sees is zeroed, what is not finite is noted, the largest gives a power of two
+//   scan       two, tiles in turn: one look at a raw tile's scales: what no row sees is zeroed, what is not finite is noted, the largest gives a power of two
 //   producers  eight: codes to f16 (whole number, zero taken off, times its scale, rounded once) into the swizzled operand tiles. Keys stay rows of
 //              positions; the values' words hold pairs of positions of a dim, so that V^T's rows of dims need no exchange either. The order of the dims in a
 //              run of 8 (Q has the same) and of the pairs of positions in a run of 8 is the unpacking's own.
-//   MMA        issues S = Q K^T for the next step behind O += P V of this one, P read from tensor memory, where it replaces its scores
-//   softmax    four a row tile, a thread a row: maximum, 2^x, sum, P as f16; rescales O when a maximum has grown by more than 2^8
+//   MMA        issues O += P V of a half and S = Q K^T of the half after next, P read from tensor memory, where it replaces its scores
+//   softmax    four a row tile, a thread a row: 2^x, sum, P as f16; rescales O where a score has passed its reference by more than 2^12
 // Tensor memory: the scores of both tiles and both outputs, all 512 columns. f16 operands for bf16 queries too: q is exact after a power of two a row,
 // and K, V and P lose 2^-12 instead of bf16's 2^-9.
 //
@@ -25,9 +26,12 @@ namespace {
 
 __device__ unsigned int g_kv_prompt_status;
 
-constexpr int BN = 128;                     // positions of a step
+constexpr int BN = 128, HALF = BN / 2;     // positions of a step, of a half
 constexpr int STEP_TILES = BN / KV_TILE;
-constexpr int PRODUCER0 = 8, LOADER = 16, SCAN = 17, MMA = 18, PROMPT_THREADS = 19 * 32;
+constexpr int PRODUCER0 = 8, LOADER = 16, SCAN = 17, SCANS = 2, MMA = 19, PROMPT_THREADS = 20 * 32;
+// Registers a thread: launched with 96; the softmax warps hold two tiles' scores at a time.
+constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 144, PRODUCER_REGS = 72, OTHER_REGS = 48;
+static_assert(256 * SOFTMAX_REGS + 256 * PRODUCER_REGS + 128 * OTHER_REGS <= PROMPT_THREADS * LAUNCH_REGS, "an increase beyond what the CTA was launched with waits forever");
 constexpr int META_STEPS = 8;               // more than steps are between the scan and softmax
 
 // ---- barriers, bulk copies, tensor memory ----
@@ -100,6 +104,22 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(idesc), "r"(add)
       : "memory");
 }
+// two at a time
+__device__ __forceinline__ float2 fma2(uint32_t x, uint32_t y, float f, float add) { // (x f + add, y f + add)
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(x), "r"(y), "f"(f), "f"(add));
+  return r;
+}
+__device__ __forceinline__ void add2(float2 &a, float2 b) {
+  asm("{\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a.x), "+f"(a.y)
+      : "f"(b.x), "f"(b.y));
+}
 #define XNQ_R16(r, o) \
   "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7]), "=r"(r[o + 8]), "=r"(r[o + 9]), \
       "=r"(r[o + 10]), "=r"(r[o + 11]), "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]), "=r"(r[o + 15])
@@ -157,7 +177,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   using L = KvTile<BITS, HD>;
   constexpr int NB = L::NB, W = L::W, PANEL = 128 * 128; // bytes of 64 columns of an operand
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[3 * 16 + 8 + 2 * 2 + 1 + 2];
+  __shared__ __align__(8) uint64_t bars[3 * 16 + 8 + 4 + 4 + 2 + 2 + 1];
   __shared__ Meta meta[META_STEPS][STEP_TILES];
   __shared__ int s_null[16];
   __shared__ int s_dead, s_last;
@@ -167,13 +187,13 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   uint8_t *const smem = smem_raw + (base - (uint32_t)__cvta_generic_to_shared(smem_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
   const uint32_t raw_full = bar, raw_scanned = bar + 16 * 8, raw_empty = bar + 32 * 8, k_full = bar + 48 * 8, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16,
-                 s_full = v_empty + 16, p_full = s_full + 16, q_ready = p_full + 16, o_done = q_ready + 8;
+                 s_full = v_empty + 16, p_full = s_full + 32, pv_done = p_full + 32, o_done = pv_done + 16, q_ready = o_done + 16; // s_full, p_full: [row tile][buffer] (softmax may be two halves ahead of the MMAs)
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 16; i++) mbar_init(raw_full + 8 * i, 1), mbar_init(raw_scanned + 8 * i, 1), mbar_init(raw_empty + 8 * i, 2);
     for (int i = 0; i < 2; i++) {
       mbar_init(k_full + 8 * i, STEP_TILES), mbar_init(v_full + 8 * i, STEP_TILES), mbar_init(k_empty + 8 * i, 1), mbar_init(v_empty + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_done + 8 * i, 1);
+      mbar_init(s_full + 16 * i, 1), mbar_init(s_full + 16 * i + 8, 1), mbar_init(p_full + 16 * i, 4), mbar_init(p_full + 16 * i + 8, 4), mbar_init(pv_done + 8 * i, 1), mbar_init(o_done + 8 * i, 1);
     }
     mbar_init(q_ready, QT * 4);
     s_dead = 0;
@@ -186,7 +206,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   pdl_wait();
 
   // ---- which rows, which positions; the row tiles with the most positions first ----
@@ -204,6 +224,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   if (threadIdx.x == 0 && pos + a.seq > a.c.max_seq) atomicOr(&g_kv_prompt_status, KV_PAST_ATTEND);
   volatile int *const dead = &s_dead;
 
+  if (warp >= LOADER) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
   if (warp == LOADER) {
     const uint8_t *ahead = nullptr;
     for (int i = 0; i < n * STEP_TILES; i++) {
@@ -226,39 +247,51 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     if (*dead) // none of this CTA's copies is in flight when it ends
       for (int i = 0; i < P::SLOTS; i++)
         for (int k = 0; k < 1000 && !mbar_try(raw_full + 8 * i, 0) && !mbar_try(raw_full + 8 * i, 1); k++) {}
-  } else if (warp == SCAN) {
-    for (int i = 0; i < n * STEP_TILES; i++) {
+  } else if (warp < MMA && warp >= SCAN) { // tiles in turn
+    for (int i = warp - SCAN; i < n * STEP_TILES; i += SCANS) {
       const int slot = i % P::SLOTS;
       if (!wait_for(raw_full + 8 * slot, (i / P::SLOTS) & 1, dead)) break;
       uint8_t *tile = smem + P::RAW0 + slot * L::BYTES;
       const bool null = s_null[slot];
       const int j0 = (t0 + i) * KV_TILE;
-      unsigned bad = 0, k_top = 0, v_top = 0;
-      auto look = [&](uint32_t *at, uint32_t keep, unsigned bit0, unsigned bit1, unsigned &top) {
-        const uint32_t old = *at;
-        uint32_t x = null ? 0u : old & keep;
-        if ((x & 0x7c00u) == 0x7c00u) x &= 0xffff0000u, bad |= bit0;
-        if ((x & 0x7c000000u) == 0x7c000000u) x &= 0xffffu, bad |= bit1;
-        if (x != old) *at = x;
-        top = max(top, max(x & 0x7fffu, (x >> 16) & 0x7fffu));
-      };
-      const bool k_in = j0 + lane >= lo && j0 + lane <= hi;
+      // a lane's scales: a position's keys, half a pair's values (NB words a pair)
+      constexpr int KW = NB / 2;
+      uint32_t *const kp = reinterpret_cast<uint32_t *>(tile + L::k_scale(lane, 0)), *const vp = reinterpret_cast<uint32_t *>(tile + L::v_scale(lane / 2, (lane & 1) * KW));
+      uint32_t x[2 * KW];
 #pragma unroll
-      for (int q = 0; q < NB / 2; q++) look(reinterpret_cast<uint32_t *>(tile + L::k_scale(lane, 2 * q)), k_in ? 0xffffffffu : 0u, 1u << lane, 1u << lane, k_top);
-      if (lane < 16) {
-        const int j = j0 + 2 * lane;
-        const uint32_t keep = (j >= lo && j <= hi ? 0xffffu : 0u) | (j + 1 >= lo && j + 1 <= hi ? 0xffff0000u : 0u);
+      for (int k = 0; k < KW; k++) x[k] = kp[k], x[KW + k] = vp[k];
+      uint32_t top[2] = {0u, 0u};
 #pragma unroll
-        for (int q = 0; q < NB; q++) look(reinterpret_cast<uint32_t *>(tile + L::v_scale(lane, q)), keep, 1u << (2 * lane), 2u << (2 * lane), v_top);
+      for (int k = 0; k < KW; k++) top[0] = __vmaxu2(top[0], x[k] & 0x7fff7fffu), top[1] = __vmaxu2(top[1], x[KW + k] & 0x7fff7fffu);
+      const uint32_t k_top = max(top[0] & 0xffffu, top[0] >> 16), v_top = max(top[1] & 0xffffu, top[1] >> 16);
+      // Most tiles: all of their positions are seen by some row, every scale is below 4 and the largest ones are not below 2^-6.
+      const bool plain = !null && j0 >= lo && j0 + KV_TILE - 1 <= hi && __all_sync(0xffffffffu, max(k_top, v_top) < 0x4400u) && __any_sync(0xffffffffu, k_top >= 0x2400u) &&
+                         __any_sync(0xffffffffu, v_top >= 0x2400u);
+      Meta mt{0, 0, 0u, 0};
+      if (!plain) {
+        unsigned bad = 0, most[2] = {0u, 0u};
+#pragma unroll
+        for (int k = 0; k < 2 * KW; k++) {
+          const bool is_k = k < KW;
+          const int in = is_k ? lane : lane & ~1, j = j0 + in; // keys: both halves are of position j; values: of j and j + 1
+          const bool in0 = j >= lo && j <= hi, in1 = is_k ? in0 : j + 1 >= lo && j + 1 <= hi;
+          uint32_t y = null ? 0u : x[k] & ((in0 ? 0xffffu : 0u) | (in1 ? 0xffff0000u : 0u));
+          if ((y & 0x7c00u) == 0x7c00u) y &= 0xffff0000u, bad |= 1u << in;
+          if ((y & 0x7c000000u) == 0x7c000000u) y &= 0xffffu, bad |= (is_k ? 1u : 2u) << in;
+          if (is_k) kp[k] = y;
+          else vp[k - KW] = y;
+          most[is_k ? 0 : 1] = max(most[is_k ? 0 : 1], max(y & 0x7fffu, (y >> 16) & 0x7fffu));
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        mt = Meta{scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[0])))),
+                  scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[1])))), bad, null ? 1 : 0};
       }
-      bad = __reduce_or_sync(0xffffffffu, bad), k_top = __reduce_max_sync(0xffffffffu, k_top), v_top = __reduce_max_sync(0xffffffffu, v_top);
-      if (lane == 0)
-        meta[(i / STEP_TILES) % META_STEPS][i % STEP_TILES] = Meta{scale_shift(__half2float(__ushort_as_half((unsigned short)k_top))),
-                                                                 scale_shift(__half2float(__ushort_as_half((unsigned short)v_top))), bad, null ? 1 : 0};
+      if (lane == 0) meta[(i / STEP_TILES) % META_STEPS][i % STEP_TILES] = mt;
       __syncwarp();
       if (lane == 0) mbar_arrive(raw_scanned + 8 * slot);
     }
   } else if (warp >= PRODUCER0 && warp < LOADER) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGS));
     const int in_step = (warp - PRODUCER0) >> 1;
     const bool is_v = (warp - PRODUCER0) & 1;
     const uint32_t full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty;
@@ -349,41 +382,48 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       __syncwarp();
     }
   } else if (warp == MMA) {
-    bool alive = n > 0 && wait_for(q_ready, 0, dead) && wait_for(k_full, 0, dead);
-    auto scores = [&](int q, int stage) {
+    // The loops' course and the descriptors are functions of what the compiler knows to be uniform, so that descriptors stay in uniform registers: moved there
+    // one by one they hold an MMA up for longer than it takes. After a wait that gave up nothing more is issued.
+    const int halves = 2 * __shfl_sync(0xffffffffu, n, 0);
+    bool alive = halves > 0 && wait_for(q_ready, 0, dead) && wait_for(k_full, 0, dead);
+    auto scores = [&](int q, int h) { // of half h
+      const int stage = (h >> 1) & 1, rows_at = (h & 1) * (HALF * 128);
+      const uint64_t qd = operand(base + P::Q0 + q * P::OPERAND), kd = operand(base + P::K0 + stage * P::OPERAND + rows_at);
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ks++)
-        mma_ss(tmem + q * 128, operand(base + P::Q0 + q * P::OPERAND + (ks >> 2) * PANEL) + (ks & 3) * 2, operand(base + P::K0 + stage * P::OPERAND + (ks >> 2) * PANEL) + (ks & 3) * 2,
-               instruction(BN), ks ? 1u : 0u);
-      commit(s_full + 8 * q);
+        mma_ss(tmem + q * 128 + (h & 1) * HALF, qd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), instruction(HALF),
+               ks ? 1u : 0u);
+      commit(s_full + 16 * q + 8 * (h & 1));
     };
-    if (alive) {
-      tc_fence_after();
-      if (elect_one()) {
+    tc_fence_after();
+    if (elect_one() && alive) {
 #pragma unroll
-        for (int q = 0; q < QT; q++) scores(q, 0);
-        commit(k_empty);
-      }
-      __syncwarp();
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int q = 0; q < QT; q++) scores(q, h);
+      commit(k_empty);
     }
-    for (int j = 0; j < n && alive; j++) {
-      const int stage = j & 1;
-      const int v_stage = P::V_STAGES == 2 ? stage : 0;
-      alive = wait_for(v_full + 8 * v_stage, (P::V_STAGES == 2 ? j >> 1 : j) & 1, dead);
-      const bool more = j + 1 < n;
-      if (alive && more) alive = wait_for(k_full + 8 * (stage ^ 1), ((j + 1) >> 1) & 1, dead);
+    __syncwarp();
+    for (int h = 0; h < halves; h++) {
+      const int j = h >> 1, stage = j & 1, v_stage = P::V_STAGES == 2 ? stage : 0;
+      const bool more = h + 2 < halves;
+      if (!(h & 1)) {
+        if (alive) alive = wait_for(v_full + 8 * v_stage, (P::V_STAGES == 2 ? j >> 1 : j) & 1, dead);
+        if (alive && more) alive = wait_for(k_full + 8 * (stage ^ 1), ((j + 1) >> 1) & 1, dead);
+      }
+      const uint64_t vd = operand(base + P::V0 + v_stage * P::OPERAND + (h & 1) * (HD * 128));
 #pragma unroll
       for (int q = 0; q < QT; q++) {
-        if (alive) alive = wait_for(p_full + 8 * q, j & 1, dead);
-        if (!alive) break;
+        if (alive) alive = wait_for(p_full + 16 * q + 8 * (h & 1), (h >> 1) & 1, dead);
         tc_fence_after();
-        if (elect_one()) {
+        __syncwarp();
+        if (elect_one() && alive) {
 #pragma unroll
-          for (int ks = 0; ks < BN / 16; ks++)
-            mma_ts(tmem + 256 + q * HD, tmem + q * 128 + ks * 8, operand(base + P::V0 + v_stage * P::OPERAND + (ks >> 2) * (HD * 128)) + (ks & 3) * 2, instruction(HD), j | ks ? 1u : 0u);
-          if (more) scores(q, stage ^ 1);
-          else commit(o_done + 8 * q);
-          if (q == QT - 1) {
+          for (int ks = 0; ks < HALF / 16; ks++) mma_ts(tmem + 256 + q * HD, tmem + q * 128 + (h & 1) * HALF + ks * 8, vd + (uint64_t)(ks * 2), instruction(HD), h | ks ? 1u : 0u);
+          commit(pv_done + 8 * q);
+          if (more) scores(q, h + 2);
+          else if (h & 1) commit(o_done + 8 * q);
+          if (q == QT - 1 && (h & 1)) {
             commit(v_empty + 8 * v_stage);
             if (more) commit(k_empty + 8 * (stage ^ 1));
           }
@@ -393,8 +433,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     }
   } else if (warp < QT * 4) {
     // ---- a row a thread ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     const int q = warp >> 2, r = (warp & 3) * 32 + lane; // row tile, row of it
-    const uint32_t tm = tmem + ((uint32_t)(warp & 3) << 21), scores = tm + q * 128, o_acc = tm + 256 + q * HD;
+    const uint32_t tm = tmem + ((uint32_t)(warp & 3) << 21), buffers = tm + q * 128, o_acc = tm + 256 + q * HD;
     const int row = q * 128 + r;
     const bool valid = row < rows;
     const long long at = row0 + row, tok = at / a.group;
@@ -440,108 +481,116 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
-    float m = -INFINITY, ref = 0.f, l = 0.f;
-    int v_ref = 0; // O holds the sums times 2^v_ref
+    float ref = -INFINITY, l = 0.f; // the reference: 4 below a maximum when it was set; none yet: -inf
+    int v_ref = 0;                  // O holds the sums times 2^v_ref
     bool alive = true;
-    for (int j = 0; j < n; j++) {
-      alive = wait_for(s_full + 8 * q, j & 1, dead);
-      if (!alive) break;
-      tc_fence_after();
-      int hidden = 0, cut = 0; // bit c: tile c of the step is seen by no row of the warp; not by all
-      float top = -INFINITY;
-      int v_new = v_ref;
+    int h2 = 0; // the half at hand
+    // Rows with a score more than 2^12 over their reference (or that have none) get another: what they have summed is scaled, P of the half's first tile
+    // included; o_by: O and P alone (the values' scales).
+    auto rescale = [&](int c, float top, float o_by) {
+      const bool grew = top > ref + 12.f;
+      const float to = grew ? top - 4.f : ref, by = ref == -INFINITY ? 0.f : exp2_approx(ref - to);
+      ref = to, l *= by;
+      const float f32 = by * o_by;
+      if (h2) {
+        if (!wait_for(pv_done + 8 * q, (h2 - 1) & 1, dead)) alive = false; // (the half before that one was done before this one's scores)
+        tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < STEP_TILES; c++) {
-        const Meta mt = meta[j % META_STEPS][c];
-        const int j0 = (t0 + j * STEP_TILES + c) * KV_TILE;
-        if (mt.gone || j0 > hi_any || j0 + KV_TILE - 1 < lo_any) {
-          hidden |= 1 << c;
-          continue;
+        for (int x = 0; x < HD; x += 16) {
+          uint32_t o[16];
+          tmem_ld16(o_acc + x, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f32);
+          tmem_st16(o_acc + x, o);
         }
-        if (j0 < lo_all || j0 + KV_TILE - 1 > hi_all) cut |= 1 << c;
-        v_new = min(v_new, mt.v_shift);
-        uint32_t s[32];
-        tmem_ld32(scores + c * 32, s);
+      }
+      if (c) {
+        const __half2 f16 = __float2half2_rn(f32); // (0 or less than one: P loses no more than its own rounding)
+        uint32_t o[16];
+        tmem_ld16(buffers + (h2 & 1) * HALF, o);
         tmem_ld_wait();
-        float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, x = -INFINITY;
-        if ((cut >> c) & 1) {
 #pragma unroll
-          for (int i = 0; i < 32; i++) {
-            const int p = j0 + position_at(i);
-            if (p >= r_lo && p <= r_hi) x = fmaxf(x, __uint_as_float(s[i]));
-          }
-          if (mt.bad) {
-            const int first = max(r_lo - j0, 0), last = min(r_hi - j0, 31);
-            if (first <= last && (mt.bad >> first) << (31 - last + first)) l = NAN;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) y[(i >> 1) & 3] = fmaxf(y[(i >> 1) & 3], fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 1])));
-          x = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-          if (mt.bad) l = NAN;
-        }
-        top = fmaxf(top, x == -INFINITY ? x : x * (mt.k_shift ? ldexpf(f, -mt.k_shift) : f));
+        for (int i = 0; i < 16; i++) o[i] = as_u32(__hmul2(as_half2(o[i]), f16));
+        tmem_st16(buffers + (h2 & 1) * HALF, o);
       }
-      top = fmaxf(top, m);
-      const bool grew = top > ref + 12.f || (m == -INFINITY && top != -INFINITY); // the reference lies 4 below a maximum
-      if (__any_sync(0xffffffffu, grew) || v_new != v_ref) {
-        const float r2 = top == -INFINITY ? 0.f : top - 4.f;
-        const float by = m == -INFINITY ? 0.f : exp2_approx(ref - r2);
-        m = top, ref = r2, l *= by;
-        if (j) {
-          const float o_by = by * ldexpf(1.f, v_new - v_ref);
-#pragma unroll 1
-          for (int c = 0; c < HD; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(o_acc + c, o);
-            tmem_ld_wait();
+      tmem_st_wait();
+    };
+    // scores of tile c of the half to weights
+    auto weigh = [&](uint32_t (&s)[32], int c) {
+      const uint32_t at_s = buffers + (h2 & 1) * HALF + c * 32, at_p = buffers + (h2 & 1) * HALF + c * 16; // P over scores that have been read
+      const Meta mt = meta[(h2 >> 1) % META_STEPS][(h2 & 1) * 2 + c];
+      const int j0 = (t0 + h2 * 2 + c) * KV_TILE;
+      uint32_t pk[16];
+      const bool out = mt.gone || j0 > hi_any || j0 + KV_TILE - 1 < lo_any, cut = j0 < lo_all || j0 + KV_TILE - 1 > hi_all; // seen by no row of the warp; not by all
+      bool general = out | cut | (mt.bad != 0) | (mt.k_shift != 0) | (mt.v_shift != v_ref) | __any_sync(0xffffffffu, ref == -INFINITY);
+      if (!general) {
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        __half2 most = __float2half2_rn(0.f);
 #pragma unroll
-            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * o_by);
-            tmem_st16(o_acc + c, o);
-          }
+        for (int i = 0; i < 32; i += 2) {
+          float2 p = fma2(s[i], s[i + 1], f, -ref);
+          p.x = exp2_approx(p.x), p.y = exp2_approx(p.y);
+          add2(sum[(i >> 1) & 1], p);
+          pk[i / 2] = pack_half2(p.x, p.y);
+          most = __hmax2(most, as_half2(pk[i / 2]));
         }
-        v_ref = v_new;
+        general = __any_sync(0xffffffffu, fmaxf(__low2float(most), __high2float(most)) > 4096.f); // (an overflow is infinite)
+        if (!general) l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        else {
+          tmem_ld32(at_s, s);
+          tmem_ld_wait();
+        }
       }
-#pragma unroll 1
-      for (int c = 0; c < STEP_TILES; c++) {
-        uint32_t pk[16];
-        if ((hidden >> c) & 1) {
+      if (general) {
+        if (out) {
 #pragma unroll
           for (int i = 0; i < 16; i++) pk[i] = 0u;
         } else {
-          const Meta mt = meta[j % META_STEPS][c];
-          const int j0 = (t0 + j * STEP_TILES + c) * KV_TILE;
-          const float ft = mt.k_shift ? ldexpf(f, -mt.k_shift) : f;
-          uint32_t s[32];
-          tmem_ld32(scores + c * 32, s);
-          tmem_ld_wait();
+          if (cut) {
+            const int first = max(r_lo - j0, 0), last = min(r_hi - j0, 31);
+            const unsigned seen = first <= last ? (0xffffffffu >> (31 - last + first)) << first : 0u;
+            if (mt.bad & seen) l = NAN;
 #pragma unroll
-          for (int i = 0; i < 32; i++) s[i] = __float_as_uint(exp2_approx(fmaf(__uint_as_float(s[i]), ft, -ref)));
-          if ((cut >> c) & 1) {
+            for (int i = 0; i < 32; i++)
+              if (!((seen >> position_at(i)) & 1)) s[i] = 0xff800000u;
+          } else if (mt.bad) l = NAN;
+          const float ft = ldexpf(f, -mt.k_shift);
+          float x = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
-              const int p = j0 + position_at(i);
-              if (p < r_lo || p > r_hi) s[i] = 0u;
-            }
+          for (int i = 0; i < 32; i++) x = fmaxf(x, __uint_as_float(s[i]));
+          const float top = x == -INFINITY ? x : x * ft;
+          if (__any_sync(0xffffffffu, top > ref + 12.f) || mt.v_shift < v_ref) {
+            const int v_new = min(mt.v_shift, v_ref);
+            rescale(c, top, ldexpf(1.f, v_new - v_ref));
+            v_ref = v_new;
           }
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          const float from = ref == -INFINITY ? 0.f : ref, by = ldexpf(1.f, v_ref - mt.v_shift); // (scales that far from the others)
 #pragma unroll
-          for (int i = 0; i < 32; i++) sum[i & 3] += __uint_as_float(s[i]);
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          if (mt.v_shift != v_ref) { // (scales that far from the others)
-            const float by = ldexpf(1.f, v_ref - mt.v_shift);
-#pragma unroll
-            for (int i = 0; i < 32; i++) s[i] = __float_as_uint(__uint_as_float(s[i]) * by);
+          for (int i = 0; i < 32; i += 2) {
+            const float p0 = exp2_approx(fmaf(__uint_as_float(s[i]), ft, -from)), p1 = exp2_approx(fmaf(__uint_as_float(s[i + 1]), ft, -from));
+            l += p0 + p1;
+            pk[i / 2] = pack_half2(p0 * by, p1 * by);
           }
-#pragma unroll
-          for (int i = 0; i < 16; i++) pk[i] = pack_half2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
         }
-        tmem_st16(scores + c * 16, pk);
       }
+      tmem_st16(at_p, pk);
+    };
+    for (; h2 < 2 * n && alive; h2++) {
+      alive = wait_for(s_full + 16 * q + 8 * (h2 & 1), (h2 >> 1) & 1, dead);
+      if (!alive) break;
+      tc_fence_after();
+      uint32_t x[32], y[32];
+      tmem_ld32(buffers + (h2 & 1) * HALF, x);
+      tmem_ld_wait();
+      tmem_ld32(buffers + (h2 & 1) * HALF + 32, y);
+      weigh(x, 0);
+      tmem_ld_wait();
+      weigh(y, 1);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * q);
+      if (lane == 0) mbar_arrive(p_full + 16 * q + 8 * (h2 & 1));
     }
     if (alive && n) alive = wait_for(o_done + 8 * q, 0, dead);
     tc_fence_after();
@@ -575,7 +624,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       if (valid && a.lse) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (ref + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
     } else {
       float *rec = a.records + (size_t)blockIdx.x * P::RECORD;
-      rec[row] = l == 0.f ? -INFINITY : ref, rec[QT * 128 + row] = l;
+      rec[row] = ref, rec[QT * 128 + row] = l;
       const float by = ldexpf(1.f, -v_ref);
       float *dst = rec + 2 * QT * 128 + (size_t)row * HD;
 #pragma unroll 1
@@ -592,49 +641,50 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       }
     }
     tc_fence_before();
-  }
-  __syncthreads();
-  if (a.splits > 1) {
-    const int unit = (int)(blockIdx.x / per) * (per / a.splits) + bk;
-    if (threadIdx.x == 0) {
-      __threadfence();
-      s_last = atomicInc(a.tickets + unit, (unsigned)(a.splits - 1)) == (unsigned)(a.splits - 1);
-      __threadfence();
-    }
-    __syncthreads();
-    if (s_last) {
-      const float *first = a.records + (size_t)(blockIdx.x - split) * P::RECORD;
-      for (int i = threadIdx.x; i < rows * (HD / 8); i += PROMPT_THREADS) {
-        const int row = i / (HD / 8), c = (i - row * (HD / 8)) * 8;
-        const long long at = row0 + row, tok = at / a.group;
-        const int h = kvh * a.group + (int)(at - tok * a.group);
-        float m = -INFINITY, l = 0.f, v[8] = {};
-        for (int k = 0; k < a.splits; k++) m = fmaxf(m, __ldcg(first + (size_t)k * P::RECORD + row));
-        for (int k = 0; k < a.splits; k++) {
-          const float *p = first + (size_t)k * P::RECORD;
-          const float mp = __ldcg(p + row), lp = __ldcg(p + QT * 128 + row);
-          const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + 2 * QT * 128 + (size_t)row * HD + c)), y = __ldcg(reinterpret_cast<const float4 *>(p + 2 * QT * 128 + (size_t)row * HD + c + 4));
-          const float by = mp == -INFINITY ? 0.f : exp2_approx(mp - m);
-          if (by == 0.f) continue;
-          l += by * lp;
-          v[0] += by * x.x, v[1] += by * x.y, v[2] += by * x.z, v[3] += by * x.w, v[4] += by * y.x, v[5] += by * y.y, v[6] += by * y.z, v[7] += by * y.w;
-        }
-        const float by = l > 0.f ? 1.f / l : l;
-        uint32_t w[4];
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const float x = v[2 * q] * by, y = v[2 * q + 1] * by;
-          if (a.dtype == XNQ_F16) w[q] = pack_half2(x, y);
-          else {
-            const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
-            w[q] = *reinterpret_cast<const uint32_t *>(&z);
+    if (a.splits > 1) { // the softmax warps alone
+      asm volatile("bar.sync 1, %0;" ::"n"(QT * 128) : "memory");
+      const int unit = (int)(blockIdx.x / per) * (per / a.splits) + bk;
+      if (threadIdx.x == 0) {
+        __threadfence();
+        s_last = atomicInc(a.tickets + unit, (unsigned)(a.splits - 1)) == (unsigned)(a.splits - 1);
+        __threadfence();
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(QT * 128) : "memory");
+      if (s_last) {
+        const float *first = a.records + (size_t)(blockIdx.x - split) * P::RECORD;
+        for (int i = threadIdx.x; i < rows * (HD / 8); i += QT * 128) {
+          const int row = i / (HD / 8), c = (i - row * (HD / 8)) * 8;
+          const long long at = row0 + row, tok = at / a.group;
+          const int h = kvh * a.group + (int)(at - tok * a.group);
+          float m = -INFINITY, l = 0.f, v[8] = {};
+          for (int k = 0; k < a.splits; k++) m = fmaxf(m, __ldcg(first + (size_t)k * P::RECORD + row));
+          for (int k = 0; k < a.splits; k++) {
+            const float *p = first + (size_t)k * P::RECORD;
+            const float mp = __ldcg(p + row), lp = __ldcg(p + QT * 128 + row);
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + 2 * QT * 128 + (size_t)row * HD + c)), y = __ldcg(reinterpret_cast<const float4 *>(p + 2 * QT * 128 + (size_t)row * HD + c + 4));
+            const float by = mp == -INFINITY ? 0.f : exp2_approx(mp - m);
+            if (by == 0.f) continue;
+            l += by * lp;
+            v[0] += by * x.x, v[1] += by * x.y, v[2] += by * x.z, v[3] += by * x.w, v[4] += by * y.x, v[5] += by * y.y, v[6] += by * y.z, v[7] += by * y.w;
           }
+          const float by = l > 0.f ? 1.f / l : l;
+          uint32_t w[4];
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            const float x = v[2 * q] * by, y = v[2 * q + 1] * by;
+            if (a.dtype == XNQ_F16) w[q] = pack_half2(x, y);
+            else {
+              const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
+              w[q] = *reinterpret_cast<const uint32_t *>(&z);
+            }
+          }
+          *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out.p) + b * a.out.sb + tok * a.out.ss + h * a.out.sh + c) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (a.lse && c == 0) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
         }
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out.p) + b * a.out.sb + tok * a.out.ss + h * a.out.sh + c) = make_uint4(w[0], w[1], w[2], w[3]);
-        if (a.lse && c == 0) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
       }
     }
   }
+  __syncthreads();
   if (warp == MMA) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
