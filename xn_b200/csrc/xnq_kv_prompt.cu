@@ -6,11 +6,11 @@
 // step, in two halves. Two row tiles take turns, and a tile's scores are in two buffers: the tensor core forms the next half's while this one's are in
 // softmax. Warps have roles:
 //   loader     one bulk copy (1-D, never multicast) a cache tile, into a ring of raw tiles
-//   scan       two, tiles in turn: one look at a raw tile's scales: what no row sees is zeroed, what is not finite is noted, the largest gives a power of two
+//   scan       one look at a raw tile's scales: what no row sees is zeroed, what is not finite is noted, the largest gives a power of two
 //   producers  eight: codes to f16 (whole number, zero taken off, times its scale, rounded once) into the swizzled operand tiles. Keys stay rows of
 //              positions; the values' words hold pairs of positions of a dim, so that V^T's rows of dims need no exchange either. The order of the dims in a
 //              run of 8 (Q has the same) and of the pairs of positions in a run of 8 is the unpacking's own.
-//   MMA        issues O += P V of a half and S = Q K^T of the half after next, P read from tensor memory, where it replaces its scores
+//   MMA        one a row tile: issues O += P V of a half and S = Q K^T of the half after next, P read from tensor memory, where it replaces its scores
 //   softmax    four a row tile, a thread a row: 2^x, sum, P as f16; rescales O where a score has passed its reference by more than 2^12
 // Tensor memory: the scores of both tiles and both outputs, all 512 columns. f16 operands for bf16 queries too: q is exact after a power of two a row,
 // and K, V and P lose 2^-12 instead of bf16's 2^-9.
@@ -28,7 +28,7 @@ __device__ unsigned int g_kv_prompt_status;
 
 constexpr int BN = 128, HALF = BN / 2;     // positions of a step, of a half
 constexpr int STEP_TILES = BN / KV_TILE;
-constexpr int PRODUCER0 = 8, LOADER = 16, SCAN = 17, SCANS = 2, MMA = 19, PROMPT_THREADS = 20 * 32;
+constexpr int PRODUCER0 = 8, LOADER = 16, SCAN = 17, MMA = 18, PROMPT_THREADS = 20 * 32;
 // Registers a thread: launched with 96; the softmax warps hold two tiles' scores at a time.
 constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 144, PRODUCER_REGS = 72, OTHER_REGS = 48;
 static_assert(256 * SOFTMAX_REGS + 256 * PRODUCER_REGS + 128 * OTHER_REGS <= PROMPT_THREADS * LAUNCH_REGS, "an increase beyond what the CTA was launched with waits forever");
@@ -140,6 +140,23 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld64(uint32_t addr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+      "%24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, "
+      "%56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
+      : XNQ_R16(r, 0), XNQ_R16(r, 16), XNQ_R16(r, 32), XNQ_R16(r, 48)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, "
+      "%25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -177,7 +194,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   using L = KvTile<BITS, HD>;
   constexpr int NB = L::NB, W = L::W, PANEL = 128 * 128; // bytes of 64 columns of an operand
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[3 * 16 + 8 + 4 + 4 + 2 + 2 + 1];
+  __shared__ __align__(8) uint64_t bars[3 * 16 + 8 + 4 + 4 + 2 + 2 + 2];
   __shared__ Meta meta[META_STEPS][STEP_TILES];
   __shared__ int s_null[16];
   __shared__ int s_dead, s_last;
@@ -192,10 +209,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   if (threadIdx.x == 0) {
     for (int i = 0; i < 16; i++) mbar_init(raw_full + 8 * i, 1), mbar_init(raw_scanned + 8 * i, 1), mbar_init(raw_empty + 8 * i, 2);
     for (int i = 0; i < 2; i++) {
-      mbar_init(k_full + 8 * i, STEP_TILES), mbar_init(v_full + 8 * i, STEP_TILES), mbar_init(k_empty + 8 * i, 1), mbar_init(v_empty + 8 * i, 1);
+      mbar_init(k_full + 8 * i, STEP_TILES), mbar_init(v_full + 8 * i, STEP_TILES), mbar_init(k_empty + 8 * i, QT), mbar_init(v_empty + 8 * i, QT);
       mbar_init(s_full + 16 * i, 1), mbar_init(s_full + 16 * i + 8, 1), mbar_init(p_full + 16 * i, 4), mbar_init(p_full + 16 * i + 8, 4), mbar_init(pv_done + 8 * i, 1), mbar_init(o_done + 8 * i, 1);
     }
-    mbar_init(q_ready, QT * 4);
+    mbar_init(q_ready, 4), mbar_init(q_ready + 8, 4);
     s_dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -247,8 +264,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     if (*dead) // none of this CTA's copies is in flight when it ends
       for (int i = 0; i < P::SLOTS; i++)
         for (int k = 0; k < 1000 && !mbar_try(raw_full + 8 * i, 0) && !mbar_try(raw_full + 8 * i, 1); k++) {}
-  } else if (warp < MMA && warp >= SCAN) { // tiles in turn
-    for (int i = warp - SCAN; i < n * STEP_TILES; i += SCANS) {
+  } else if (warp == SCAN) {
+    for (int i = 0; i < n * STEP_TILES; i++) {
       const int slot = i % P::SLOTS;
       if (!wait_for(raw_full + 8 * slot, (i / P::SLOTS) & 1, dead)) break;
       uint8_t *tile = smem + P::RAW0 + slot * L::BYTES;
@@ -381,26 +398,25 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       if (lane == 0) mbar_arrive(full + 8 * (is_v ? v_stage : stage)), mbar_arrive(raw_empty + 8 * slot);
       __syncwarp();
     }
-  } else if (warp == MMA) {
+  } else if (warp >= MMA && warp < MMA + QT) {
     // The loops' course and the descriptors are functions of what the compiler knows to be uniform, so that descriptors stay in uniform registers: moved there
-    // one by one they hold an MMA up for longer than it takes. After a wait that gave up nothing more is issued.
-    const int halves = 2 * __shfl_sync(0xffffffffu, n, 0);
-    bool alive = halves > 0 && wait_for(q_ready, 0, dead) && wait_for(k_full, 0, dead);
-    auto scores = [&](int q, int h) { // of half h
-      const int stage = (h >> 1) & 1, rows_at = (h & 1) * (HALF * 128);
-      const uint64_t qd = operand(base + P::Q0 + q * P::OPERAND), kd = operand(base + P::K0 + stage * P::OPERAND + rows_at);
+    // one by one they hold an MMA up for longer than it takes. After a wait that gave up nothing more is issued. (One warp for both row tiles was held up by
+    // the one while the other was ready: 307 us for 2048 queries at 8192 positions.)
+    const int q = warp - MMA, halves = 2 * __shfl_sync(0xffffffffu, n, 0);
+    bool alive = halves > 0 && wait_for(q_ready + 8 * q, 0, dead) && wait_for(k_full, 0, dead);
+    const uint64_t qd = operand(base + P::Q0 + q * P::OPERAND);
+    const uint32_t s_acc = tmem + q * 128, o_acc = tmem + 256 + q * HD, sf = s_full + 16 * q, pf = p_full + 16 * q;
+    auto scores = [&](int h) { // of half h
+      const uint64_t kd = operand(base + P::K0 + ((h >> 1) & 1) * P::OPERAND + (h & 1) * (HALF * 128));
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ks++)
-        mma_ss(tmem + q * 128 + (h & 1) * HALF, qd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), instruction(HALF),
-               ks ? 1u : 0u);
-      commit(s_full + 16 * q + 8 * (h & 1));
+        mma_ss(s_acc + (h & 1) * HALF, qd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), instruction(HALF), ks ? 1u : 0u);
+      commit(sf + 8 * (h & 1));
     };
     tc_fence_after();
     if (elect_one() && alive) {
-#pragma unroll
-      for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int q = 0; q < QT; q++) scores(q, h);
+      scores(0);
+      scores(1);
       commit(k_empty);
     }
     __syncwarp();
@@ -412,24 +428,21 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         if (alive && more) alive = wait_for(k_full + 8 * (stage ^ 1), ((j + 1) >> 1) & 1, dead);
       }
       const uint64_t vd = operand(base + P::V0 + v_stage * P::OPERAND + (h & 1) * (HD * 128));
+      if (alive) alive = wait_for(pf + 8 * (h & 1), (h >> 1) & 1, dead);
+      tc_fence_after();
+      __syncwarp();
+      if (elect_one() && alive) {
 #pragma unroll
-      for (int q = 0; q < QT; q++) {
-        if (alive) alive = wait_for(p_full + 16 * q + 8 * (h & 1), (h >> 1) & 1, dead);
-        tc_fence_after();
-        __syncwarp();
-        if (elect_one() && alive) {
-#pragma unroll
-          for (int ks = 0; ks < HALF / 16; ks++) mma_ts(tmem + 256 + q * HD, tmem + q * 128 + (h & 1) * HALF + ks * 8, vd + (uint64_t)(ks * 2), instruction(HD), h | ks ? 1u : 0u);
-          commit(pv_done + 8 * q);
-          if (more) scores(q, h + 2);
-          else if (h & 1) commit(o_done + 8 * q);
-          if (q == QT - 1 && (h & 1)) {
-            commit(v_empty + 8 * v_stage);
-            if (more) commit(k_empty + 8 * (stage ^ 1));
-          }
+        for (int ks = 0; ks < HALF / 16; ks++) mma_ts(o_acc, s_acc + (h & 1) * HALF + ks * 8, vd + (uint64_t)(ks * 2), instruction(HD), h | ks ? 1u : 0u);
+        commit(pv_done + 8 * q);
+        if (more) scores(h + 2);
+        else if (h & 1) commit(o_done + 8 * q);
+        if (h & 1) {
+          commit(v_empty + 8 * v_stage);
+          if (more) commit(k_empty + 8 * (stage ^ 1));
         }
-        __syncwarp();
       }
+      __syncwarp();
     }
   } else if (warp < QT * 4) {
     // ---- a row a thread ----
@@ -479,7 +492,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       }
       fence_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
+      if (lane == 0) mbar_arrive(q_ready + 8 * q);
     }
     float ref = -INFINITY, l = 0.f; // the reference: 4 below a maximum when it was set; none yet: -inf
     int v_ref = 0;                  // O holds the sums times 2^v_ref
@@ -516,77 +529,84 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       }
       tmem_st_wait();
     };
-    // scores of tile c of the half to weights
-    auto weigh = [&](uint32_t (&s)[32], int c) {
-      const uint32_t at_s = buffers + (h2 & 1) * HALF + c * 32, at_p = buffers + (h2 & 1) * HALF + c * 16; // P over scores that have been read
-      const Meta mt = meta[(h2 >> 1) % META_STEPS][(h2 & 1) * 2 + c];
-      const int j0 = (t0 + h2 * 2 + c) * KV_TILE;
-      uint32_t pk[16];
-      const bool out = mt.gone || j0 > hi_any || j0 + KV_TILE - 1 < lo_any, cut = j0 < lo_all || j0 + KV_TILE - 1 > hi_all; // seen by no row of the warp; not by all
-      bool general = out | cut | (mt.bad != 0) | (mt.k_shift != 0) | (mt.v_shift != v_ref) | __any_sync(0xffffffffu, ref == -INFINITY);
+    // A half's scores to weights. Where every row sees every position, no scales are far off and no score is far over its row's reference, both tiles at once.
+    auto weigh = [&](uint32_t (&s)[64]) {
+      const uint32_t at = buffers + (h2 & 1) * HALF; // P takes the place of the first half of the scores
+      const Meta *mt2 = &meta[(h2 >> 1) % META_STEPS][(h2 & 1) * 2];
+      const Meta ma = mt2[0], mb = mt2[1];
+      const int j0 = (t0 + h2 * 2) * KV_TILE;
+      bool general = (ma.gone | mb.gone | ma.k_shift | mb.k_shift | (ma.v_shift ^ v_ref) | (mb.v_shift ^ v_ref)) != 0 || (ma.bad | mb.bad) != 0u || j0 < lo_all ||
+                     j0 + HALF - 1 > hi_all || __any_sync(0xffffffffu, ref == -INFINITY);
+      uint32_t pk[32];
       if (!general) {
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        __half2 most = __float2half2_rn(0.f);
+        float2 sum[4] = {};
+        __half2 most[2] = {__float2half2_rn(0.f), __float2half2_rn(0.f)};
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
+        for (int i = 0; i < 64; i += 2) {
           float2 p = fma2(s[i], s[i + 1], f, -ref);
           p.x = exp2_approx(p.x), p.y = exp2_approx(p.y);
-          add2(sum[(i >> 1) & 1], p);
+          add2(sum[(i >> 1) & 3], p);
           pk[i / 2] = pack_half2(p.x, p.y);
-          most = __hmax2(most, as_half2(pk[i / 2]));
+          most[(i >> 1) & 1] = __hmax2(most[(i >> 1) & 1], as_half2(pk[i / 2]));
         }
-        general = __any_sync(0xffffffffu, fmaxf(__low2float(most), __high2float(most)) > 4096.f); // (an overflow is infinite)
-        if (!general) l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        else {
-          tmem_ld32(at_s, s);
-          tmem_ld_wait();
-        }
+        most[0] = __hmax2(most[0], most[1]);
+        general = __any_sync(0xffffffffu, fmaxf(__low2float(most[0]), __high2float(most[0])) > 4096.f); // (an overflow is infinite)
+        if (!general) l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
       }
-      if (general) {
-        if (out) {
+      if (!general) {
+        tmem_st32(at, pk);
+        return;
+      }
+#pragma unroll 1
+      for (int c = 0; c < 2; c++) {
+        const Meta mt = mt2[c];
+        const int i0 = j0 + c * KV_TILE;
+        uint32_t x[32], out[16];
+        if (mt.gone || i0 > hi_any || i0 + KV_TILE - 1 < lo_any) { // seen by no row of the warp
 #pragma unroll
-          for (int i = 0; i < 16; i++) pk[i] = 0u;
+          for (int i = 0; i < 16; i++) out[i] = 0u;
         } else {
-          if (cut) {
-            const int first = max(r_lo - j0, 0), last = min(r_hi - j0, 31);
+          tmem_ld32(at + c * 32, x);
+          tmem_ld_wait();
+          if (i0 < lo_all || i0 + KV_TILE - 1 > hi_all) { // not by all
+            const int first = max(r_lo - i0, 0), last = min(r_hi - i0, 31);
             const unsigned seen = first <= last ? (0xffffffffu >> (31 - last + first)) << first : 0u;
             if (mt.bad & seen) l = NAN;
 #pragma unroll
             for (int i = 0; i < 32; i++)
-              if (!((seen >> position_at(i)) & 1)) s[i] = 0xff800000u;
+              if (!((seen >> position_at(i)) & 1)) x[i] = 0xff800000u;
           } else if (mt.bad) l = NAN;
           const float ft = ldexpf(f, -mt.k_shift);
-          float x = -INFINITY;
+          float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; i++) x = fmaxf(x, __uint_as_float(s[i]));
-          const float top = x == -INFINITY ? x : x * ft;
+          for (int i = 0; i < 32; i += 2) y[(i >> 1) & 3] = fmaxf(y[(i >> 1) & 3], fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+          const float z = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), top = z == -INFINITY ? z : z * ft;
           if (__any_sync(0xffffffffu, top > ref + 12.f) || mt.v_shift < v_ref) {
             const int v_new = min(mt.v_shift, v_ref);
             rescale(c, top, ldexpf(1.f, v_new - v_ref));
             v_ref = v_new;
           }
           const float from = ref == -INFINITY ? 0.f : ref, by = ldexpf(1.f, v_ref - mt.v_shift); // (scales that far from the others)
+          float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const float p0 = exp2_approx(fmaf(__uint_as_float(s[i]), ft, -from)), p1 = exp2_approx(fmaf(__uint_as_float(s[i + 1]), ft, -from));
-            l += p0 + p1;
-            pk[i / 2] = pack_half2(p0 * by, p1 * by);
+            const float p0 = exp2_approx(fmaf(__uint_as_float(x[i]), ft, -from)), p1 = exp2_approx(fmaf(__uint_as_float(x[i + 1]), ft, -from));
+            sum += p0 + p1;
+            out[i / 2] = pack_half2(p0 * by, p1 * by);
           }
+          l += sum;
         }
+        tmem_st16(at + c * 16, out); // over scores of this tile and the one before, which have been read
       }
-      tmem_st16(at_p, pk);
     };
     for (; h2 < 2 * n && alive; h2++) {
       alive = wait_for(s_full + 16 * q + 8 * (h2 & 1), (h2 >> 1) & 1, dead);
       if (!alive) break;
       tc_fence_after();
-      uint32_t x[32], y[32];
-      tmem_ld32(buffers + (h2 & 1) * HALF, x);
+      uint32_t x[64];
+      tmem_ld64(buffers + (h2 & 1) * HALF, x);
       tmem_ld_wait();
-      tmem_ld32(buffers + (h2 & 1) * HALF + 32, y);
-      weigh(x, 0);
-      tmem_ld_wait();
-      weigh(y, 1);
+      weigh(x);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
