@@ -28,6 +28,7 @@ __device__ unsigned int g_kv_prompt_status;
 
 constexpr int BN = 128, HALF = BN / 2;     // positions of a step, of a half
 constexpr int STEP_TILES = BN / KV_TILE;
+constexpr int RING = 3;                      // halves of operands
 constexpr int PRODUCER0 = 8, LOADER = 16, SCAN = 17, MMA = 18, PROMPT_THREADS = 20 * 32;
 // Registers a thread: launched with 96; the softmax warps hold two tiles' scores at a time.
 constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 144, PRODUCER_REGS = 72, OTHER_REGS = 48;
@@ -166,13 +167,13 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
 template <int BITS, int HD, int QT>
 struct PromptShape {
   using L = KvTile<BITS, HD>;
-  static constexpr int OPERAND = 128 * HD * 2; // a tile of Q, K or V^T
-  static constexpr int V_STAGES = BITS == 8 && HD == 128 && QT == 2 ? 1 : 2; // (two would leave three raw tiles)
-  static constexpr int Q0 = 0, K0 = QT * OPERAND, V0 = K0 + 2 * OPERAND, RAW0 = V0 + V_STAGES * OPERAND;
+  static constexpr int Q_TILE = 128 * HD * 2, KV_HALF = HALF * HD * 2; // operands: a row tile, the keys or values of a half
+  static constexpr int Q0 = 0, K0 = QT * Q_TILE, V0 = K0 + RING * KV_HALF, RAW0 = V0 + RING * KV_HALF;
   static constexpr int MOST = 227 * 1024 - 3072; // (1024 of them to start on 1024 bytes, the rest for what is static)
   static constexpr int SLOTS = (MOST - RAW0) / L::BYTES < 16 ? (MOST - RAW0) / L::BYTES : 16;
   // A producer waits for its tile's scan and then not before the tile STEP_TILES further on, whose barrier must by then be in the phase before, not two
-  // before, which reads as complete: the tile that had the slot last lies no nearer than STEP_TILES.
+  // before, which reads as complete: the tile that had the slot last lies no nearer than STEP_TILES. (For the rings of operands the releases come in order:
+  // whoever has seen half h - 5 released has seen half h - 6.)
   static_assert(SLOTS >= STEP_TILES, "raw tiles");
   static constexpr int SMEM_USED = RAW0 + SLOTS * L::BYTES + 1024;
   static constexpr int SMEM = SMEM_USED > 120 * 1024 ? SMEM_USED : 120 * 1024; // one CTA an SM: each takes all of the tensor memory
@@ -192,9 +193,9 @@ template <int BITS, int HD, int QT>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(const __grid_constant__ AttendArgs a) {
   using P = PromptShape<BITS, HD, QT>;
   using L = KvTile<BITS, HD>;
-  constexpr int NB = L::NB, W = L::W, PANEL = 128 * 128; // bytes of 64 columns of an operand
+  constexpr int NB = L::NB, W = L::W, PANEL = 128 * 128, K_PANEL = HALF * 128; // bytes of 64 columns of Q, of a half's keys
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[3 * 16 + 8 + 4 + 4 + 2 + 2 + 2];
+  __shared__ __align__(8) uint64_t bars[3 * 16 + 4 * RING + 4 + 4 + 2 + 2 + 2];
   __shared__ Meta meta[META_STEPS][STEP_TILES];
   __shared__ int s_null[16];
   __shared__ int s_dead, s_last;
@@ -203,13 +204,13 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - (uint32_t)__cvta_generic_to_shared(smem_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
-  const uint32_t raw_full = bar, raw_scanned = bar + 16 * 8, raw_empty = bar + 32 * 8, k_full = bar + 48 * 8, k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16,
-                 s_full = v_empty + 16, p_full = s_full + 32, pv_done = p_full + 32, o_done = pv_done + 16, q_ready = o_done + 16; // s_full, p_full: [row tile][buffer] (softmax may be two halves ahead of the MMAs)
+  const uint32_t raw_full = bar, raw_scanned = bar + 16 * 8, raw_empty = bar + 32 * 8, k_full = bar + 48 * 8, k_empty = k_full + 8 * RING, v_full = k_empty + 8 * RING, v_empty = v_full + 8 * RING,
+                 s_full = v_empty + 8 * RING, p_full = s_full + 32, pv_done = p_full + 32, o_done = pv_done + 16, q_ready = o_done + 16; // s_full, p_full: [row tile][buffer] (softmax may be two halves ahead of the MMAs)
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 16; i++) mbar_init(raw_full + 8 * i, 1), mbar_init(raw_scanned + 8 * i, 1), mbar_init(raw_empty + 8 * i, 2);
+    for (int i = 0; i < RING; i++) mbar_init(k_full + 8 * i, 2), mbar_init(v_full + 8 * i, 2), mbar_init(k_empty + 8 * i, QT), mbar_init(v_empty + 8 * i, QT);
     for (int i = 0; i < 2; i++) {
-      mbar_init(k_full + 8 * i, STEP_TILES), mbar_init(v_full + 8 * i, STEP_TILES), mbar_init(k_empty + 8 * i, QT), mbar_init(v_empty + 8 * i, QT);
       mbar_init(s_full + 16 * i, 1), mbar_init(s_full + 16 * i + 8, 1), mbar_init(p_full + 16 * i, 4), mbar_init(p_full + 16 * i + 8, 4), mbar_init(pv_done + 8 * i, 1), mbar_init(o_done + 8 * i, 1);
     }
     mbar_init(q_ready, 4), mbar_init(q_ready + 8, 4);
@@ -264,65 +265,72 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     if (*dead) // none of this CTA's copies is in flight when it ends
       for (int i = 0; i < P::SLOTS; i++)
         for (int k = 0; k < 1000 && !mbar_try(raw_full + 8 * i, 0) && !mbar_try(raw_full + 8 * i, 1); k++) {}
-  } else if (warp == SCAN) {
-    for (int i = 0; i < n * STEP_TILES; i++) {
-      const int slot = i % P::SLOTS;
-      if (!wait_for(raw_full + 8 * slot, (i / P::SLOTS) & 1, dead)) break;
-      uint8_t *tile = smem + P::RAW0 + slot * L::BYTES;
-      const bool null = s_null[slot];
-      const int j0 = (t0 + i) * KV_TILE;
-      // a lane's scales: a position's keys, half a pair's values (NB words a pair)
-      constexpr int KW = NB / 2;
-      uint32_t *const kp = reinterpret_cast<uint32_t *>(tile + L::k_scale(lane, 0)), *const vp = reinterpret_cast<uint32_t *>(tile + L::v_scale(lane / 2, (lane & 1) * KW));
-      uint32_t x[2 * KW];
+  } else if (warp == SCAN) { // two tiles at a time
+    constexpr int KW = NB / 2;
+    for (int i = 0; i < n * STEP_TILES; i += 2) {
+      uint32_t *kp[2], *vp[2], x[2][2 * KW];
+      bool null[2];
+      bool ok = true;
 #pragma unroll
-      for (int k = 0; k < KW; k++) x[k] = kp[k], x[KW + k] = vp[k];
-      uint32_t top[2] = {0u, 0u};
+      for (int e = 0; e < 2; e++) {
+        const int slot = (i + e) % P::SLOTS;
+        ok = ok && wait_for(raw_full + 8 * slot, ((i + e) / P::SLOTS) & 1, dead);
+        uint8_t *tile = smem + P::RAW0 + slot * L::BYTES;
+        null[e] = s_null[slot];
+        // a lane's scales: a position's keys, half a pair's values (NB words a pair)
+        kp[e] = reinterpret_cast<uint32_t *>(tile + L::k_scale(lane, 0)), vp[e] = reinterpret_cast<uint32_t *>(tile + L::v_scale(lane / 2, (lane & 1) * KW));
 #pragma unroll
-      for (int k = 0; k < KW; k++) top[0] = __vmaxu2(top[0], x[k] & 0x7fff7fffu), top[1] = __vmaxu2(top[1], x[KW + k] & 0x7fff7fffu);
-      const uint32_t k_top = max(top[0] & 0xffffu, top[0] >> 16), v_top = max(top[1] & 0xffffu, top[1] >> 16);
-      // Most tiles: all of their positions are seen by some row, every scale is below 4 and the largest ones are not below 2^-6.
-      const bool plain = !null && j0 >= lo && j0 + KV_TILE - 1 <= hi && __all_sync(0xffffffffu, max(k_top, v_top) < 0x4400u) && __any_sync(0xffffffffu, k_top >= 0x2400u) &&
-                         __any_sync(0xffffffffu, v_top >= 0x2400u);
-      Meta mt{0, 0, 0u, 0};
-      if (!plain) {
-        unsigned bad = 0, most[2] = {0u, 0u};
-#pragma unroll
-        for (int k = 0; k < 2 * KW; k++) {
-          const bool is_k = k < KW;
-          const int in = is_k ? lane : lane & ~1, j = j0 + in; // keys: both halves are of position j; values: of j and j + 1
-          const bool in0 = j >= lo && j <= hi, in1 = is_k ? in0 : j + 1 >= lo && j + 1 <= hi;
-          uint32_t y = null ? 0u : x[k] & ((in0 ? 0xffffu : 0u) | (in1 ? 0xffff0000u : 0u));
-          if ((y & 0x7c00u) == 0x7c00u) y &= 0xffff0000u, bad |= 1u << in;
-          if ((y & 0x7c000000u) == 0x7c000000u) y &= 0xffffu, bad |= (is_k ? 1u : 2u) << in;
-          if (is_k) kp[k] = y;
-          else vp[k - KW] = y;
-          most[is_k ? 0 : 1] = max(most[is_k ? 0 : 1], max(y & 0x7fffu, (y >> 16) & 0x7fffu));
-        }
-        bad = __reduce_or_sync(0xffffffffu, bad);
-        mt = Meta{scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[0])))),
-                  scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[1])))), bad, null ? 1 : 0};
+        for (int k = 0; k < KW; k++) x[e][k] = kp[e][k], x[e][KW + k] = vp[e][k];
       }
-      if (lane == 0) meta[(i / STEP_TILES) % META_STEPS][i % STEP_TILES] = mt;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(raw_scanned + 8 * slot);
+      if (!ok) break;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int j0 = (t0 + i + e) * KV_TILE;
+        uint32_t top[2] = {0u, 0u};
+#pragma unroll
+        for (int k = 0; k < KW; k++) top[0] = __vmaxu2(top[0], x[e][k] & 0x7fff7fffu), top[1] = __vmaxu2(top[1], x[e][KW + k] & 0x7fff7fffu);
+        const uint32_t k_top = max(top[0] & 0xffffu, top[0] >> 16), v_top = max(top[1] & 0xffffu, top[1] >> 16);
+        // Most tiles: all of their positions are seen by some row, every scale is below 4 and the largest ones are not below 2^-6.
+        const bool plain = !null[e] && j0 >= lo && j0 + KV_TILE - 1 <= hi && __all_sync(0xffffffffu, max(k_top, v_top) < 0x4400u) && __any_sync(0xffffffffu, k_top >= 0x2400u) &&
+                           __any_sync(0xffffffffu, v_top >= 0x2400u);
+        Meta mt{0, 0, 0u, 0};
+        if (!plain) {
+          unsigned bad = 0, most[2] = {0u, 0u};
+#pragma unroll
+          for (int k = 0; k < 2 * KW; k++) {
+            const bool is_k = k < KW;
+            const int in = is_k ? lane : lane & ~1, j = j0 + in; // keys: both halves are of position j; values: of j and j + 1
+            const bool in0 = j >= lo && j <= hi, in1 = is_k ? in0 : j + 1 >= lo && j + 1 <= hi;
+            uint32_t y = null[e] ? 0u : x[e][k] & ((in0 ? 0xffffu : 0u) | (in1 ? 0xffff0000u : 0u));
+            if ((y & 0x7c00u) == 0x7c00u) y &= 0xffff0000u, bad |= 1u << in;
+            if ((y & 0x7c000000u) == 0x7c000000u) y &= 0xffffu, bad |= (is_k ? 1u : 2u) << in;
+            if (is_k) kp[e][k] = y;
+            else vp[e][k - KW] = y;
+            most[is_k ? 0 : 1] = max(most[is_k ? 0 : 1], max(y & 0x7fffu, (y >> 16) & 0x7fffu));
+          }
+          bad = __reduce_or_sync(0xffffffffu, bad);
+          mt = Meta{scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[0])))),
+                    scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[1])))), bad, null[e] ? 1 : 0};
+        }
+        if (lane == 0) meta[((i + e) / STEP_TILES) % META_STEPS][(i + e) % STEP_TILES] = mt;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(raw_scanned + 8 * ((i + e) % P::SLOTS));
+      }
     }
   } else if (warp >= PRODUCER0 && warp < LOADER) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PRODUCER_REGS));
-    const int in_step = (warp - PRODUCER0) >> 1;
+    const int in_half = ((warp - PRODUCER0) >> 1) & 1; // every other half: tile 0 or 1 of it
     const bool is_v = (warp - PRODUCER0) & 1;
     const uint32_t full = is_v ? v_full : k_full, empty = is_v ? v_empty : k_empty;
-    for (int j = 0; j < n; j++) {
-      const int i = j * STEP_TILES + in_step, slot = i % P::SLOTS, stage = j & 1;
+    for (int h = (warp - PRODUCER0) >> 2; h < 2 * n; h += 2) {
+      const int i = h * 2 + in_half, slot = i % P::SLOTS, stage = h % RING, lap = h / RING;
       if (!wait_for(raw_scanned + 8 * slot, (i / P::SLOTS) & 1, dead)) break;
-      const int v_stage = P::V_STAGES == 2 ? stage : 0;
-      if (is_v && P::V_STAGES == 1) {
-        if (j >= 1 && !wait_for(v_empty, (j - 1) & 1, dead)) break;
-      } else if (j >= 2 && !wait_for(empty + 8 * stage, ((j >> 1) - 1) & 1, dead)) break;
+      if (lap && !wait_for(empty + 8 * stage, (lap - 1) & 1, dead)) break;
       const uint8_t *tile = smem + P::RAW0 + slot * L::BYTES;
-      const int shift = is_v ? meta[j % META_STEPS][in_step].v_shift : meta[j % META_STEPS][in_step].k_shift;
+      const Meta &mt = meta[(h >> 1) % META_STEPS][(h & 1) * 2 + in_half];
+      const int shift = is_v ? mt.v_shift : mt.k_shift;
       if (!is_v) {
-        const uint32_t dst = base + P::K0 + stage * P::OPERAND + in_step * (KV_TILE * 128);
+        const uint32_t dst = base + P::K0 + stage * P::KV_HALF + in_half * (KV_TILE * 128);
 #pragma unroll 1
         for (int it = 0; it < 4; it++) {
           const int r = it * 8 + (lane & 7), t = (lane >> 3) ^ ((r >> 1) & 3), from = position_at(r);
@@ -349,12 +357,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
             uint32_t x[4];
 #pragma unroll
             for (int q = 0; q < 4; q++) x[q] = as_u32(__hmul2(as_half2(signed_pair<BITS>(BITS == 4 ? w[bl] : w[2 * bl + q / 2], BITS == 4 ? q : q & 1)), d2));
-            sts128(dst + (bl >> 1) * PANEL + r * 128 + ((((bl & 1) * 4 + t) ^ (r & 7)) << 4), x[0], x[1], x[2], x[3]);
+            sts128(dst + (bl >> 1) * K_PANEL + r * 128 + ((((bl & 1) * 4 + t) ^ (r & 7)) << 4), x[0], x[1], x[2], x[3]);
           }
         }
       } else {
         const int pq = lane & 3, g = lane >> 2;
-        const uint32_t dst = base + P::V0 + v_stage * P::OPERAND + (in_step >> 1) * (HD * 128);
+        const uint32_t dst = base + P::V0 + stage * P::KV_HALF;
         uint32_t w[4][W], d[4][NB];
 #pragma unroll
         for (int q = 0; q < 4; q++) {
@@ -390,12 +398,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
             for (int q = 0; q < 4; q++)
               x[q] = as_u32(__hmul2(as_half2(signed_pair<BITS>(BITS == 4 ? w[q][bl] : w[q][2 * bl + k / 2], BITS == 4 ? k : k & 1)), as_half2(d[q][bl])));
             const int dim = bl * 32 + g * 4 + k;
-            sts128(dst + dim * 128 + ((((in_step & 1) * 4 + pq) ^ (dim & 7)) << 4), x[0], x[1], x[2], x[3]);
+            sts128(dst + dim * 128 + (((in_half * 4 + pq) ^ (dim & 7)) << 4), x[0], x[1], x[2], x[3]);
           }
       }
       fence_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(full + 8 * (is_v ? v_stage : stage)), mbar_arrive(raw_empty + 8 * slot);
+      if (lane == 0) mbar_arrive(full + 8 * stage), mbar_arrive(raw_empty + 8 * slot);
       __syncwarp();
     }
   } else if (warp >= MMA && warp < MMA + QT) {
@@ -403,31 +411,28 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     // one by one they hold an MMA up for longer than it takes. After a wait that gave up nothing more is issued. (One warp for both row tiles was held up by
     // the one while the other was ready: 307 us for 2048 queries at 8192 positions.)
     const int q = warp - MMA, halves = 2 * __shfl_sync(0xffffffffu, n, 0);
-    bool alive = halves > 0 && wait_for(q_ready + 8 * q, 0, dead) && wait_for(k_full, 0, dead);
-    const uint64_t qd = operand(base + P::Q0 + q * P::OPERAND);
+    bool alive = halves > 0 && wait_for(q_ready + 8 * q, 0, dead) && wait_for(k_full, 0, dead) && wait_for(k_full + 8, 0, dead);
+    const uint64_t qd = operand(base + P::Q0 + q * P::Q_TILE);
     const uint32_t s_acc = tmem + q * 128, o_acc = tmem + 256 + q * HD, sf = s_full + 16 * q, pf = p_full + 16 * q;
     auto scores = [&](int h) { // of half h
-      const uint64_t kd = operand(base + P::K0 + ((h >> 1) & 1) * P::OPERAND + (h & 1) * (HALF * 128));
+      const uint64_t kd = operand(base + P::K0 + (h % RING) * P::KV_HALF);
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ks++)
-        mma_ss(s_acc + (h & 1) * HALF, qd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), instruction(HALF), ks ? 1u : 0u);
+        mma_ss(s_acc + (h & 1) * HALF, qd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (K_PANEL / 16) + (ks & 3) * 2), instruction(HALF), ks ? 1u : 0u);
       commit(sf + 8 * (h & 1));
+      commit(k_empty + 8 * (h % RING));
     };
     tc_fence_after();
     if (elect_one() && alive) {
       scores(0);
       scores(1);
-      commit(k_empty);
     }
     __syncwarp();
     for (int h = 0; h < halves; h++) {
-      const int j = h >> 1, stage = j & 1, v_stage = P::V_STAGES == 2 ? stage : 0;
       const bool more = h + 2 < halves;
-      if (!(h & 1)) {
-        if (alive) alive = wait_for(v_full + 8 * v_stage, (P::V_STAGES == 2 ? j >> 1 : j) & 1, dead);
-        if (alive && more) alive = wait_for(k_full + 8 * (stage ^ 1), ((j + 1) >> 1) & 1, dead);
-      }
-      const uint64_t vd = operand(base + P::V0 + v_stage * P::OPERAND + (h & 1) * (HD * 128));
+      if (alive) alive = wait_for(v_full + 8 * (h % RING), (h / RING) & 1, dead);
+      if (alive && more) alive = wait_for(k_full + 8 * ((h + 2) % RING), ((h + 2) / RING) & 1, dead);
+      const uint64_t vd = operand(base + P::V0 + (h % RING) * P::KV_HALF);
       if (alive) alive = wait_for(pf + 8 * (h & 1), (h >> 1) & 1, dead);
       tc_fence_after();
       __syncwarp();
@@ -435,12 +440,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
 #pragma unroll
         for (int ks = 0; ks < HALF / 16; ks++) mma_ts(o_acc, s_acc + (h & 1) * HALF + ks * 8, vd + (uint64_t)(ks * 2), instruction(HD), h | ks ? 1u : 0u);
         commit(pv_done + 8 * q);
+        commit(v_empty + 8 * (h % RING));
         if (more) scores(h + 2);
         else if (h & 1) commit(o_done + 8 * q);
-        if (h & 1) {
-          commit(v_empty + 8 * v_stage);
-          if (more) commit(k_empty + 8 * (stage ^ 1));
-        }
       }
       __syncwarp();
     }
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       e = max(-100, min(100, e));
       const float up = ldexpf(a.scale < 0.f ? -1.f : 1.f, e); // the scale's sign goes into q
       f = ldexpf(fabsf(a.scale) * LOG2E, -e);
-      const uint32_t dst = base + P::Q0 + q * P::OPERAND + r * 128;
+      const uint32_t dst = base + P::Q0 + q * P::Q_TILE + r * 128;
 #pragma unroll
       for (int c = 0; c < HD / 8; c++) {
         const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
