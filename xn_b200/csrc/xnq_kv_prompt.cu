@@ -52,22 +52,40 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) { // may
       : "memory");
   return ok != 0;
 }
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) { // now
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
 // By a whole converged warp; one answer for all lanes. A wait of two seconds is given up: the status bit is set and `dead` makes every other wait return.
+// (Nothing but the barrier is looked at on most turns: with a vote and a look at `dead` on each, waiting warps took half of the SM's issue slots.)
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int *dead) {
-  unsigned long long t0 = 0;
-  for (unsigned attempt = 1;; attempt++) {
-    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-    if (__any_sync(0xffffffffu, *dead)) return false;
-    if ((attempt & 15u) == 0) {
-      unsigned long long now;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-      if (t0 == 0) t0 = now;
-      if (__any_sync(0xffffffffu, now - t0 > 2000000000ull)) break;
+  bool ok = mbar_try(bar, parity);
+  if (!__all_sync(0xffffffffu, ok)) {
+    unsigned long long t0 = 0;
+    for (unsigned attempt = 1; !ok; attempt++) {
+      ok = mbar_try(bar, parity);
+      if (!ok && (attempt & 63u) == 0) {
+        if (*dead) break;
+        unsigned long long now;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+        if (t0 == 0) t0 = now;
+        if (now - t0 > 2000000000ull) {
+          *dead = 1;
+          atomicOr(&g_kv_prompt_status, KV_WAIT);
+          break;
+        }
+      }
     }
+    ok = __all_sync(0xffffffffu, ok);
   }
-  *dead = 1;
-  atomicOr(&g_kv_prompt_status, KV_WAIT);
-  return false;
+  return ok;
 }
 __device__ __forceinline__ bool elect_one() {
   uint32_t e;
@@ -197,7 +215,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[3 * 16 + 4 * RING + 4 + 4 + 2 + 2 + 2];
   __shared__ Meta meta[META_STEPS][STEP_TILES];
-  __shared__ int s_null[16];
+  __shared__ int s_null[16], s_plain[META_STEPS * 2]; // of a half: nothing in its tiles' scales to look at
   __shared__ int s_dead, s_last;
   __shared__ uint32_t s_tmem;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -283,6 +301,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         for (int k = 0; k < KW; k++) x[e][k] = kp[e][k], x[e][KW + k] = vp[e][k];
       }
       if (!ok) break;
+      bool both = true;
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const int j0 = (t0 + i + e) * KV_TILE;
@@ -312,7 +331,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
           mt = Meta{scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[0])))),
                     scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[1])))), bad, null[e] ? 1 : 0};
         }
+        both = both && plain;
         if (lane == 0) meta[((i + e) / STEP_TILES) % META_STEPS][(i + e) % STEP_TILES] = mt;
+        if (e && lane == 0) s_plain[(i / 2) % (2 * META_STEPS)] = both;
         __syncwarp();
         if (lane == 0) mbar_arrive(raw_scanned + 8 * ((i + e) % P::SLOTS));
       }
@@ -414,37 +435,49 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     bool alive = halves > 0 && wait_for(q_ready + 8 * q, 0, dead) && wait_for(k_full, 0, dead) && wait_for(k_full + 8, 0, dead);
     const uint64_t qd = operand(base + P::Q0 + q * P::Q_TILE);
     const uint32_t s_acc = tmem + q * 128, o_acc = tmem + 256 + q * HD, sf = s_full + 16 * q, pf = p_full + 16 * q;
-    auto scores = [&](int h) { // of half h
-      const uint64_t kd = operand(base + P::K0 + (h % RING) * P::KV_HALF);
+    auto scores = [&](uint32_t buf, uint32_t k_at) {
+      const uint64_t kd = operand(base + P::K0 + k_at * P::KV_HALF);
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ks++)
-        mma_ss(s_acc + (h & 1) * HALF, qd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (K_PANEL / 16) + (ks & 3) * 2), instruction(HALF), ks ? 1u : 0u);
-      commit(sf + 8 * (h & 1));
-      commit(k_empty + 8 * (h % RING));
+        mma_ss(s_acc + buf * HALF, qd + (uint64_t)((ks >> 2) * (PANEL / 16) + (ks & 3) * 2), kd + (uint64_t)((ks >> 2) * (K_PANEL / 16) + (ks & 3) * 2), instruction(HALF), ks ? 1u : 0u);
+      commit(sf + 8 * buf);
+      commit(k_empty + 8 * k_at);
     };
     tc_fence_after();
     if (elect_one() && alive) {
-      scores(0);
-      scores(1);
+      scores(0, 0);
+      scores(1, 1);
     }
     __syncwarp();
+    // The three barriers of a half are looked at together: one after the other they took 220 cycles each when there was nothing to wait for, and the loop
+    // 2200 a half. v_at, k_at: places of half h's values and of half h + 2's keys in their rings; *_odd: the rings' laps.
+    uint32_t v_at = 0, v_odd = 0, k_at = 2, k_odd = 0, p_odd = 0;
     for (int h = 0; h < halves; h++) {
+      const uint32_t buf = h & 1;
       const bool more = h + 2 < halves;
-      if (alive) alive = wait_for(v_full + 8 * (h % RING), (h / RING) & 1, dead);
-      if (alive && more) alive = wait_for(k_full + 8 * ((h + 2) % RING), ((h + 2) / RING) & 1, dead);
-      const uint64_t vd = operand(base + P::V0 + (h % RING) * P::KV_HALF);
-      if (alive) alive = wait_for(pf + 8 * (h & 1), (h >> 1) & 1, dead);
+      const uint32_t pb = pf + 8 * buf, vb = v_full + 8 * v_at, kb = k_full + 8 * k_at;
+      const uint32_t v_ok = mbar_test(vb, v_odd), k_ok = more ? mbar_test(kb, k_odd) : 1u, p_ok = mbar_test(pb, p_odd);
+      if (!__all_sync(0xffffffffu, v_ok & k_ok & p_ok) && alive) {
+        alive = wait_for(vb, v_odd, dead);
+        if (alive && more) alive = wait_for(kb, k_odd, dead);
+        if (alive) alive = wait_for(pb, p_odd, dead);
+      }
       tc_fence_after();
       __syncwarp();
       if (elect_one() && alive) {
+        const uint64_t vd = operand(base + P::V0 + v_at * P::KV_HALF);
 #pragma unroll
-        for (int ks = 0; ks < HALF / 16; ks++) mma_ts(o_acc, s_acc + (h & 1) * HALF + ks * 8, vd + (uint64_t)(ks * 2), instruction(HD), h | ks ? 1u : 0u);
+        for (int ks = 0; ks < HALF / 16; ks++)
+          mma_ts(o_acc, s_acc + buf * HALF + ks * 8, vd + (uint64_t)(ks * 2), instruction(HD), h | ks ? 1u : 0u);
         commit(pv_done + 8 * q);
-        commit(v_empty + 8 * (h % RING));
-        if (more) scores(h + 2);
-        else if (h & 1) commit(o_done + 8 * q);
+        commit(v_empty + 8 * v_at);
+        if (more) scores(buf, k_at);
+        else if (buf) commit(o_done + 8 * q);
       }
       __syncwarp();
+      if (++v_at == RING) v_at = 0, v_odd ^= 1;
+      if (++k_at == RING) k_at = 0, k_odd ^= 1;
+      p_odd ^= buf;
     }
   } else if (warp < QT * 4) {
     // ---- a row a thread ----
@@ -498,7 +531,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     }
     float ref = -INFINITY, l = 0.f; // the reference: 4 below a maximum when it was set; none yet: -inf
     int v_ref = 0;                  // O holds the sums times 2^v_ref
-    bool alive = true;
+    bool alive = true, have_ref = false; // of all 32 rows
     int h2 = 0; // the half at hand
     // Rows with a score more than 2^12 over their reference (or that have none) get another: what they have summed is scaled, P of the half's first tile
     // included; o_by: O and P alone (the values' scales).
@@ -534,31 +567,28 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     // A half's scores to weights. Where every row sees every position, no scales are far off and no score is far over its row's reference, both tiles at once.
     auto weigh = [&](uint32_t (&s)[64]) {
       const uint32_t at = buffers + (h2 & 1) * HALF; // P takes the place of the first half of the scores
-      const Meta *mt2 = &meta[(h2 >> 1) % META_STEPS][(h2 & 1) * 2];
-      const Meta ma = mt2[0], mb = mt2[1];
       const int j0 = (t0 + h2 * 2) * KV_TILE;
-      bool general = (ma.gone | mb.gone | ma.k_shift | mb.k_shift | (ma.v_shift ^ v_ref) | (mb.v_shift ^ v_ref)) != 0 || (ma.bad | mb.bad) != 0u || j0 < lo_all ||
-                     j0 + HALF - 1 > hi_all || __any_sync(0xffffffffu, ref == -INFINITY);
+      bool general = !have_ref || v_ref != 0 || j0 < lo_all || j0 + HALF - 1 > hi_all || !s_plain[h2 % (2 * META_STEPS)];
       uint32_t pk[32];
+      tmem_ld_wait();
       if (!general) {
         float2 sum[4] = {};
-        __half2 most[2] = {__float2half2_rn(0.f), __float2half2_rn(0.f)};
 #pragma unroll
         for (int i = 0; i < 64; i += 2) {
           float2 p = fma2(s[i], s[i + 1], f, -ref);
           p.x = exp2_approx(p.x), p.y = exp2_approx(p.y);
           add2(sum[(i >> 1) & 3], p);
           pk[i / 2] = pack_half2(p.x, p.y);
-          most[(i >> 1) & 1] = __hmax2(most[(i >> 1) & 1], as_half2(pk[i / 2]));
         }
-        most[0] = __hmax2(most[0], most[1]);
-        general = __any_sync(0xffffffffu, fmaxf(__low2float(most[0]), __high2float(most[0])) > 4096.f); // (an overflow is infinite)
-        if (!general) l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+        const float add = ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+        general = __any_sync(0xffffffffu, !(add <= 4096.f)); // so is any weight that is, and sums below it are a few hundred
+        if (!general) l += add;
       }
       if (!general) {
         tmem_st32(at, pk);
         return;
       }
+      const Meta *mt2 = &meta[(h2 >> 1) % META_STEPS][(h2 & 1) * 2];
 #pragma unroll 1
       for (int c = 0; c < 2; c++) {
         const Meta mt = mt2[c];
@@ -587,6 +617,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
             const int v_new = min(mt.v_shift, v_ref);
             rescale(c, top, ldexpf(1.f, v_new - v_ref));
             v_ref = v_new;
+            have_ref = __all_sync(0xffffffffu, ref != -INFINITY);
           }
           const float from = ref == -INFINITY ? 0.f : ref, by = ldexpf(1.f, v_ref - mt.v_shift); // (scales that far from the others)
           float sum = 0.f;
@@ -607,7 +638,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       tc_fence_after();
       uint32_t x[64];
       tmem_ld64(buffers + (h2 & 1) * HALF, x);
-      tmem_ld_wait();
       weigh(x);
       tmem_st_wait();
       tc_fence_before();
