@@ -1,9 +1,15 @@
 // The quantized KV cache is written (quantized as it is stored, after an optional rotary embedding of q and k) and read back.
 //
-// Both kernels are bound by their bytes: one pass, each value read once and written once. A thread takes 8 consecutive dims of a PAIR of
-// positions (2 i, 2 i + 1) that share the words of V's codes, so a pair is stored in whole words; where only one of the two is new, the other
-// half of a word is left alone (2-byte stores). Four neighbouring threads hold a block of 32.
-#include "xnq_kv_cache.cuh"
+// Both kernels are bound by their bytes: one pass, each value read once and written once.
+//
+// Store: a thread takes 8 consecutive dims of a PAIR of positions (2 i, 2 i + 1) that share the words of V's codes, so a pair is stored in whole words;
+// where only one of the two is new, the other half of a word is left alone (2-byte stores). Four neighbouring threads hold a block of 32. A warp stays with
+// its pair (a query's position) and goes over heads, so that sequence, page and rotation are looked up once; few positions are shared by several
+// warps (`slices`). Read back: a warp takes a tile of a head, keys or values, in the order of its words. (A thread a unit of 8 dims, each with its own
+// divisions of 64-bit indexes: 8 x 4096 tokens with rotation and their read-back 354 us, read-back of 16 x 8192 positions 211 us.)
+#include <algorithm>
+
+#include "xnq_kv_attend.cuh"
 #include "xnq_quantize_act.cuh"
 
 namespace xnq {
@@ -38,6 +44,38 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16 *p, const fl
 #pragma unroll
   for (int i = 0; i < 4; i++) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
   *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(h);
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T *p, const float (&v)[4]);
+template <>
+__device__ __forceinline__ void store4<float>(float *p, const float (&v)[4]) {
+  *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+template <>
+__device__ __forceinline__ void store4<__half>(__half *p, const float (&v)[4]) {
+  const __half2 h[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
+  *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(h);
+}
+template <>
+__device__ __forceinline__ void store4<__nv_bfloat16>(__nv_bfloat16 *p, const float (&v)[4]) {
+  const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+  *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(h);
+}
+template <int N> // 1, 2 or 4 words at p, or 8 in two fours
+__device__ __forceinline__ void load_words(const uint8_t *p, const uint8_t *p2, uint32_t (&w)[N]) {
+  if (N == 1) w[0] = *reinterpret_cast<const uint32_t *>(p);
+  else if (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2 *>(p);
+    w[0] = x.x, w[N - 1] = x.y;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4 *>(p);
+    w[0] = x.x, w[1 % N] = x.y, w[2 % N] = x.z, w[3 % N] = x.w;
+    if (N == 8) {
+      const uint4 y = *reinterpret_cast<const uint4 *>(p2);
+      w[4 % N] = y.x, w[5 % N] = y.y, w[6 % N] = y.z, w[7 % N] = y.w;
+    }
+  }
 }
 
 // One block of 32 in four neighbouring lanes, 8 values each: the arithmetic of BlockQ4_0::from_float and BlockQ8_0::from_float
@@ -79,7 +117,7 @@ __device__ __forceinline__ Codes8 quantize8(const float (&v)[8]) {
   const float d = __fdiv_rn(mx, -8.0f), id = d != 0.f ? __fdiv_rn(1.0f, d) : 0.f;
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i++) w |= (uint32_t)min(max(__float2int_rz(__fadd_rn(__fmul_rn(v[i], id), 8.5f)), 0), 15) << (4 * i);
+  for (int i = 0; i < 8; i++) w |= min(__float2uint_rz(__fadd_rn(__fmul_rn(v[i], id), 8.5f)), 15u) << (4 * i); // (saturates below 0; NaN: 0)
   o.lo = w, o.hi = 0u, o.d = __float2half_rn(d);
   return o;
 }
@@ -89,212 +127,268 @@ __device__ __forceinline__ float rope_of(float x, float other, float c, float s,
 }
 // this thread's 8 values of a head rotated; its partner, half a head away, holds the other half of the pairs
 template <int HD>
-__device__ __forceinline__ void rope8(float (&v)[8], const RopeArgs &r, long long pos, int l, bool valid) {
-  const bool upper = l >= HD / 16;
-  float c[8], s[8];
+__device__ __forceinline__ void rope8(float (&v)[8], const float (&c)[8], const float (&s)[8], bool upper) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) v[i] = rope_of(v[i], __shfl_xor_sync(0xffffffffu, v[i], HD / 16), c[i], s[i], upper);
+}
+template <int HD>
+__device__ __forceinline__ void load_tables(const RopeArgs &r, long long pos, int l, bool valid, float (&c)[8], float (&s)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i++) c[i] = s[i] = 0.f;
-  if (valid) {
-    load8(r.cos + pos * (HD / 2) + (l & (HD / 16 - 1)) * 8, c);
-    load8(r.sin + pos * (HD / 2) + (l & (HD / 16 - 1)) * 8, s);
+  if (!valid) return;
+  load8(r.cos + pos * (HD / 2) + (l & (HD / 16 - 1)) * 8, c);
+  load8(r.sin + pos * (HD / 2) + (l & (HD / 16 - 1)) * 8, s);
+}
+
+struct StoreUnits { // warps: [0, kv) store keys and values, the rest rotate queries
+  unsigned kv, all, pairs, kv_slices, q_slices;
+};
+
+template <int BITS, int HD, typename T, bool ROPE>
+__global__ void __launch_bounds__(256) kv_store_kernel(KvView c, KvRows k, KvRows v, RopeArgs r, StoreUnits un, long long seq, const long long *pos_p, int pos_stride) {
+  using L = KvTile<BITS, HD>;
+  constexpr int LANES = HD / 8, ROWS = 32 / LANES; // threads of a head's row, rows of a warp
+  const int lane = threadIdx.x & 31, l = lane % LANES, sub = lane / LANES;
+  unsigned u = blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_launch_dependents();
+  pdl_wait();
+  if (u >= un.all) return;
+  if (ROPE && u >= un.kv) { // queries
+    u -= un.kv;
+    const unsigned bs = u / un.q_slices, slice = u - bs * un.q_slices, b = bs / (unsigned)seq, s = bs - b * (unsigned)seq;
+    const long long p = pos_p[(long long)b * pos_stride] + s;
+    const bool valid = p >= 0 && p < r.rows;
+    float cs[8], sn[8];
+    load_tables<HD>(r, p, l, valid, cs, sn);
+    const T *src = static_cast<const T *>(r.q.p) + b * r.q.sb + s * r.q.ss + l * 8;
+    const long long dst = b * r.q_out.sb + s * r.q_out.ss + l * 8;
+#pragma unroll 4
+    for (int base = slice * ROWS; base < r.heads; base += un.q_slices * ROWS) {
+      const int h = base + sub;
+      float x[8] = {};
+      if (valid && h < r.heads) load8(src + h * r.q.sh, x);
+      rope8<HD>(x, cs, sn, l >= HD / 16);
+      if (h >= r.heads) continue;
+      const long long at = dst + h * r.q_out.sh;
+      if (r.q_out_dtype == XNQ_F32) store8(static_cast<float *>(r.q_out.p) + at, x);
+      else if (r.q_out_dtype == XNQ_F16) store8(static_cast<__half *>(r.q_out.p) + at, x);
+      else store8(static_cast<__nv_bfloat16 *>(r.q_out.p) + at, x);
+    }
+    return;
   }
+  const unsigned bp = u / un.kv_slices, slice = u - bp * un.kv_slices, b = bp / un.pairs;
+  const long long first = pos_p[(long long)b * pos_stride], p0 = ((first >> 1) + (bp - b * un.pairs)) * 2, s0 = p0 - first; // the pair's even position and its token
+  bool has[2], past = false;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float other = __shfl_xor_sync(0xffffffffu, v[i], HD / 16);
-    v[i] = rope_of(v[i], other, c[i], s[i], upper);
+  for (int e = 0; e < 2; e++) {
+    const long long p = p0 + e, s = s0 + e;
+    has[e] = s >= 0 && s < seq && p >= 0;
+    if (has[e] && (p >= c.max_seq || (ROPE && p >= r.rows))) has[e] = false, past = true;
+  }
+  if (past && lane == 0) atomicOr(&g_kv_store_status, KV_PAST_STORE);
+  if (!has[0] && !has[1]) return;
+  uint8_t *tile0 = kv_tile_at(c, (int)b, 0, (int)(p0 / KV_TILE), L::BYTES); // head 0's
+  if (!tile0) {
+    if (lane == 0) atomicOr(&g_kv_store_status, KV_NO_PAGE);
+    return;
+  }
+  const int row = (int)p0 % KV_TILE, pair = row / 2, blk = l / 4, t = l % 4;
+  float cs[2][8], sn[2][8];
+  if (ROPE) load_tables<HD>(r, p0, l, has[0], cs[0], sn[0]), load_tables<HD>(r, p0 + 1, l, has[1], cs[1], sn[1]);
+  const T *const kp = static_cast<const T *>(k.p) + b * k.sb + s0 * k.ss + l * 8, *const vp = static_cast<const T *>(v.p) + b * v.sb + s0 * v.ss + l * 8;
+  auto row_of = [&](int x, float (&val)[2][8]) { // rows 0 .. KV - 1: keys, the next KV: values
+    const bool is_v = x >= c.kv_heads, in = x < 2 * c.kv_heads;
+    const T *p = is_v ? vp + (x - c.kv_heads) * v.sh : kp + x * k.sh;
+    const long long ss = is_v ? v.ss : k.ss;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) val[e][i] = 0.f;
+      if (in && has[e]) load8(p + e * ss, val[e]);
+    }
+  };
+  float next[2][8];
+  row_of(slice * ROWS + sub, next);
+  for (int base = slice * ROWS; base < 2 * c.kv_heads; base += un.kv_slices * ROWS) { // the next rows are on their way meanwhile
+    const int x = base + sub;
+    const bool is_v = x >= c.kv_heads;
+    float val[2][8];
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) val[e][i] = next[e][i];
+    if (base + un.kv_slices * ROWS < 2 * c.kv_heads) row_of(x + un.kv_slices * ROWS, next);
+    Codes8 q[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      if (ROPE) { // values keep theirs; the shuffles want every lane
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = val[e][i];
+        rope8<HD>(y, cs[e], sn[e], l >= HD / 16);
+#pragma unroll
+        for (int i = 0; i < 8; i++) val[e][i] = is_v ? val[e][i] : y[i];
+      }
+      q[e] = quantize8<BITS>(val[e]);
+    }
+    if (x >= 2 * c.kv_heads) continue;
+    uint8_t *tile = tile0 + (is_v ? x - c.kv_heads : x) * c.head_bytes;
+    if (!is_v) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        if (!has[e]) continue;
+        if (BITS == 4) *reinterpret_cast<uint32_t *>(tile + L::k_word(row + e, t, blk)) = q[e].lo;
+        else *reinterpret_cast<uint2 *>(tile + L::k_word(row + e, t, 2 * blk)) = make_uint2(q[e].lo, q[e].hi);
+        if (t == 0) *reinterpret_cast<__half *>(tile + L::k_scale(row + e, blk)) = q[e].d;
+      }
+      continue;
+    }
+    constexpr int G = BITS / 4; // words a granule of four dims takes
+#pragma unroll
+    for (int half = 0; half < 2; half++) { // dims 8 t + 4 half ..: chunk g = 2 t + half
+#pragma unroll
+      for (int j = 0; j < G; j++) {
+        uint32_t g[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const uint32_t w = BITS == 4 ? q[e].lo : (half ? q[e].hi : q[e].lo);
+          g[e] = (BITS == 4 ? w >> (16 * half) : w >> (16 * j)) & 0xffffu;
+        }
+        uint8_t *at = tile + L::v_word(pair, 2 * t + half, G * blk + j);
+        if (has[0] && has[1]) *reinterpret_cast<uint32_t *>(at) = g[0] | (g[1] << 16);
+        else *reinterpret_cast<uint16_t *>(at + (has[0] ? 0 : 2)) = (uint16_t)(has[0] ? g[0] : g[1]);
+      }
+    }
+    if (t == 0) {
+      __half *at = reinterpret_cast<__half *>(tile + L::v_scale(pair, blk));
+      if (has[0] && has[1]) *reinterpret_cast<__half2 *>(at) = __halves2half2(q[0].d, q[1].d);
+      else at[has[0] ? 0 : 1] = has[0] ? q[0].d : q[1].d;
+    }
   }
 }
 
-// Blocks [0, kv_blocks) store keys and values, the rest rotate queries. Whole warps work or leave together.
-template <int BITS, int HD, typename T, bool ROPE>
-__global__ void __launch_bounds__(256) kv_store_kernel(KvView c, KvRows k, KvRows v, RopeArgs r, long long batch, long long seq, const long long *pos_p, int pos_stride,
-                                                       long long kv_blocks) {
-  using L = KvTile<BITS, HD>;
-  constexpr int LANES = HD / 8; // threads of a head's row
-  pdl_launch_dependents();
-  pdl_wait();
-  const int l = threadIdx.x % LANES;
-  if (blockIdx.x >= kv_blocks) { // queries
-    const long long u = (long long)(blockIdx.x - kv_blocks) * (256 / LANES) + threadIdx.x / LANES; // row (b, s, head)
-    const bool in = u < batch * seq * r.heads;
-    const long long bs = in ? u / r.heads : 0, b = bs / seq, s = bs - b * seq;
-    const int h = in ? (int)(u - bs * r.heads) : 0;
-    const long long p = pos_p[b * pos_stride] + s;
-    const bool valid = in && p >= 0 && p < r.rows;
-    float x[8] = {};
-    if (valid) load8(static_cast<const T *>(r.q.p) + b * r.q.sb + s * r.q.ss + h * r.q.sh + l * 8, x);
-    rope8<HD>(x, r, p, l, valid);
-    const long long at = b * r.q_out.sb + s * r.q_out.ss + h * r.q_out.sh + l * 8;
-    if (!in) return;
-    if (r.q_out_dtype == XNQ_F32) store8(static_cast<float *>(r.q_out.p) + at, x);
-    else if (r.q_out_dtype == XNQ_F16) store8(static_cast<__half *>(r.q_out.p) + at, x);
-    else store8(static_cast<__nv_bfloat16 *>(r.q_out.p) + at, x);
-    return;
-  }
-  const long long pairs = seq / 2 + 1; // pairs that `seq` positions may touch
-  const long long u = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; // (b, pair, K or V, head)
-  const bool in = u < batch * pairs * 2 * c.kv_heads;
-  const long long bp = in ? u / (2 * c.kv_heads) : 0, b = bp / pairs;
-  const int kh = in ? (int)(u - bp * (2 * c.kv_heads)) : 0;
-  const bool is_v = kh >= c.kv_heads;
-  const int head = is_v ? kh - c.kv_heads : kh;
-  const long long first = pos_p[b * pos_stride];
-  const long long p0 = ((first >> 1) + (bp - b * pairs)) * 2; // the pair's even position
-  const KvRows &x = is_v ? v : k;
-  bool has[2];
-  float val[2][8];
-#pragma unroll
-  for (int e = 0; e < 2; e++) {
-    const long long p = p0 + e, s = p - first;
-    has[e] = in && s >= 0 && s < seq && p >= 0;
-    if (has[e] && (p >= c.max_seq || (ROPE && p >= r.rows))) {
-      has[e] = false;
-      if (l == 0) atomicOr(&g_kv_store_status, KV_PAST_STORE);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) val[e][i] = 0.f;
-    if (has[e]) load8(static_cast<const T *>(x.p) + b * x.sb + s * x.ss + head * x.sh + l * 8, val[e]);
-  }
-  Codes8 q[2];
-#pragma unroll
-  for (int e = 0; e < 2; e++) {
-    if (ROPE) { // values keep theirs; the shuffles want every lane
-      float t[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) t[i] = val[e][i];
-      rope8<HD>(t, r, p0 + e, l, has[e]);
-#pragma unroll
-      for (int i = 0; i < 8; i++) val[e][i] = is_v ? val[e][i] : t[i];
-    }
-    q[e] = quantize8<BITS>(val[e]);
-  }
-  if (!has[0] && !has[1]) return;
-  uint8_t *tile = kv_tile_at(c, (int)b, head, (int)(p0 / KV_TILE), L::BYTES);
-  if (!tile) {
-    if (l == 0) atomicOr(&g_kv_store_status, KV_NO_PAGE);
-    return;
-  }
-  const int row = (int)(p0 % KV_TILE), pair = row / 2, blk = l / 4, t = l % 4;
-  if (!is_v) {
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      if (!has[e]) continue;
-      if (BITS == 4) *reinterpret_cast<uint32_t *>(tile + L::k_word(row + e, t, blk)) = q[e].lo;
-      else *reinterpret_cast<uint2 *>(tile + L::k_word(row + e, t, 2 * blk)) = make_uint2(q[e].lo, q[e].hi);
-      if (t == 0) *reinterpret_cast<__half *>(tile + L::k_scale(row + e, blk)) = q[e].d;
-    }
-    return;
-  }
-  constexpr int G = BITS / 4; // words a granule of four dims takes
-#pragma unroll
-  for (int half = 0; half < 2; half++) { // dims 8 t + 4 half ..: chunk g = 2 t + half
-#pragma unroll
-    for (int j = 0; j < G; j++) {
-      uint32_t g[2];
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const uint32_t w = BITS == 4 ? q[e].lo : (half ? q[e].hi : q[e].lo);
-        g[e] = (BITS == 4 ? w >> (16 * half) : w >> (16 * j)) & 0xffffu;
-      }
-      uint8_t *at = tile + L::v_word(pair, 2 * t + half, G * blk + j);
-      if (has[0] && has[1]) *reinterpret_cast<uint32_t *>(at) = g[0] | (g[1] << 16);
-      else *reinterpret_cast<uint16_t *>(at + (has[0] ? 0 : 2)) = (uint16_t)(has[0] ? g[0] : g[1]);
-    }
-  }
-  if (t == 0) {
-    __half *at = reinterpret_cast<__half *>(tile + L::v_scale(pair, blk));
-#pragma unroll
-    for (int e = 0; e < 2; e++)
-      if (has[e]) at[e] = q[e].d;
-  }
+__device__ __forceinline__ float2 pair_values(uint32_t codes, __half2 d) { // two codes as whole numbers in f16, two scales: the exact products
+  const float2 c = __half22float2(as_half2(codes)), s = __half22float2(d);
+  return make_float2(c.x * s.x, c.y * s.y);
 }
 
 // k_out, v_out [batch, kv_heads, n, head_dim]: positions start .. start + n - 1. Positions outside [0, max_seq) or without a page: zeros.
 template <int BITS, int HD, typename T>
-__global__ void __launch_bounds__(256) kv_load_kernel(KvView c, T *k_out, T *v_out, long long batch, long long n, const long long *start_p, int start_stride,
+__global__ void __launch_bounds__(256) kv_load_kernel(KvView c, T *k_out, T *v_out, unsigned units, unsigned tiles, long long n, const long long *start_p, int start_stride,
                                                       long long start0) {
   using L = KvTile<BITS, HD>;
-  constexpr int LANES = HD / 8;
+  constexpr int NB = L::NB, W = L::W;
+  const int lane = threadIdx.x & 31;
+  const unsigned u = blockIdx.x * 8 + (threadIdx.x >> 5); // (b, head, K or V, tile)
   pdl_launch_dependents();
   pdl_wait();
-  const int l = threadIdx.x % LANES, blk = l / 4, t = l % 4;
-  const long long pairs = n / 2 + 1;
-  const long long u = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; // (b, K or V, head, pair)
-  if (u >= batch * 2 * c.kv_heads * pairs) return;
-  const long long bk = u / pairs, b = bk / (2 * c.kv_heads);
-  const int kh = (int)(bk - b * (2 * c.kv_heads));
-  const bool is_v = kh >= c.kv_heads;
-  const int head = is_v ? kh - c.kv_heads : kh;
-  const long long first = start_p ? start_p[b * start_stride] : start0;
-  const long long p0 = ((first >> 1) + (u - bk * pairs)) * 2;
-  T *out = (is_v ? v_out : k_out) + (b * c.kv_heads + head) * n * HD + l * 8;
-  uint8_t *tile = nullptr;
-  if (p0 >= 0 && p0 < c.max_seq) {
-    tile = kv_tile_at(c, (int)b, head, (int)(p0 / KV_TILE), L::BYTES);
-    if (!tile && l == 0) atomicOr(&g_kv_store_status, KV_NO_PAGE);
+  if (u >= units) return;
+  const unsigned bh = u / tiles, b = bh / (2 * c.kv_heads);
+  const int kh = (int)(bh - b * (2 * c.kv_heads)), head = kh >> 1;
+  const long long first = start_p ? start_p[(long long)b * start_stride] : start0;
+  const long long tile_i = (first >> 5) + (u - bh * tiles), j0 = tile_i * KV_TILE; // positions j0 .. j0 + 31, of which [lo, hi) are asked for
+  static_assert(KV_TILE == 32, "a shift");
+  const int lo = (int)max(first - j0, 0ll), hi = (int)min(first + n - j0, (long long)KV_TILE);
+  if (lo >= hi) return;
+  const int there = (int)min(max(c.max_seq - j0, 0ll), (long long)KV_TILE); // positions of the tile that the cache has
+  const uint8_t *tile = j0 >= 0 && there > 0 ? kv_tile_at(c, (int)b, head, (int)tile_i, L::BYTES) : nullptr;
+  if (lane == 0) {
+    if (j0 >= 0 && there < hi) atomicOr(&g_kv_store_status, KV_PAST_STORE);
+    if (j0 >= 0 && there > 0 && !tile) atomicOr(&g_kv_store_status, KV_NO_PAGE);
   }
-  const int row = (int)(p0 % KV_TILE), pair = row / 2;
-  uint32_t w[2][2] = {}; // [position][lo, hi]: codes as the quantizer made them
-  float d[2] = {};
-  if (tile) {
-    if (!is_v) {
+  T *const out = (kh & 1 ? v_out : k_out) + (((long long)b * c.kv_heads + head) * n + (j0 - first)) * HD;
+  if (!(kh & 1)) { // keys: a lane takes the chunk of 8 dims of every block of a row
+#pragma unroll
+    for (int it = 0; it < 4; it++) {
+      const int row = it * 8 + lane / 4, t = lane % 4;
+      if (row < lo || row >= hi) continue;
+      const bool ok = tile && row < there;
+      uint32_t w[W], d[NB / 2];
+#pragma unroll
+      for (int i = 0; i < W; i++) w[i] = 0u;
+#pragma unroll
+      for (int i = 0; i < NB / 2; i++) d[i] = 0u;
+      if (ok) {
+        load_words<W>(tile + L::k_word(row, t, 0), W == 8 ? tile + L::k_word(row, t, 4) : nullptr, w);
+        load_words<NB / 2>(tile + L::k_scale(row, 0), nullptr, d);
+      }
+#pragma unroll
+      for (int bl = 0; bl < NB; bl++) {
+        const __half2 d2 = bl & 1 ? __high2half2(as_half2(d[bl / 2])) : __low2half2(as_half2(d[bl / 2]));
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) { // dims (i, i + 4), or (0, 2), (1, 3), (4, 6), (5, 7)
+          const float2 x = pair_values(signed_pair<BITS>(BITS == 4 ? w[bl] : w[2 * bl + i / 2], BITS == 4 ? i : i & 1), d2);
+          const int y = BITS == 4 ? i : (i >> 1) * 4 + (i & 1), z = BITS == 4 ? i + 4 : y + 2;
+          v[y] = x.x, v[z] = x.y;
+        }
+        store8(out + (long long)row * HD + bl * 32 + t * 8, v);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int it = 0; it < 4; it++) { // values: a lane takes the chunk of 4 dims of every block of a pair of positions
+    const int pair = it * 4 + lane / 8, g = lane % 8;
+    if (2 * pair + 1 < lo || 2 * pair >= hi) continue;
+    uint32_t w[W], d[NB];
+#pragma unroll
+    for (int i = 0; i < W; i++) w[i] = 0u;
+#pragma unroll
+    for (int i = 0; i < NB; i++) d[i] = 0u;
+    if (tile && 2 * pair < there) {
+      load_words<W>(tile + L::v_word(pair, g, 0), W == 8 ? tile + L::v_word(pair, g, 4) : nullptr, w);
+      load_words<NB>(tile + L::v_scale(pair, 0), nullptr, d);
+    }
+    const bool odd = 2 * pair + 1 < there;
+#pragma unroll
+    for (int bl = 0; bl < NB; bl++) {
+      float v[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float2 x = pair_values(signed_pair<BITS>(BITS == 4 ? w[bl] : w[2 * bl + i / 2], BITS == 4 ? i : i & 1), as_half2(d[bl]));
+        v[0][i] = x.x, v[1][i] = odd ? x.y : 0.f;
+      }
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        if (BITS == 4) w[e][0] = *reinterpret_cast<const uint32_t *>(tile + L::k_word(row + e, t, blk));
-        else {
-          const uint2 x = *reinterpret_cast<const uint2 *>(tile + L::k_word(row + e, t, 2 * blk));
-          w[e][0] = x.x, w[e][1] = x.y;
-        }
-        d[e] = __half2float(*reinterpret_cast<const __half *>(tile + L::k_scale(row + e, blk)));
+        const int row = 2 * pair + e;
+        if (row >= lo && row < hi) store4(out + (long long)row * HD + bl * 32 + g * 4, v[e]);
       }
-    } else {
-      constexpr int G = BITS / 4;
-#pragma unroll
-      for (int half = 0; half < 2; half++)
-#pragma unroll
-        for (int j = 0; j < G; j++) {
-          const uint32_t x = *reinterpret_cast<const uint32_t *>(tile + L::v_word(pair, 2 * t + half, G * blk + j));
-          const int at = BITS == 4 ? 0 : half, sh = BITS == 4 ? 16 * half : 16 * j;
-          w[0][at] |= (x & 0xffffu) << sh, w[1][at] |= (x >> 16) << sh;
-        }
-      const __half2 s = *reinterpret_cast<const __half2 *>(tile + L::v_scale(pair, blk));
-      d[0] = __low2float(s), d[1] = __high2float(s);
     }
-  }
-#pragma unroll
-  for (int e = 0; e < 2; e++) {
-    const long long p = p0 + e, s = p - first;
-    if (s < 0 || s >= n) continue;
-    const bool ok = tile && p < c.max_seq;
-    if (!ok && p >= c.max_seq && l == 0) atomicOr(&g_kv_store_status, KV_PAST_STORE);
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int code = BITS == 4 ? (int)(w[e][0] >> (4 * i)) & 15 : (int)(w[e][i / 4] >> (8 * (i % 4))) & 255;
-      v[i] = ok ? d[e] * (float)(code - L::ZERO) : 0.f;
-    }
-    store8(out + s * HD, v);
   }
 }
 
+// Warps that share a position's rows: as many as it takes to fill the GPU (148 SMs of 32 warps), a row group each at most.
+unsigned slices_for(int64_t positions, int64_t groups) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(groups, 4736 / std::max<int64_t>(positions, 1))); }
+
 template <int BITS, int HD, typename T>
 int run_store(const KvView &c, const KvRows &k, const KvRows &v, const RopeArgs &r, int64_t batch, int64_t seq, const long long *pos, int pos_stride, cudaStream_t s) {
-  const int64_t rows_per_block = 256 / (HD / 8);
-  const int64_t kv = (batch * (seq / 2 + 1) * 2 * c.kv_heads + rows_per_block - 1) / rows_per_block;
-  const int64_t q = r.cos && r.q.p ? (batch * seq * r.heads + rows_per_block - 1) / rows_per_block : 0;
-  if (kv + q > INT32_MAX) return fail(XNQ_ERR_SIZE, "kv_store: %lld x %lld tokens are more than one launch takes", (long long)batch, (long long)seq);
-  const dim3 grid((unsigned)(kv + q)), block(256);
-  if (r.cos) XNQ_CUDA(launch_pdl(kv_store_kernel<BITS, HD, T, true>, grid, block, 0, s, c, k, v, r, batch, seq, pos, pos_stride, kv));
-  else XNQ_CUDA(launch_pdl(kv_store_kernel<BITS, HD, T, false>, grid, block, 0, s, c, k, v, r, batch, seq, pos, pos_stride, kv));
+  constexpr int ROWS = 32 / (HD / 8);
+  const int64_t pairs = seq / 2 + 1; // that `seq` positions may touch
+  StoreUnits un{};
+  un.pairs = (unsigned)pairs;
+  un.kv_slices = slices_for(batch * pairs, (2 * c.kv_heads + ROWS - 1) / ROWS);
+  const int64_t kv = batch * pairs * un.kv_slices;
+  int64_t all = kv;
+  if (r.cos && r.q.p) {
+    un.q_slices = slices_for(batch * seq, (r.heads + ROWS - 1) / ROWS);
+    all += batch * seq * un.q_slices;
+  }
+  if (all > INT32_MAX) return fail(XNQ_ERR_SIZE, "kv_store: %lld x %lld tokens are more than one launch takes", (long long)batch, (long long)seq);
+  un.kv = (unsigned)kv, un.all = (unsigned)all;
+  const dim3 grid((unsigned)((all + 7) / 8)), block(256);
+  if (r.cos) XNQ_CUDA(launch_pdl(kv_store_kernel<BITS, HD, T, true>, grid, block, 0, s, c, k, v, r, un, seq, pos, pos_stride));
+  else XNQ_CUDA(launch_pdl(kv_store_kernel<BITS, HD, T, false>, grid, block, 0, s, c, k, v, r, un, seq, pos, pos_stride));
   count_launch();
   return XNQ_OK;
 }
 template <int BITS, int HD, typename T>
 int run_load(const KvView &c, void *k, void *v, int64_t batch, int64_t n, const long long *start, int start_stride, int64_t start0, cudaStream_t s) {
-  const int64_t rows_per_block = 256 / (HD / 8);
-  const int64_t blocks = (batch * 2 * c.kv_heads * (n / 2 + 1) + rows_per_block - 1) / rows_per_block;
-  if (blocks > INT32_MAX) return fail(XNQ_ERR_SIZE, "kv_load: %lld x %lld positions are more than one launch takes", (long long)batch, (long long)n);
-  XNQ_CUDA(launch_pdl(kv_load_kernel<BITS, HD, T>, dim3((unsigned)blocks), dim3(256), 0, s, c, static_cast<T *>(k), static_cast<T *>(v), batch, n, start, start_stride, start0));
+  const int64_t tiles = start || start0 % KV_TILE ? (n + KV_TILE - 2) / KV_TILE + 1 : (n + KV_TILE - 1) / KV_TILE; // that n positions may touch
+  const int64_t units = batch * 2 * c.kv_heads * tiles;
+  if (units > INT32_MAX) return fail(XNQ_ERR_SIZE, "kv_load: %lld x %lld positions are more than one launch takes", (long long)batch, (long long)n);
+  XNQ_CUDA(launch_pdl(kv_load_kernel<BITS, HD, T>, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, s, c, static_cast<T *>(k), static_cast<T *>(v), (unsigned)units, (unsigned)tiles, n,
+                      start, start_stride, start0));
   count_launch();
   return XNQ_OK;
 }
