@@ -9,7 +9,7 @@
 // (O) by 8 query rows; scales meet the f32 sums (keys) or the weights (values). Bound by the cache's bytes, if unpacking stays cheap: a tile's 32
 // positions are 4608 bytes, which an SM gets in 200 cycles. So no code is converted: masked out of its word, a nibble or byte in the low ten
 // bits of a half is the f16 SUBNORMAL c 2^-24 (bits 4..7: 16 c 2^-24, the 16 undone in q or in the result), exact in the product; one shift and four masks a
-// word of eight 4-bit codes. The -z term comes from the sums' start value (S) or from one product of the weights with ones (O).
+// word of eight 4-bit codes. The -z term comes from the sums' start value (S) or from one more product, of the weights with -z (O).
 //
 // The rows of a KV head's query heads (and of a few tokens) are the 8 NT columns of a tile; a wider group takes several row tiles. The work is the
 // flattened list of (sequence, KV head, row tile, tile of 32 positions), cut into equal runs, one a CTA, so that ragged batches balance. The four
@@ -20,7 +20,8 @@
 // f32 queries (SPLIT): q and the weights are taken apart into two f16 each (22 bits), and the codes have their zero taken off first and are whole numbers in
 // f16: a subnormal operand's products are summed with the bits that a number of 2^-14 would have, some 2^-18 of the score (an output's error 3e-6 of its
 // norm with 4-bit codes; 5e-7 now, as much as f32 products), and with many weights the two sums in O would cancel. 16-bit queries: q is exact in f16 after a power of two a row, the weights are rounded to f16.
-// Ranges: p is held within 2^12 (rescaled when a maximum grows by more than 2^4), the values' scales are brought near one by a power of two a warp.
+// Ranges: a row's reference lies 8 below its maximum of the time and is renewed when a score passes it by more than 12, so that nothing need be known
+// of a tile's maximum beforehand; the values' scales are brought near one by a power of two a warp.
 #include <algorithm>
 #include <cmath>
 
@@ -325,17 +326,14 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
     }
 
     // ---- this warp's tiles ----
-    float acc[NT][2 * NB][4], zsum[SPLIT ? 1 : NT][4], m[NT][2], ref[NT][2], l[NT][2];
+    float acc[NT][2 * NB][4], ref[NT][2], limit[NT][2], l[NT][2]; // limit: a score above it asks for another reference
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
       for (int i = 0; i < 2 * NB; i++)
 #pragma unroll
         for (int c = 0; c < 4; c++) acc[n][i][c] = 0.f;
-      if (!SPLIT)
-#pragma unroll
-        for (int c = 0; c < 4; c++) zsum[n][c] = 0.f;
-      m[n][0] = m[n][1] = -INFINITY, ref[n][0] = ref[n][1] = 0.f, l[n][0] = l[n][1] = 0.f;
+      ref[n][0] = ref[n][1] = 0.f, limit[n][0] = limit[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
     }
     int k = 0;                 // the values' scales are taken times 2^k
     bool k_set = false;
@@ -377,7 +375,12 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
             }
           }
 #pragma unroll
-          for (int q2 = 0; q2 < NB / 2; q2++) dk[e][q2] = *reinterpret_cast<const uint32_t *>(tile + L::k_scale(row, 2 * q2));
+          for (int q2 = 0; q2 < NB / 2; q2 += 2) {
+            if (NB == 4) {
+              const uint2 x = *reinterpret_cast<const uint2 *>(tile + L::k_scale(row, 0));
+              dk[e][0] = x.x, dk[e][NB / 2 - 1] = x.y;
+            } else dk[e][0] = *reinterpret_cast<const uint32_t *>(tile + L::k_scale(row, 0));
+          }
         }
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -411,7 +414,6 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
       }
       // the values' scales: half2 of a pair of positions [group][pair t or t + 4][block]
       uint32_t dv[2][2][NB];
-      __half2 d_top = __float2half2_rn(0.f);
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -457,44 +459,6 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
             }
         }
       }
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-          for (int bl = 0; bl < NB; bl++) d_top = __hmax2(d_top, __habs2(as_half2(dv[u][e][bl])));
-      const float d_max = fmaxf(__low2float(d_top), __high2float(d_top));
-      if (__any_sync(0xffffffffu, d_max > d_most || !k_set)) {
-        float top = d_max;
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int k_new = scale_shift(top);
-        if (top > 0.f) {
-          const float by = k_set ? ldexpf(1.f, k_new - k) : 0.f;
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-#pragma unroll
-            for (int x = 0; x < 2 * NB; x++)
-#pragma unroll
-              for (int c = 0; c < 4; c++) acc[n][x][c] *= by;
-            if (!SPLIT)
-#pragma unroll
-              for (int c = 0; c < 4; c++) zsum[n][c] *= by;
-          }
-          k = k_new, k_set = true, d_most = ldexpf(4.f, -k);
-        }
-      }
-      if (k != 0) {
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int e = 0; e < 2; e++)
-#pragma unroll
-            for (int bl = 0; bl < NB; bl++) dv[u][e][bl] = raise_pair(dv[u][e][bl], k);
-      }
-      // softmax
-      bool grew = false;
-      float top[NT][2];
       if (masked) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -506,29 +470,67 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
               if (j < lo[n][c & 1] || j > hi[n][c & 1]) s[u][n][c] = -INFINITY;
             }
       }
+      // One vote a tile: a score over its limit, or (where scales are taken as they are) a scale of two or more, seen in the union of the bits
+      bool look = k != 0 || !k_set;
+      {
+        uint32_t bits = 0;
 #pragma unroll
-      for (int n = 0; n < NT; n++) {
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int bl = 0; bl < NB; bl++) bits |= dv[u][e][bl];
+        look |= (bits & 0x40004000u) != 0;
+      }
+      float top[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          float x = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
-#pragma unroll
-          for (int o = 4; o <= 16; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-          top[n][c] = fmaxf(m[n][c], x == -INFINITY ? x : x * factor[n][c]);
-          grew |= top[n][c] > ref[n][c] + 12.f || (m[n][c] == -INFINITY && top[n][c] != -INFINITY); // the reference lies 8 below a maximum
+          const float x = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
+          top[n][c] = x == -INFINITY ? x : x * factor[n][c];
+          look |= top[n][c] > limit[n][c];
         }
-      }
-      if (__any_sync(0xffffffffu, grew)) {
+      if (__any_sync(0xffffffffu, look)) {
+        __half2 d_top = __float2half2_rn(0.f);
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int bl = 0; bl < NB; bl++) d_top = __hmax2(d_top, __habs2(as_half2(dv[u][e][bl])));
+        float d_max = fmaxf(__low2float(d_top), __high2float(d_top)), o_by = 1.f;
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) d_max = fmaxf(d_max, __shfl_xor_sync(0xffffffffu, d_max, o));
+        if (d_max > 0.f && (d_max > d_most || !k_set)) {
+          const int k_new = scale_shift(d_max);
+          o_by = k_set ? ldexpf(1.f, k_new - k) : 0.f;
+          k = k_new, k_set = true, d_most = ldexpf(4.f, -k);
+        }
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int c = 0; c < 2; c++) {
-            const float r2 = top[n][c] == -INFINITY ? 0.f : top[n][c] - 8.f;
-            const float by = m[n][c] == -INFINITY ? 0.f : exp2_approx(ref[n][c] - r2);
-            m[n][c] = top[n][c], ref[n][c] = r2, l[n][c] *= by;
 #pragma unroll
-            for (int x = 0; x < 2 * NB; x++) acc[n][x][c] *= by, acc[n][x][c + 2] *= by;
-            if (!SPLIT) zsum[SPLIT ? 0 : n][c] *= by, zsum[SPLIT ? 0 : n][c + 2] *= by;
+            for (int o = 4; o <= 16; o <<= 1) top[n][c] = fmaxf(top[n][c], __shfl_xor_sync(0xffffffffu, top[n][c], o));
+            float by = 1.f;
+            if (top[n][c] > limit[n][c]) {
+              const float to = top[n][c] - 8.f;
+              by = limit[n][c] == -INFINITY ? 0.f : exp2_approx(ref[n][c] - to);
+              ref[n][c] = to, limit[n][c] = to + 12.f, l[n][c] *= by;
+            }
+            const float a_by = by * o_by;
+#pragma unroll
+            for (int x = 0; x < 2 * NB; x++) acc[n][x][c] *= a_by, acc[n][x][c + 2] *= a_by;
           }
+      }
+      if (k != 0) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int bl = 0; bl < NB; bl++) dv[u][e][bl] = raise_pair(dv[u][e][bl], k);
       }
       uint32_t ph[2][NT][2], pl[2][SPLIT ? NT : 1][2]; // weights of positions (2 t, 2 t + 1), (+ 8) of the group, query row g
 #pragma unroll
@@ -544,6 +546,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
             if (SPLIT) pl[u][SPLIT ? n : 0][e] = transpose8x8(pack_half2(p0 - __low2float(as_half2(h2)), p1 - __high2float(as_half2(h2))));
           }
       // values
+      const uint32_t z0 = BITS == 4 ? 0x80088008u : 0x80808080u, z1 = 0x80808080u, minus_zero[4] = {z0, z1, z0, z1}; // -z of an operand's even and odd dims
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         uint32_t w[2][W];
@@ -592,12 +595,8 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
 #pragma unroll
             for (int half = 0; half < 2; half++) {
               mma(acc[n][2 * bl + half], op[half], bh[0], bh[1]);
+              if (!SPLIT) mma(acc[n][2 * bl + half], minus_zero, bh[0], bh[1]);
               if (SPLIT) mma(acc[n][2 * bl + half], op[half], bl2[0], bl2[1]);
-            }
-            if (!SPLIT) { // row bl of one more product: the block's sum of weights
-              const uint32_t one = g == bl ? 0x3c003c00u : 0u;
-              const uint32_t ones[4] = {one, 0u, one, 0u};
-              mma(zsum[SPLIT ? 0 : n], ones, bh[0], bh[1]);
             }
           }
         }
@@ -616,7 +615,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
         float sum = l[n][c];
 #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (g == 0) s_m[warp * R + col] = m[n][c] == -INFINITY ? -INFINITY : ref[n][c], s_l[warp * R + col] = sum;
+        if (g == 0) s_m[warp * R + col] = limit[n][c] == -INFINITY ? -INFINITY : ref[n][c], s_l[warp * R + col] = sum;
         const float down = ldexpf(1.f, -k);
 #pragma unroll
         for (int bl = 0; bl < NB; bl++) {
@@ -624,8 +623,8 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
           const float *x = acc[n][2 * bl], *y = acc[n][2 * bl + 1];
           if (SPLIT) v = make_float4(x[c] * down, x[c + 2] * down, y[c] * down, y[c + 2] * down);
           else { // codes came as c 2^-24, those of the odd dims 16 times as much with 4 bits
-            const float z = __shfl_sync(0xffffffffu, zsum[SPLIT ? 0 : n][c], bl * 4 + t) * (float)L::ZERO, one = 16777216.f, odd = BITS == 4 ? 1048576.f : 16777216.f;
-            v = make_float4((x[c] * one - z) * down, (x[c + 2] * odd - z) * down, (y[c] * one - z) * down, (y[c + 2] * odd - z) * down);
+            const float one = 16777216.f * down, odd = BITS == 4 ? 1048576.f * down : one;
+            v = make_float4(x[c] * one, x[c + 2] * odd, y[c] * one, y[c + 2] * odd);
           }
           *reinterpret_cast<float4 *>(s_acc + (warp * R + col) * P::COL + bl * 32 + g * 4) = v;
         }
