@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
   __shared__ long long s_sum[SPLIT_WARPS];
   __shared__ long long s_before;
   __shared__ int s_b, s_last;
+  __shared__ Span s_span;
+  __shared__ unsigned s_runs[4][SPLIT_WARPS];
   __shared__ long long s_row[R], s_lse_row[R]; // where an item's rows go
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float *const merge = reinterpret_cast<float *>(smem + SPLIT_WARPS * SPLIT_STAGES * L::BYTES);
@@ -163,40 +165,74 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
   // ---- this CTA's run of the flattened list: [t0, t1) of `total` tiles ----
   const int per_seq = a.c.kv_heads * a.row_tiles; // items of a sequence, all of its count of tiles
   const int batch = (int)a.batch;
-  const int some = threadIdx.x < batch ? span_of(a, threadIdx.x).count : 0; // (most batches: the one look at the positions)
-  long long mine = some;
-  for (int b = threadIdx.x + SPLIT_WARPS * 32; b < batch; b += SPLIT_WARPS * 32) mine += span_of(a, b).count;
+  Span own{0, 0, 0}; // (most batches: the one look at the positions)
+  if ((int)threadIdx.x < batch) own = span_of(a, threadIdx.x);
+  long long mine = own.count;
+  bool look = (int)threadIdx.x < batch && (own.count == 0 || own.pos + a.seq > a.c.max_seq); // a sequence that sees nothing, or that lies past the cache
+  for (int b = threadIdx.x + SPLIT_WARPS * 32; b < batch; b += SPLIT_WARPS * 32) {
+    const Span sp = span_of(a, b);
+    mine += sp.count, look |= sp.count == 0 || sp.pos + a.seq > a.c.max_seq;
+  }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) s_sum[warp] = mine;
-  __syncthreads();
+  look = __syncthreads_or(look);
   long long total = 0;
 #pragma unroll
   for (int w = 0; w < SPLIT_WARPS; w++) total += s_sum[w];
   total *= per_seq;
   // Short items go to CTAs of their own: a run shorter than a tile a warp only where the items are shorter too.
   const long long items = (long long)batch * per_seq, at_least = min((long long)SPLIT_WARPS, max(total / items, 1ll));
-  const long long share = max((total + gridDim.x - 1) / gridDim.x, at_least);
-  const long long t0 = blockIdx.x * share, t1 = min(total, t0 + share);
-
-  // sequences that see nothing: rows of zeros
-  for (int b = blockIdx.x; b < batch; b += gridDim.x) {
-    const Span sp = span_of(a, b);
-    if (threadIdx.x == 0 && sp.pos + a.seq > a.c.max_seq) atomicOr(&g_kv_attend_status, KV_PAST_ATTEND);
-    if (sp.count) continue;
-    for (long long i = threadIdx.x; i < a.seq * a.heads * HD; i += SPLIT_WARPS * 32) {
-      const long long row = i / HD, s = row / a.heads;
-      const int h = (int)(row - s * a.heads), d = (int)(i - row * HD);
-      store_any(a.out.p, a.dtype, b * a.out.sb + s * a.out.ss + h * a.out.sh + d, 0.f);
-      if (a.lse && d == 0) a.lse[(b * a.seq + s) * a.heads + h] = -INFINITY;
+  long long share = max((total + gridDim.x - 1) / gridDim.x, at_least);
+  // A run that goes on into a second item pays for another start and end, about as long as 15 tiles take: where a run of a few more tiles keeps every
+  // CTA within one item, the items are rounded up to whole runs.
+  bool whole_runs = false;
+  {
+    const long long more[4] = {share, share + max(share / 8, 1ll), share + max(share / 4, 2ll), share + max(share / 2, 3ll)};
+    unsigned runs[4] = {0u, 0u, 0u, 0u};
+    if (share <= 24) {
+      for (int b = threadIdx.x; b < batch; b += SPLIT_WARPS * 32) {
+        const unsigned n = (unsigned)(b == (int)threadIdx.x ? own.count : span_of(a, b).count);
+#pragma unroll
+        for (int k = 0; k < 4; k++) runs[k] += (n + (unsigned)more[k] - 1) / (unsigned)more[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) runs[k] = __reduce_add_sync(0xffffffffu, runs[k]);
+      if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < 4; k++) s_runs[k][warp] = runs[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 3; k >= 0; k--) {
+        unsigned long long sum = 0;
+#pragma unroll
+        for (int w = 0; w < SPLIT_WARPS; w++) sum += s_runs[k][w];
+        if (sum * per_seq <= gridDim.x) share = more[k], whole_runs = true, total = sum * per_seq * more[k];
+      }
     }
   }
+  auto length = [&](int count) { return whole_runs ? (count + share - 1) / share * share : (long long)count; }; // of an item in the list
+  const long long t0 = blockIdx.x * share, t1 = min(total, t0 + share);
+
+  if (look) // sequences that see nothing: rows of zeros
+    for (int b = blockIdx.x; b < batch; b += gridDim.x) {
+      const Span sp = span_of(a, b);
+      if (threadIdx.x == 0 && sp.pos + a.seq > a.c.max_seq) atomicOr(&g_kv_attend_status, KV_PAST_ATTEND);
+      if (sp.count) continue;
+      for (long long i = threadIdx.x; i < a.seq * a.heads * HD; i += SPLIT_WARPS * 32) {
+        const long long row = i / HD, s = row / a.heads;
+        const int h = (int)(row - s * a.heads), d = (int)(i - row * HD);
+        store_any(a.out.p, a.dtype, b * a.out.sb + s * a.out.ss + h * a.out.sh + d, 0.f);
+        if (a.lse && d == 0) a.lse[(b * a.seq + s) * a.heads + h] = -INFINITY;
+      }
+    }
   if (t0 >= t1) return;
-  // the sequence of tile t0: a scan of the counts, a block of threads at a time
+  // the sequence of tile t0: a scan of the lengths, a block of threads at a time
   if (threadIdx.x == 0) s_b = batch;
   long long before = 0;
   for (int base = 0; base < batch; base += SPLIT_WARPS * 32) {
-    const long long n = (base == 0 ? (long long)some : base + (int)threadIdx.x < batch ? (long long)span_of(a, base + threadIdx.x).count : 0ll) * per_seq;
+    const Span sp = base == 0 ? own : base + (int)threadIdx.x < batch ? span_of(a, base + threadIdx.x) : Span{0, 0, 0};
+    const long long n = length(sp.count) * per_seq;
     long long inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -212,17 +248,16 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
       if (w < warp) here += s_sum[w];
       before += s_sum[w];
     }
-    if (n && here + inc - n <= t0 && t0 < here + inc) s_b = base + threadIdx.x, s_before = here + inc - n; // one thread
+    if (n && here + inc - n <= t0 && t0 < here + inc) s_b = base + threadIdx.x, s_before = here + inc - n, s_span = sp; // one thread
     if (before > t0) break;
   }
   __syncthreads();
   int b = s_b;
   if (b >= batch) return; // (only where pos changes under the kernel)
   long long item0 = s_before; // first tile of the item at hand in the flattened list
-  Span sp = span_of(a, b);
-  if (sp.count == 0) return; // (as above)
-  int item = (int)((t0 - item0) / sp.count); // of the sequence: (KV head, row tile)
-  item0 += (long long)item * sp.count;
+  Span sp = s_span;
+  int item = (int)((t0 - item0) / length(sp.count)); // of the sequence: (KV head, row tile)
+  item0 += item * length(sp.count);
 
   for (long long at = t0; at < t1;) {
     while (item == per_seq || sp.count == 0) { // on to the next sequence that has tiles
@@ -663,7 +698,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
     }
     if (!whole) {
       const long long c_first = item0 / share; // the CTAs that hold parts of the item: c_first .. c_first + others
-      const int others = (int)((item0 + sp.count - 1) / share - c_first);
+      const int others = (int)((item0 + length(sp.count) - 1) / share - c_first);
       __syncthreads();
       if (threadIdx.x == 0) {
         __threadfence(); // the CTA's parts, which the barrier has ordered before, become visible before the count does
@@ -705,6 +740,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
         }
       }
     }
+    if (whole_runs) return; // one item a CTA
     at = item0 + tb;
     item0 += sp.count;
     item++;
