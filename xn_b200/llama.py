@@ -19,6 +19,10 @@ Tensor parallelism over ``world`` ranks (one process per GPU):
 Prefill runs attention and the mean of its RMSNorms as torch ops, the rest as the library's operators. A decode step uses the
 library's fused operators between the linears (residual-add + RMSNorm, RoPE + KV-cache store + single-query attention, SwiGLU), so
 one layer is six launches for one sequence and nine for a batch on Q4_K weights, and the whole step is one CUDA graph.
+
+With ``kv_dtype`` the KV cache is a ``QuantizedKVCache`` a layer, and both prefill and decode rotate, quantize and store the
+projection's output in one kernel and attend to the codes in the next: one launch more in a decode step's layer, a quarter (Q4_0) or
+half (Q8_0) of the cache's memory and of what the attention reads, and no torch attention in a prompt.
 """
 from __future__ import annotations
 
@@ -32,6 +36,7 @@ import torch.nn.functional as F
 
 from . import decoder_ops as ops
 from .dtypes import GgmlDType
+from .kv_cache import QuantizedKVCache
 from .parallel import PeerGather
 from .quantized import QCudaTensor, init
 
@@ -73,21 +78,26 @@ def _dense(shape, std, seed, device):
 
 
 class _Layer:
-    __slots__ = ("wqkv", "wo", "wgu", "wdown", "norm1", "norm2", "k_cache", "v_cache")
+    __slots__ = ("wqkv", "wo", "wgu", "wdown", "norm1", "norm2", "k_cache", "v_cache", "kv")
 
 
 class QLlama:
     """Random-init weights (N(0, 0.02), quantized on the device with the reference's quantizers), a
-    KV cache of ``max_seq`` positions for ``batch`` sequences, prefill and CUDA-graphed decode."""
+    KV cache of ``max_seq`` positions for ``batch`` sequences, prefill and CUDA-graphed decode.
+
+    ``kv_dtype``: the KV cache is held in blocks of that format (Q4_0 or Q8_0) instead of bf16 rows, quantized as tokens are stored
+    and read as codes by the attention, in prefill and decode alike; heads of 64 or 128."""
 
     def __init__(self, cfg: LlamaConfig, device: torch.device, batch: int = 1, max_seq: int = 1024, rank: int = 0, world: int = 1,
-                 group=None, seed: int = 0, max_prefill_rows: int = 512, fused_decode: bool = True, fused_norm: Optional[bool] = None, fused_rope: bool = True):
+                 group=None, seed: int = 0, max_prefill_rows: int = 512, fused_decode: bool = True, fused_norm: Optional[bool] = None, fused_rope: bool = True,
+                 kv_dtype: Optional[GgmlDType] = None):
         if cfg.n_kv_heads % world or cfg.n_heads % world or cfg.ffn % world or cfg.vocab % world or cfg.d_model % world:
             raise ValueError(f"config does not divide over {world} ranks")
         init(device)
         self.cfg, self.device, self.batch, self.max_seq, self.rank, self.world = cfg, device, batch, max_seq, rank, world
         self.hl, self.kvl = cfg.n_heads // world, cfg.n_kv_heads // world
-        self.fused_decode = fused_decode and cfg.head_dim == 128
+        self.kv_dtype = kv_dtype
+        self.fused_decode = fused_decode and (cfg.head_dim == 128 or kv_dtype is not None)
         # One-row decode: residual add + RMSNorm in the prologue of the matvec that follows (same bits either way): two launches
         # fewer per layer (690 against 661 tok/s on one GPU), and sharded it is where the exchange of the row-parallel linears is
         # awaited, off the producing kernel's critical path. XN_FUSED_NORM=0/1 overrides the default for measurements.
@@ -118,8 +128,12 @@ class QLlama:
             L.wdown = self._kshard(_dense((c.d_model, c.ffn), 0.02, s0 + 6, device), c.linear_dtype)
             L.norm1 = torch.ones(c.d_model, device=device)
             L.norm2 = torch.ones(c.d_model, device=device)
-            L.k_cache = torch.zeros((batch, self.kvl, max_seq, hd), device=device, dtype=torch.bfloat16)
-            L.v_cache = torch.zeros_like(L.k_cache)
+            L.k_cache = L.v_cache = L.kv = None
+            if kv_dtype is not None:
+                L.kv = QuantizedKVCache(kv_dtype, batch, self.kvl, max_seq, hd, device)
+            else:
+                L.k_cache = torch.zeros((batch, self.kvl, max_seq, hd), device=device, dtype=torch.bfloat16)
+                L.v_cache = torch.zeros_like(L.k_cache)
             self.layers.append(L)
         self.norm = torch.ones(c.d_model, device=device)
         self.embed = _dense((c.vocab, c.d_model), 0.02, seed * 1_000_003 + 900_001, device).to(torch.bfloat16)
@@ -229,13 +243,16 @@ class QLlama:
         B, S, _ = x.shape
         eps = self.cfg.rms_eps
         qkv = L.wqkv.matmul_t(ops.add_rmsnorm_rows(x, delta, L.norm1, eps))
-        if prompt and self.cfg.head_dim % 8 == 0:
-            q = ops.rope_kv_store_prompt(qkv, self.cos, self.sin, L.k_cache, L.v_cache, self.hl, self.kvl)
+        if L.kv is not None:
+            a = self._attend_blocks(L, qkv, pos_idx[:1])
         else:
-            q = self._rope_store(L, qkv, pos_idx)
-        kv = mask.shape[-1]
-        a = F.scaled_dot_product_attention(q, L.k_cache[:, :, :kv], L.v_cache[:, :, :kv], attn_mask=mask, enable_gqa=True)
-        a = a.transpose(1, 2).reshape(B, S, self.hl * self.cfg.head_dim)
+            if prompt and self.cfg.head_dim % 8 == 0:
+                q = ops.rope_kv_store_prompt(qkv, self.cos, self.sin, L.k_cache, L.v_cache, self.hl, self.kvl)
+            else:
+                q = self._rope_store(L, qkv, pos_idx)
+            kv = mask.shape[-1]
+            a = F.scaled_dot_product_attention(q, L.k_cache[:, :, :kv], L.v_cache[:, :, :kv], attn_mask=mask, enable_gqa=True)
+            a = a.transpose(1, 2).reshape(B, S, self.hl * self.cfg.head_dim)
         if self.pg is None:   # the linear takes the bf16 rows as they are
             o = L.wo.matmul_t(a, out=torch.empty_like(x))
         else:
@@ -244,6 +261,13 @@ class QLlama:
         gu = L.wgu.matmul_t(ops.add_rmsnorm_rows(x, o, L.norm2, eps)).view(B * S, 2 * f)
         h = ops.swiglu(gu, torch.empty((B * S, f), device=self.device)).view(B, S, f)
         return self._sum_parts(self._linear_parts(L.wdown, h))
+
+    def _attend_blocks(self, L: _Layer, qkv: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
+        """The attention of a layer over its block-quantized cache: qkv [B, S, ..] of consecutive tokens, the first at ``pos`` [1].
+        Returns [B, S, heads * hd] in bf16, the type the cache's queries are rounded to in prefill and decode (the rows become 8-bit
+        activations in the next linear)."""
+        q = L.kv.rope_store(qkv, self.cos, self.sin, pos, self.hl, out_dtype=torch.bfloat16)
+        return L.kv.attend(q, pos).flatten(2)
 
     def _rope_store(self, L: _Layer, qkv: torch.Tensor, pos_idx: torch.Tensor) -> torch.Tensor:
         """q and k rotated at ``pos_idx``, k and v stored into the caches at these positions; returns q [B, H, S, hd] bf16."""
@@ -299,13 +323,17 @@ class QLlama:
             else:
                 ops.add_rmsnorm(cur, delta, L.norm1, c.rms_eps, None if xi else self._xn, xi)
                 L.wqkv.matmul_t(xi or self._xn, out=self._qkv)
-            if self.fused_rope:   # RoPE and the KV-cache store inside the attention kernel: one launch less per layer, same bits
+            a = self._a
+            if L.kv is not None:
+                a = self._attend_blocks(L, self._qkv.unsqueeze(1), self.pos).squeeze(1)
+                a = a if self.pg is None else a.float()
+            elif self.fused_rope:   # RoPE and the KV-cache store inside the attention kernel: one launch less per layer, same bits
                 ops.rope_attn_decode(self._qkv, self.cos, self.sin, self.pos, L.k_cache, L.v_cache, self._a.view(self.batch, self.hl, c.head_dim), self.hl, self.kvl)
             else:
                 ops.rope_kv_store(self._qkv, self.cos, self.sin, self.pos, self._q, L.k_cache, L.v_cache, self.hl, self.kvl)
                 ops.attn_decode(self._q, L.k_cache, L.v_cache, self.pos, self._a.view(self.batch, self.hl, c.head_dim), self.hl, self.kvl)
             hint(L.wgu)
-            o = self._linear_parts(L.wo, self._a, self._o, defer=defer)           # world summands per row when sharded
+            o = self._linear_parts(L.wo, a, self._o, defer=defer)           # world summands per row when sharded
             hint(L.wdown)
             if fused:
                 L.wgu.matvec_normed(cur, o, L.norm2, c.rms_eps, nxt, self._gu, await_comm=self.pg if defer else None)
