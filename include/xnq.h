@@ -374,7 +374,9 @@ int xnq_kv_load(const xnq_kv_cache *cache, int64_t batch, const long long *start
  * of sequence b is at p = pos[b] + i and sees j <= p (causal) or j < pos[b] + seq, and with a window > 0 only j > p - window. One that sees nothing gives
  * zeros (lse -inf). q and out [batch, seq, heads, head_dim] have one type; lse (may be NULL): f32 [batch, seq, heads], the natural logarithm of the sum of
  * exponentials. f32 queries: products and sums to f32 accuracy. f16 / bf16: the softmax weights are rounded to 16 bits before they meet v.
- * workspace: xnq_kv_attend_workspace_bytes, 16-byte aligned, zeroed once after it was allocated; one call at a time may use it. */
+ * workspace: xnq_kv_attend_workspace_bytes, 16-byte aligned, its first XNQ_KV_WORKSPACE_ZEROED bytes zeroed once after it was allocated
+ * (a call leaves them so); one call at a time may use it. */
+#define XNQ_KV_WORKSPACE_ZEROED 4096
 size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim);
 int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
                   int pos_stride, float scale, int causal, int64_t window, void *workspace, size_t ws_bytes, void *stream);

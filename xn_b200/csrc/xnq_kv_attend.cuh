@@ -23,6 +23,7 @@ struct AttendArgs {
 // Workspace: the tickets, at one place whatever the call, then the parts.
 constexpr int KV_TICKETS = 1024;
 constexpr size_t KV_TICKET_BYTES = KV_TICKETS * 4;
+static_assert(KV_TICKET_BYTES == XNQ_KV_WORKSPACE_ZEROED, "what a caller zeroes");
 constexpr unsigned KV_WAIT = 8; // status: a wait of the kernel for many rows expired (with the bits of xnq_kv_cache.cuh)
 
 // xnq_kv_prompt.cu: many 16-bit query rows

@@ -23,6 +23,7 @@ from . import _lib
 from .dtypes import GgmlDType
 from .quantized import _TORCH_TO_XNQ, _XNQ_IDS, _stream_ptr, init
 
+_ZEROED = 4096  # XNQ_KV_WORKSPACE_ZEROED: the front of attention's workspace, zero before its first use
 PAGE_UNIT = 32  # positions of a tile: page sizes are multiples of it
 
 
@@ -55,7 +56,9 @@ _workspaces: dict[tuple[int, int], torch.Tensor] = {}   # (device, stream) -> ze
 
 def _workspace(device: torch.device, need: int) -> torch.Tensor:
     if torch.cuda.is_current_stream_capturing():   # a graph may be replayed beside others: scratch of its own, zeroed in every replay
-        return torch.zeros(need, dtype=torch.uint8, device=device)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws[:_ZEROED].zero_()
+        return ws
     key = (device.index, int(_stream_ptr(device).value or 0))
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < need:
