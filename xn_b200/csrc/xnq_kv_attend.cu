@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
   // Short items go to CTAs of their own: a run shorter than a tile a warp only where the items are shorter too.
   const long long at_least = min((long long)SPLIT_WARPS, max(total / max(items, 1ll), 1ll));
   long long share = max((total + gridDim.x - 1) / gridDim.x, at_least);
+  if (share > at_least) share = (share + SPLIT_WARPS - 1) / SPLIT_WARPS * SPLIT_WARPS; // as long for the warps, and fewer parts to join
   // A run that goes on into a second item pays for another start and end, about as long as 15 tiles take: where a run of a few more tiles keeps every
   // CTA within one item, the items are rounded up to whole runs.
   bool whole_runs = false;
