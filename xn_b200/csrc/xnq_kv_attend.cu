@@ -68,40 +68,6 @@ __device__ __forceinline__ void load_vec(const float *p, float (&v)[V]) {
     v[0] = x.x, v[1] = x.y;
   }
 }
-template <int V>
-__device__ __forceinline__ void load_vec_cg(const float *p, float (&v)[V]) {
-  if (V == 4) {
-    const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
-    v[0] = x.x, v[1] = x.y, v[V - 2] = x.z, v[V - 1] = x.w;
-  } else {
-    const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
-    v[0] = x.x, v[1] = x.y;
-  }
-}
-template <int V>
-__device__ __forceinline__ void store_vec(void *p, int dtype, long long at, const float (&v)[V]) {
-  if (dtype == XNQ_F32) {
-    float *q = static_cast<float *>(p) + at;
-    if (V == 4) *reinterpret_cast<float4 *>(q) = make_float4(v[0], v[1], v[V - 2], v[V - 1]);
-    else *reinterpret_cast<float2 *>(q) = make_float2(v[0], v[1]);
-    return;
-  }
-  uint32_t w[V / 2];
-#pragma unroll
-  for (int i = 0; i < V / 2; i++) {
-    if (dtype == XNQ_F16) {
-      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t *>(&h);
-    }
-  }
-  uint16_t *q = static_cast<uint16_t *>(p) + at;
-  if (V == 4) *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[V / 2 - 1]);
-  else *reinterpret_cast<uint32_t *>(q) = w[0];
-}
-
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -774,9 +740,19 @@ struct SplitLaunch {
     return XNQ_OK;
   }
 };
-// Query rows of a KV head to an item of the split kernel.
-int split_nt(int64_t rows) { return rows <= 8 ? 1 : 2; }
-// Rows from which the kernel for many rows takes 16-bit queries.
+// Query rows of a KV head to an item of the split kernel: 8 or 16. Sixteen read a tile half as often and take 1.3 to 1.6 times as long for
+// it, with two CTAs an SM instead of three. Where the items fill the GPU that gains (16 rows, 64 sequences of 4096 positions and 8 KV heads: 131 us against 145,
+// Q8_0 184 against 252), unless the second half of the last sixteen is empty (4 bits, 24 rows: 229 against 204). Where they do not, items of 8 go to more SMs
+// and are done sooner (16 rows of one sequence of 8192: 37 us against 25, of 512: 22 against 16).
+int split_nt(int bits, int64_t rows, int64_t heads, int sms) {
+  const int64_t eights = (rows + 7) / 8;
+  return eights == 1 || heads * eights <= sms || (bits == 4 && eights == 3) ? 1 : 2;
+}
+// 16-bit query rows of a KV head from which the kernel for many rows takes them, whose time hardly depends on their number up to 128. Below it they keep this
+// kernel's scores, exact products of the codes, where the other's keys are rounded to 16 bits (an error of 1e-4 of a row's log sum), also where the other is
+// sooner. 8 KV heads, us, this kernel against that: Q4_0, 32 rows, one sequence of 8192 27 against 28, of 32768 52 against 52, 16 sequences of 8192 123 against
+// 129; 64 rows, 36 against 32, 78 against 52, 219 against 131. Q8_0, 16 rows, 29 against 28, 47 against 50, 98 against 135; 64 rows, 46 against 32, 92 against
+// 54, 309 against 136.
 constexpr int64_t PROMPT_ROWS = 64;
 
 template <int BITS, int HD, int NT, bool SPLIT>
@@ -807,7 +783,7 @@ int for_each_split(F f) { // f<BITS, HD, NT, SPLIT>()
 
 template <int BITS, int HD>
 int run_attend(const AttendArgs &a, int sms, cudaStream_t s) {
-  const bool one = split_nt(a.seq * a.group) == 1;
+  const bool one = split_nt(BITS, a.seq * a.group, a.batch * a.c.kv_heads, sms) == 1;
   if (a.dtype == XNQ_F32) return one ? run_split<BITS, HD, 1, true>(a, sms, s) : run_split<BITS, HD, 2, true>(a, sms, s);
   return one ? run_split<BITS, HD, 1, false>(a, sms, s) : run_split<BITS, HD, 2, false>(a, sms, s);
 }
@@ -866,8 +842,9 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
   a.tickets = static_cast<unsigned int *>(workspace);
   a.records = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + KV_TICKET_BYTES);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (q->dtype != XNQ_F32 && seq * a.group >= PROMPT_ROWS) return launch_kv_prompt(a, kv_bits(cache->ggml_dtype), cache->head_dim, sms, s);
-  if (kv_bits(cache->ggml_dtype) == 4) return cache->head_dim == 64 ? run_attend<4, 64>(a, sms, s) : run_attend<4, 128>(a, sms, s);
+  const int bits = kv_bits(cache->ggml_dtype);
+  if (q->dtype != XNQ_F32 && seq * a.group >= PROMPT_ROWS) return launch_kv_prompt(a, bits, cache->head_dim, sms, s);
+  if (bits == 4) return cache->head_dim == 64 ? run_attend<4, 64>(a, sms, s) : run_attend<4, 128>(a, sms, s);
   return cache->head_dim == 64 ? run_attend<8, 64>(a, sms, s) : run_attend<8, 128>(a, sms, s);
 }
 

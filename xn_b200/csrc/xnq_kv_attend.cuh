@@ -51,6 +51,39 @@ __device__ __forceinline__ float exp2_approx(float x) { // 2^x within 2 ulp
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+template <int V> // 2 or 4 values
+__device__ __forceinline__ void load_vec_cg(const float *p, float (&v)[V]) {
+  if (V == 4) {
+    const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
+    v[0] = x.x, v[1] = x.y, v[V - 2] = x.z, v[V - 1] = x.w;
+  } else {
+    const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
+    v[0] = x.x, v[1] = x.y;
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_vec(void *p, int dtype, long long at, const float (&v)[V]) {
+  if (dtype == XNQ_F32) {
+    float *q = static_cast<float *>(p) + at;
+    if (V == 4) *reinterpret_cast<float4 *>(q) = make_float4(v[0], v[1], v[V - 2], v[V - 1]);
+    else *reinterpret_cast<float2 *>(q) = make_float2(v[0], v[1]);
+    return;
+  }
+  uint32_t w[V / 2];
+#pragma unroll
+  for (int i = 0; i < V / 2; i++) {
+    if (dtype == XNQ_F16) {
+      const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+  }
+  uint16_t *q = static_cast<uint16_t *>(p) + at;
+  if (V == 4) *reinterpret_cast<uint2 *>(q) = make_uint2(w[0], w[V / 2 - 1]);
+  else *reinterpret_cast<uint32_t *>(q) = w[0];
+}
 // Pair i of a word's codes (16 bits apart) as f16 subnormals, c 2^-24; 4 bits: 16 times that where i is odd.
 template <int BITS>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {

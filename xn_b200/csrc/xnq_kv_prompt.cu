@@ -15,7 +15,7 @@
 // Tensor memory: the scores of both tiles and both outputs, all 512 columns. f16 operands for bf16 queries too: q is exact after a power of two a row,
 // and K, V and P lose 2^-12 instead of bf16's 2^-9.
 //
-// Where the row tiles are fewer than the SMs, `splits` CTAs share a tile's positions; the last to arrive adds their parts, in order.
+// Where the row tiles are fewer than the SMs, `splits` CTAs share a tile's positions; a second kernel adds their parts, in order.
 #include <algorithm>
 #include <climits>
 
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   __shared__ __align__(8) uint64_t bars[3 * 16 + 4 * RING + 4 + 4 + 2 + 2 + 2];
   __shared__ Meta meta[META_STEPS][STEP_TILES];
   __shared__ int s_null[16], s_plain[META_STEPS * 2]; // of a half: nothing in its tiles' scales to look at
-  __shared__ int s_dead, s_last;
+  __shared__ int s_dead;
   __shared__ uint32_t s_tmem;
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
@@ -675,8 +675,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       }
       if (valid && a.lse) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (ref + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
     } else {
-      float *rec = a.records + (size_t)blockIdx.x * P::RECORD;
-      rec[row] = ref, rec[QT * 128 + row] = l;
+      float *rec = a.records + (((size_t)(a.row_tiles - 1 - rt) * (per / a.splits) + bk) * a.splits + split) * P::RECORD;
+      if (valid) rec[row] = ref, rec[QT * 128 + row] = l;
       const float by = ldexpf(1.f, -v_ref);
       float *dst = rec + 2 * QT * 128 + (size_t)row * HD;
 #pragma unroll 1
@@ -687,60 +687,68 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
           tmem_ld_wait();
         }
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
+        for (int i = 0; i < 16 && valid; i += 4)
           *reinterpret_cast<float4 *>(dst + c + i) = n ? make_float4(__uint_as_float(o[i]) * by, __uint_as_float(o[i + 1]) * by, __uint_as_float(o[i + 2]) * by, __uint_as_float(o[i + 3]) * by)
                                                        : make_float4(0.f, 0.f, 0.f, 0.f);
       }
     }
     tc_fence_before();
-    if (a.splits > 1) { // the softmax warps alone
-      asm volatile("bar.sync 1, %0;" ::"n"(QT * 128) : "memory");
-      const int unit = (int)(blockIdx.x / per) * (per / a.splits) + bk;
-      if (threadIdx.x == 0) {
-        __threadfence();
-        s_last = atomicInc(a.tickets + unit, (unsigned)(a.splits - 1)) == (unsigned)(a.splits - 1);
-        __threadfence();
-      }
-      asm volatile("bar.sync 1, %0;" ::"n"(QT * 128) : "memory");
-      if (s_last) {
-        const float *first = a.records + (size_t)(blockIdx.x - split) * P::RECORD;
-        for (int i = threadIdx.x; i < rows * (HD / 8); i += QT * 128) {
-          const int row = i / (HD / 8), c = (i - row * (HD / 8)) * 8;
-          const long long at = row0 + row, tok = at / a.group;
-          const int h = kvh * a.group + (int)(at - tok * a.group);
-          float m = -INFINITY, l = 0.f, v[8] = {};
-          for (int k = 0; k < a.splits; k++) m = fmaxf(m, __ldcg(first + (size_t)k * P::RECORD + row));
-          for (int k = 0; k < a.splits; k++) {
-            const float *p = first + (size_t)k * P::RECORD;
-            const float mp = __ldcg(p + row), lp = __ldcg(p + QT * 128 + row);
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p + 2 * QT * 128 + (size_t)row * HD + c)), y = __ldcg(reinterpret_cast<const float4 *>(p + 2 * QT * 128 + (size_t)row * HD + c + 4));
-            const float by = mp == -INFINITY ? 0.f : exp2_approx(mp - m);
-            if (by == 0.f) continue;
-            l += by * lp;
-            v[0] += by * x.x, v[1] += by * x.y, v[2] += by * x.z, v[3] += by * x.w, v[4] += by * y.x, v[5] += by * y.y, v[6] += by * y.z, v[7] += by * y.w;
-          }
-          const float by = l > 0.f ? 1.f / l : l;
-          uint32_t w[4];
-#pragma unroll
-          for (int q = 0; q < 4; q++) {
-            const float x = v[2 * q] * by, y = v[2 * q + 1] * by;
-            if (a.dtype == XNQ_F16) w[q] = pack_half2(x, y);
-            else {
-              const __nv_bfloat162 z = __floats2bfloat162_rn(x, y);
-              w[q] = *reinterpret_cast<const uint32_t *>(&z);
-            }
-          }
-          *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out.p) + b * a.out.sb + tok * a.out.ss + h * a.out.sh + c) = make_uint4(w[0], w[1], w[2], w[3]);
-          if (a.lse && c == 0) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
-        }
-      }
-    }
   }
   __syncthreads();
   if (warp == MMA) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
+}
+
+// The parts of rows whose positions `splits` CTAs shared, added in the order of their places: a warp a row, a lane HD / 32 dims. A kernel of its own, because
+// every SM has a share of it: one CTA of the attention adding 18 parts of 128 rows, 1.2 MB, had taken longer than the attention (128 rows of one sequence of 8192 positions: 139 us, now 32).
+template <int HD>
+__global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int V = HD / 32, RECORD = 128 * (HD + 2), AHEAD = 8;
+  const int lane = threadIdx.x & 31, units = (int)a.batch * a.c.kv_heads;
+  const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5), all_rows = a.seq * a.group;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rt = (int)(at / (128ll * units)), bk = (int)(at / 128 % units), row = (int)(at % 128), b = bk / a.c.kv_heads, kvh = bk % a.c.kv_heads;
+  const long long at_row = rt * 128ll + row;
+  if (rt >= a.row_tiles || at_row >= all_rows) return;
+  const float *const first = a.records + ((size_t)(a.row_tiles - 1 - rt) * units + bk) * a.splits * RECORD; // (the last row tiles' CTAs come first)
+  float m = -INFINITY, l = 0.f, v[V] = {};
+  for (int k = lane; k < a.splits; k += 32) m = fmaxf(m, __ldcg(first + (size_t)k * RECORD + row));
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int k0 = 0; k0 < a.splits; k0 += 32) {
+    const int left = min(32, a.splits - k0);
+    float mine = 0.f;
+    if (lane < left) {
+      const float *p = first + (size_t)(k0 + lane) * RECORD;
+      const float mp = __ldcg(p + row);
+      mine = mp == -INFINITY ? 0.f : exp2_approx(mp - m);
+      l += mine * __ldcg(p + 128 + row); // (a part of NaN stays one)
+    }
+    for (int k = 0; k < left; k += AHEAD) {
+      float x[AHEAD][V];
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) load_vec_cg<V>(first + (size_t)(k0 + min(k + i, left - 1)) * RECORD + 256 + (size_t)row * HD + lane * V, x[i]);
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) {
+        const float by = __shfl_sync(0xffffffffu, mine, (k + i) & 31);
+        if (k + i < left && by != 0.f)
+#pragma unroll
+          for (int c = 0; c < V; c++) v[c] += by * x[i][c];
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const long long tok = at_row / a.group;
+  const int h = kvh * a.group + (int)(at_row - tok * a.group);
+  const float by = l > 0.f ? 1.f / l : l; // nothing seen: zeros; NaN stays
+#pragma unroll
+  for (int c = 0; c < V; c++) v[c] = l == 0.f ? 0.f : v[c] * by;
+  store_vec<V>(a.out.p, a.dtype, b * a.out.sb + tok * a.out.ss + h * a.out.sh + lane * V, v);
+  if (a.lse && lane == 0) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
 }
 
 // Row tiles of 256 rows where they fill the GPU, else of 128; CTAs that share a tile's positions where those do not fill it either.
@@ -759,6 +767,9 @@ int launch(const AttendArgs &a, cudaStream_t s) {
   const int64_t grid = (int64_t)a.row_tiles * a.batch * a.c.kv_heads * a.splits;
   if (grid > INT_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of query rows are more than one launch takes", (long long)grid);
   XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
+  count_launch();
+  if (a.splits == 1) return XNQ_OK;
+  XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD>, dim3((unsigned)(a.row_tiles * a.batch * a.c.kv_heads * 16)), dim3(256), 0, s, a));
   count_launch();
   return XNQ_OK;
 }
