@@ -102,6 +102,21 @@ def test_stored_blocks_are_the_oracles(O, fmt, dt, B, KV, S, L, hd, page, start)
 
 
 @pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_of_two_equal_magnitudes_the_first_gives_the_sign(O, fmt, dt):
+    """Every ordered pair of places of a block's largest values, one positive and one negative."""
+    x = (_rand(21, 992, 32).clamp(-1, 1) * 0.9)
+    pairs = [(i, j) for i in range(32) for j in range(32) if i != j]
+    for n, (i, j) in enumerate(pairs):
+        x[n, i], x[n, j] = 2.0, -2.0
+    x = x.view(1, 496, 1, 64).to(TYPES[dt])
+    c = _cache(fmt, 1, 1, 496, 64)
+    c.store(x.to(DEV), x.flip(1).contiguous().to(DEV), _pos(0))
+    got_k, got_v = c.load(0, 496, dtype=torch.float32)
+    assert torch.equal(got_k, _held(O, fmt, x).transpose(1, 2)) and torch.equal(got_v, _held(O, fmt, x.flip(1)).transpose(1, 2))
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
 def test_tokens_one_at_a_time_and_at_own_positions(O, fmt):
     """Positions of their own, odd and even, in any order: a pair of positions shares words of the values' codes."""
     B, KV, L, hd = 3, 2, 65, 128

@@ -117,12 +117,11 @@ __device__ __forceinline__ Codes8 quantize8(const float (&v)[8]) {
   float m = mx >= -mn ? mx : mn;
   if (mx == -INFINITY) m = 0.f; // NaN alone
   if (__any_sync(0xffffffffu, mx == -mn && mx > 0.f)) { // both signs: whichever comes first
-    int at = 32;
+    int at = 64; // twice the place, and the sign; 64: none of this thread's
     const int t = threadIdx.x & 3;
 #pragma unroll
     for (int i = 7; i >= 0; i--)
       if (fabsf(v[i]) == mx) at = 2 * (t * 8 + i) + (v[i] < 0.f);
-    at = min(at == 32 ? 64 : at, 64);
     at = min(at, __shfl_xor_sync(0xffffffffu, at, 1));
     at = min(at, __shfl_xor_sync(0xffffffffu, at, 2));
     if (mx == -mn && mx > 0.f) m = at & 1 ? mn : mx;
