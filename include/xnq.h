@@ -373,7 +373,8 @@ int xnq_kv_load(const xnq_kv_cache *cache, int64_t batch, const long long *start
 /* out[b, i, h] = softmax over the positions j that query i sees of (scale q k_j), times v_j; heads / kv_heads query heads share a KV head. Query i
  * of sequence b is at p = pos[b] + i and sees j <= p (causal) or j < pos[b] + seq, and with a window > 0 only j > p - window. One that sees nothing gives
  * zeros (lse -inf). q and out [batch, seq, heads, head_dim] have one type; lse (may be NULL): f32 [batch, seq, heads], the natural logarithm of the sum of
- * exponentials. f32 queries: products and sums to f32 accuracy. f16 / bf16: the softmax weights are rounded to 16 bits before they meet v.
+ * exponentials. f32 queries: products and sums to f32 accuracy. f16 / bf16: the softmax weights are rounded to f16 before they meet v, and
+ * from 64 query rows of a KV head (seq * heads / kv_heads) the keys and values are, too (relative 2^-12 each).
  * workspace: xnq_kv_attend_workspace_bytes, 16-byte aligned, its first XNQ_KV_WORKSPACE_ZEROED bytes zeroed once after it was allocated
  * (a call leaves them so); one call at a time may use it. */
 #define XNQ_KV_WORKSPACE_ZEROED 4096

@@ -22,6 +22,11 @@
 // norm with 4-bit codes; 5e-7 now, as much as f32 products), and with many weights the two sums in O would cancel. 16-bit queries: q is exact in f16 after a power of two a row, the weights are rounded to f16.
 // Ranges: a row's reference lies 8 below its maximum of the time and is renewed when a score passes it by more than 12, so that nothing need be known
 // of a tile's maximum beforehand; the values' scales are brought near one by a power of two a warp.
+//
+// Measured (bf16 queries, 32 heads over 8 of 128): 16 sequences of 8192 positions in Q4_0 blocks 42 us, 64 of 330 to 16384 in pages 144 us (4.1 TB/s of cache),
+// one of 131072 47 us, of 512 9.7 us in a captured step; Q8_0, 16 of 8192, 65 us (4.4 TB/s). Few rows of many positions are bound by instructions: 570 a tile and
+// warp, of which the codes' masks and shifts are the most, 12 warps an SM (with 128 registers and 16 warps it was slower). Few positions are bound by the
+// chain of latencies: positions, first tile, a tile's arithmetic, the meeting of the parts.
 #include <algorithm>
 #include <cmath>
 

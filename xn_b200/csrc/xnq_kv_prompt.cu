@@ -16,6 +16,10 @@
 // and K, V and P lose 2^-12 instead of bf16's 2^-9.
 //
 // Where the row tiles are fewer than the SMs, `splits` CTAs share a tile's positions; a second kernel adds their parts, in order.
+//
+// Measured (bf16, 32 heads over 8 of 128, Q4_0): 2048 tokens at the end of 8192 positions 282 us, 850 TFLOP/s, 512 tokens of their own 17 us. A step of 128 positions
+// takes about 4500 cycles for two row tiles, of which the tensor core works 2560 and softmax's 2^x 2048 of each scheduler; the rest is roles that wait for one another, and 256
+// CTAs on 148 SMs (the longest first). Two threads a row, or one buffer of scores a tile, were slower.
 #include <algorithm>
 #include <climits>
 
@@ -751,13 +755,16 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_consta
   if (a.lse && lane == 0) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
 }
 
-// Row tiles of 256 rows where they fill the GPU, else of 128; CTAs that share a tile's positions where those do not fill it either.
+// Row tiles of 128 rows where an SM each is enough for them, or the rows are no more; CTAs that share a tile's positions where the SMs are more. Else tiles
+// of 256, which take less time than two of 128. 32 heads over 8 of 128, us with tiles of 128 against 256: 512 tokens of their own 22 against 27, 400 of 8192
+// positions 121 against 154, 8 sequences of 64 tokens of 4096 72 against 88, 64 of 32 260 against 299; 1024 tokens of 8192 234 against 163, 600 of 4096
+// 119 against 90, 16 sequences of 60 of 4096 136 against 94.
 struct Plan {
   int qt, row_tiles, splits;
 };
 Plan plan_of(int64_t batch, int64_t seq, int group, int kv_heads, int64_t max_seq, int sms) {
   const int64_t rows = seq * group, heads = batch * kv_heads, two = (rows + 255) / 256, one = (rows + 127) / 128;
-  if (heads * two >= sms) return Plan{2, (int)two, 1};
+  if (one > 1 && heads * one > sms) return Plan{2, (int)two, 1};
   const int64_t steps = (max_seq + BN - 1) / BN;
   return Plan{1, (int)one, (int)std::max<int64_t>(1, std::min<int64_t>(sms / (heads * one), steps / 2))};
 }
