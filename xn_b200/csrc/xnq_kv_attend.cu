@@ -124,7 +124,9 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
   __shared__ int s_b, s_last;
   __shared__ Span s_span;
   __shared__ unsigned s_runs[4][SPLIT_WARPS];
-  __shared__ long long s_row[R], s_lse_row[R]; // where an item's rows go
+  // Where an item's rows go; of an item and the next one: warp 0 writes the next one's while other warps still store this one's rows. Between an item and
+  // the one after the next lie barriers that every warp reaches when it is done with the first.
+  __shared__ long long s_row[2][R], s_lse_row[2][R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float *const merge = reinterpret_cast<float *>(smem + SPLIT_WARPS * SPLIT_STAGES * L::BYTES);
   float *const s_m = merge, *const s_l = merge + SPLIT_WARPS * R, *const s_acc = merge + 2 * SPLIT_WARPS * R;
@@ -240,6 +242,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
   int item = (int)((t0 - item0) / length(sp.count)); // of the sequence: (KV head, row tile)
   item0 += item * length(sp.count);
 
+  int turn = 0; // which of the two copies is the item's
   for (long long at = t0; at < t1;) {
     while (item == per_seq || sp.count == 0) { // on to the next sequence that has tiles
       item = 0;
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
       const int r = n * 8 + g; // this lane's row as an operand's column
       const long long row = (long long)rt * R + r, s = row / a.group;
       const int h = kvh * a.group + (int)(row - s * a.group);
-      if (warp == 0 && t == 0) s_row[r] = b * a.out.sb + s * a.out.ss + h * a.out.sh, s_lse_row[r] = ((long long)b * a.seq + s) * a.heads + h;
+      if (warp == 0 && t == 0) s_row[turn][r] = b * a.out.sb + s * a.out.ss + h * a.out.sh, s_lse_row[turn][r] = ((long long)b * a.seq + s) * a.heads + h;
       float v[NB][8], top = 0.f;
 #pragma unroll
       for (int bl = 0; bl < NB; bl++) {
@@ -626,7 +629,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
     asm volatile("cp.async.wait_all;" ::: "memory");
 
     // ---- the warps meet ----
-    __syncthreads(); // (of the item before, everything has been read)
+    __syncthreads(); // (of the item before, everything in s_m, s_l and s_acc has been read)
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -657,8 +660,8 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
       const float by = l_all > 0.f ? 1.f / l_all : l_all; // 0: nothing seen, zeros; NaN stays
 #pragma unroll
       for (int i = 0; i < V; i++) v[i] *= by;
-      store_vec<V>(a.out.p, a.dtype, s_row[r] + lane * V, v);
-      if (a.lse && lane == 0) a.lse[s_lse_row[r]] = l_all > 0.f ? (m_all + log2f(l_all)) * LN2 : l_all == 0.f ? -INFINITY : l_all;
+      store_vec<V>(a.out.p, a.dtype, s_row[turn][r] + lane * V, v);
+      if (a.lse && lane == 0) a.lse[s_lse_row[turn][r]] = l_all > 0.f ? (m_all + log2f(l_all)) * LN2 : l_all == 0.f ? -INFINITY : l_all;
     };
     float *const rec = a.records + (blockIdx.x * 2 + (ta == 0 ? 1 : 0)) * (long long)RECORD_STRIDE;
     for (int r = warp; r < rows; r += SPLIT_WARPS) {
@@ -732,7 +735,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
     }
     if (whole_runs) return; // one item a CTA
     at = item0 + length(sp.count), item0 = at;
-    item++;
+    item++, turn ^= 1;
   }
 }
 
