@@ -32,3 +32,30 @@ def test_rows_of_items_that_follow_one_another(fmt, dt, S, H, group_of, lse):
     for out, sums in made[1:]:
         assert torch.equal(out, made[0][0]) and (not lse or torch.equal(sums, made[0][1]))
     assert _status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("S,hd", [(20, 128), (150, 128), (150, 64)])
+def test_weights_stored_before_a_half_renews_its_reference(fmt, dt, S, hd):
+    """Scores rise by some 13 (weights by 2^19) from the first tile of 32 of a half to the second, twice: the second tile asks for another reference when the
+    first one's weights are already stored, and they are brought to it. The keys are whole multiples of a power of two, so that scores are exact however large:
+    what is left is the tolerance's own terms."""
+    B, H, KV, L = 2, 16, 4, 512
+    c = _cache(fmt, B, KV, L, hd)
+    level = ((torch.arange(L) >= 32).int() + (torch.arange(L) >= 160))[None, :, None, None]
+    code = 3 * level + torch.randint(-1, 2, (B, L, KV, hd), generator=torch.Generator().manual_seed(4))
+    code[..., ::32] = -8 if fmt == "q4_0" else 127        # a block's largest: its scale is 1/2
+    c.store((code * 0.5).to(DEV), _rand(5, B, L, KV, hd).to(DEV), _pos(0))
+    k, v = c.load(0, L, dtype=torch.float32)
+    assert torch.equal(k.transpose(1, 2), (code * 0.5).to(DEV))
+    q = _rand(6, B, S, H, hd, gain=1.0 if hd == 128 else 1.4).abs()
+    q[..., ::32] = 0
+    q = q.to(TYPES[dt]).to(DEV)
+    first = [L - S, L - S - 45]
+    got = c.attend(q, _pos(*first))
+    want, _, tol = _reference(k, v, q, first)
+    _check(got, want, tol, (fmt, dt, S))
+    for _ in range(100):
+        assert torch.equal(c.attend(q, _pos(*first)), got)
+    assert _status() == 0

@@ -560,6 +560,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       if (c) {
         const __half2 f16 = __float2half2_rn(f32); // (0 or less than one: P loses no more than its own rounding)
         uint32_t o[16];
+        tmem_st_wait(); // the first tile's P is there
         tmem_ld16(buffers + (h2 & 1) * HALF, o);
         tmem_ld_wait();
 #pragma unroll
