@@ -228,7 +228,6 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
   const uint32_t raw_full = bar, raw_scanned = bar + 16 * 8, raw_empty = bar + 32 * 8, k_full = bar + 48 * 8, k_empty = k_full + 8 * RING, v_full = k_empty + 8 * RING, v_empty = v_full + 8 * RING,
                  s_full = v_empty + 8 * RING, p_full = s_full + 32, pv_done = p_full + 32, o_done = pv_done + 16, q_ready = o_done + 16; // s_full, p_full: [row tile][buffer] (softmax may be two halves ahead of the MMAs)
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 16; i++) mbar_init(raw_full + 8 * i, 1), mbar_init(raw_scanned + 8 * i, 1), mbar_init(raw_empty + 8 * i, 2);
     for (int i = 0; i < RING; i++) mbar_init(k_full + 8 * i, 2), mbar_init(v_full + 8 * i, 2), mbar_init(k_empty + 8 * i, QT), mbar_init(v_empty + 8 * i, QT);
@@ -247,6 +246,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+  // Not before this CTA has its tensor memory: a kernel that is let in takes its own and then waits for this one to end.
+  pdl_launch_dependents();
   pdl_wait();
 
   // ---- which rows, which positions; the row tiles with the most positions first ----
