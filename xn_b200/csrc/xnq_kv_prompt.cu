@@ -268,7 +268,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   if (warp >= LOADER) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
   if (warp == LOADER) {
     const uint8_t *ahead = nullptr;
-    for (int i = 0; i < n * STEP_TILES; i++) {
+    int i = 0;
+    for (; i < n * STEP_TILES; i++) {
       const int slot = i % P::SLOTS, lap = i / P::SLOTS;
       if ((i & 31) == 0) ahead = i + lane < n_tiles ? kv_tile_at(a.c, b, kvh, t0 + i + lane, L::BYTES) : nullptr;
       const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ahead), i & 31));
@@ -285,9 +286,11 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       }
       __syncwarp();
     }
-    if (*dead) // none of this CTA's copies is in flight when it ends
-      for (int i = 0; i < P::SLOTS; i++)
-        for (int k = 0; k < 1000 && !mbar_try(raw_full + 8 * i, 0) && !mbar_try(raw_full + 8 * i, 1); k++) {}
+    // None of this CTA's copies is in flight when it ends, whatever the other roles gave up: the last one into each slot (`i` were asked for) is waited for.
+    for (int slot = 0; slot < P::SLOTS && slot < i; slot++) {
+      const uint32_t parity = (uint32_t)((i - 1 - slot) / P::SLOTS) & 1u;
+      for (int k = 0; k < 1000 && !mbar_try(raw_full + 8 * slot, parity); k++) {}
+    }
   } else if (warp == SCAN) { // two tiles at a time
     constexpr int KW = NB / 2;
     for (int i = 0; i < n * STEP_TILES; i += 2) {
@@ -483,6 +486,11 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       if (++v_at == RING) v_at = 0, v_odd ^= 1;
       if (++k_at == RING) k_at = 0, k_odd ^= 1;
       p_odd ^= buf;
+    }
+    if (!alive && halves > 0) { // given up: what has been issued ends before the operands and the tensor memory go
+      if (elect_one()) commit(o_done + 8 * q);
+      __syncwarp();
+      for (int k = 0; k < 1000 && !mbar_try(o_done + 8 * q, 0); k++) {}
     }
   } else if (warp < QT * 4) {
     // ---- a row a thread ----
