@@ -1,5 +1,8 @@
 """The quantized KV cache where it can go wrong between items, warps, halves and calls. Tolerances are those of test_gpu_kv_cache.py."""
 import math
+import sys
+import threading
+import time
 
 import pytest
 import torch
@@ -59,3 +62,79 @@ def test_weights_stored_before_a_half_renews_its_reference(fmt, dt, S, hd):
     for _ in range(100):
         assert torch.equal(c.attend(q, _pos(*first)), got)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("S,own", [(64, True), (3, True), (64, False)])
+def test_two_threads_on_one_stream(S, own):
+    """Each call's parts stay its own, with results that it makes (C++) and with given ones (Python): the interpreter's lock is free while a call launches.
+    A kernel that takes its time comes first, and the calls are more than the device's queue holds, so that launches block."""
+    B, H, KV, hd, L = 1, 8, 2, 128, 16384
+    c = _filled("q4_0", B, KV, L, hd)
+    qs = [_rand(20 + i, B, S, H, hd).to(torch.bfloat16).to(DEV) for i in range(4)]
+    pos = _pos(L - S)
+    call = lambda q: c.attend(q, pos, out=torch.empty_like(q)) if own else c.attend(q, pos)
+    want = [call(q) for q in qs]
+    wrong, start = [], threading.Barrier(4)
+
+    def work(i):
+        for n in range(3):
+            torch.cuda._sleep(100_000_000 if i == 0 else 1)
+            start.wait()
+            got = [call(qs[i]) for _ in range(400)]
+            wrong.extend((i, n) for g in got if not torch.equal(g, want[i]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    assert not wrong, (len(wrong), wrong[:5])
+
+
+def test_one_call_at_a_time_uses_a_workspace(monkeypatch):
+    """The Python path: a call's kernels (two, where parts are joined) are enqueued before another call may use the same scratch."""
+    from xn_b200 import kv_cache
+    real, inside, together = kv_cache._lib.lib(), [], []
+
+    class Slow:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def xnq_kv_attend(self, *args):
+            ws, here = args[12].value, threading.get_ident()
+            inside.append((ws, here))
+            time.sleep(0.005)
+            together.extend(other for other in list(inside) if other[0] == ws and other[1] != here)
+            rc = real.xnq_kv_attend(*args)
+            inside.remove((ws, here))
+            return rc
+    c = _filled("q4_0", 1, 2, 256, 64)
+    q, pos = _rand(2, 1, 1, 4, 64).to(DEV), _pos(255)
+    c.attend(q, pos, out=torch.empty_like(q))
+    monkeypatch.setattr(kv_cache._lib, "lib", Slow)
+    threads = [threading.Thread(target=lambda: [c.attend(q, pos, out=torch.empty_like(q)) for _ in range(5)]) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not together and not inside
+
+
+def test_scratch_is_kept_for_a_few_streams():
+    from xn_b200 import kv_cache
+    B, S, H, KV, hd, L = 1, 3, 8, 2, 64, 600
+    c = _filled("q8_0", B, KV, L, hd)
+    q, pos = _rand(3, B, S, H, hd).to(DEV), _pos(L - S)
+    want = c.attend(q, pos, out=torch.empty_like(q))
+    streams = [torch.cuda.Stream() for _ in range(40)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got = c.attend(q, pos, out=torch.empty_like(q))
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(got, want)
+    assert len(kv_cache._workspaces) <= 16

@@ -14,7 +14,9 @@ the batch, padding on the left): it is not stored, and its query gives zeros. Ev
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import threading
 from typing import Optional
 
 import torch
@@ -51,19 +53,24 @@ def _rows(t: torch.Tensor) -> _Rows:
     return _Rows(t.data_ptr(), int(_TORCH_TO_XNQ[t.dtype]), *strides)
 
 
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}   # (device, stream) -> zeroed once; a kernel leaves its counters at zero
+_MOST_WORKSPACES = 16   # streams that have scratch of their own; a call of another one takes and clears its own
+_workspaces: dict[tuple[int, int], tuple[torch.Tensor, threading.Lock]] = {}   # (device, stream) -> zeroed once; a kernel leaves its counters at zero
+_NO_LOCK = contextlib.nullcontext()
 
 
-def _workspace(device: torch.device, need: int) -> torch.Tensor:
-    if torch.cuda.is_current_stream_capturing():   # a graph may be replayed beside others: scratch of its own, zeroed in every replay
+def _workspace(device: torch.device, need: int):
+    """Scratch on the current stream, and the lock to hold while a call that uses it is enqueued (its kernels follow one another on the stream)."""
+    capturing = torch.cuda.is_current_stream_capturing()   # a graph may be replayed beside others: scratch of its own, zeroed in every replay
+    key = (device.index, int(_stream_ptr(device).value or 0))
+    kept = None if capturing else _workspaces.get(key)
+    if kept is not None and kept[0].numel() >= need:
+        return kept
+    if capturing or (kept is None and len(_workspaces) >= _MOST_WORKSPACES):
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         ws[:_ZEROED].zero_()
-        return ws
-    key = (device.index, int(_stream_ptr(device).value or 0))
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < need:
-        ws = _workspaces[key] = torch.zeros(need, dtype=torch.uint8, device=device)
-    return ws
+        return ws, _NO_LOCK
+    kept = _workspaces[key] = (torch.zeros(need, dtype=torch.uint8, device=device), threading.Lock())
+    return kept
 
 
 class QuantizedKVCache:
@@ -202,8 +209,10 @@ class QuantizedKVCache:
         pp, stride = self._positions(pos)
         L = _lib.lib()
         with torch.cuda.device(self.device):
-            ws = _workspace(self.device, max(16, int(L.xnq_kv_attend_workspace_bytes(self.batch, seq, heads, self.kv_heads, self.head_dim))))
-            _lib.check(L.xnq_kv_attend(ctypes.byref(self._view), ctypes.byref(_rows(q)), ctypes.byref(_rows(out)), None if lse is None else ctypes.c_void_p(lse.data_ptr()),
-                                       self.batch, seq, heads, pp, stride, self.head_dim ** -0.5 if scale is None else float(scale), int(causal), int(window),
-                                       ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(self.device)))
+            ws, lock = _workspace(self.device, max(16, int(L.xnq_kv_attend_workspace_bytes(self.batch, seq, heads, self.kv_heads, self.head_dim))))
+            with lock:   # (the interpreter's is free during the call, which may enqueue two kernels)
+                rc = L.xnq_kv_attend(ctypes.byref(self._view), ctypes.byref(_rows(q)), ctypes.byref(_rows(out)), None if lse is None else ctypes.c_void_p(lse.data_ptr()),
+                                     self.batch, seq, heads, pp, stride, self.head_dim ** -0.5 if scale is None else float(scale), int(causal), int(window),
+                                     ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(self.device))
+            _lib.check(rc)
         return out
