@@ -7,7 +7,7 @@ import time
 import pytest
 import torch
 
-from test_gpu_kv_cache import DEV, TYPES, _cache, _check, _filled, _init, _pos, _rand, _reference, _status  # noqa: F401 (_init: the module's fixture)
+from test_gpu_kv_cache import DEV, TYPES, _cache, _check, _filled, _fmt, _init, _pos, _rand, _reference, _status  # noqa: F401 (_init: the module's fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -138,3 +138,29 @@ def test_scratch_is_kept_for_a_few_streams():
         torch.cuda.current_stream().wait_stream(s)
         assert torch.equal(got, want)
     assert len(kv_cache._workspaces) <= 16
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_blocks_with_infinities_and_nans_are_the_oracles(O, fmt, dt):
+    inf, nan = math.inf, math.nan
+    x = _rand(12, 16, 32)
+    x[0], x[1], x[2], x[3] = inf, -inf, nan, 0.0
+    x[4, ::2], x[4, 1::2] = -inf, nan
+    x[5, ::2], x[5, 1::2] = inf, nan
+    x[6, :16], x[6, 16:] = -inf, inf
+    x[7, :16], x[7, 16:] = inf, -inf
+    x[8, 31], x[9, 31], x[10, 31] = inf, -inf, nan
+    x[11, 0], x[11, 31] = nan, -inf
+    x[12], x[12, 5] = nan, 2.0
+    x[13], x[13, 30] = nan, -2.0
+    x[14], x[15] = -0.0, -1e-30
+    x = x.view(1, 4, 2, 64).to(TYPES[dt])
+    c = _cache(fmt, 1, 2, 4, 64)
+    c.store(x.to(DEV), x.flip(1).contiguous().to(DEV), _pos(0))
+    got = c.load(0, 4, dtype=torch.float32)
+    for g, w in zip(got, (x, x.flip(1))):
+        a = w.float().numpy()
+        want = torch.from_numpy(O.to_float(int(_fmt(fmt)), O.from_float(int(_fmt(fmt)), a), a.size).reshape(a.shape)).transpose(1, 2).to(DEV)
+        near = torch.equal if fmt == "q4_0" else lambda p, q: torch.allclose(p, q, rtol=2.0 ** -7, atol=0.0)   # (Q8_0's scale: a product with 1 / 127)
+        assert torch.equal(torch.isnan(g), torch.isnan(want)) and near(torch.nan_to_num(g, nan=0.0), torch.nan_to_num(want, nan=0.0))

@@ -115,7 +115,7 @@ __device__ __forceinline__ Codes8 quantize8(const float (&v)[8]) {
 #pragma unroll
   for (int off = 1; off <= 2; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off)), mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, off));
   float m = mx >= -mn ? mx : mn;
-  if (mx == -INFINITY) m = 0.f; // NaN alone
+  if (mx == -INFINITY && mn == INFINITY) m = 0.f; // NaN alone
   if (__any_sync(0xffffffffu, mx == -mn && mx > 0.f)) { // both signs: whichever comes first
     int at = 64; // twice the place, and the sign; 64: none of this thread's
     const int t = threadIdx.x & 3;
