@@ -164,3 +164,36 @@ def test_blocks_with_infinities_and_nans_are_the_oracles(O, fmt, dt):
         want = torch.from_numpy(O.to_float(int(_fmt(fmt)), O.from_float(int(_fmt(fmt)), a), a.size).reshape(a.shape)).transpose(1, 2).to(DEV)
         near = torch.equal if fmt == "q4_0" else lambda p, q: torch.allclose(p, q, rtol=2.0 ** -7, atol=0.0)   # (Q8_0's scale: a product with 1 / 127)
         assert torch.equal(torch.isnan(g), torch.isnan(want)) and near(torch.nan_to_num(g, nan=0.0), torch.nan_to_num(want, nan=0.0))
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("S", [20, 70, 300])
+@pytest.mark.parametrize("k_gain,v_gain,q_gain", [(1e-3, 1e-6, 1e3), (300.0, 3e3, 1e-2), (1.0, 1e-3, 1.0), (1.0, 1e-6, 1.0), (1e-6, 1.0, 1.0)])
+def test_scales_far_from_one_with_many_rows(fmt, dt, S, k_gain, v_gain, q_gain):
+    """f16 results below its smallest normal number, 2^-14, keep that number's rounding: 2^-25 each."""
+    B, KV, H, hd, L = 1, 2, 8, 128, 700
+    c = _filled(fmt, B, KV, L, hd, k_gain=k_gain, v_gain=v_gain)
+    k, v = c.load(0, L, dtype=torch.float32)
+    q = _rand(9, B, S, H, hd, gain=q_gain).to(TYPES[dt]).to(DEV)
+    want, _, tol = _reference(k, v, q, [L - S])
+    got = c.attend(q, _pos(L - S))
+    if dt == "f16" and v_gain < 1e-2:
+        assert float((got.double() - want).norm()) <= 2.0 ** -10 * float(want.norm()) + 2.0 ** -25 * want.numel() ** 0.5
+    else:
+        _check(got, want, tol, (fmt, dt, S, k_gain, v_gain, q_gain))
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("S", [1, 70, 300])
+@pytest.mark.parametrize("gains", [(0.0, 1e-5, 1.0, 1e-3), (1.0, 1e-5, 30.0, 0.0), (1e-5, 0.0, 1e-3, 1e-5), (1e-4, 1e-5, 1e-4, 1e-6)])
+def test_values_whose_size_changes_from_tile_to_tile(fmt, S, gains):
+    """A whole tile of 32 positions after another, of zeros too, growing and shrinking."""
+    B, KV, H, hd, L = 1, 2, 8, 128, 700
+    c = _cache(fmt, B, KV, L, hd)
+    size = torch.tensor(gains)[torch.arange(L) // 32 % 4][None, :, None, None]
+    c.store(_rand(3, B, L, KV, hd).to(DEV), (_rand(4, B, L, KV, hd) * size).to(DEV), _pos(0))
+    k, v = c.load(0, L, dtype=torch.float32)
+    q = _rand(9, B, S, H, hd, gain=1.5).to(torch.bfloat16).to(DEV)
+    want, _, tol = _reference(k, v, q, [L - S])
+    _check(c.attend(q, _pos(L - S)), want, tol, (fmt, S, gains))

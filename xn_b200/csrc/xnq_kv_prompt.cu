@@ -37,6 +37,7 @@ constexpr int PRODUCER0 = 8, LOADER = 16, SCAN = 17, MMA = 18, PROMPT_THREADS = 
 // Registers a thread: launched with 96; the softmax warps hold two tiles' scores at a time.
 constexpr int LAUNCH_REGS = 96, SOFTMAX_REGS = 144, PRODUCER_REGS = 72, OTHER_REGS = 48;
 static_assert(256 * SOFTMAX_REGS + 256 * PRODUCER_REGS + 128 * OTHER_REGS <= PROMPT_THREADS * LAUNCH_REGS, "an increase beyond what the CTA was launched with waits forever");
+constexpr int MOST_SHIFT = 24;              // the smallest scale, 2^-24, is raised to 1
 constexpr int META_STEPS = 8;               // more than steps are between the scan and softmax
 
 // ---- barriers, bulk copies, tensor memory ----
@@ -337,7 +338,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
           }
           bad = __reduce_or_sync(0xffffffffu, bad);
           mt = Meta{scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[0])))),
-                    scale_shift(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xffffffffu, most[1])))), bad, null[e] ? 1 : 0};
+                    0, bad, null[e] ? 1 : 0};
+          const unsigned v_most = __reduce_max_sync(0xffffffffu, most[1]);
+          mt.v_shift = v_most ? scale_shift(__half2float(__ushort_as_half((unsigned short)v_most))) : MOST_SHIFT; // (zeros: any power does)
         }
         both = both && plain;
         if (lane == 0) meta[((i + e) / STEP_TILES) % META_STEPS][(i + e) % STEP_TILES] = mt;
@@ -543,7 +546,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       if (lane == 0) mbar_arrive(q_ready + 8 * q);
     }
     float ref = -INFINITY, l = 0.f; // the reference: 4 below a maximum when it was set; none yet: -inf
-    int v_ref = 0;                  // O holds the sums times 2^v_ref
+    // O holds the sums times 2^v_ref, the least shift of the tiles so far. (Were it 0 before the first tile, small values would be raised and their weights
+    // lowered by as much, into f16's smallest numbers.)
+    int v_ref = MOST_SHIFT;
     bool alive = true, have_ref = false; // of all 32 rows
     int h2 = 0; // the half at hand
     // Rows with a score more than 2^12 over their reference (or that have none) get another: what they have summed is scaled, P of the half's first tile
