@@ -197,3 +197,18 @@ def test_values_whose_size_changes_from_tile_to_tile(fmt, S, gains):
     q = _rand(9, B, S, H, hd, gain=1.5).to(torch.bfloat16).to(DEV)
     want, _, tol = _reference(k, v, q, [L - S])
     _check(c.attend(q, _pos(L - S)), want, tol, (fmt, S, gains))
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("S", [1, 70])
+@pytest.mark.parametrize("scale", [0.0, 1e-30, -1e-38, 1e-45])
+def test_a_scale_near_nothing_averages_what_is_seen(dt, S, scale):
+    """Also with queries near nothing: a hidden position's weight stays zero however small a score's factor is."""
+    B, KV, H, hd, L = 2, 2, 8, 64, 200
+    c = _filled("q4_0", B, KV, L, hd)
+    k, v = c.load(0, L, dtype=torch.float32)
+    for gain in (1.0, 1e-30):
+        q = _rand(9, B, S, H, hd, gain=gain).to(TYPES[dt]).to(DEV)
+        first = [L - S, 40 - S // 2]
+        want, _, tol = _reference(k, v, q, first, scale=0.0)
+        _check(c.attend(q, _pos(*first), scale=scale), want, tol, (dt, S, scale, gain))

@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
       if (r >= rows) l0 = 0, h0 = INT32_MAX; // no row: its weights are thrown away
       else hi_any = max(hi_any, h0), lo_any = min(lo_any, l0);
       lo_all = max(lo_all, l0), hi_all = min(hi_all, h0);
-      const float f = ldexpf(fabsf(a.scale) * LOG2E, (SPLIT ? 0 : 24) - e);
+      const float f = fmaxf(ldexpf(fabsf(a.scale) * LOG2E, (SPLIT ? 0 : 24) - e), LEAST_FACTOR);
 #pragma unroll
       for (int c = 0; c < 2; c++) { // from the lane that holds row 2 t + c
         const int from = (2 * t + c) * 4;
@@ -851,7 +851,7 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
   const int sms = device < 64 ? g_sms[device] : 0;
   if (!sms) return fail(XNQ_ERR_UNSUPPORTED, "kv_attend: xnq_init has not run for device %d", device);
   a.lse = lse, a.batch = batch, a.seq = seq, a.heads = heads, a.group = heads / cache->kv_heads, a.dtype = q->dtype;
-  a.pos_stride = pos_stride, a.causal = causal, a.pos = pos, a.scale = scale == 0.f ? 1e-30f : scale /* (a masked score is -inf times it) */, a.window = std::min<int64_t>(window, INT32_MAX);
+  a.pos_stride = pos_stride, a.causal = causal, a.pos = pos, a.scale = scale, a.window = std::min<int64_t>(window, INT32_MAX);
   a.tickets = static_cast<unsigned int *>(workspace);
   a.records = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + KV_TICKET_BYTES);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -6,6 +6,9 @@
 namespace xnq {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// What scores are multiplied by is no less: a hidden position's is -inf, whose product with a factor that has sunk to zero is not. (Scores of the
+// operands, below 2^45, times this are nothing, as those of a scale of 0 are.)
+constexpr float LEAST_FACTOR = 1e-30f;
 
 struct AttendArgs {
   KvView c;

@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       int e = top > 0.f && top < INFINITY ? 8 - ilogbf(top) : 0; // the largest |q| to [2^8, 2^9)
       e = max(-100, min(100, e));
       const float up = ldexpf(a.scale < 0.f ? -1.f : 1.f, e); // the scale's sign goes into q
-      f = ldexpf(fabsf(a.scale) * LOG2E, -e);
+      f = fmaxf(ldexpf(fabsf(a.scale) * LOG2E, -e), LEAST_FACTOR);
       const uint32_t dst = base + P::Q0 + q * P::Q_TILE + r * 128;
 #pragma unroll
       for (int c = 0; c < HD / 8; c++) {
