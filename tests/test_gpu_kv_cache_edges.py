@@ -212,3 +212,13 @@ def test_a_scale_near_nothing_averages_what_is_seen(dt, S, scale):
         first = [L - S, 40 - S // 2]
         want, _, tol = _reference(k, v, q, first, scale=0.0)
         _check(c.attend(q, _pos(*first), scale=scale), want, tol, (dt, S, scale, gain))
+
+
+def test_what_a_cache_is_made_of_is_not_replaced():
+    """The kernels hold the addresses of its memory and its page table: both are filled in, never exchanged for others."""
+    c = _cache("q4_0", 2, 2, 64, 64, 32)
+    for name in ("pages", "page_table", "max_seq", "batch", "kv_heads", "head_dim", "page_size", "num_pages", "dtype", "device"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name))
+    c.page_table.copy_(torch.arange(4).view(2, 2))
+    assert c.page_table.data_ptr() == c._view.page_table and c.pages.data_ptr() == c._view.pages

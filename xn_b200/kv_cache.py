@@ -77,8 +77,15 @@ class QuantizedKVCache:
     """Keys and values of ``batch`` sequences of up to ``max_seq`` positions, ``dtype`` blocks (Q4_0, Q8_0), ``head_dim`` 64 or 128.
 
     ``page_size`` (a multiple of 32): the memory is ``num_pages`` pages of that many positions, and ``page_table`` (int32 ``[batch, ceil(max_seq /
-    page_size)]`` on the device, all -1 at first) says which page holds positions ``i * page_size ..`` of a sequence; the program fills it in. Without it
-    every sequence has one run of memory."""
+    page_size)]`` on the device, all -1 at first) says which page holds positions ``i * page_size ..`` of a sequence; the program fills it in (in place: the
+    kernels hold its address, and a cache's attributes are not exchanged). Without it every sequence has one run of memory."""
+
+    _FIXED = frozenset(("pages", "page_table", "dtype", "batch", "kv_heads", "max_seq", "head_dim", "page_size", "num_pages", "device"))
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and name in self.__dict__:
+            raise AttributeError(f"QuantizedKVCache.{name} is fixed when the cache is made" + (": fill it in place" if name in ("pages", "page_table") else ""))
+        super().__setattr__(name, value)
 
     def __init__(self, dtype: GgmlDType, batch: int, kv_heads: int, max_seq: int, head_dim: int, device: torch.device | str = "cuda:0",
                  page_size: Optional[int] = None, num_pages: Optional[int] = None):
