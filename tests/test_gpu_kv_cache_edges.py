@@ -222,3 +222,33 @@ def test_what_a_cache_is_made_of_is_not_replaced():
             setattr(c, name, getattr(c, name))
     c.page_table.copy_(torch.arange(4).view(2, 2))
     assert c.page_table.data_ptr() == c._view.page_table and c.pages.data_ptr() == c._view.pages
+
+
+def test_calls_that_torch_would_have_to_see_through_are_refused():
+    """No gradient, tangent or trace comes out of these calls: with tensors that ask for one they say so."""
+    from torch.autograd import forward_ad
+    B, S, KV, H, hd, L = 1, 2, 2, 4, 64, 64
+    c = _filled("q8_0", B, KV, L, hd)
+    q, k, pos = _rand(1, B, S, H, hd).to(DEV), _rand(2, B, S, KV, hd).to(DEV), _pos(10)
+    qkv, table = _rand(3, B, S, (H + 2 * KV) * hd).to(DEV), torch.zeros(L, hd // 2, device=DEV)
+    want, before = c.attend(q, pos), c.pages.clone()
+    ask = lambda t: t.clone().requires_grad_()
+    calls = [lambda: c.attend(ask(q), pos), lambda: c.attend(ask(q), pos, out=torch.empty_like(q)), lambda: c.attend(ask(q).half(), pos), lambda: c.store(ask(k), k, pos),
+             lambda: c.store(k, ask(k), pos), lambda: c.rope_store(ask(qkv), table, table, pos, H), lambda: c.rope_store(qkv, ask(table), table, pos, H),
+             lambda: torch.func.vmap(lambda t: c.attend(t, pos))(q[None]), lambda: torch.func.grad(lambda t: c.attend(t, pos).sum())(q),
+             lambda: torch.func.jvp(lambda t: c.attend(t, pos), (q,), (q,)), lambda: torch.jit.trace(lambda t: c.attend(t, pos), q, check_trace=False),
+             lambda: torch.jit.trace(lambda t: (c.store(t, k, pos), t + 1)[1], k, check_trace=False)]
+
+    def dual():
+        with forward_ad.dual_level():
+            c.attend(forward_ad.make_dual(q, q), pos)
+    for i, call in enumerate(calls + [dual]):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail(f"call {i}")
+    assert torch.equal(c.pages, before)
+    with torch.no_grad():
+        assert torch.equal(c.attend(ask(q), pos), want) and torch.equal(c.attend(ask(q), pos, out=torch.empty_like(q)), want)
+    with torch.inference_mode():
+        assert torch.equal(c.attend(ask(q), pos), want)
+    assert torch.equal(c.attend(ask(q).detach(), pos), want) and not c.attend(q, pos).requires_grad

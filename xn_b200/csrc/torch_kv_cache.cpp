@@ -3,6 +3,7 @@
 // the host, some four times what its kernels take for a few tokens. Everything that is not ordinary returns None, and the Python code takes the call.
 #include "torch_common.h"
 
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -122,6 +123,8 @@ bool rows(const Cache &c, const at::Tensor &t, xnq_rows *out) {
   }
   return reinterpret_cast<uintptr_t>(out->data) % 16 == 0;
 }
+// A gradient or a tangent is asked for: the Python code refuses the call.
+bool asks(const at::Tensor &t) { return (t.requires_grad() && c10::GradMode::is_enabled()) || t._fw_grad(0).defined(); }
 bool positions(const Cache &c, PyObject *o, const long long **p, int *stride) {
   if (!plain(o)) return false;
   const at::Tensor &t = THPVariable_Unpack(o);
@@ -174,7 +177,7 @@ PyObject *kv_store(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   int stride;
   if (!plain(args[1]) || !plain(args[2]) || observed() || c10::cuda::current_device() != c->device) Py_RETURN_NONE;
   const at::Tensor &kt = THPVariable_Unpack(args[1]), &vt = THPVariable_Unpack(args[2]);
-  if (!rows(*c, kt, &k) || !rows(*c, vt, &v) || k.dtype != v.dtype || kt.size(1) != vt.size(1) || kt.size(2) != c->c.kv_heads || vt.size(2) != c->c.kv_heads ||
+  if (asks(kt) || asks(vt) || !rows(*c, kt, &k) || !rows(*c, vt, &v) || k.dtype != v.dtype || kt.size(1) != vt.size(1) || kt.size(2) != c->c.kv_heads || vt.size(2) != c->c.kv_heads ||
       !positions(*c, args[3], &pos, &stride))
     Py_RETURN_NONE;
   int rc;
@@ -202,7 +205,7 @@ PyObject *kv_rope_store(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   const at::Tensor &x = THPVariable_Unpack(args[1]), &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]);
   const int64_t hd = c->c.head_dim, kv = c->c.kv_heads;
   const int dtype = xnq_dtype(x.scalar_type());
-  if (dtype < 0 || heads < 1 || heads > 65535 || x.dim() != 3 || x.size(0) != c->batch || x.size(1) == 0 || x.size(2) != (heads + 2 * kv) * hd || x.stride(2) != 1 ||
+  if (asks(x) || asks(cos) || asks(sin) || dtype < 0 || heads < 1 || heads > 65535 || x.dim() != 3 || x.size(0) != c->batch || x.size(1) == 0 || x.size(2) != (heads + 2 * kv) * hd || x.stride(2) != 1 ||
       x.device().index() != c->device || !positions(*c, args[4], &pos, &stride))
     Py_RETURN_NONE;
   for (const at::Tensor *t : {&cos, &sin})
@@ -271,7 +274,7 @@ PyObject *kv_attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   xnq_rows q;
   const long long *pos;
   int stride;
-  if (!rows(*c, qt, &q) || qt.size(2) < 1 || qt.size(2) % c->c.kv_heads || !positions(*c, args[2], &pos, &stride)) Py_RETURN_NONE;
+  if (asks(qt) || !rows(*c, qt, &q) || qt.size(2) < 1 || qt.size(2) % c->c.kv_heads || !positions(*c, args[2], &pos, &stride)) Py_RETURN_NONE;
   const int causal = PyObject_IsTrue(args[3]);
   const long long window = PyLong_AsLongLong(args[4]);
   const double scale = PyFloat_AsDouble(args[5]);

@@ -10,7 +10,8 @@ blocks it is 144 bytes, as Q8_0 272. ``QLlama(kv_dtype=...)`` uses it; any other
     k, v = cache.load(0, n)                               # what the blocks stand for
 
 ``pos`` is the position of the first of a call's ``seq`` tokens, one for every sequence or one for all. A token at a negative position is none (an idle slot of
-the batch, padding on the left): it is not stored, and its query gives zeros. Everything is enqueued on the current stream.
+the batch, padding on the left): it is not stored, and its query gives zeros. Everything is enqueued on the current stream. There are no derivatives: tensors
+that require a gradient are refused, but under ``torch.no_grad()``, and so are tracers.
 """
 from __future__ import annotations
 
@@ -20,6 +21,7 @@ import threading
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .dtypes import GgmlDType
@@ -51,6 +53,15 @@ def _served(t: torch.Tensor) -> bool:
 def _rows(t: torch.Tensor) -> _Rows:
     strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]   # of a dimension of one entry torch may say anything
     return _Rows(t.data_ptr(), int(_TORCH_TO_XNQ[t.dtype]), *strides)
+
+
+def _refuse_derivatives(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    """These calls are torch operators of no kind: no gradient, tangent or trace comes out of them, and a call that asks for one says so."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{who} cannot be traced")
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and ((t.requires_grad and torch.is_grad_enabled()) or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None)):
+            raise RuntimeError(f"{who} has no derivative, and one of its tensors asks for it: call it under torch.no_grad(), or with detached tensors")
 
 
 _MOST_WORKSPACES = 16   # streams that have scratch of their own; a call of another one takes and clears its own
@@ -136,6 +147,7 @@ class QuantizedKVCache:
         ``BlockQ4_0`` / ``BlockQ8_0::from_float`` make of the f32 values (k_quants.rs:235-270, 636-661), Q8_0's scale being ``max|x| * float32(1 / 127)``."""
         if self._native.kv_store(self._handle, k, v, pos):
             return
+        _refuse_derivatives("store", k, v)
         self._tokens("k", k, self.kv_heads), self._tokens("v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype is not v.dtype:
             raise ValueError(f"k is {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}")
@@ -148,6 +160,7 @@ class QuantizedKVCache:
             q = self._native.kv_rope_store(self._handle, qkv, cos, sin, pos, heads, -1 if out_dtype is None else _XNQ_IDS[out_dtype])
             if q is not None:
                 return q
+        _refuse_derivatives("rope_store", qkv, cos, sin)
         hd, width = self.head_dim, (heads + 2 * self.kv_heads) * self.head_dim
         if heads < 1 or qkv.dim() != 3 or qkv.shape[2] != width:
             raise ValueError(f"rope_store: qkv is {tuple(qkv.shape)}; {heads} + 2 * {self.kv_heads} heads of {hd}")
@@ -180,6 +193,7 @@ class QuantizedKVCache:
         both = self._native.kv_load(self._handle, start, length, _XNQ_IDS[dtype])
         if both is not None:
             return both
+        _refuse_derivatives("load")
         k = torch.empty((self.batch, self.kv_heads, length, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         sp, stride = self._positions(start, "start") if isinstance(start, torch.Tensor) else (None, 0)
@@ -199,6 +213,7 @@ class QuantizedKVCache:
             res = self._native.kv_attend(self._handle, q, pos, causal, window, self.head_dim ** -0.5 if scale is None else scale)
             if res is not None:
                 return res
+        _refuse_derivatives("attend", q, out, lse)
         self._tokens("q", q)
         heads, seq = q.shape[2], q.shape[1]
         if heads < 1 or heads % self.kv_heads:
