@@ -252,3 +252,21 @@ def test_calls_that_torch_would_have_to_see_through_are_refused():
     with torch.inference_mode():
         assert torch.equal(c.attend(ask(q), pos), want)
     assert torch.equal(c.attend(ask(q).detach(), pos), want) and not c.attend(q, pos).requires_grad
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("S", [1, 6, 70])
+@pytest.mark.parametrize("sizes", [(0.3,), (0.05,), (0.05, 0.7, 0.02, 260.0, 0.3), (300.0, 0.05)])
+def test_values_of_ordinary_and_other_sizes(fmt, dt, S, sizes):
+    """On both sides of the ranges in which scales are taken as they are, and from one side to the other."""
+    B, KV, H, hd, L = 2, 2, 8, 128, 500
+    c = _cache(fmt, B, KV, L, hd)
+    size = torch.tensor(sizes)[torch.arange(L) // 32 % len(sizes)][None, :, None, None]
+    c.store((_rand(3, B, L, KV, hd) * size.clamp(max=1.0)).to(DEV), (_rand(4, B, L, KV, hd) * size).to(DEV), _pos(0))
+    k, v = c.load(0, L, dtype=torch.float32)
+    q = _rand(9, B, S, H, hd, gain=1.5).to(TYPES[dt]).to(DEV)
+    first = [L - S, 333 - S]
+    want, _, tol = _reference(k, v, q, first)
+    _check(c.attend(q, _pos(*first)), want, tol, (fmt, dt, S, sizes))
+    assert _status() == 0

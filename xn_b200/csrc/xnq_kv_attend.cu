@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) d_max = fmaxf(d_max, __shfl_xor_sync(0xffffffffu, d_max, o));
         if (d_max > 0.f && (d_max > d_most || !k_set)) {
-          const int k_new = scale_shift(d_max);
+          const int k_new = scale_shift(d_max, -6, 2);
           o_by = k_set ? ldexpf(1.f, k_new - k) : 0.f;
           k = k_new, k_set = true, d_most = ldexpf(4.f, -k);
         }

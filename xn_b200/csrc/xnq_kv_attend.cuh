@@ -101,10 +101,10 @@ __device__ __forceinline__ uint32_t signed_pair(uint32_t w, int i) { // the same
   }
   return as_u32(__hsub2(as_half2(code_pair<8>(w, i) | 0x64006400u), __float2half2_rn(1152.f)));
 }
-// How much the scales of a run of blocks, the largest of which is `top`, are raised (a power of two): not at all from 2^-6 to 4
-__device__ __forceinline__ int scale_shift(float top) {
+// How much the scales of a run of blocks, the largest of which is `top`, are raised (a power of two): not at all from 2^least to 2^most
+__device__ __forceinline__ int scale_shift(float top, int least, int most) {
   const int e = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
-  return e > 1 || e < -6 ? -e : 0;
+  return e >= most || e < least ? -e : 0;
 }
 __device__ __forceinline__ uint32_t raise_pair(uint32_t d, int k) { // two scales times 2^k, -15 <= k <= 24
   const __half2 by = __float2half2_rn(ldexpf(1.f, min(k, 15))), by2 = __float2half2_rn(ldexpf(1.f, max(k - 15, 0))); // 2^24 is past f16
