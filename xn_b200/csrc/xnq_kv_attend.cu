@@ -20,8 +20,8 @@
 // f32 queries (SPLIT): q and the weights are taken apart into two f16 each (22 bits), and the codes have their zero taken off first and are whole numbers in
 // f16: a subnormal operand's products are summed with the bits that a number of 2^-14 would have, some 2^-18 of the score (an output's error 3e-6 of its
 // norm with 4-bit codes; 5e-7 now, as much as f32 products), and with many weights the two sums in O would cancel. 16-bit queries: q is exact in f16 after a power of two a row, the weights are rounded to f16.
-// Ranges: a row's reference lies 8 below its maximum of the time and is renewed when a score passes it by more than 12, so that nothing need be known
-// of a tile's maximum beforehand; the values' scales are brought near one by a power of two a warp.
+// Ranges: a row's reference lies 8 (8 bits: 11) below its maximum of the time and is renewed when a score passes it by more than 12 (14), so that nothing need
+// be known of a tile's maximum beforehand; the values' scales are brought near one by a power of two a warp.
 //
 // Measured (bf16 queries, 32 heads over 8 of 128): 16 sequences of 8192 positions in Q4_0 blocks 42 us, 64 of 330 to 16384 in pages 144 us (4.1 TB/s of cache),
 // one of 131072 47 us, of 512 9.7 us in a captured step; Q8_0, 16 of 8192, 65 us (4.4 TB/s). Few rows of many positions are bound by instructions: 570 a tile and
@@ -88,11 +88,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) { // of 16-bit valu
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
-template <int HD, int NT>
+template <int BITS, int HD, int NT>
 struct SplitShape {
   static constexpr int R = 8 * NT;        // query rows of an item
   static constexpr int COL = HD + 4;      // floats from row to row of the accumulators in shared memory
   static constexpr int MERGE = SPLIT_WARPS * R * (COL + 2) * 4; // bytes
+  // Ranges of the weights, 2^BELOW at a row's maximum when its reference was set and at most 2^OVER, and of the values' scales, 2^LEAST to 2^MOST before
+  // they are brought near one, so that a weight times a scale stays below 2^16 and is 4 or more at the maximum: f16 holds it to its rounding
+  // down to 2^-16 of that. Q8_0's scales are a sixteenth of Q4_0's for the same values.
+  static constexpr float BELOW = BITS == 4 ? 8.f : 11.f, OVER = BITS == 4 ? 12.f : 14.f;
+  static constexpr int LEAST = BITS == 4 ? -6 : -9, MOST = BITS == 4 ? 2 : 1;
 };
 
 // Parts of items in the workspace, two places a CTA: references [R], sums [R], accumulators [R][HD]. A cut item's ticket is that of the CTA which holds its
@@ -116,7 +121,7 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t *src, cons
 template <int BITS, int HD, int NT, bool SPLIT>
 __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_split_kernel(const AttendArgs a) {
   using L = KvTile<BITS, HD>;
-  using P = SplitShape<HD, NT>;
+  using P = SplitShape<BITS, HD, NT>;
   constexpr int NB = L::NB, W = L::W, R = P::R;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_sum[SPLIT_WARPS];
@@ -493,8 +498,20 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
               if (j < lo[n][c & 1] || j > hi[n][c & 1]) s[u][n][c] = -INFINITY;
             }
       }
-      // One vote a tile: a score over its limit, or (where scales are taken as they are) a scale of two or more, seen in the union of the bits
-      bool look = k != 0 || !k_set;
+      // One vote a tile: a score over its limit, or a scale over the others' range. Where scales are taken as they are: one of two or more, seen in the union
+      // of the bits; else the largest of this lane's. (With a vote that was always taken there, and Q8_0's range as Q4_0's: 64 sequences of 4096
+      // positions, Q8_0, 242 us with values of 0.3 and 135 with values of 0.7; now 137 and 138, and 214 with values of 0.05.)
+      auto largest = [&]() {
+        __half2 d_top = __float2half2_rn(0.f);
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int bl = 0; bl < NB; bl++) d_top = __hmax2(d_top, __habs2(as_half2(dv[u][e][bl])));
+        return fmaxf(__low2float(d_top), __high2float(d_top));
+      };
+      bool look = !k_set;
       {
         uint32_t bits = 0;
 #pragma unroll
@@ -505,6 +522,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
             for (int bl = 0; bl < NB; bl++) bits |= dv[u][e][bl];
         look |= (bits & 0x40004000u) != 0;
       }
+      if (k != 0) look |= largest() > d_most;
       float top[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; n++)
@@ -515,20 +533,13 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
           look |= top[n][c] > limit[n][c];
         }
       if (__any_sync(0xffffffffu, look)) {
-        __half2 d_top = __float2half2_rn(0.f);
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int e = 0; e < 2; e++)
-#pragma unroll
-            for (int bl = 0; bl < NB; bl++) d_top = __hmax2(d_top, __habs2(as_half2(dv[u][e][bl])));
-        float d_max = fmaxf(__low2float(d_top), __high2float(d_top)), o_by = 1.f;
+        float d_max = largest(), o_by = 1.f;
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) d_max = fmaxf(d_max, __shfl_xor_sync(0xffffffffu, d_max, o));
         if (d_max > 0.f && (d_max > d_most || !k_set)) {
-          const int k_new = scale_shift(d_max, -6, 2);
+          const int k_new = scale_shift(d_max, P::LEAST, P::MOST);
           o_by = k_set ? ldexpf(1.f, k_new - k) : 0.f;
-          k = k_new, k_set = true, d_most = ldexpf(4.f, -k);
+          k = k_new, k_set = true, d_most = ldexpf(1.f, P::MOST - k);
         }
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -538,9 +549,9 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_s
             for (int o = 4; o <= 16; o <<= 1) top[n][c] = fmaxf(top[n][c], __shfl_xor_sync(0xffffffffu, top[n][c], o));
             float by = 1.f;
             if (top[n][c] > limit[n][c]) {
-              const float to = top[n][c] - 8.f;
+              const float to = top[n][c] - P::BELOW;
               by = limit[n][c] == -INFINITY ? 0.f : exp2_approx(ref[n][c] - to);
-              ref[n][c] = to, limit[n][c] = to + 12.f, l[n][c] *= by;
+              ref[n][c] = to, limit[n][c] = to + P::OVER, l[n][c] *= by;
             }
             const float a_by = by * o_by;
 #pragma unroll
@@ -743,7 +754,7 @@ int g_sms[64]; // of the devices that xnq_init has seen
 
 template <int BITS, int HD, int NT, bool SPLIT>
 struct SplitLaunch {
-  static constexpr size_t smem() { return SPLIT_WARPS * SPLIT_STAGES * KvTile<BITS, HD>::BYTES + SplitShape<HD, NT>::MERGE; }
+  static constexpr size_t smem() { return SPLIT_WARPS * SPLIT_STAGES * KvTile<BITS, HD>::BYTES + SplitShape<BITS, HD, NT>::MERGE; }
   static inline int per_sm = 0;
   static int init() {
     XNQ_CUDA(cudaFuncSetAttribute(kv_attend_split_kernel<BITS, HD, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem()));
