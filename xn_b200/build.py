@@ -1,5 +1,5 @@
-"""Builds, in-tree, ``libxnq.so`` (the C-ABI CUDA library; nvcc alone, for sm_100a only) and ``_xnq_torch.so`` (the torch side of a linear's call; the host
-compiler, and the headers of the torch that is installed).
+"""Builds, in-tree, ``libxnq.so`` (the C-ABI CUDA library; nvcc alone, for sm_100a only) and ``_xnq_torch.so`` (the torch side of a linear's and of the quantized KV
+cache's calls; the host compiler, and the headers of the torch that is installed).
 
 Usage: ``python -m xn_b200.build [--force] [--library]``.  No other architecture, no PTX fallback.  ``--library``: ``libxnq.so`` alone.
 """
@@ -64,7 +64,7 @@ def torch_sources() -> list[str]:
 
 
 def torch_module_is_stale() -> bool:
-    deps = [*torch_sources(), *(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.startswith("torch_") and f.endswith(".h"))]
+    deps = [*torch_sources(), *(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.startswith("torch_") and f.endswith(".h")), os.path.join(HERE, "..", "include", "xnq.h")]
     if not os.path.exists(TORCH_MODULE) or os.path.getmtime(TORCH_MODULE) < max(os.path.getmtime(p) for p in deps):
         return True
     try:
