@@ -363,7 +363,7 @@ typedef struct xnq_kv_rope {
 size_t xnq_kv_page_bytes(int ggml_dtype, int kv_heads, int head_dim, int64_t page_size); /* 0: not a cache this library serves */
 /* k and v [batch, seq, kv_heads, head_dim] of one type into the cache. k is rotated first with `rope` (may be NULL), in f32. The codes and scales are
  * those of BlockQ4_0 / BlockQ8_0::from_float (k_quants.rs:235-270, 636-661) on the f32 values, bit for bit for Q4_0; Q8_0's scale is max|x| times the
- * f32 nearest 1 / 127 instead of divided by 127. */
+ * f32 nearest 1 / 127 instead of divided by 127, by which a code whose value lies half way between two may be the other one. */
 int xnq_kv_store(const xnq_kv_cache *cache, const xnq_rows *k, const xnq_rows *v, int64_t batch, int64_t seq, const long long *pos, int pos_stride,
                  const xnq_kv_rope *rope, void *stream);
 /* What n positions of every sequence stand for: k_out, v_out [batch, kv_heads, n, head_dim] contiguous, 16-byte aligned. They start at start_dev

@@ -83,9 +83,10 @@ __device__ __forceinline__ void load_words(const uint8_t *p, const uint8_t *p2, 
 }
 
 // One block of 32 in four neighbouring lanes, 8 values each: the arithmetic of BlockQ4_0::from_float and BlockQ8_0::from_float
-// (k_quants.rs:235-270, 636-661), every operation rounded for itself, but for Q8_0's scale: max|x| times the f32 nearest 1 / 127, where the file's quantizer
-// divides by 127 (the two differ in the scale's last f32 bit, one f16 scale in some 4000 and one code at a tie). The codes come back unsigned: 4 bits, eight
-// nibbles in lo; 8 bits, code + 128.
+// (k_quants.rs:235-270, 636-661), every operation rounded for itself, but for Q8_0's scale: max|x| times the f32 nearest 1 / 127, which is what torch makes of
+// a division by 127 on a GPU, where the file's quantizer (and the one of this library's activations) divides. The two differ in the scale's last f32 bit and, by that,
+// in codes where x / scale is a half: 5 of 100000 bf16 values, 7 of a million f16 ones, one in four million f32 ones, by one, to the other side of the tie. No f16
+// scale differs where x is f16 or bf16, one in a few million where it is f32. The codes come back unsigned: 4 bits, eight nibbles in lo; 8 bits, code + 128.
 struct Codes8 {
   uint32_t lo, hi;
   __half d;
