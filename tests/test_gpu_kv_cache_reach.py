@@ -159,3 +159,23 @@ def test_q8_0_blocks_are_the_oracles_but_at_ties(O, dt):
     assert np.all(np.abs(got[0] - want)[same] <= 2.0 ** -10 * np.abs(want)[same])   # the f16 scale's last bit, if that
     if dt != "f32":
         assert np.array_equal(got[0][same], want[same])
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("B,S,H,KV,hd,L", [(1, 1, 8, 2, 128, 131072), (4, 1, 4, 2, 64, 40000), (1, 5, 14, 2, 64, 16384), (1, 64, 8, 2, 128, 8192), (16, 1, 8, 2, 128, 200)])
+def test_f32_queries_are_as_exact_as_f32_products(fmt, B, S, H, KV, hd, L):
+    """At most one and a half times the error that products, weights and sums in f32 have on the same blocks, or 1e-6 of the result's norm."""
+    c = _filled(fmt, B, KV, L, hd, v_gain=0.7)
+    k, v = c.load(0, L, dtype=torch.float32)
+    q = _rand(9, B, S, H, hd, gain=1.5).to(DEV)
+    at = torch.arange(L, device=DEV) > torch.arange(L - S, L, device=DEV)[:, None]
+
+    def result(kind):
+        rows = q.to(kind).view(B, S, KV, H // KV, hd).permute(0, 2, 3, 1, 4).reshape(B, KV, -1, hd)
+        score = (rows @ k.to(kind).transpose(-1, -2) * hd ** -0.5).view(B, KV, H // KV, S, L).masked_fill(at, -math.inf)
+        weight = torch.exp(score - score.amax(-1, keepdim=True))
+        out = (weight.view(B, KV, -1, L) @ v.to(kind)).view(B, KV, H // KV, S, hd) / weight.sum(-1, keepdim=True)
+        return out.permute(0, 3, 1, 2, 4).reshape(B, S, H, hd).double()
+    want = result(torch.float64)
+    error = lambda x: float((x.double() - want).norm() / want.norm())
+    assert error(c.attend(q, _pos(L - S))) <= max(1.5 * error(result(torch.float32)), 1e-6)
