@@ -374,7 +374,8 @@ int xnq_kv_load(const xnq_kv_cache *cache, int64_t batch, const long long *start
  * of sequence b is at p = pos[b] + i and sees j <= p (causal) or j < pos[b] + seq, and with a window > 0 only j > p - window. One that sees nothing gives
  * zeros (lse -inf). q and out [batch, seq, heads, head_dim] have one type; lse (may be NULL): f32 [batch, seq, heads], the natural logarithm of the sum of
  * exponentials. f32 queries: products and sums to f32 accuracy. f16 / bf16: the softmax weights are rounded to f16 before they meet v, and
- * from 64 query rows of a KV head (seq * heads / kv_heads) the keys and values are, too (relative 2^-12 each).
+ * from 64 query rows of a KV head (seq * heads / kv_heads) the keys and values are, too (relative 2^-12 each). Scores are served up to 2^22 in
+ * magnitude; far beyond it a row may come out as NaN.
  * workspace: xnq_kv_attend_workspace_bytes, 16-byte aligned, its first XNQ_KV_WORKSPACE_ZEROED bytes zeroed once after it was allocated
  * (a call leaves them so); one call at a time may use it. */
 #define XNQ_KV_WORKSPACE_ZEROED 4096
