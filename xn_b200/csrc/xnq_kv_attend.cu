@@ -20,7 +20,7 @@
 // f32 queries (SPLIT): q and the weights are taken apart into two f16 each (22 bits), and the codes have their zero taken off first and are whole numbers in
 // f16: a subnormal operand's products are summed with the bits that a number of 2^-14 would have, some 2^-18 of the score, and with many weights the two
 // sums in O would cancel. The instruction's sums cut off what is too small for the larger summand, always downwards, so sixteen positions are summed by themselves and added to
-// O by f32 additions: an output's error is 3e-7 to 5e-7 of its norm at any length (one sum through all of them: 5e-6 for 131072 positions of Q8_0 at 92 us, now 102;
+// O by f32 additions: an output's error is 3e-7 to 5e-7 of its norm at any length (one sum through all of them: 5e-6 for 131072 positions of Q8_0;
 // f32 products 9e-7). 16-bit queries: q is exact in f16 after a power of two a row, the weights are rounded to f16.
 // Ranges: a row's reference lies 8 (8 bits: 11) below its maximum of the time and is renewed when a score passes it by more than 12 (14), so that nothing need
 // be known of a tile's maximum beforehand; the values' scales are brought near one by a power of two a warp.
@@ -120,8 +120,12 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t *src, cons
   }
 }
 
+// CTAs an SM that registers are to leave room for. f32 queries over 128 dims: with three, sums of their own spill (Q4_0, 131072 positions, 78 us against 70,
+// 512 positions 12.7 against 10.7); over 64 dims two are slower (16 sequences of 8192 positions, Q8_0, 51 us against 49).
+constexpr int split_ctas(int hd, int nt, bool split) { return nt == 1 && !(split && hd == 128) ? 3 : 2; }
+
 template <int BITS, int HD, int NT, bool SPLIT>
-__global__ void __launch_bounds__(SPLIT_WARPS * 32, NT == 1 ? 3 : 2) kv_attend_split_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) kv_attend_split_kernel(const AttendArgs a) {
   using L = KvTile<BITS, HD>;
   using P = SplitShape<BITS, HD, NT>;
   constexpr int NB = L::NB, W = L::W, R = P::R;
