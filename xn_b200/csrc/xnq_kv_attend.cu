@@ -25,10 +25,10 @@
 // Ranges: a row's reference lies 8 (8 bits: 11) below its maximum of the time and is renewed when a score passes it by more than 12 (14), so that nothing need
 // be known of a tile's maximum beforehand; the values' scales are brought near one by a power of two a warp.
 //
-// Measured (bf16 queries, 32 heads over 8 of 128): 16 sequences of 8192 positions in Q4_0 blocks 42 us, 64 of 330 to 16384 in pages 144 us (4.1 TB/s of cache),
-// one of 131072 47 us, of 512 9.7 us in a captured step; Q8_0, 16 of 8192, 65 us (4.4 TB/s). Few rows of many positions are bound by instructions: 570 a tile and
-// warp, of which the codes' masks and shifts are the most, 12 warps an SM (with 128 registers and 16 warps it was slower). Few positions are bound by the
-// chain of latencies: positions, first tile, a tile's arithmetic, the meeting of the parts.
+// Measured (bf16 queries, 32 heads over 8 of 128): 16 sequences of 8192 positions in Q4_0 blocks 43 us, 64 of 330 to 16384 in pages 140 us (4.2 TB/s of cache),
+// one of 131072 47 us, of 512 10 us in a captured step; Q8_0, 16 of 8192, 66 us (4.3 TB/s). Few rows of many positions are bound by latency: a tile is one chain of 570
+// instructions a warp, and with 12 warps an SM (128 registers and 16 warps were slower) issue, the ALU, tensor and memory pipes are each busy for less than half
+// of the time. Few positions are bound by the chain of positions, first tile, a tile's arithmetic and the meeting of the parts.
 #include <algorithm>
 #include <cmath>
 
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
   const long long at_least = min((long long)SPLIT_WARPS, max(total / max(items, 1ll), 1ll));
   long long share = max((total + gridDim.x - 1) / gridDim.x, at_least);
   if (share > at_least) share = (share + SPLIT_WARPS - 1) / SPLIT_WARPS * SPLIT_WARPS; // as long for the warps, and fewer parts to join
-  // A run that goes on into a second item pays for another start and end, about as long as 15 tiles take: where a run of a few more tiles keeps every
+  // A run that goes on into a second item pays for another start and end, about as long as START_TILES take: where a run of a few more tiles keeps every
   // CTA within one item, the items are rounded up to whole runs.
   bool whole_runs = false;
   {
@@ -198,8 +198,8 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
       }
     }
   }
-  // Else every item is as long in the list as its tiles and a start and end: with tiles alone the CTAs with many short items were the last (64 sequences of
-  // 330 to 16384 positions: 165 us, now 147).
+  // Else every item is as long in the list as its tiles and a start and end: with tiles alone the CTAs with many short items are the last (64 sequences of
+  // 330 to 16384 positions: 149 us against 143).
   const int lead = whole_runs ? 0 : (int)min((long long)START_TILES, share / 2);
   if (lead) {
     total += items * lead;

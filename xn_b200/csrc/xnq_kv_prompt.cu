@@ -17,7 +17,7 @@
 //
 // Where the row tiles are fewer than the SMs, `splits` CTAs share a tile's positions; a second kernel adds their parts, in order.
 //
-// Measured (bf16, 32 heads over 8 of 128, Q4_0): 2048 tokens at the end of 8192 positions 282 us, 850 TFLOP/s, 512 tokens of their own 17 us. A step of 128 positions
+// Measured (bf16, 32 heads over 8 of 128, Q4_0): 2048 tokens at the end of 8192 positions 285 us, 845 TFLOP/s, 512 tokens of their own 18 us. A step of 128 positions
 // takes about 4500 cycles for two row tiles, of which the tensor core works 2560 and softmax's 2^x 2048 of each scheduler; the rest is roles that wait for one another, and 256
 // CTAs on 148 SMs (the longest first). Two threads a row, or one buffer of scores a tile, were slower.
 #include <algorithm>
