@@ -383,6 +383,49 @@ size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int 
 int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
                   int pos_stride, float scale, int causal, int64_t window, void *workspace, size_t ws_bytes, void *stream);
 
+/* ---- the quantized KV cache between requests: page tables, packed tokens, trees of drafted tokens -----------------------------------------------------
+ * Page tables from request lengths. Entry i of row b is needed when i * page_size < length[b] and, with `first` (may be NULL), when the page reaches past
+ * first[b] or begins before `sinks` (positions below first[b] are seen no more, but for the first `sinks`). `table` receives, for `from` (the table of before;
+ * may be `table` itself, else apart from it): needed entries that are pages as they are; the other needed ones the pages that no such entry names, in
+ * ascending order, row by row; -1 where there are none left, and for every entry that is not needed. room[b]: the positions that sequence b has pages for now
+ * (length[b], or where its first missing page begins); *free_pages: pages that no entry names. A page may be named by several rows (a shared beginning): it
+ * is free when none does. Rows have ceil(max_seq / page_size) entries. Device memory, up to 2^20 pages. workspace: xnq_kv_reserve_workspace_bytes, 16-byte
+ * aligned, of any contents; one call at a time may use it. */
+size_t xnq_kv_reserve_workspace_bytes(int64_t num_pages);
+int xnq_kv_reserve(int32_t *table, int64_t table_stride, const int32_t *from, int64_t from_stride, int64_t batch, int64_t page_size, int64_t num_pages, int64_t max_seq,
+                   const long long *length, const long long *first, int64_t sinks, long long *room, long long *free_pages, void *workspace, size_t ws_bytes, void *stream);
+/* Packed tokens: `tokens` rows, those of sequence 0 first, then sequence 1's .., then rows that are no sequence's. Sequence b brings count[b] tokens, for the
+ * places pos[b] .. of the cache; no more than `longest`, and no more in all than `tokens` (what is beyond is cut off and sets a status bit). Device memory,
+ * the caller's:
+ *   start[batch] = pos; offsets[batch + 1]: sequence b has the rows offsets[b] .. offsets[b + 1] - 1
+ *   sequence[tokens], position[tokens], slot[tokens] (page * page_size + place in the page); each -1 for a row that is no sequence's, position and slot for a token that
+ *     is none (its place is negative or past max_seq), slot for one whose place has no page
+ * With trees (sees and nodes not NULL; longest <= XNQ_KV_TREE_MOST): parents[tokens] holds for each token the index, in its sequence, of the one that it follows,
+ * a smaller one than its own; -1: it follows what is in the cache; -2: it is none (so is one whose parent is none or is no smaller index, and every token of a
+ * sequence at a negative pos). Its position is pos + its depth.
+ *   sees[tokens, ceil(longest / 32)]: bit t of a row: the token sees token t of its tree, itself included; nodes[batch, ..]: the tokens that are not none. */
+#define XNQ_KV_TREE_MOST 256
+typedef struct xnq_kv_plan {
+  int64_t tokens, batch, longest;
+  long long *start, *offsets;
+  int32_t *sequence;
+  long long *position, *slot;
+  uint32_t *sees, *nodes;
+} xnq_kv_plan;
+int xnq_kv_plan_make(const xnq_kv_cache *cache, const long long *pos, int pos_stride, const long long *count, const int32_t *parents, const xnq_kv_plan *plan, void *stream);
+/* xnq_kv_store for packed tokens: k and v [tokens, kv_heads, head_dim] (stride_b is not looked at) go to the plan's slots; with `rope` rotated at its positions. */
+int xnq_kv_store_packed(const xnq_kv_cache *cache, const xnq_rows *k, const xnq_rows *v, const xnq_kv_plan *plan, const xnq_kv_rope *rope, void *stream);
+/* Of each tree the path to the token node[b] (an index in it; -1: none) is kept: its tokens' keys and values move to the places pos[b], pos[b] + 1, ..,
+ * and pos_out[b] becomes the place behind them. What lies behind that is left as it is. */
+int xnq_kv_keep(const xnq_kv_cache *cache, const xnq_kv_plan *plan, const long long *node, long long *pos_out, void *stream);
+/* xnq_kv_attend with first positions that stay visible and for packed tokens. A query at p sees j <= p (causal) or j < pos + its sequence's new tokens, and with
+ * a window > 0 only j > p - window or j < sinks. plan NULL: q and out [batch, seq, heads, head_dim], p = pos[b] + i. Else q, out [tokens, heads, head_dim] and lse
+ * [tokens, heads] (batch, seq, pos and stride_b are not looked at), p the plan's position; with trees a token sees the cache below its tree (p and the window as
+ * above; a window of at least `longest`) and the tokens of its tree that it descends from. A token that is none gives zeros; rows behind the last sequence
+ * are left as they are, or set to zero (lse -inf) with `clear`. Workspace: xnq_kv_attend_workspace_bytes of (batch, seq), or of (plan->batch, plan->longest). */
+int xnq_kv_attend_packed(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
+                         int pos_stride, const xnq_kv_plan *plan, int clear, float scale, int causal, int64_t window, int64_t sinks, void *workspace, size_t ws_bytes, void *stream);
+
 /* Sticky device-side status bits of this library's kernels on the current device (0 = healthy).
  * Bits 0-7, one-row ring kernel: bit 0 a consumer's bounded mbarrier wait expired, bit 1 a producer's, bit 2 a
  * self-check refused an access. Bits 8-15: the same for the fp16 tensor-core kernel. Bits 16-23, integer
@@ -390,7 +433,7 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
  * expired. Bits 24-25: a decode position outside [0, max_seq) reached xnq_rope_kv_store (24) or
  * xnq_attn_decode (25); bit 26: xnq_embed_rows met a token outside the table.
  * Bits 27-29, the quantized KV cache: 27 a position past it was to be stored or read back, 28 attended to, 29 a page table's entry was no page,
- * 30 a wait inside the kernel for many query rows expired.
+ * 30 a wait inside the kernel for many query rows expired; 31 a plan of packed tokens cut off what was more than it holds, or met a parent that is none.
  * Synchronizes the device.
  * No counterpart in the reference (its kernels never wait on anything). */
 int xnq_device_status(unsigned int *bits);

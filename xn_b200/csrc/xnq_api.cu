@@ -270,6 +270,7 @@ int xnq_init(int device) {
   if ((rc = decoder_ops_init()) != XNQ_OK) return rc;
   if ((rc = kv_store_init()) != XNQ_OK) return rc;
   if ((rc = kv_attend_init(device)) != XNQ_OK) return rc;
+  if ((rc = kv_plan_init()) != XNQ_OK) return rc;
   if ((rc = generic_init(device)) != XNQ_OK) return rc;
   return XNQ_OK;
 }
@@ -277,14 +278,15 @@ int xnq_init(int device) {
 int xnq_device_status(unsigned int *bits) {
   clear_error();
   if (!bits) return fail(XNQ_ERR_NULL, "device_status: bits is NULL");
-  unsigned int mv = 0, pf = 0, im = 0, dc = 0, ks = 0, ka = 0;
+  unsigned int mv = 0, pf = 0, im = 0, dc = 0, ks = 0, ka = 0, kp = 0;
   int rc = matvec_status(&mv);
   if (rc == XNQ_OK) rc = prefill_status(&pf);
   if (rc == XNQ_OK) rc = imma_status(&im);
   if (rc == XNQ_OK) rc = decoder_status(&dc);
   if (rc == XNQ_OK) rc = kv_store_status(&ks);
   if (rc == XNQ_OK) rc = kv_attend_status(&ka);
-  *bits = (mv & 0xffu) | ((pf & 0xffu) << 8) | ((im & 0xffu) << 16) | ((dc & 7u) << 24) | (((ks | ka) & 31u) << 27);
+  if (rc == XNQ_OK) rc = kv_plan_status(&kp);
+  *bits = (mv & 0xffu) | ((pf & 0xffu) << 8) | ((im & 0xffu) << 16) | ((dc & 7u) << 24) | (((ks | ka | kp) & 31u) << 27);
   return rc;
 }
 

@@ -344,6 +344,8 @@ int kv_store_status(unsigned int *bits);
 int kv_store_init();
 int kv_attend_status(unsigned int *bits);
 int kv_attend_init(int device);
+int kv_plan_status(unsigned int *bits);
+int kv_plan_init();
 int decoder_status(unsigned int *bits); // 1 rope/store, 2 attention: a position outside [0, max_seq)
 // Activation OPERAND image (XNQ_ACT_OPERAND): up to 64 rows quantized to Q8_K and laid out as the integer tensor-core kernel reads them,
 // so that a producer (add+RMSNorm, SwiGLU) can write them directly and the matmul needs no activation kernel of its own:

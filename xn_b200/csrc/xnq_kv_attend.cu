@@ -31,6 +31,7 @@
 // of the time. Few positions are bound by the chain of positions, first tile, a tile's arithmetic and the meeting of the parts.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "xnq_kv_attend.cuh"
 #include "xnq_quantize_act.cuh"
@@ -42,17 +43,25 @@ __device__ unsigned int g_kv_attend_status;
 
 constexpr int SPLIT_WARPS = 4, SPLIT_STAGES = 3, START_TILES = 12;
 // What sequence b's queries see, as tiles [first, first + count).
-struct Span {
+struct PlainSpan {
   int first, count;
   long long pos;
+  __device__ __forceinline__ int tile(int i) const { return first + i; }
 };
-__device__ __forceinline__ Span span_of(const AttendArgs &a, int b) {
-  Span s;
+struct MoreSpan : Sequence {
+  int row_tiles;
+};
+template <int R>
+__device__ __forceinline__ void span_of(const AttendArgs &a, int b, MoreSpan &s) {
+  static_cast<Sequence &>(s) = sequence_of(a, b);
+  s.row_tiles = (int)(((long long)s.seq * a.group + R - 1) / R);
+}
+template <int R>
+__device__ __forceinline__ void span_of(const AttendArgs &a, int b, PlainSpan &s) {
   s.pos = a.pos[(long long)b * a.pos_stride];
   const long long hi = min(s.pos + a.seq - 1, a.c.max_seq - 1), p0 = max(s.pos, 0ll), lo = a.window ? max(p0 - a.window + 1, 0ll) : 0ll;
   s.first = (int)(min(lo, a.c.max_seq) / KV_TILE);
   s.count = hi < lo ? 0 : (int)(hi / KV_TILE) - s.first + 1;
-  return s;
 }
 __device__ __forceinline__ void load8_any(const void *p, int dtype, long long at, float (&v)[8]) {
   if (dtype == XNQ_F32) load8(static_cast<const float *>(p) + at, v);
@@ -124,8 +133,11 @@ __device__ __forceinline__ void copy_tile(uint32_t dst, const uint8_t *src, cons
 // 512 positions 12.7 against 10.7); over 64 dims two are slower (16 sequences of 8192 positions, Q8_0, 51 us against 49).
 constexpr int split_ctas(int hd, int nt, bool split) { return nt == 1 && !(split && hd == 128) ? 3 : 2; }
 
-template <int BITS, int HD, int NT, bool SPLIT>
+// MORE: first positions that stay visible, packed tokens and trees; the list is then of the tiles that a sequence sees, which may be two runs, and a sequence
+// has as many row tiles as its own tokens take. Which positions of a tile a row sees is a word of 32 bits.
+template <int BITS, int HD, int NT, bool SPLIT, bool MORE>
 __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) kv_attend_split_kernel(const AttendArgs a) {
+  using Span = typename std::conditional<MORE, MoreSpan, PlainSpan>::type;
   using L = KvTile<BITS, HD>;
   using P = SplitShape<BITS, HD, NT>;
   constexpr int NB = L::NB, W = L::W, R = P::R;
@@ -147,16 +159,29 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
   pdl_wait();
 
   // ---- this CTA's run of the flattened list: [t0, t1) of `total` tiles ----
-  const int per_seq = a.c.kv_heads * a.row_tiles; // items of a sequence, all of its count of tiles
+  const int per_seq = MORE ? a.c.kv_heads : a.c.kv_heads * a.row_tiles; // items of a sequence (MORE: of a row tile), all of its count of tiles
   const int batch = (int)a.batch;
-  Span own{0, 0, 0}; // (most batches: the one look at the positions)
-  if ((int)threadIdx.x < batch) own = span_of(a, threadIdx.x);
-  const auto counted = [](int n) { return n ? n + (1ll << 40) : 0ll; }; // tiles, and above them sequences that have some
-  long long mine = counted(own.count);
-  bool look = (int)threadIdx.x < batch && (own.count == 0 || own.pos + a.seq > a.c.max_seq); // a sequence that sees nothing, or that lies past the cache
+  const auto look_up = [&](int b) {
+    Span s;
+    span_of<R>(a, b, s);
+    return s;
+  };
+  Span own{}; // (most batches: the one look at the positions)
+  if ((int)threadIdx.x < batch) own = look_up(threadIdx.x);
+  const auto weight = [](const Span &s) {
+    if constexpr (MORE) return s.row_tiles;
+    else return 1;
+  };
+  const auto counted = [&](const Span &s) { return s.count ? ((long long)s.count + (1ll << 40)) * weight(s) : 0ll; }; // tiles, and above them sequences that have some
+  const auto odd = [&](const Span &s) { // sees nothing, or lies past the cache
+    if constexpr (MORE) return s.here && (s.count == 0 || (!a.offsets && s.pos + a.seq > a.c.max_seq));
+    else return s.count == 0 || s.pos + a.seq > a.c.max_seq;
+  };
+  long long mine = counted(own);
+  bool look = (int)threadIdx.x < batch && odd(own);
   for (int b = threadIdx.x + SPLIT_WARPS * 32; b < batch; b += SPLIT_WARPS * 32) {
-    const Span sp = span_of(a, b);
-    mine += counted(sp.count), look |= sp.count == 0 || sp.pos + a.seq > a.c.max_seq;
+    const Span sp = look_up(b);
+    mine += counted(sp), look |= odd(sp);
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -179,9 +204,10 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
     unsigned runs[4] = {0u, 0u, 0u, 0u};
     if (share <= 24) {
       for (int b = threadIdx.x; b < batch; b += SPLIT_WARPS * 32) {
-        const unsigned n = (unsigned)(b == (int)threadIdx.x ? own.count : span_of(a, b).count);
+        const Span sp = b == (int)threadIdx.x ? own : look_up(b);
+        const unsigned n = (unsigned)sp.count;
 #pragma unroll
-        for (int k = 0; k < 4; k++) runs[k] += (n + (unsigned)more[k] - 1) / (unsigned)more[k];
+        for (int k = 0; k < 4; k++) runs[k] += (n + (unsigned)more[k] - 1) / (unsigned)more[k] * (unsigned)weight(sp);
       }
 #pragma unroll
       for (int k = 0; k < 4; k++) runs[k] = __reduce_add_sync(0xffffffffu, runs[k]);
@@ -210,23 +236,31 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
 
   if (look) // sequences that see nothing: rows of zeros
     for (int b = blockIdx.x; b < batch; b += gridDim.x) {
-      const Span sp = span_of(a, b);
-      if (threadIdx.x == 0 && sp.pos + a.seq > a.c.max_seq) atomicOr(&g_kv_attend_status, KV_PAST_ATTEND);
+      const Span sp = look_up(b);
+      if (threadIdx.x == 0 && !(MORE && a.offsets) && sp.pos + a.seq > a.c.max_seq) atomicOr(&g_kv_attend_status, KV_PAST_ATTEND);
       if (sp.count) continue;
-      for (long long i = threadIdx.x; i < a.seq * a.heads * HD; i += SPLIT_WARPS * 32) {
+      long long seq = a.seq, first = b * a.seq, base = b * a.out.sb;
+      if constexpr (MORE) {
+        if (!sp.here) continue;
+        seq = sp.seq, first = sp.first_row, base = a.offsets ? first * a.out.ss : base;
+      }
+      for (long long i = threadIdx.x; i < seq * a.heads * HD; i += SPLIT_WARPS * 32) {
         const long long row = i / HD, s = row / a.heads;
         const int h = (int)(row - s * a.heads), d = (int)(i - row * HD);
-        store_any(a.out.p, a.dtype, b * a.out.sb + s * a.out.ss + h * a.out.sh + d, 0.f);
-        if (a.lse && d == 0) a.lse[(b * a.seq + s) * a.heads + h] = -INFINITY;
+        store_any(a.out.p, a.dtype, base + s * a.out.ss + h * a.out.sh + d, 0.f);
+        if (a.lse && d == 0) a.lse[(first + s) * a.heads + h] = -INFINITY;
       }
     }
+  if constexpr (MORE) {
+    if (a.offsets && a.clear) clear_behind(a, HD);
+  }
   if (t0 >= t1) return;
   // the sequence of tile t0: a scan of the lengths, a block of threads at a time
   if (threadIdx.x == 0) s_b = batch;
   long long before = 0;
   for (int base = 0; base < batch; base += SPLIT_WARPS * 32) {
-    const Span sp = base == 0 ? own : base + (int)threadIdx.x < batch ? span_of(a, base + threadIdx.x) : Span{0, 0, 0};
-    const long long n = length(sp.count) * per_seq;
+    const Span sp = base == 0 ? own : base + (int)threadIdx.x < batch ? look_up(base + threadIdx.x) : Span{};
+    const long long n = length(sp.count) * per_seq * weight(sp);
     long long inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -255,18 +289,24 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
 
   int turn = 0; // which of the two copies is the item's
   for (long long at = t0; at < t1;) {
-    while (item == per_seq || sp.count == 0) { // on to the next sequence that has tiles
+    while (item == per_seq * weight(sp) || sp.count == 0) { // on to the next sequence that has tiles
       item = 0;
       if (++b >= batch) return; // (only where pos changes under the kernel)
-      sp = span_of(a, b);
+      sp = look_up(b);
     }
-    const int kvh = item / a.row_tiles, rt = item - kvh * a.row_tiles;
+    int row_tiles = a.row_tiles;
+    long long seq = a.seq, lse_row = (long long)b * a.seq, q_at = b * a.q.sb, out_at = b * a.out.sb;
+    if constexpr (MORE) {
+      row_tiles = sp.row_tiles, seq = sp.seq, lse_row = sp.first_row;
+      if (a.offsets) q_at = sp.first_row * a.q.ss, out_at = sp.first_row * a.out.ss;
+    }
+    const int kvh = item / row_tiles, rt = item - kvh * row_tiles;
     const int ta = (int)max(0ll, at - item0 - lead), tb = (int)min((long long)sp.count, t1 - item0 - lead); // tiles [ta, tb) of the item are this CTA's
     if (tb <= ta) { // (a run that ends or starts before the item's first tile)
       at = item0 + length(sp.count), item0 = at, item++;
       continue;
     }
-    const int rows = (int)min((long long)R, a.seq * a.group - (long long)rt * R);
+    const int rows = (int)min((long long)R, seq * a.group - (long long)rt * R);
 
     // ---- start the ring: this warp's tiles are ta + warp, + 4, ...; lane i looks up the page of the i-th of a batch of 32 ----
     const int n_tiles = tb - ta > warp ? (tb - ta - warp + SPLIT_WARPS - 1) / SPLIT_WARPS : 0;
@@ -276,7 +316,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
       if (i < n_tiles) {
         if ((i & 31) == 0) {
           const int mine_i = i + lane;
-          ahead = mine_i < n_tiles ? kv_tile_at(a.c, b, kvh, sp.first + ta + warp + mine_i * SPLIT_WARPS, L::BYTES) : nullptr;
+          ahead = mine_i < n_tiles ? kv_tile_at(a.c, b, kvh, sp.tile(ta + warp + mine_i * SPLIT_WARPS), L::BYTES) : nullptr;
         }
         const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ahead), i & 31));
         const int stage = i % SPLIT_STAGES;
@@ -291,19 +331,21 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
     // ---- the query rows as operands ----
     uint32_t qh[NT][NB][4], ql[SPLIT ? NT : 1][SPLIT ? NB : 1][4]; // [.. ][b][2 step + register]
     float start[SPLIT ? 1 : NT][SPLIT ? 1 : NB][4] = {}, factor[NT][2]; // of columns 2 t, 2 t + 1; start as the sums' registers are
-    int lo[NT][2], hi[NT][2], lo_all = 0, hi_all = INT32_MAX, hi_any = -1, lo_any = INT32_MAX;
+    int lo[MORE ? 1 : NT][2], hi[MORE ? 1 : NT][2], lo_all = 0, hi_all = INT32_MAX, hi_any = -1, lo_any = INT32_MAX;
+    Sight sight[MORE ? NT : 1];                // of this lane's rows
+    const uint32_t *tree[MORE ? NT : 1] = {};  // their bits
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       const int r = n * 8 + g; // this lane's row as an operand's column
       const long long row = (long long)rt * R + r, s = row / a.group;
       const int h = kvh * a.group + (int)(row - s * a.group);
-      if (warp == 0 && t == 0) s_row[turn][r] = b * a.out.sb + s * a.out.ss + h * a.out.sh, s_lse_row[turn][r] = ((long long)b * a.seq + s) * a.heads + h;
+      if (warp == 0 && t == 0) s_row[turn][r] = out_at + s * a.out.ss + h * a.out.sh, s_lse_row[turn][r] = (lse_row + s) * a.heads + h;
       float v[NB][8], top = 0.f;
 #pragma unroll
       for (int bl = 0; bl < NB; bl++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) v[bl][i] = 0.f;
-        if (r < rows) load8_any(a.q.p, a.dtype, b * a.q.sb + s * a.q.ss + h * a.q.sh + bl * 32 + t * 8, v[bl]);
+        if (r < rows) load8_any(a.q.p, a.dtype, q_at + s * a.q.ss + h * a.q.sh + bl * 32 + t * 8, v[bl]);
 #pragma unroll
         for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[bl][i]));
       }
@@ -336,10 +378,17 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
           if (SPLIT) ql[n][bl][i] = pack_half2(lo_v[x] * down, lo_v[y] * down);
         }
       }
-      int l0, h0;
-      seen_by(a, sp.pos, s, l0, h0);
-      if (r >= rows) l0 = 0, h0 = INT32_MAX; // no row: its weights are thrown away
-      else hi_any = max(hi_any, h0), lo_any = min(lo_any, l0);
+      int l0 = 0, h0 = INT32_MAX; // no row: its weights are thrown away
+      if constexpr (MORE) {
+        sight[n] = Sight{0, INT32_MAX};
+        if (r < rows) {
+          sight[n] = sight_of(a, sp, s), l0 = sight[n].lo, h0 = sight[n].hi;
+          tree[n] = a.sees ? a.sees + (sp.first_row + s) * a.words : nullptr;
+        }
+      } else if (r < rows) {
+        seen_by(a, sp.pos, s, l0, h0);
+        hi_any = max(hi_any, h0), lo_any = min(lo_any, l0);
+      }
       lo_all = max(lo_all, l0), hi_all = min(hi_all, h0);
       const float f = fmaxf(ldexpf(fabsf(a.scale) * LOG2E, (SPLIT ? 0 : 24) - e), LEAST_FACTOR);
 #pragma unroll
@@ -350,13 +399,13 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
           for (int bl = 0; bl < NB; bl++)
             start[SPLIT ? 0 : n][SPLIT ? 0 : bl][c] = start[SPLIT ? 0 : n][SPLIT ? 0 : bl][c + 2] = __shfl_sync(0xffffffffu, sum[bl], from) * (-(float)L::ZERO / 16777216.f);
         factor[n][c] = __shfl_sync(0xffffffffu, f, from);
-        lo[n][c] = __shfl_sync(0xffffffffu, l0, from), hi[n][c] = __shfl_sync(0xffffffffu, h0, from);
+        if constexpr (!MORE) lo[n][c] = __shfl_sync(0xffffffffu, l0, from), hi[n][c] = __shfl_sync(0xffffffffu, h0, from);
       }
     }
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) {
       lo_all = max(lo_all, __shfl_xor_sync(0xffffffffu, lo_all, o)), hi_all = min(hi_all, __shfl_xor_sync(0xffffffffu, hi_all, o));
-      lo_any = min(lo_any, __shfl_xor_sync(0xffffffffu, lo_any, o)), hi_any = max(hi_any, __shfl_xor_sync(0xffffffffu, hi_any, o));
+      if constexpr (!MORE) lo_any = min(lo_any, __shfl_xor_sync(0xffffffffu, lo_any, o)), hi_any = max(hi_any, __shfl_xor_sync(0xffffffffu, hi_any, o));
     }
 
     // ---- this warp's tiles ----
@@ -378,14 +427,33 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
       __syncwarp();
       const int stage = i % SPLIT_STAGES;
       const uint8_t *tile = ring + stage * L::BYTES;
-      const int j0 = (sp.first + ta + warp + i * SPLIT_WARPS) * KV_TILE;
-      const bool masked = j0 < lo_all || j0 + KV_TILE - 1 > hi_all;
+      const int j0 = sp.tile(ta + warp + i * SPLIT_WARPS) * KV_TILE;
+      bool masked;
+      uint32_t col[MORE ? NT : 1][2], any = 0u; // MORE, masked: the positions that columns 2 t + c see, and that some row sees
+      if constexpr (MORE) masked = !all_seen(a, lo_all, hi_all, j0);
+      else masked = j0 < lo_all || j0 + KV_TILE - 1 > hi_all;
       if ((gone >> stage) & 1) { // no page: not attended to
         if (lane == 0) atomicOr(&g_kv_attend_status, KV_NO_PAGE);
         __syncwarp();
         continue;
       }
-      if (j0 > hi_any || j0 + KV_TILE - 1 < lo_any) { // (other row tiles of the sequence see it)
+      bool nothing; // (other row tiles of the sequence see it)
+      if constexpr (MORE) {
+        nothing = false;
+        if (masked) {
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            const bool real = n * 8 + g < rows;
+            const uint32_t m = seen_in_tile(a, sight[n], tree[n], sp.pos, j0);
+            any |= real ? m : 0u;
+#pragma unroll
+            for (int c = 0; c < 2; c++) col[n][c] = __shfl_sync(0xffffffffu, m, (2 * t + c) * 4);
+          }
+          any = __reduce_or_sync(0xffffffffu, any);
+          nothing = any == 0u;
+        }
+      } else nothing = j0 > hi_any || j0 + KV_TILE - 1 < lo_any;
+      if (nothing) {
         __syncwarp();
         continue;
       }
@@ -470,7 +538,9 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const int in = u * 16 + e * 8 + 2 * t, j = j0 + in;
-            const uint32_t keep = (j >= lo_any && j <= hi_any ? 0xffffu : 0u) | (j + 1 >= lo_any && j + 1 <= hi_any ? 0xffff0000u : 0u);
+            uint32_t keep;
+            if constexpr (MORE) keep = ((any >> in) & 1u ? 0xffffu : 0u) | ((any >> in) & 2u ? 0xffff0000u : 0u);
+            else keep = (j >= lo_any && j <= hi_any ? 0xffffu : 0u) | (j + 1 >= lo_any && j + 1 <= hi_any ? 0xffff0000u : 0u);
 #pragma unroll
             for (int bl = 0; bl < NB; bl++) {
               uint32_t x = dv[u][e][bl] & keep;
@@ -485,8 +555,13 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
           for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-              const int first = max(lo[n][c] - j0, 0), last = min(hi[n][c] - j0, 31);
-              if (first <= last && (bad >> first) << (31 - last + first)) {
+              bool hit;
+              if constexpr (MORE) hit = (bad & col[n][c]) != 0u;
+              else {
+                const int first = max(lo[n][c] - j0, 0), last = min(hi[n][c] - j0, 31);
+                hit = first <= last && (bad >> first) << (31 - last + first);
+              }
+              if (hit) {
 #pragma unroll
                 for (int x = 0; x < 2 * NB; x++) acc[n][x][c] = acc[n][x][c + 2] = NAN;
               }
@@ -500,8 +575,11 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
           for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-              const int j = j0 + u * 16 + (c >> 1) * 8 + g;
-              if (j < lo[n][c & 1] || j > hi[n][c & 1]) s[u][n][c] = -INFINITY;
+              const int in = u * 16 + (c >> 1) * 8 + g, j = j0 + in;
+              bool hidden;
+              if constexpr (MORE) hidden = !((col[n][c & 1] >> in) & 1u);
+              else hidden = j < lo[n][c & 1] || j > hi[n][c & 1];
+              if (hidden) s[u][n][c] = -INFINITY;
             }
       }
       // One vote a tile: a score over its limit, or a scale over the others' range. Where scales are taken as they are: one of two or more, seen in the union
@@ -766,14 +844,14 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
 
 int g_sms[64]; // of the devices that xnq_init has seen
 
-template <int BITS, int HD, int NT, bool SPLIT>
+template <int BITS, int HD, int NT, bool SPLIT, bool MORE>
 struct SplitLaunch {
   static constexpr size_t smem() { return SPLIT_WARPS * SPLIT_STAGES * KvTile<BITS, HD>::BYTES + SplitShape<BITS, HD, NT>::MERGE; }
   static inline int per_sm = 0;
   static int init() {
-    XNQ_CUDA(cudaFuncSetAttribute(kv_attend_split_kernel<BITS, HD, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem()));
+    XNQ_CUDA(cudaFuncSetAttribute(kv_attend_split_kernel<BITS, HD, NT, SPLIT, MORE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem()));
     int n = 0;
-    XNQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attend_split_kernel<BITS, HD, NT, SPLIT>, SPLIT_WARPS * 32, smem()));
+    XNQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attend_split_kernel<BITS, HD, NT, SPLIT, MORE>, SPLIT_WARPS * 32, smem()));
     per_sm = std::max(1, std::min(n, 4));
     return XNQ_OK;
   }
@@ -793,37 +871,50 @@ int split_nt(int bits, int64_t rows, int64_t heads, int sms) {
 // 54, 309 against 136.
 constexpr int64_t PROMPT_ROWS = 64;
 
-template <int BITS, int HD, int NT, bool SPLIT>
+template <int BITS, int HD, int NT, bool SPLIT, bool MORE>
 int run_split(AttendArgs a, int sms, cudaStream_t s) {
-  const int64_t rows = a.seq * a.group;
+  const int64_t rows = std::min<int64_t>(a.seq * a.group, MORE ? a.rows_to - 1 : INT64_MAX);
   a.row_tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
-  using Launch = SplitLaunch<BITS, HD, NT, SPLIT>;
+  if (MORE && a.batch * a.row_tiles >= 1 << 22) return fail(XNQ_ERR_SIZE, "kv_attend: %lld x %lld query rows are more than one launch takes", (long long)a.batch, (long long)rows);
+  using Launch = SplitLaunch<BITS, HD, NT, SPLIT, MORE>;
   // no more CTAs than the longest caches could fill
   const int64_t most = a.batch * a.c.kv_heads * a.row_tiles * ((a.c.max_seq + KV_TILE - 1) / KV_TILE);
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(std::min(sms * Launch::per_sm, MAX_SPLIT_GRID), std::max<int64_t>(most, a.batch)));
-  XNQ_CUDA(launch_pdl(kv_attend_split_kernel<BITS, HD, NT, SPLIT>, dim3((unsigned)grid), dim3(SPLIT_WARPS * 32), Launch::smem(), s, a));
+  XNQ_CUDA(launch_pdl(kv_attend_split_kernel<BITS, HD, NT, SPLIT, MORE>, dim3((unsigned)grid), dim3(SPLIT_WARPS * 32), Launch::smem(), s, a));
   count_launch();
   return XNQ_OK;
 }
 
 template <typename F>
-int for_each_split(F f) { // f<BITS, HD, NT, SPLIT>()
+int for_each_split(F f) { // f(a launch)
   int rc = XNQ_OK;
   auto one = [&](auto l) {
     if (rc == XNQ_OK) rc = f(l);
   };
-  one(SplitLaunch<4, 64, 1, false>{}), one(SplitLaunch<4, 64, 2, false>{}), one(SplitLaunch<4, 64, 1, true>{}), one(SplitLaunch<4, 64, 2, true>{});
-  one(SplitLaunch<4, 128, 1, false>{}), one(SplitLaunch<4, 128, 2, false>{}), one(SplitLaunch<4, 128, 1, true>{}), one(SplitLaunch<4, 128, 2, true>{});
-  one(SplitLaunch<8, 64, 1, false>{}), one(SplitLaunch<8, 64, 2, false>{}), one(SplitLaunch<8, 64, 1, true>{}), one(SplitLaunch<8, 64, 2, true>{});
-  one(SplitLaunch<8, 128, 1, false>{}), one(SplitLaunch<8, 128, 2, false>{}), one(SplitLaunch<8, 128, 1, true>{}), one(SplitLaunch<8, 128, 2, true>{});
+  auto both = [&](auto bits, auto hd) {
+    constexpr int B = decltype(bits)::value, H = decltype(hd)::value;
+    one(SplitLaunch<B, H, 1, false, false>{}), one(SplitLaunch<B, H, 2, false, false>{}), one(SplitLaunch<B, H, 1, true, false>{}), one(SplitLaunch<B, H, 2, true, false>{});
+    one(SplitLaunch<B, H, 1, false, true>{}), one(SplitLaunch<B, H, 2, false, true>{}), one(SplitLaunch<B, H, 1, true, true>{}), one(SplitLaunch<B, H, 2, true, true>{});
+  };
+  const std::integral_constant<int, 4> four;
+  const std::integral_constant<int, 8> eight;
+  const std::integral_constant<int, 64> hd64;
+  const std::integral_constant<int, 128> hd128;
+  both(four, hd64), both(four, hd128), both(eight, hd64), both(eight, hd128);
   return rc;
 }
 
-template <int BITS, int HD>
+template <int BITS, int HD, bool MORE>
 int run_attend(const AttendArgs &a, int sms, cudaStream_t s) {
-  const bool one = split_nt(BITS, a.seq * a.group, a.batch * a.c.kv_heads, sms) == 1;
-  if (a.dtype == XNQ_F32) return one ? run_split<BITS, HD, 1, true>(a, sms, s) : run_split<BITS, HD, 2, true>(a, sms, s);
-  return one ? run_split<BITS, HD, 1, false>(a, sms, s) : run_split<BITS, HD, 2, false>(a, sms, s);
+  const int64_t rows = std::min<int64_t>(a.seq * a.group, MORE ? a.rows_to - 1 : INT64_MAX);
+  const bool one = split_nt(BITS, rows, a.batch * a.c.kv_heads, sms) == 1;
+  if (a.dtype == XNQ_F32) return one ? run_split<BITS, HD, 1, true, MORE>(a, sms, s) : run_split<BITS, HD, 2, true, MORE>(a, sms, s);
+  return one ? run_split<BITS, HD, 1, false, MORE>(a, sms, s) : run_split<BITS, HD, 2, false, MORE>(a, sms, s);
+}
+template <bool MORE>
+int run_attend(const AttendArgs &a, int bits, int head_dim, int sms, cudaStream_t s) {
+  if (bits == 4) return head_dim == 64 ? run_attend<4, 64, MORE>(a, sms, s) : run_attend<4, 128, MORE>(a, sms, s);
+  return head_dim == 64 ? run_attend<8, 64, MORE>(a, sms, s) : run_attend<8, 128, MORE>(a, sms, s);
 }
 
 } // namespace
@@ -847,18 +938,11 @@ int kv_attend_init(int device) {
 
 using namespace xnq;
 
-extern "C" {
-
-size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim) {
-  if (batch <= 0 || seq <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
-  // (for the kernel for many rows at its most: a part for every SM)
-  return KV_TICKET_BYTES + std::max(RECORDS_BYTES, seq * (heads / kv_heads) >= PROMPT_ROWS ? kv_prompt_parts_bytes(head_dim) : 0);
-}
-
-int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
-                  int pos_stride, float scale, int causal, int64_t window, void *workspace, size_t ws_bytes, void *stream) {
-  clear_error();
-  AttendArgs a{};
+namespace {
+// The checks and arguments of both forms (nothing more where batch or seq is 0).
+int attend_args(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos, int pos_stride, float scale,
+                int causal, int64_t window, void *workspace, size_t ws_bytes, AttendArgs *args, int *sms) {
+  AttendArgs &a = *args;
   int rc = kv_view("kv_attend", cache, batch, &a.c);
   if (rc != XNQ_OK) return rc;
   if (!q || !out || !pos) return fail(XNQ_ERR_NULL, "kv_attend: NULL argument");
@@ -873,17 +957,67 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(XNQ_ERR_ALIGN, "kv_attend: the workspace must be 16-byte aligned");
   int device = 0;
   XNQ_CUDA(cudaGetDevice(&device));
-  const int sms = device < 64 ? g_sms[device] : 0;
-  if (!sms) return fail(XNQ_ERR_UNSUPPORTED, "kv_attend: xnq_init has not run for device %d", device);
+  *sms = device < 64 ? g_sms[device] : 0;
+  if (!*sms) return fail(XNQ_ERR_UNSUPPORTED, "kv_attend: xnq_init has not run for device %d", device);
   a.lse = lse, a.batch = batch, a.seq = seq, a.heads = heads, a.group = heads / cache->kv_heads, a.dtype = q->dtype;
   a.pos_stride = pos_stride, a.causal = causal, a.pos = pos, a.scale = scale, a.window = std::min<int64_t>(window, INT32_MAX);
   a.tickets = static_cast<unsigned int *>(workspace);
   a.records = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + KV_TICKET_BYTES);
+  return XNQ_OK;
+}
+} // namespace
+
+extern "C" {
+
+size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim) {
+  if (batch <= 0 || seq <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+  // (for the kernel for many rows at its most: a part for every SM)
+  return KV_TICKET_BYTES + std::max(RECORDS_BYTES, seq * (heads / kv_heads) >= PROMPT_ROWS ? kv_prompt_parts_bytes(head_dim) : 0);
+}
+
+int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
+                  int pos_stride, float scale, int causal, int64_t window, void *workspace, size_t ws_bytes, void *stream) {
+  clear_error();
+  AttendArgs a{};
+  int sms = 0;
+  const int rc = attend_args(cache, q, out, lse, batch, seq, heads, pos, pos_stride, scale, causal, window, workspace, ws_bytes, &a, &sms);
+  if (rc != XNQ_OK || batch == 0 || seq == 0) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int bits = kv_bits(cache->ggml_dtype);
-  if (q->dtype != XNQ_F32 && seq * a.group >= PROMPT_ROWS) return launch_kv_prompt(a, bits, cache->head_dim, sms, s);
-  if (bits == 4) return cache->head_dim == 64 ? run_attend<4, 64>(a, sms, s) : run_attend<4, 128>(a, sms, s);
-  return cache->head_dim == 64 ? run_attend<8, 64>(a, sms, s) : run_attend<8, 128>(a, sms, s);
+  if (q->dtype != XNQ_F32 && seq * a.group >= PROMPT_ROWS) return launch_kv_prompt(a, false, bits, cache->head_dim, sms, s);
+  return run_attend<false>(a, bits, cache->head_dim, sms, s);
+}
+
+int xnq_kv_attend_packed(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
+                         int pos_stride, const xnq_kv_plan *plan, int clear, float scale, int causal, int64_t window, int64_t sinks, void *workspace, size_t ws_bytes, void *stream) {
+  clear_error();
+  if (sinks < 0) return fail(XNQ_ERR_SHAPE, "kv_attend: sinks %lld", (long long)sinks);
+  if (plan) {
+    const int rc = kv_plan_check("kv_attend", plan);
+    if (rc != XNQ_OK) return rc;
+    if (plan->sees && window > 0 && window < plan->longest)
+      return fail(XNQ_ERR_SHAPE, "kv_attend: a window of %lld is shorter than trees of up to %lld tokens", (long long)window, (long long)plan->longest);
+    batch = plan->batch, seq = plan->longest, pos = plan->start, pos_stride = 1;
+  }
+  AttendArgs a{};
+  int sms = 0;
+  const int rc = attend_args(cache, q, out, lse, batch, seq, heads, pos, pos_stride, scale, causal, window, workspace, ws_bytes, &a, &sms);
+  if (rc != XNQ_OK || batch == 0 || seq == 0 || (plan && plan->tokens == 0)) return rc;
+  a.sinks = window ? std::min<int64_t>(sinks, INT32_MAX) : 0, a.rows_to = INT64_MAX;
+  if (plan) {
+    a.tokens = plan->tokens, a.offsets = plan->offsets, a.position = plan->position, a.start = plan->start, a.sees = plan->sees, a.nodes = plan->nodes;
+    a.words = (int)((plan->longest + 31) / 32), a.clear = clear;
+    a.seq = std::min<int64_t>(plan->longest, plan->tokens);
+  }
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int bits = kv_bits(cache->ggml_dtype), hd = cache->head_dim;
+  if (q->dtype == XNQ_F32 || a.seq * a.group < PROMPT_ROWS) return run_attend<true>(a, bits, hd, sms, s);
+  if (!plan || batch == 1) return launch_kv_prompt(a, true, bits, hd, sms, s);
+  // Sequences of their own numbers of tokens: each goes to the kernel for its number of rows.
+  AttendArgs few = a;
+  a.rows_from = few.rows_to = PROMPT_ROWS, few.clear = 0;
+  const int rc2 = launch_kv_prompt(a, true, bits, hd, sms, s);
+  return rc2 != XNQ_OK ? rc2 : run_attend<true>(few, bits, hd, sms, s);
 }
 
 } // extern "C"

@@ -21,6 +21,12 @@ struct AttendArgs {
   int row_tiles, splits;  // tiles of query rows of a KV head; CTAs that share a row tile's positions (many rows)
   unsigned int *tickets;  // KV_TICKETS words, zero between calls
   float *records;         // parts of rows
+  // What the kernels look at in their second form (MORE): first positions that stay visible, and packed tokens (offsets null: none).
+  long long sinks, tokens;
+  const long long *offsets, *position, *start;
+  const uint32_t *sees, *nodes; // null: no trees
+  int words, clear;             // words of a token's bits; rows behind the last sequence: zeros
+  long long rows_from, rows_to; // this launch's sequences: those with that many query rows of a KV head, [from, to)
 };
 
 // Workspace: the tickets, at one place whatever the call, then the parts.
@@ -33,7 +39,7 @@ constexpr unsigned KV_WAIT = 8; // status: a wait of the kernel for many rows ex
 int kv_prompt_init(int device);
 int kv_prompt_status(unsigned int *bits);
 size_t kv_prompt_parts_bytes(int head_dim);
-int launch_kv_prompt(const AttendArgs &a, int bits, int head_dim, int sms, cudaStream_t s);
+int launch_kv_prompt(const AttendArgs &a, bool more, int bits, int head_dim, int sms, cudaStream_t s);
 
 #ifdef __CUDACC__
 // positions [lo, hi] that the query at token s of a sequence at `pos` sees
@@ -42,6 +48,73 @@ __device__ __forceinline__ void seen_by(const AttendArgs &a, long long pos, long
   const long long h = p < 0 ? -1 : min(a.causal ? p : pos + a.seq - 1, a.c.max_seq - 1);
   const long long l = a.window ? max(p - a.window + 1, 0ll) : 0ll;
   hi = (int)h, lo = (int)min(l, a.c.max_seq);
+}
+// What a sequence's queries are, and which tiles of the cache they see between them: the first `head` and `count - head` more, `gap` tiles on.
+struct Sequence {
+  long long pos, first_row; // place of its first token; its first row among all tokens
+  int seq, head, gap, count;
+  bool here;                // of this launch
+  __device__ __forceinline__ int tile(int i) const { return i < head ? i : i + gap; }
+};
+// tiles of what tokens [s0, s1] of the sequence see
+__device__ __forceinline__ void tiles_seen(const AttendArgs &a, Sequence &x, long long s0, long long s1) {
+  const long long end = a.sees || !a.causal ? x.pos + x.seq - 1 : x.pos + s1, hi = min(end, a.c.max_seq - 1);
+  const long long p0 = max(a.sees ? x.pos : x.pos + s0, 0ll), lo = a.window ? min(max(p0 - a.window + 1, 0ll), a.c.max_seq) : 0ll;
+  const int first = (int)(lo / KV_TILE);
+  x.head = hi < 0 ? 0 : min((int)((min(a.sinks, hi + 1) + KV_TILE - 1) / KV_TILE), first);
+  x.gap = first - x.head;
+  x.count = x.head + (hi < lo ? 0 : (int)(hi / KV_TILE) - first + 1);
+}
+__device__ __forceinline__ Sequence sequence_of(const AttendArgs &a, int b) {
+  Sequence x;
+  if (a.offsets) {
+    x.pos = a.start[b], x.first_row = a.offsets[b], x.seq = (int)(a.offsets[b + 1] - x.first_row);
+    const long long rows = (long long)x.seq * a.group;
+    x.here = rows >= a.rows_from && rows < a.rows_to;
+  } else x.pos = a.pos[(long long)b * a.pos_stride], x.first_row = b * a.seq, x.seq = (int)a.seq, x.here = true;
+  x.head = x.gap = x.count = 0;
+  if (x.here && x.seq > 0) tiles_seen(a, x, 0, x.seq - 1);
+  return x;
+}
+// What one of a sequence's tokens sees: positions [lo, hi], the first `sinks` up to hi, and tokens of its tree (whose first is at place pos).
+struct Sight {
+  int lo, hi;
+};
+__device__ __forceinline__ Sight sight_of(const AttendArgs &a, const Sequence &x, long long s) {
+  const long long p = a.offsets ? a.position[x.first_row + s] : x.pos + s;
+  const long long h = p < 0 ? -1 : min(a.sees ? x.pos - 1 : a.causal ? p : x.pos + x.seq - 1, a.c.max_seq - 1);
+  const long long l = a.window ? min(max(p - a.window + 1, 0ll), a.c.max_seq) : 0ll;
+  return Sight{(int)l, (int)h};
+}
+__device__ __forceinline__ uint32_t bits_between(int from, int to) { // bits [from, to] of 32
+  from = max(from, 0), to = min(to, 31);
+  return from <= to ? (0xffffffffu >> (31 - to + from)) << from : 0u;
+}
+__device__ __forceinline__ uint32_t bits_at(const uint32_t *row, int words, int off) { // 32 bits from bit `off` on (it may be negative, or past the row)
+  if (off <= -32 || off >= words * 32) return 0u;
+  if (off < 0) return row[0] << -off;
+  const int w = off >> 5;
+  return __funnelshift_r(row[w], w + 1 < words ? row[w + 1] : 0u, off & 31);
+}
+// of the 32 positions from j0 on; row: the token's bits
+__device__ __forceinline__ uint32_t seen_in_tile(const AttendArgs &a, const Sight &v, const uint32_t *row, long long pos, int j0) {
+  uint32_t m = bits_between(v.lo - j0, v.hi - j0) | bits_between(-j0, (int)min(a.sinks - 1, (long long)v.hi) - j0);
+  if (row && j0 + KV_TILE > pos) m |= bits_at(row, a.words, (int)(j0 - pos));
+  return m;
+}
+// whether every one of some tokens sees all of a tile: lo and hi are the largest and the smallest of theirs
+__device__ __forceinline__ bool all_seen(const AttendArgs &a, int lo, int hi, int j0) { return j0 + KV_TILE - 1 <= hi && (j0 >= lo || j0 + KV_TILE <= a.sinks); }
+// Rows behind the last sequence: zeros. By every block of a launch.
+__device__ __forceinline__ void clear_behind(const AttendArgs &a, int head_dim) {
+  const int chunks = a.heads * (head_dim * (a.dtype == XNQ_F32 ? 4 : 2) / 16), each = chunks / a.heads;
+  for (long long t = a.offsets[a.batch] + blockIdx.x; t < a.tokens; t += gridDim.x)
+    for (int i = threadIdx.x; i < chunks; i += blockDim.x) {
+      const int h = i / each, x = i - h * each;
+      const long long row = t * a.out.ss + h * a.out.sh;
+      uint8_t *const p = static_cast<uint8_t *>(a.out.p) + row * (a.dtype == XNQ_F32 ? 4 : 2) + x * 16;
+      *reinterpret_cast<uint4 *>(p) = make_uint4(0u, 0u, 0u, 0u);
+      if (a.lse && x == 0) a.lse[t * a.heads + h] = -INFINITY;
+    }
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);

@@ -77,10 +77,11 @@ int kv_dispatch(int bits, int head_dim, int dtype, F f) {
 }
 
 int kv_view(const char *who, const xnq_kv_cache *c, int64_t batch, KvView *v); // checks the descriptor
+int kv_plan_check(const char *who, const xnq_kv_plan *p);
 
 // status bits (xnq_device_status bits 27 and up): a position past the cache was asked for, by a store or load (1) or by attention (2); a page table's
-// entry was outside the cache (4)
-constexpr unsigned KV_PAST_STORE = 1, KV_PAST_ATTEND = 2, KV_NO_PAGE = 4;
+// entry was outside the cache (4); a plan of packed tokens cut something off (16)
+constexpr unsigned KV_PAST_STORE = 1, KV_PAST_ATTEND = 2, KV_NO_PAGE = 4, KV_PLAN_CUT = 16;
 
 #ifdef __CUDACC__
 // The tile of (sequence, head) that holds positions 32 * tile .. ; null where the page table has no page there.

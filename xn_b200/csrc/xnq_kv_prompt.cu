@@ -212,7 +212,8 @@ struct Meta { // of a tile
 // In a run of 8 positions, the place of pair i is taken by pair (i + run) & 3: what lies at column n of a tile
 __host__ __device__ constexpr int position_at(int n) { return (n & ~7) | ((((n >> 1) + (n >> 3)) & 3) << 1) | (n & 1); }
 
-template <int BITS, int HD, int QT>
+// MORE: first positions that stay visible, packed tokens and trees; a CTA's tiles may then be two runs of the cache.
+template <int BITS, int HD, int QT, bool MORE>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(const __grid_constant__ AttendArgs a) {
   using P = PromptShape<BITS, HD, QT>;
   using L = KvTile<BITS, HD>;
@@ -227,6 +228,15 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - (uint32_t)__cvta_generic_to_shared(smem_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
+  if constexpr (MORE) {
+    if (a.offsets) { // (before this CTA takes anything: most of a ragged batch's grid has no rows)
+      pdl_wait();
+      const int per = (int)a.batch * a.c.kv_heads * a.splits, bk = (int)(blockIdx.x % per) / a.splits, b = bk / a.c.kv_heads;
+      if (a.clear) clear_behind(a, HD);
+      const long long all_rows = (a.offsets[b + 1] - a.offsets[b]) * a.group;
+      if (all_rows < a.rows_from || (a.row_tiles - 1 - (int)(blockIdx.x / per)) * (long long)(QT * 128) >= all_rows) return;
+    }
+  }
   const uint32_t raw_full = bar, raw_scanned = bar + 16 * 8, raw_empty = bar + 32 * 8, k_full = bar + 48 * 8, k_empty = k_full + 8 * RING, v_full = k_empty + 8 * RING, v_empty = v_full + 8 * RING,
                  s_full = v_empty + 8 * RING, p_full = s_full + 32, pv_done = p_full + 32, o_done = pv_done + 16, q_ready = o_done + 16; // s_full, p_full: [row tile][buffer] (softmax may be two halves ahead of the MMAs)
   if (threadIdx.x == 0) {
@@ -254,16 +264,39 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   // ---- which rows, which positions; the row tiles with the most positions first ----
   const int per = (int)a.batch * a.c.kv_heads * a.splits, rem = (int)(blockIdx.x % per);
   const int rt = a.row_tiles - 1 - (int)(blockIdx.x / per), split = rem % a.splits, bk = rem / a.splits, kvh = bk % a.c.kv_heads, b = bk / a.c.kv_heads;
-  const long long all_rows = a.seq * a.group, row0 = (long long)rt * (QT * 128);
+  Sequence sq; // MORE
+  long long all_rows = a.seq * a.group, q_at = b * a.q.sb, out_at = b * a.out.sb, lse_row = (long long)b * a.seq;
+  const long long row0 = (long long)rt * (QT * 128);
+  if constexpr (MORE) {
+    sq = sequence_of(a, b);
+    all_rows = (long long)sq.seq * a.group, lse_row = sq.first_row;
+    if (a.offsets) q_at = sq.first_row * a.q.ss, out_at = sq.first_row * a.out.ss;
+  }
   const int rows = (int)min((long long)(QT * 128), all_rows - row0);
-  const long long pos = a.pos[(long long)b * a.pos_stride], s_first = row0 / a.group, s_end = (row0 + rows - 1) / a.group;
-  const long long hi_l = pos + s_end < 0 ? -1 : min(a.causal ? pos + s_end : pos + a.seq - 1, a.c.max_seq - 1);
-  const long long lo_l = a.window ? min(max(max(pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0ll;
-  const int hi = (int)hi_l, lo = (int)lo_l, tiles = hi < lo ? 0 : hi / KV_TILE - lo / KV_TILE + 1;
+  const long long s_first = row0 / a.group, s_end = (row0 + rows - 1) / a.group;
+  long long pos;
+  int hi, lo, tiles;
+  if constexpr (MORE) {
+    pos = sq.pos;
+    tiles_seen(a, sq, s_first, s_end);
+    tiles = sq.count;
+    // what the rows see of the cache, but for the first positions and a tree's tokens
+    hi = (int)max(min(a.sees ? pos - 1 : a.causal ? pos + s_end : pos + sq.seq - 1, a.c.max_seq - 1), -1ll);
+    lo = a.window ? (int)min(max(max(a.sees ? pos : pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0;
+  } else {
+    pos = a.pos[(long long)b * a.pos_stride];
+    const long long hi_l = pos + s_end < 0 ? -1 : min(a.causal ? pos + s_end : pos + a.seq - 1, a.c.max_seq - 1);
+    const long long lo_l = a.window ? min(max(max(pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0ll;
+    hi = (int)hi_l, lo = (int)lo_l, tiles = hi < lo ? 0 : hi / KV_TILE - lo / KV_TILE + 1;
+  }
   const int steps_all = (tiles + STEP_TILES - 1) / STEP_TILES, steps_each = (steps_all + a.splits - 1) / a.splits, step0 = min(split * steps_each, steps_all);
   const int n = min(steps_all - step0, steps_each); // steps of this CTA
-  const int t0 = lo / KV_TILE + step0 * STEP_TILES, n_tiles = min(tiles - step0 * STEP_TILES, n * STEP_TILES);
-  if (threadIdx.x == 0 && pos + a.seq > a.c.max_seq) atomicOr(&g_kv_prompt_status, KV_PAST_ATTEND);
+  const int t0 = (MORE ? 0 : lo / KV_TILE) + step0 * STEP_TILES, n_tiles = min(tiles - step0 * STEP_TILES, n * STEP_TILES);
+  const auto tile_of = [&](int i) { // this CTA's i-th tile, in the cache
+    if constexpr (MORE) return sq.tile(t0 + i);
+    else return t0 + i;
+  };
+  if (threadIdx.x == 0 && !(MORE && a.offsets) && pos + a.seq > a.c.max_seq) atomicOr(&g_kv_prompt_status, KV_PAST_ATTEND);
   volatile int *const dead = &s_dead;
 
   if (warp >= LOADER) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
@@ -272,7 +305,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     int i = 0;
     for (; i < n * STEP_TILES; i++) {
       const int slot = i % P::SLOTS, lap = i / P::SLOTS;
-      if ((i & 31) == 0) ahead = i + lane < n_tiles ? kv_tile_at(a.c, b, kvh, t0 + i + lane, L::BYTES) : nullptr;
+      if ((i & 31) == 0) ahead = i + lane < n_tiles ? kv_tile_at(a.c, b, kvh, tile_of(i + lane), L::BYTES) : nullptr;
       const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ahead), i & 31));
       if (lap && !wait_for(raw_empty + 8 * slot, (lap - 1) & 1, dead)) break;
       if (lane == 0) {
@@ -314,7 +347,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       bool both = true;
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int j0 = (t0 + i + e) * KV_TILE;
+        const int j0 = tile_of(i + e) * KV_TILE;
         uint32_t top[2] = {0u, 0u};
 #pragma unroll
         for (int k = 0; k < KW; k++) top[0] = __vmaxu2(top[0], x[e][k] & 0x7fff7fffu), top[1] = __vmaxu2(top[1], x[e][KW + k] & 0x7fff7fffu);
@@ -322,16 +355,21 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         // Most tiles: all of their positions are seen by some row, every scale is below 4 and the largest keys and values are not below 2^-3, f16's middle:
         // largest scales of 2^-6 (codes up to 8) or 2^-10 (up to 127). (With 2^-6 for 8 bits too, 2048 queries over 8192 positions took 699 us with values
         // of 0.3 and 293 with values of 0.7.)
-        const bool plain = !null[e] && j0 >= lo && j0 + KV_TILE - 1 <= hi && __all_sync(0xffffffffu, max(k_top, v_top) < 0x4400u) && __any_sync(0xffffffffu, k_top >= LEAST_BITS) &&
+        const bool inside = MORE ? all_seen(a, lo, hi, j0) : j0 >= lo && j0 + KV_TILE - 1 <= hi;
+        const bool plain = !null[e] && inside && __all_sync(0xffffffffu, max(k_top, v_top) < 0x4400u) && __any_sync(0xffffffffu, k_top >= LEAST_BITS) &&
                            __any_sync(0xffffffffu, v_top >= LEAST_BITS);
         Meta mt{0, 0, 0u, 0};
         if (!plain) {
           unsigned bad = 0, most[2] = {0u, 0u};
+          uint32_t seen = 0u; // MORE: positions of the tile that some row may see
+          if constexpr (MORE) seen = seen_in_tile(a, Sight{lo, hi}, a.nodes ? a.nodes + (long long)b * a.words : nullptr, pos, j0);
 #pragma unroll
           for (int k = 0; k < 2 * KW; k++) {
             const bool is_k = k < KW;
             const int in = is_k ? lane : lane & ~1, j = j0 + in; // keys: both halves are of position j; values: of j and j + 1
-            const bool in0 = j >= lo && j <= hi, in1 = is_k ? in0 : j + 1 >= lo && j + 1 <= hi;
+            bool in0, in1;
+            if constexpr (MORE) in0 = (seen >> in) & 1u, in1 = is_k ? in0 : (seen >> in) & 2u;
+            else in0 = j >= lo && j <= hi, in1 = is_k ? in0 : j + 1 >= lo && j + 1 <= hi;
             uint32_t y = null[e] ? 0u : x[e][k] & ((in0 ? 0xffffu : 0u) | (in1 ? 0xffff0000u : 0u));
             if ((y & 0x7c00u) == 0x7c00u) y &= 0xffff0000u, bad |= 1u << in;
             if ((y & 0x7c000000u) == 0x7c000000u) y &= 0xffffu, bad |= (is_k ? 1u : 2u) << in;
@@ -508,13 +546,19 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     const long long at = row0 + row, tok = at / a.group;
     const int h = kvh * a.group + (int)(at - tok * a.group);
     int r_lo = 0, r_hi = INT_MAX;
-    if (valid) seen_by(a, pos, tok, r_lo, r_hi);
+    const uint32_t *tree = nullptr; // MORE: the row's bits
+    if constexpr (MORE) {
+      if (valid) {
+        const Sight v = sight_of(a, sq, tok);
+        r_lo = v.lo, r_hi = v.hi, tree = a.sees ? a.sees + (sq.first_row + tok) * a.words : nullptr;
+      }
+    } else if (valid) seen_by(a, pos, tok, r_lo, r_hi);
     const int lo_all = __reduce_max_sync(0xffffffffu, valid ? r_lo : 0), hi_all = __reduce_min_sync(0xffffffffu, r_hi);
     const int lo_any = __reduce_min_sync(0xffffffffu, valid ? r_lo : INT_MAX), hi_any = __reduce_max_sync(0xffffffffu, valid ? r_hi : -1);
     float f = 0.f;
     { // the row as an operand
       uint4 x[HD / 8];
-      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q.p) + b * a.q.sb + tok * a.q.ss + h * a.q.sh);
+      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q.p) + q_at + tok * a.q.ss + h * a.q.sh);
 #pragma unroll
       for (int c = 0; c < HD / 8; c++) x[c] = valid && n > 0 ? src[c] : make_uint4(0, 0, 0, 0);
       auto value = [&](uint32_t w, int half) {
@@ -589,8 +633,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     // A half's scores to weights. Where every row sees every position, no scales are far off and no score is far over its row's reference, both tiles at once.
     auto weigh = [&](uint32_t (&s)[64]) {
       const uint32_t at = buffers + (h2 & 1) * HALF; // P takes the place of the first half of the scores
-      const int j0 = (t0 + h2 * 2) * KV_TILE;
-      bool general = !have_ref || v_ref != 0 || j0 < lo_all || j0 + HALF - 1 > hi_all || !s_plain[h2 % (2 * META_STEPS)];
+      const int j0 = tile_of(h2 * 2) * KV_TILE;
+      bool general = !have_ref || v_ref != 0 || !s_plain[h2 % (2 * META_STEPS)];
+      if constexpr (MORE) general = general || !all_seen(a, lo_all, hi_all, j0) || !all_seen(a, lo_all, hi_all, tile_of(h2 * 2 + 1) * KV_TILE);
+      else general = general || j0 < lo_all || j0 + HALF - 1 > hi_all;
       uint32_t pk[32];
       tmem_ld_wait();
       if (!general) {
@@ -614,17 +660,23 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
 #pragma unroll 1
       for (int c = 0; c < 2; c++) {
         const Meta mt = mt2[c];
-        const int i0 = j0 + c * KV_TILE;
-        uint32_t x[32], out[16];
-        if (mt.gone || i0 > hi_any || i0 + KV_TILE - 1 < lo_any) { // seen by no row of the warp
+        const int i0 = MORE ? tile_of(h2 * 2 + c) * KV_TILE : j0 + c * KV_TILE;
+        uint32_t x[32], out[16], mine = 0u; // MORE: positions that the row sees
+        bool every, nothing; // row of the warp sees all of them; sees any
+        if constexpr (MORE) {
+          every = all_seen(a, lo_all, hi_all, i0);
+          if (!every) mine = seen_in_tile(a, Sight{r_lo, r_hi}, tree, pos, i0);
+          nothing = !every && !__any_sync(0xffffffffu, valid && mine);
+        } else every = i0 >= lo_all && i0 + KV_TILE - 1 <= hi_all, nothing = i0 > hi_any || i0 + KV_TILE - 1 < lo_any;
+        if (mt.gone || nothing) { // seen by no row of the warp
 #pragma unroll
           for (int i = 0; i < 16; i++) out[i] = 0u;
         } else {
           tmem_ld32(at + c * 32, x);
           tmem_ld_wait();
-          if (i0 < lo_all || i0 + KV_TILE - 1 > hi_all) { // not by all
-            const int first = max(r_lo - i0, 0), last = min(r_hi - i0, 31);
-            const unsigned seen = first <= last ? (0xffffffffu >> (31 - last + first)) << first : 0u;
+          if (!every) { // not by all
+            unsigned seen = mine;
+            if constexpr (!MORE) seen = bits_between(r_lo - i0, r_hi - i0);
             if (mt.bad & seen) l = NAN;
 #pragma unroll
             for (int i = 0; i < 32; i++)
@@ -671,7 +723,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     // ---- the row's result, or its part ----
     if (a.splits == 1) {
       const float by = l > 0.f ? ldexpf(1.f / l, -v_ref) : l; // nothing seen: zeros; NaN stays
-      uint16_t *dst = static_cast<uint16_t *>(a.out.p) + b * a.out.sb + tok * a.out.ss + h * a.out.sh;
+      uint16_t *dst = static_cast<uint16_t *>(a.out.p) + out_at + tok * a.out.ss + h * a.out.sh;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 16) {
         uint32_t o[16];
@@ -695,7 +747,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         }
         __syncwarp();
       }
-      if (valid && a.lse) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (ref + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
+      if (valid && a.lse) a.lse[(lse_row + tok) * a.heads + h] = l > 0.f ? (ref + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
     } else {
       float *rec = a.records + (((size_t)(a.row_tiles - 1 - rt) * (per / a.splits) + bk) * a.splits + split) * P::RECORD;
       if (valid) rec[row] = ref, rec[QT * 128 + row] = l;
@@ -725,16 +777,26 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
 
 // The parts of rows whose positions `splits` CTAs shared, added in the order of their places: a warp a row, a lane HD / 32 dims. A kernel of its own, because
 // every SM has a share of it: one CTA of the attention adding 18 parts of 128 rows, 1.2 MB, had taken longer than the attention (128 rows of one sequence of 8192 positions: 139 us, now 32).
-template <int HD>
+template <int HD, bool MORE>
 __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int V = HD / 32, RECORD = 128 * (HD + 2), AHEAD = 8;
   const int lane = threadIdx.x & 31, units = (int)a.batch * a.c.kv_heads;
-  const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5), all_rows = a.seq * a.group;
+  const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  long long all_rows = a.seq * a.group;
   pdl_launch_dependents();
   pdl_wait();
   const int rt = (int)(at / (128ll * units)), bk = (int)(at / 128 % units), row = (int)(at % 128), b = bk / a.c.kv_heads, kvh = bk % a.c.kv_heads;
   const long long at_row = rt * 128ll + row;
-  if (rt >= a.row_tiles || at_row >= all_rows) return;
+  if (rt >= a.row_tiles) return;
+  long long out_at = b * a.out.sb, lse_row = (long long)b * a.seq;
+  if constexpr (MORE) {
+    if (a.offsets) {
+      const long long first = a.offsets[b];
+      all_rows = (a.offsets[b + 1] - first) * a.group, out_at = first * a.out.ss, lse_row = first;
+      if (all_rows < a.rows_from) return;
+    }
+  }
+  if (at_row >= all_rows) return;
   const float *const first = a.records + ((size_t)(a.row_tiles - 1 - rt) * units + bk) * a.splits * RECORD; // (the last row tiles' CTAs come first)
   float m = -INFINITY, l = 0.f, v[V] = {};
   for (int k = lane; k < a.splits; k += 32) m = fmaxf(m, __ldcg(first + (size_t)k * RECORD + row));
@@ -769,8 +831,8 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_consta
   const float by = l > 0.f ? 1.f / l : l; // nothing seen: zeros; NaN stays
 #pragma unroll
   for (int c = 0; c < V; c++) v[c] = l == 0.f ? 0.f : v[c] * by;
-  store_vec<V>(a.out.p, a.dtype, b * a.out.sb + tok * a.out.ss + h * a.out.sh + lane * V, v);
-  if (a.lse && lane == 0) a.lse[((long long)b * a.seq + tok) * a.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
+  store_vec<V>(a.out.p, a.dtype, out_at + tok * a.out.ss + h * a.out.sh + lane * V, v);
+  if (a.lse && lane == 0) a.lse[(lse_row + tok) * a.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
 }
 
 // Row tiles of 128 rows where an SM each is enough for them, or the rows are no more; CTAs that share a tile's positions where the SMs are more. Else tiles
@@ -787,25 +849,27 @@ Plan plan_of(int64_t batch, int64_t seq, int group, int kv_heads, int64_t max_se
   return Plan{1, (int)one, (int)std::max<int64_t>(1, std::min<int64_t>(sms / (heads * one), steps / 2))};
 }
 
-template <int BITS, int HD, int QT>
+template <int BITS, int HD, int QT, bool MORE>
 int launch(const AttendArgs &a, cudaStream_t s) {
   const int64_t grid = (int64_t)a.row_tiles * a.batch * a.c.kv_heads * a.splits;
   if (grid > INT_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of query rows are more than one launch takes", (long long)grid);
-  XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
+  XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT, MORE>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
   count_launch();
   if (a.splits == 1) return XNQ_OK;
-  XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD>, dim3((unsigned)(a.row_tiles * a.batch * a.c.kv_heads * 16)), dim3(256), 0, s, a));
+  XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD, MORE>, dim3((unsigned)(a.row_tiles * a.batch * a.c.kv_heads * 16)), dim3(256), 0, s, a));
   count_launch();
   return XNQ_OK;
 }
 template <int BITS, int HD, int QT>
 int init_one() {
-  XNQ_CUDA(cudaFuncSetAttribute(kv_attend_prompt_kernel<BITS, HD, QT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<BITS, HD, QT>::SMEM));
+  XNQ_CUDA(cudaFuncSetAttribute(kv_attend_prompt_kernel<BITS, HD, QT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<BITS, HD, QT>::SMEM));
+  XNQ_CUDA(cudaFuncSetAttribute(kv_attend_prompt_kernel<BITS, HD, QT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<BITS, HD, QT>::SMEM));
   return XNQ_OK;
 }
 template <int BITS, int HD>
-int launch_hd(const AttendArgs &a, int qt, cudaStream_t s) {
-  return qt == 2 ? launch<BITS, HD, 2>(a, s) : launch<BITS, HD, 1>(a, s);
+int launch_hd(const AttendArgs &a, bool more, int qt, cudaStream_t s) {
+  if (more) return qt == 2 ? launch<BITS, HD, 2, true>(a, s) : launch<BITS, HD, 1, true>(a, s);
+  return qt == 2 ? launch<BITS, HD, 2, false>(a, s) : launch<BITS, HD, 1, false>(a, s);
 }
 
 } // namespace
@@ -825,12 +889,12 @@ int kv_prompt_init(int) {
 }
 constexpr int MAX_PARTS = 160; // CTAs of a launch that shares positions: no more than SMs
 size_t kv_prompt_parts_bytes(int head_dim) { return (size_t)MAX_PARTS * 128 * (head_dim + 2) * 4; }
-int launch_kv_prompt(const AttendArgs &args, int bits, int head_dim, int sms, cudaStream_t s) {
+int launch_kv_prompt(const AttendArgs &args, bool more, int bits, int head_dim, int sms, cudaStream_t s) {
   AttendArgs a = args;
   const Plan p = plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_PARTS));
   a.row_tiles = p.row_tiles, a.splits = p.splits;
-  if (bits == 4) return head_dim == 64 ? launch_hd<4, 64>(a, p.qt, s) : launch_hd<4, 128>(a, p.qt, s);
-  return head_dim == 64 ? launch_hd<8, 64>(a, p.qt, s) : launch_hd<8, 128>(a, p.qt, s);
+  if (bits == 4) return head_dim == 64 ? launch_hd<4, 64>(a, more, p.qt, s) : launch_hd<4, 128>(a, more, p.qt, s);
+  return head_dim == 64 ? launch_hd<8, 64>(a, more, p.qt, s) : launch_hd<8, 128>(a, more, p.qt, s);
 }
 
 } // namespace xnq

@@ -157,13 +157,18 @@ __device__ __forceinline__ void load_tables(const RopeArgs &r, long long pos, in
   load8(r.sin + pos * (HD / 2) + (l & (HD / 16 - 1)) * 8, s);
 }
 
+struct PackedRows { // of a plan: where each token goes, and the position that it is rotated at
+  const long long *slot, *position;
+};
+
 struct StoreUnits { // warps: [0, kv) store keys and values, the rest rotate queries
   unsigned kv, all, pairs, kv_slices, q_slices;
 };
 
-template <int BITS, int HD, typename T, bool ROPE>
+// PACKED: the tokens of all sequences one after the other (seq: how many). A warp has a token, and the next one with it where the two share a pair.
+template <int BITS, int HD, typename T, bool ROPE, bool PACKED>
 // Four blocks an SM: with the 120 registers that it would take, and two blocks, 8 x 4096 bf16 tokens with rotation took half as long again.
-__global__ void __launch_bounds__(256, 4) kv_store_kernel(KvView c, KvRows k, KvRows v, RopeArgs r, StoreUnits un, long long seq, const long long *pos_p, int pos_stride) {
+__global__ void __launch_bounds__(256, 4) kv_store_kernel(KvView c, KvRows k, KvRows v, RopeArgs r, StoreUnits un, long long seq, const long long *pos_p, int pos_stride, PackedRows pk) {
   using L = KvTile<BITS, HD>;
   constexpr int LANES = HD / 8, ROWS = 32 / LANES; // threads of a head's row, rows of a warp
   const int lane = threadIdx.x & 31, l = lane % LANES, sub = lane / LANES;
@@ -173,8 +178,8 @@ __global__ void __launch_bounds__(256, 4) kv_store_kernel(KvView c, KvRows k, Kv
   if (u >= un.all) return;
   if (ROPE && u >= un.kv) { // queries
     u -= un.kv;
-    const unsigned bs = u / un.q_slices, slice = u - bs * un.q_slices, b = bs / (unsigned)seq, s = bs - b * (unsigned)seq;
-    const long long p = pos_p[(long long)b * pos_stride] + s;
+    const unsigned bs = u / un.q_slices, slice = u - bs * un.q_slices, b = PACKED ? 0u : bs / (unsigned)seq, s = bs - b * (unsigned)seq;
+    const long long p = PACKED ? pk.position[s] : pos_p[(long long)b * pos_stride] + s;
     const bool valid = p >= 0 && p < r.rows;
     // A lane takes four dims and their partners half a head on; U rows are on their way at a time. (16-bit types: with eight dims, 252 us instead of 157 for
     // 8 x 4096 tokens.)
@@ -217,25 +222,49 @@ __global__ void __launch_bounds__(256, 4) kv_store_kernel(KvView c, KvRows k, Kv
     }
     return;
   }
-  const unsigned bp = u / un.kv_slices, slice = u - bp * un.kv_slices, b = bp / un.pairs;
-  const long long first = pos_p[(long long)b * pos_stride], p0 = ((first >> 1) + (bp - b * un.pairs)) * 2, s0 = p0 - first; // the pair's even position and its token
+  const unsigned bp = u / un.kv_slices, slice = u - bp * un.kv_slices, b = PACKED ? 0u : bp / un.pairs;
+  long long p0, s0, turn[2]; // the pair's even position (a slot is one, too) and its token; the positions of the two for their rotation
   bool has[2], past = false;
+  if constexpr (PACKED) {
+    const long long t = bp, at = pk.slot[t];
+    if (at < 0 || ((at & 1) && t > 0 && pk.slot[t - 1] == at - 1)) return; // no token, or the one before has taken it along
+    p0 = at & ~1ll, s0 = t - (at & 1);
+    has[0] = !(at & 1), has[1] = (at & 1) || (t + 1 < seq && pk.slot[t + 1] == at + 1);
 #pragma unroll
-  for (int e = 0; e < 2; e++) {
-    const long long p = p0 + e, s = s0 + e;
-    has[e] = s >= 0 && s < seq && p >= 0;
-    if (has[e] && (p >= c.max_seq || (ROPE && p >= r.rows))) has[e] = false, past = true;
+    for (int e = 0; e < 2; e++) {
+      turn[e] = has[e] ? pk.position[s0 + e] : 0;
+      if (ROPE && has[e] && turn[e] >= r.rows) has[e] = false, past = true;
+    }
+  } else {
+    const long long first = pos_p[(long long)b * pos_stride];
+    p0 = ((first >> 1) + (bp - b * un.pairs)) * 2, s0 = p0 - first;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const long long p = p0 + e, s = s0 + e;
+      has[e] = s >= 0 && s < seq && p >= 0;
+      if (has[e] && (p >= c.max_seq || (ROPE && p >= r.rows))) has[e] = false, past = true;
+      turn[e] = p;
+    }
   }
   if (past && lane == 0) atomicOr(&g_kv_store_status, KV_PAST_STORE);
   if (!has[0] && !has[1]) return;
-  uint8_t *tile0 = kv_tile_at(c, (int)b, 0, (int)(p0 / KV_TILE), L::BYTES); // head 0's
-  if (!tile0) {
-    if (lane == 0) atomicOr(&g_kv_store_status, KV_NO_PAGE);
-    return;
+  uint8_t *tile0; // head 0's
+  int row;
+  if constexpr (PACKED) {
+    const long long size = (long long)c.page_tiles * KV_TILE, page = p0 / size;
+    const int in = (int)(p0 - page * size);
+    if (page >= c.num_pages) return; // (the plan is another cache's)
+    tile0 = c.pages + page * c.page_bytes + (long long)(in / KV_TILE) * L::BYTES, row = in % KV_TILE;
+  } else {
+    tile0 = kv_tile_at(c, (int)b, 0, (int)(p0 / KV_TILE), L::BYTES), row = (int)p0 % KV_TILE;
+    if (!tile0) {
+      if (lane == 0) atomicOr(&g_kv_store_status, KV_NO_PAGE);
+      return;
+    }
   }
-  const int row = (int)p0 % KV_TILE, pair = row / 2, blk = l / 4, t = l % 4;
+  const int pair = row / 2, blk = l / 4, t = l % 4;
   float cs[2][8], sn[2][8];
-  if (ROPE) load_tables<HD>(r, p0, l, has[0], cs[0], sn[0]), load_tables<HD>(r, p0 + 1, l, has[1], cs[1], sn[1]);
+  if (ROPE) load_tables<HD>(r, turn[0], l, has[0], cs[0], sn[0]), load_tables<HD>(r, turn[1], l, has[1], cs[1], sn[1]);
   const T *const kp = static_cast<const T *>(k.p) + b * k.sb + s0 * k.ss + l * 8, *const vp = static_cast<const T *>(v.p) + b * v.sb + s0 * v.ss + l * 8;
   auto row_of = [&](int x, float (&val)[2][8]) { // rows 0 .. KV - 1: keys, the next KV: values
     const bool is_v = x >= c.kv_heads, in = x < 2 * c.kv_heads;
@@ -396,10 +425,10 @@ __global__ void __launch_bounds__(256) kv_load_kernel(KvView c, T *k_out, T *v_o
 // Warps that share a position's rows: as many as it takes to fill the GPU (148 SMs of 32 warps), a row group each at most.
 unsigned slices_for(int64_t positions, int64_t groups) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(groups, 4736 / std::max<int64_t>(positions, 1))); }
 
-template <int BITS, int HD, typename T>
-int run_store(const KvView &c, const KvRows &k, const KvRows &v, const RopeArgs &r, int64_t batch, int64_t seq, const long long *pos, int pos_stride, cudaStream_t s) {
+template <int BITS, int HD, typename T, bool PACKED>
+int run_store(const KvView &c, const KvRows &k, const KvRows &v, const RopeArgs &r, int64_t batch, int64_t seq, const long long *pos, int pos_stride, const PackedRows &pk, cudaStream_t s) {
   constexpr int ROWS = 32 / (HD / 8);
-  const int64_t pairs = seq / 2 + 1; // that `seq` positions may touch
+  const int64_t pairs = PACKED ? seq : seq / 2 + 1; // that `seq` positions may touch
   StoreUnits un{};
   un.pairs = (unsigned)pairs;
   un.kv_slices = slices_for(batch * pairs, (2 * c.kv_heads + ROWS - 1) / ROWS);
@@ -413,8 +442,8 @@ int run_store(const KvView &c, const KvRows &k, const KvRows &v, const RopeArgs 
   if (all > INT32_MAX) return fail(XNQ_ERR_SIZE, "kv_store: %lld x %lld tokens are more than one launch takes", (long long)batch, (long long)seq);
   un.kv = (unsigned)kv, un.all = (unsigned)all;
   const dim3 grid((unsigned)((all + 7) / 8)), block(256);
-  if (r.cos) XNQ_CUDA(launch_pdl(kv_store_kernel<BITS, HD, T, true>, grid, block, 0, s, c, k, v, r, un, seq, pos, pos_stride));
-  else XNQ_CUDA(launch_pdl(kv_store_kernel<BITS, HD, T, false>, grid, block, 0, s, c, k, v, r, un, seq, pos, pos_stride));
+  if (r.cos) XNQ_CUDA(launch_pdl(kv_store_kernel<BITS, HD, T, true, PACKED>, grid, block, 0, s, c, k, v, r, un, seq, pos, pos_stride, pk));
+  else XNQ_CUDA(launch_pdl(kv_store_kernel<BITS, HD, T, false, PACKED>, grid, block, 0, s, c, k, v, r, un, seq, pos, pos_stride, pk));
   count_launch();
   return XNQ_OK;
 }
@@ -458,6 +487,25 @@ int kv_view(const char *who, const xnq_kv_cache *c, int64_t batch, KvView *v) {
   *v = KvView{static_cast<uint8_t *>(c->pages), c->page_table, c->table_stride, c->num_pages, tile * tiles * c->kv_heads, tile * tiles, c->max_seq, (int)tiles, c->kv_heads};
   return XNQ_OK;
 }
+namespace {
+// rows and rotation of a store
+int store_args(const xnq_rows *k, const xnq_rows *v, const xnq_kv_rope *rope, KvRows *kr, KvRows *vr, RopeArgs *r) {
+  int rc;
+  if ((rc = kv_rows("kv_store", "k", k, kr)) != XNQ_OK || (rc = kv_rows("kv_store", "v", v, vr)) != XNQ_OK) return rc;
+  if (v->dtype != k->dtype) return fail(XNQ_ERR_DTYPE, "kv_store: k has type %d, v %d", k->dtype, v->dtype);
+  if (!rope) return XNQ_OK;
+  if (!rope->cos_table || !rope->sin_table) return fail(XNQ_ERR_NULL, "kv_store: a rotation without tables");
+  if (rope->table_rows < 1 || rope->heads < 0 || rope->heads > 65535) return fail(XNQ_ERR_SHAPE, "kv_store: tables of %lld rows, %d heads", (long long)rope->table_rows, rope->heads);
+  if ((reinterpret_cast<uintptr_t>(rope->cos_table) | reinterpret_cast<uintptr_t>(rope->sin_table)) & 15) return fail(XNQ_ERR_ALIGN, "kv_store: the tables must be 16-byte aligned");
+  r->cos = rope->cos_table, r->sin = rope->sin_table, r->rows = rope->table_rows, r->heads = rope->heads;
+  if (rope->heads) {
+    if ((rc = kv_rows("kv_store", "q", &rope->q, &r->q)) != XNQ_OK || (rc = kv_rows("kv_store", "q_out", &rope->q_out, &r->q_out)) != XNQ_OK) return rc;
+    if (rope->q.dtype != k->dtype) return fail(XNQ_ERR_DTYPE, "kv_store: k has type %d, q %d", k->dtype, rope->q.dtype);
+    r->q_out_dtype = rope->q_out.dtype;
+  }
+  return XNQ_OK;
+}
+} // namespace
 int kv_store_status(unsigned int *bits) {
   XNQ_CUDA(cudaMemcpyFromSymbol(bits, g_kv_store_status, sizeof(*bits)));
   return XNQ_OK;
@@ -490,22 +538,26 @@ int xnq_kv_store(const xnq_kv_cache *cache, const xnq_rows *k, const xnq_rows *v
   if (seq < 0 || seq > INT32_MAX || pos_stride < 0 || pos_stride > 1) return fail(XNQ_ERR_SHAPE, "kv_store: seq %lld, pos_stride %d (0 or 1)", (long long)seq, pos_stride);
   if (batch == 0 || seq == 0) return XNQ_OK;
   KvRows kr, vr;
-  if ((rc = kv_rows("kv_store", "k", k, &kr)) != XNQ_OK || (rc = kv_rows("kv_store", "v", v, &vr)) != XNQ_OK) return rc;
-  if (v->dtype != k->dtype) return fail(XNQ_ERR_DTYPE, "kv_store: k has type %d, v %d", k->dtype, v->dtype);
   RopeArgs r{};
-  if (rope) {
-    if (!rope->cos_table || !rope->sin_table) return fail(XNQ_ERR_NULL, "kv_store: a rotation without tables");
-    if (rope->table_rows < 1 || rope->heads < 0 || rope->heads > 65535) return fail(XNQ_ERR_SHAPE, "kv_store: tables of %lld rows, %d heads", (long long)rope->table_rows, rope->heads);
-    if ((reinterpret_cast<uintptr_t>(rope->cos_table) | reinterpret_cast<uintptr_t>(rope->sin_table)) & 15) return fail(XNQ_ERR_ALIGN, "kv_store: the tables must be 16-byte aligned");
-    r.cos = rope->cos_table, r.sin = rope->sin_table, r.rows = rope->table_rows, r.heads = rope->heads;
-    if (rope->heads) {
-      if ((rc = kv_rows("kv_store", "q", &rope->q, &r.q)) != XNQ_OK || (rc = kv_rows("kv_store", "q_out", &rope->q_out, &r.q_out)) != XNQ_OK) return rc;
-      if (rope->q.dtype != k->dtype) return fail(XNQ_ERR_DTYPE, "kv_store: k has type %d, q %d", k->dtype, rope->q.dtype);
-      r.q_out_dtype = rope->q_out.dtype;
-    }
-  }
+  if ((rc = store_args(k, v, rope, &kr, &vr, &r)) != XNQ_OK) return rc;
   return kv_dispatch(kv_bits(cache->ggml_dtype), cache->head_dim, k->dtype, [&](auto f) {
-    return run_store<f.BITS, f.HD, typename decltype(f)::T>(c, kr, vr, r, batch, seq, pos, pos_stride, static_cast<cudaStream_t>(stream));
+    return run_store<f.BITS, f.HD, typename decltype(f)::T, false>(c, kr, vr, r, batch, seq, pos, pos_stride, PackedRows{}, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int xnq_kv_store_packed(const xnq_kv_cache *cache, const xnq_rows *k, const xnq_rows *v, const xnq_kv_plan *plan, const xnq_kv_rope *rope, void *stream) {
+  clear_error();
+  KvView c;
+  int rc = kv_plan_check("kv_store", plan);
+  if (rc != XNQ_OK || (rc = kv_view("kv_store", cache, plan->batch, &c)) != XNQ_OK) return rc;
+  if (!k || !v) return fail(XNQ_ERR_NULL, "kv_store: NULL argument");
+  if (plan->tokens == 0) return XNQ_OK;
+  KvRows kr, vr;
+  RopeArgs r{};
+  if ((rc = store_args(k, v, rope, &kr, &vr, &r)) != XNQ_OK) return rc;
+  kr.sb = vr.sb = r.q.sb = r.q_out.sb = 0;
+  return kv_dispatch(kv_bits(cache->ggml_dtype), cache->head_dim, k->dtype, [&](auto f) {
+    return run_store<f.BITS, f.HD, typename decltype(f)::T, true>(c, kr, vr, r, 1, plan->tokens, nullptr, 0, PackedRows{plan->slot, plan->position}, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -9,6 +9,15 @@ blocks it is 144 bytes, as Q8_0 272. ``QLlama(kv_dtype=...)`` uses it; any other
     out = cache.attend(q, pos)                            # q [batch, seq, heads, head_dim]: one token, a few drafts, a prompt
     k, v = cache.load(0, n)                               # what the blocks stand for
 
+Between requests, all of it on the GPU and without a look at the results::
+
+    room, free = cache.reserve(length)                    # the page table brought to the requests' lengths
+    plan = cache.plan(pos, count, tokens)                 # sequences of their own numbers of tokens, packed one after the other
+    q = cache.rope_store(qkv, cos, sin, plan, heads)      # the calls above with a plan for pos; qkv [tokens, ..], q [tokens, heads, head_dim]
+    out = cache.attend(q, plan, window=4096, sinks=4)     # a window, and first positions that stay visible
+    plan = cache.plan(pos, count, tokens, longest, parents)   # trees of drafted tokens: each sees its ancestors
+    pos = cache.keep(plan, node)                          # the accepted path stays
+
 ``pos`` is the position of the first of a call's ``seq`` tokens, one for every sequence or one for all. A token at a negative position is none (an idle slot of
 the batch, padding on the left): it is not stored, and its query gives zeros. Everything is enqueued on the current stream. There are no derivatives: tensors
 that require a gradient are refused, but under ``torch.no_grad()``, and so are tracers.
@@ -27,6 +36,7 @@ from . import _lib
 from .dtypes import GgmlDType
 from .quantized import _TORCH_TO_XNQ, _XNQ_IDS, _stream_ptr, init
 
+TREE_MOST = 256  # tokens of a tree: XNQ_KV_TREE_MOST
 _ZEROED = 4096  # XNQ_KV_WORKSPACE_ZEROED: the front of attention's workspace, zero before its first use
 PAGE_UNIT = 32  # positions of a tile: page sizes are multiples of it
 
@@ -44,15 +54,20 @@ class _Rope(ctypes.Structure):
     _fields_ = [("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("heads", ctypes.c_int), ("q", _Rows), ("q_out", _Rows)]
 
 
+class _Plan(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int64), ("batch", ctypes.c_int64), ("longest", ctypes.c_int64), ("start", ctypes.c_void_p), ("offsets", ctypes.c_void_p),
+                ("sequence", ctypes.c_void_p), ("position", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("sees", ctypes.c_void_p), ("nodes", ctypes.c_void_p)]
+
+
 def _served(t: torch.Tensor) -> bool:
-    """Whether the kernels can read this [batch, seq, heads, head_dim] tensor where it lies: rows contiguous and 16-byte aligned."""
+    """Whether the kernels can read this [batch, seq, heads, head_dim] or [tokens, heads, head_dim] tensor where it lies: rows contiguous and 16-byte aligned."""
     e = 16 // t.element_size()
-    return t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % e == 0 for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1)
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % e == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)
 
 
 def _rows(t: torch.Tensor) -> _Rows:
-    strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]   # of a dimension of one entry torch may say anything
-    return _Rows(t.data_ptr(), int(_TORCH_TO_XNQ[t.dtype]), *strides)
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]   # of a dimension of one entry torch may say anything
+    return _Rows(t.data_ptr(), int(_TORCH_TO_XNQ[t.dtype]), *([0] * (3 - len(strides))), *strides)
 
 
 def _refuse_derivatives(who: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -84,12 +99,38 @@ def _workspace(device: torch.device, need: int):
     return kept
 
 
+class KVPlan:
+    """Where the tokens of a step go: made by :meth:`QuantizedKVCache.plan`, good for every cache with the same page table (a model's layers).
+
+    ``offsets`` int64 ``[batch + 1]``: sequence ``b`` has the rows ``offsets[b] ..`` of the packed tokens. ``sequence`` (int32), ``position`` and ``slot`` (int64)
+    ``[tokens]``: of each row its sequence, the position that it is rotated at, and ``page * page_size + place`` in the cache's memory; -1: none. ``start``:
+    ``pos``, as it was. For trees ``sees`` (int32 ``[tokens, ceil(longest / 32)]``, bit ``t % 32`` of word ``t // 32``: the token sees token ``t`` of its tree) and
+    ``nodes`` (the same for all tokens of a tree ``[batch, ..]``); else None. The tensors are the plan's own and not to be written to."""
+
+    __slots__ = ("tokens", "longest", "batch", "table", "page_size", "num_pages", "max_seq", "start", "offsets", "sequence", "position", "slot", "sees", "nodes", "_view")
+
+    def __init__(self, cache: "QuantizedKVCache", tokens: int, longest: int, tree: bool):
+        dev = cache.device
+        self.tokens, self.longest, self.batch = tokens, longest, cache.batch
+        self.table, self.page_size, self.num_pages, self.max_seq = cache.page_table, cache.page_size, cache.num_pages, cache.max_seq
+        i64 = torch.empty(2 * cache.batch + 1 + 2 * tokens, dtype=torch.int64, device=dev)
+        self.start, self.offsets, self.position, self.slot = i64.split([cache.batch, cache.batch + 1, tokens, tokens])
+        words = -(-longest // 32) if tree else 0
+        i32 = torch.empty(tokens + (tokens + cache.batch) * words, dtype=torch.int32, device=dev)
+        self.sequence, sees, nodes = i32.split([tokens, tokens * words, cache.batch * words])
+        self.sees, self.nodes = (sees.view(tokens, words), nodes.view(cache.batch, words)) if tree else (None, None)
+        p = [t.data_ptr() for t in (self.start, self.offsets, self.sequence, self.position, self.slot)]
+        p = [x or i64.data_ptr() for x in p]   # (of no tokens: an address that is not NULL, which nothing is written to)
+        self._view = _Plan(tokens, cache.batch, longest, *p, (sees.data_ptr() or i32.data_ptr() or 16) if tree else None, nodes.data_ptr() if tree else None)
+
+
 class QuantizedKVCache:
     """Keys and values of ``batch`` sequences of up to ``max_seq`` positions, ``dtype`` blocks (Q4_0, Q8_0), ``head_dim`` 64 or 128.
 
     ``page_size`` (a multiple of 32): the memory is ``num_pages`` pages of that many positions, and ``page_table`` (int32 ``[batch, ceil(max_seq /
-    page_size)]`` on the device, all -1 at first) says which page holds positions ``i * page_size ..`` of a sequence; the program fills it in (in place: the
-    kernels hold its address, and a cache's attributes are not exchanged). Without it every sequence has one run of memory."""
+    page_size)]`` on the device, all -1 at first) says which page holds positions ``i * page_size ..`` of a sequence; :meth:`reserve` or the program fills it in
+    (in place: the kernels hold its address, and a cache's attributes are not exchanged). ``page_table``: another cache's, which this one shares (the layers
+    of a model: one :meth:`reserve` for all). Without pages every sequence has one run of memory."""
 
     _FIXED = frozenset(("pages", "page_table", "dtype", "batch", "kv_heads", "max_seq", "head_dim", "page_size", "num_pages", "device"))
 
@@ -99,7 +140,7 @@ class QuantizedKVCache:
         super().__setattr__(name, value)
 
     def __init__(self, dtype: GgmlDType, batch: int, kv_heads: int, max_seq: int, head_dim: int, device: torch.device | str = "cuda:0",
-                 page_size: Optional[int] = None, num_pages: Optional[int] = None):
+                 page_size: Optional[int] = None, num_pages: Optional[int] = None, page_table: Optional[torch.Tensor] = None):
         self.dtype, self.batch, self.kv_heads, self.max_seq, self.head_dim = GgmlDType(dtype), batch, kv_heads, max_seq, head_dim
         if min(batch, kv_heads, max_seq) < 1:
             raise ValueError(f"QuantizedKVCache: batch {batch}, kv_heads {kv_heads}, max_seq {max_seq}")
@@ -116,7 +157,10 @@ class QuantizedKVCache:
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
         init(self.device)
         self.pages = torch.zeros((self.num_pages, page_bytes), dtype=torch.uint8, device=self.device)
-        self.page_table = torch.full((batch, -(-max_seq // self.page_size)), -1, dtype=torch.int32, device=self.device) if paged else None
+        shape = (batch, -(-max_seq // self.page_size))
+        if page_table is not None and (not paged or page_table.shape != shape or page_table.dtype is not torch.int32 or page_table.device != self.device or not page_table.is_contiguous()):
+            raise ValueError(f"QuantizedKVCache: page_table is contiguous int32 {shape} on {self.device}, of a cache by pages")
+        self.page_table = page_table if page_table is not None else torch.full(shape, -1, dtype=torch.int32, device=self.device) if paged else None
         self._view = _Cache(int(self.dtype), kv_heads, head_dim, self.page_size, self.num_pages, self.pages.data_ptr(),
                             self.page_table.data_ptr() if paged else None, self.page_table.stride(0) if paged else 0, max_seq)
 
@@ -142,9 +186,104 @@ class QuantizedKVCache:
             raise ValueError(f"{what}: int64 on {self.device}, one for each of the {self.batch} sequences or one for all")
         return ctypes.c_void_p(pos.data_ptr()), int(pos.numel() > 1)
 
-    def store(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor) -> None:
+    def reserve(self, length: torch.Tensor, first: Optional[torch.Tensor] = None, sinks: int = 0, table: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Bring the page table to the requests' lengths: sequence ``b`` has a page wherever positions below ``length[b]`` (int64 ``[batch]``; 0: no request)
+        need one, and none beyond. Pages that are there stay; the others come, in ascending order, from those that no row names any more (a page that two rows
+        name, a shared beginning, is free when both have let go). ``first`` (int64 ``[batch]``): positions below it are seen no more, but for the first
+        ``sinks``, and their pages are given back (attention with a window). ``table``: what to start from, instead of the table as it is (its shape and type).
+
+        Returns ``room`` int64 ``[batch]``, the positions that there are pages for (``length``, or less where the pages did not suffice: sequences in their
+        order, each up to its first missing page), and ``free`` int64 ``[]``, the pages left."""
+        if self.page_table is None:
+            raise ValueError("reserve: this cache has no pages")
+        _refuse_derivatives("reserve")
+        for what, t in (("length", length), ("first", first)):
+            if t is not None and (t.dtype is not torch.int64 or t.device != self.device or t.shape != (self.batch,) or not t.is_contiguous()):
+                raise ValueError(f"reserve: {what} is contiguous int64 [{self.batch}] on {self.device}")
+        if sinks < 0:
+            raise ValueError(f"reserve: sinks {sinks}")
+        if table is None:
+            table = self.page_table
+        elif table.shape != self.page_table.shape or table.dtype is not torch.int32 or table.device != self.device or not table.is_contiguous():
+            raise ValueError(f"reserve: table is contiguous int32 {tuple(self.page_table.shape)} on {self.device}")
+        out = torch.empty(self.batch + 1, dtype=torch.int64, device=self.device)
+        L = _lib.lib()
+        need = int(L.xnq_kv_reserve_workspace_bytes(self.num_pages))
+        with torch.cuda.device(self.device):
+            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
+            p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
+            _lib.check(L.xnq_kv_reserve(p(self.page_table), self.page_table.stride(0), p(table), table.stride(0), self.batch, self.page_size, self.num_pages, self.max_seq,
+                                        p(length), p(first), sinks, p(out), ctypes.c_void_p(out.data_ptr() + 8 * self.batch), p(ws), need, _stream_ptr(self.device)))
+        return out[:-1], out[-1]
+
+    def plan(self, pos: torch.Tensor, count: torch.Tensor, tokens: int, longest: Optional[int] = None, parents: Optional[torch.Tensor] = None) -> KVPlan:
+        """Slot maps of packed tokens: sequence ``b`` brings ``count[b]`` (int64 ``[batch]``) tokens for the positions ``pos[b] ..``, all of them lie one after
+        the other in ``tokens`` rows; rows behind the last sequence are none. ``longest``: no sequence brings more (default ``tokens``). What is beyond
+        ``longest`` or ``tokens`` is cut off, and sets a status bit.
+
+        ``parents`` (int32 ``[tokens]``): the tokens of a sequence are a tree of drafts. Each one's is the index, in its sequence, of the token that it follows (a
+        smaller one than its own); -1: it follows what is in the cache; -2: the place is not used. They lie at ``pos, pos + 1, ..`` in the cache, in their
+        order, are rotated at ``pos`` + depth, and see what lies below ``pos`` and their ancestors. Up to 256 tokens a tree."""
+        _refuse_derivatives("plan")
+        if tokens < 0 or (longest is not None and longest < 1):
+            raise ValueError(f"plan: {tokens} tokens, up to {longest} a sequence")
+        longest = max(1, min(tokens, longest if longest is not None else tokens))
+        if count.dtype is not torch.int64 or count.device != self.device or count.shape != (self.batch,) or not count.is_contiguous():
+            raise ValueError(f"plan: count is contiguous int64 [{self.batch}] on {self.device}")
+        if parents is not None:
+            if parents.dtype is not torch.int32 or parents.device != self.device or parents.shape != (tokens,) or not parents.is_contiguous():
+                raise ValueError(f"plan: parents is contiguous int32 [{tokens}] on {self.device}")
+            if longest > TREE_MOST:
+                raise ValueError(f"plan: trees of up to {longest} tokens (up to {TREE_MOST} are served)")
+        pp, stride = self._positions(pos)
+        with torch.cuda.device(self.device):
+            plan = KVPlan(self, tokens, longest, parents is not None)
+            _lib.check(_lib.lib().xnq_kv_plan_make(ctypes.byref(self._view), pp, stride, ctypes.c_void_p(count.data_ptr()),
+                                                   None if parents is None else ctypes.c_void_p(parents.data_ptr() or 16), ctypes.byref(plan._view), _stream_ptr(self.device)))
+        return plan
+
+    def _planned(self, who: str, plan: KVPlan) -> None:
+        """Whether the plan's slots are this cache's."""
+        if plan.batch != self.batch or plan.start.device != self.device or plan.max_seq != self.max_seq or plan.page_size != self.page_size or plan.num_pages != self.num_pages or \
+                (plan.table is None) != (self.page_table is None) or (plan.table is not None and plan.table.data_ptr() != self.page_table.data_ptr()):
+            raise ValueError(f"{who}: the plan was made for another cache (its batch, pages and page table have to be this one's)")
+
+    def keep(self, plan: KVPlan, node: torch.Tensor) -> torch.Tensor:
+        """Of each tree of drafted tokens the path to ``node[b]`` (int64 ``[batch]``, the index in its tree; -1: no token) stays: the keys and values of its
+        tokens move up to the positions ``pos[b], pos[b] + 1, ..``. Returns where each sequence goes on, int64 ``[batch]``: ``pos`` plus the path's length. What
+        the other tokens had stored may lie behind that."""
+        _refuse_derivatives("keep")
+        self._planned("keep", plan)
+        if plan.sees is None:
+            raise ValueError("keep: the plan is not one of trees (parents)")
+        if node.dtype is not torch.int64 or node.device != self.device or node.shape != (self.batch,) or not node.is_contiguous():
+            raise ValueError(f"keep: node is contiguous int64 [{self.batch}] on {self.device}")
+        with torch.cuda.device(self.device):
+            pos = torch.empty(self.batch, dtype=torch.int64, device=self.device)
+            _lib.check(_lib.lib().xnq_kv_keep(ctypes.byref(self._view), ctypes.byref(plan._view), ctypes.c_void_p(node.data_ptr()), ctypes.c_void_p(pos.data_ptr()),
+                                              _stream_ptr(self.device)))
+        return pos
+
+    def _packed(self, what: str, t: torch.Tensor, plan: KVPlan, heads: Optional[int] = None) -> torch.Tensor:
+        if t.dim() != 3 or t.shape[0] != plan.tokens or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
+            raise ValueError(f"{what} is {tuple(t.shape)}; the plan has {plan.tokens} tokens, the cache {self.kv_heads} KV heads of {self.head_dim}")
+        if t.device != self.device:
+            raise ValueError(f"{what} is on {t.device}, the cache on {self.device}")
+        if t.dtype not in _TORCH_TO_XNQ:
+            raise ValueError(f"{what} is {t.dtype}; float32, float16 and bfloat16 are served")
+        return t
+
+    def store(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor | KVPlan) -> None:
         """Quantize ``k`` and ``v`` ``[batch, seq, kv_heads, head_dim]`` (f32 / f16 / bf16, any strides) into positions ``pos ..``: the blocks that
-        ``BlockQ4_0`` / ``BlockQ8_0::from_float`` make of the f32 values (k_quants.rs:235-270, 636-661), Q8_0's scale being ``max|x| * float32(1 / 127)``."""
+        ``BlockQ4_0`` / ``BlockQ8_0::from_float`` make of the f32 values (k_quants.rs:235-270, 636-661), Q8_0's scale being ``max|x| * float32(1 / 127)``.
+        With a plan: ``[tokens, kv_heads, head_dim]``, each token into its slot."""
+        if isinstance(pos, KVPlan):
+            _refuse_derivatives("store", k, v)
+            self._planned("store", pos)
+            self._packed("k", k, pos, self.kv_heads), self._packed("v", v, pos, self.kv_heads)
+            if k.dtype is not v.dtype:
+                raise ValueError(f"k is {k.dtype}, v {v.dtype}")
+            return self._store_packed(k, v, pos, None)
         if self._native.kv_store(self._handle, k, v, pos):
             return
         _refuse_derivatives("store", k, v)
@@ -153,30 +292,44 @@ class QuantizedKVCache:
             raise ValueError(f"k is {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}")
         self._store(k, v, pos, None)
 
-    def rope_store(self, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, heads: int, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    def rope_store(self, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor | KVPlan, heads: int, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """``qkv`` ``[batch, seq, (heads + 2 kv_heads) * head_dim]``, a fused projection's output: q and k rotated (rotate-half, f32 tables ``[rows, head_dim /
-        2]``) at their positions, k and v stored. Returns q ``[batch, seq, heads, head_dim]`` as ``out_dtype`` (default: ``qkv``'s)."""
-        if out_dtype is None or out_dtype in _TORCH_TO_XNQ:
+        2]``) at their positions, k and v stored. Returns q ``[batch, seq, heads, head_dim]`` as ``out_dtype`` (default: ``qkv``'s). With a plan: ``[tokens, ..]``,
+        and q ``[tokens, heads, head_dim]``, zeros for rows that are no token."""
+        plan = pos if isinstance(pos, KVPlan) else None
+        if plan is None and (out_dtype is None or out_dtype in _TORCH_TO_XNQ):
             q = self._native.kv_rope_store(self._handle, qkv, cos, sin, pos, heads, -1 if out_dtype is None else _XNQ_IDS[out_dtype])
             if q is not None:
                 return q
         _refuse_derivatives("rope_store", qkv, cos, sin)
         hd, width = self.head_dim, (heads + 2 * self.kv_heads) * self.head_dim
-        if heads < 1 or qkv.dim() != 3 or qkv.shape[2] != width:
+        if plan is not None:
+            self._planned("rope_store", plan)
+        if heads < 1 or qkv.dim() != (3 if plan is None else 2) or qkv.shape[-1] != width:
             raise ValueError(f"rope_store: qkv is {tuple(qkv.shape)}; {heads} + 2 * {self.kv_heads} heads of {hd}")
         for t in (cos, sin):
             if t.dtype is not torch.float32 or not t.is_contiguous() or t.dim() != 2 or t.shape[1] != hd // 2 or t.shape != cos.shape or t.device != self.device:
                 raise ValueError(f"rope_store: tables are contiguous float32 [rows, {hd // 2}] on {self.device}")
         if out_dtype is not None and out_dtype not in _TORCH_TO_XNQ:
             raise ValueError(f"rope_store: queries of type {out_dtype}")
-        x = qkv.unflatten(2, (-1, hd))
+        x = qkv.unflatten(-1, (-1, hd))
         if not _served(x):
             x = x.clone(memory_format=torch.contiguous_format)
-        self._tokens("qkv", x)
-        q, k, v = x.split([heads, self.kv_heads, self.kv_heads], dim=2)
+        self._tokens("qkv", x) if plan is None else self._packed("qkv", x, plan)
+        q, k, v = x.split([heads, self.kv_heads, self.kv_heads], dim=-2)
         out = torch.empty((*q.shape,), dtype=out_dtype or qkv.dtype, device=self.device)
-        self._store(k, v, pos, _Rope(cos.data_ptr(), sin.data_ptr(), cos.shape[0], heads, _rows(q), _rows(out)))
+        if out.numel():
+            rope = _Rope(cos.data_ptr(), sin.data_ptr(), cos.shape[0], heads, _rows(q), _rows(out))
+            self._store(k, v, pos, rope) if plan is None else self._store_packed(k, v, plan, rope)
         return out
+
+    def _store_packed(self, k, v, plan, rope) -> None:
+        if plan.tokens == 0:
+            return
+        k, v = (t if _served(t) else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.lib().xnq_kv_store_packed(ctypes.byref(self._view), ctypes.byref(_rows(k)), ctypes.byref(_rows(v)), ctypes.byref(plan._view),
+                                                      None if rope is None else ctypes.byref(rope), _stream_ptr(self.device)))
 
     def _store(self, k, v, pos, rope) -> None:
         k, v = (t if _served(t) else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
@@ -202,39 +355,59 @@ class QuantizedKVCache:
                                               ctypes.c_void_p(k.data_ptr()), ctypes.c_void_p(v.data_ptr()), _stream_ptr(self.device)))
         return k, v
 
-    def attend(self, q: torch.Tensor, pos: torch.Tensor, causal: bool = True, window: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-               lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def attend(self, q: torch.Tensor, pos: torch.Tensor | KVPlan, causal: bool = True, window: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+               lse: Optional[torch.Tensor] = None, sinks: int = 0) -> torch.Tensor:
         """Attention of ``q`` ``[batch, seq, heads, head_dim]`` (f32 / f16 / bf16, any strides) over the cache; ``heads`` is a multiple of ``kv_heads``.
 
-        Query ``i`` of a sequence is at ``p = pos + i`` and sees positions ``j <= p`` (``causal``) or ``j < pos + seq``, with a ``window`` only ``j > p - window``;
-        one that sees nothing gives zeros. ``scale``: default ``head_dim ** -0.5``. ``out``: where the result goes (``q``'s shape and type, rows contiguous and
-        16-byte aligned). ``lse``: float32 ``[batch, seq, heads]`` that receives the logarithm of the sum of exponentials (-inf: nothing seen)."""
-        if out is None and lse is None:
+        Query ``i`` of a sequence is at ``p = pos + i`` and sees positions ``j <= p`` (``causal``) or ``j < pos + seq``, with a ``window`` only ``j > p - window``
+        and, of the others, the first ``sinks``; one that sees nothing gives zeros. ``scale``: default ``head_dim ** -0.5``. ``out``: where the result goes
+        (``q``'s shape and type, rows contiguous and 16-byte aligned). ``lse``: float32 ``[batch, seq, heads]`` that receives the logarithm of the sum of
+        exponentials (-inf: nothing seen).
+
+        With a plan: ``q`` ``[tokens, heads, head_dim]``, ``lse`` ``[tokens, heads]``. A token of a tree sees what lies below its tree, with a ``window`` (at
+        least ``plan.longest``) as one at ``p`` = its position does, and its ancestors in the tree, whatever ``causal``. Rows that are no token give zeros; those
+        behind the last sequence are left as they are where ``out`` is given."""
+        plan = pos if isinstance(pos, KVPlan) else None
+        if out is None and lse is None and plan is None and not (sinks and window):
             res = self._native.kv_attend(self._handle, q, pos, causal, window, self.head_dim ** -0.5 if scale is None else scale)
             if res is not None:
                 return res
         _refuse_derivatives("attend", q, out, lse)
-        self._tokens("q", q)
-        heads, seq = q.shape[2], q.shape[1]
+        if plan is not None:
+            self._planned("attend", plan)
+            self._packed("q", q, plan)
+        else:
+            self._tokens("q", q)
+        heads = q.shape[-2]
+        batch, seq = (self.batch, q.shape[1]) if plan is None else (plan.batch, plan.longest)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"attend: {heads} query heads over {self.kv_heads} KV heads")
-        if window < 0:
-            raise ValueError(f"attend: window {window}")
+        if window < 0 or sinks < 0:
+            raise ValueError(f"attend: window {window}, sinks {sinks}")
+        if plan is not None and plan.sees is not None and 0 < window < plan.longest:
+            raise ValueError(f"attend: a window of {window} is shorter than the plan's trees of up to {plan.longest} tokens")
+        clear = out is None
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         elif out.shape != q.shape or out.dtype is not q.dtype or out.device != self.device or not _served(out) or any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
             raise ValueError(f"attend: out is {tuple(out.shape)} {out.dtype}; q is {tuple(q.shape)} {q.dtype}, and rows are contiguous, apart and 16-byte aligned")
-        if lse is not None and (lse.shape != q.shape[:3] or lse.dtype is not torch.float32 or lse.device != self.device or not lse.is_contiguous()):
-            raise ValueError(f"attend: lse is contiguous float32 {tuple(q.shape[:3])}")
+        if lse is not None and (lse.shape != q.shape[:-1] or lse.dtype is not torch.float32 or lse.device != self.device or not lse.is_contiguous()):
+            raise ValueError(f"attend: lse is contiguous float32 {tuple(q.shape[:-1])}")
         if not _served(q):
             q = q.clone(memory_format=torch.contiguous_format)
-        pp, stride = self._positions(pos)
+        pp, stride = self._positions(pos) if plan is None else (None, 0)
+        if out.numel() == 0:
+            return out
         L = _lib.lib()
+        common = (self.head_dim ** -0.5 if scale is None else float(scale), int(causal), int(window))
+        rows = (ctypes.byref(self._view), ctypes.byref(_rows(q)), ctypes.byref(_rows(out)), None if lse is None else ctypes.c_void_p(lse.data_ptr()))
         with torch.cuda.device(self.device):
-            ws, lock = _workspace(self.device, max(16, int(L.xnq_kv_attend_workspace_bytes(self.batch, seq, heads, self.kv_heads, self.head_dim))))
+            ws, lock = _workspace(self.device, max(16, int(L.xnq_kv_attend_workspace_bytes(batch, seq, heads, self.kv_heads, self.head_dim))))
+            scratch = (ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(self.device))
             with lock:   # (the interpreter's is free during the call, which may enqueue two kernels)
-                rc = L.xnq_kv_attend(ctypes.byref(self._view), ctypes.byref(_rows(q)), ctypes.byref(_rows(out)), None if lse is None else ctypes.c_void_p(lse.data_ptr()),
-                                     self.batch, seq, heads, pp, stride, self.head_dim ** -0.5 if scale is None else float(scale), int(causal), int(window),
-                                     ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(self.device))
+                if plan is None and not (sinks and window):
+                    rc = L.xnq_kv_attend(*rows, batch, seq, heads, pp, stride, *common, *scratch)
+                else:
+                    rc = L.xnq_kv_attend_packed(*rows, batch, seq, heads, pp, stride, None if plan is None else ctypes.byref(plan._view), int(clear), *common, int(sinks), *scratch)
             _lib.check(rc)
         return out
