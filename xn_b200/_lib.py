@@ -129,7 +129,8 @@ def native():
             raise RuntimeError(f"xn_b200/_xnq_torch.so cannot be loaded ({e}). Build it with `python -m xn_b200.build`.") from e
         L = lib()
         address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
-        m.kv_bind(address(L.xnq_kv_store), address(L.xnq_kv_load), address(L.xnq_kv_attend), address(L.xnq_kv_attend_workspace_bytes), check)
+        m.kv_bind(*(address(f) for f in (L.xnq_kv_store, L.xnq_kv_load, L.xnq_kv_attend, L.xnq_kv_attend_workspace_bytes, L.xnq_kv_reserve, L.xnq_kv_reserve_workspace_bytes,
+                                         L.xnq_kv_plan_make, L.xnq_kv_store_packed, L.xnq_kv_keep, L.xnq_kv_attend_packed)), check)
         m.bind(address(L.xnq_matmul_t_bias), address(L.xnq_matvec), address(L.xnq_matmul_workspace_bytes), check)
         _native = m
     return _native

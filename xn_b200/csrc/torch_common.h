@@ -47,5 +47,10 @@ PyObject *kv_store(PyObject *, PyObject *const *, Py_ssize_t);
 PyObject *kv_rope_store(PyObject *, PyObject *const *, Py_ssize_t);
 PyObject *kv_load(PyObject *, PyObject *const *, Py_ssize_t);
 PyObject *kv_attend(PyObject *, PyObject *const *, Py_ssize_t);
+PyObject *kv_reserve(PyObject *, PyObject *const *, Py_ssize_t);
+PyObject *kv_plan(PyObject *, PyObject *const *, Py_ssize_t);
+PyObject *kv_keep(PyObject *, PyObject *const *, Py_ssize_t);
+PyObject *kv_plan_handle(PyObject *, PyObject *);
+PyObject *kv_plan_view(PyObject *, PyObject *);
 
 } // namespace xnq_torch

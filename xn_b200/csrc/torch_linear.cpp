@@ -197,11 +197,16 @@ PyMethodDef methods[] = {
     {"observed", py_observed, METH_NOARGS, "observed() -> whether a mode, a transform or a tracer looks at torch's operators"},
     {"bind", bind, METH_VARARGS, "bind(matmul, matvec, workspace_bytes, check)"},
     {"kv_cache", kv_cache, METH_VARARGS, "kv_cache(address of an xnq_kv_cache, batch, device index) -> capsule"},
-    {"kv_bind", kv_bind, METH_VARARGS, "kv_bind(store, load, attend, workspace_bytes, check)"},
-    {"kv_store", FAST(kv_store), "kv_store(cache, k, v, pos) -> True or None"},
-    {"kv_rope_store", FAST(kv_rope_store), "kv_rope_store(cache, qkv, cos, sin, pos, heads, type or -1) -> q or None"},
+    {"kv_bind", kv_bind, METH_VARARGS, "kv_bind(store, load, attend, workspace_bytes, reserve, reserve_workspace_bytes, plan_make, store_packed, keep, attend_packed, check)"},
+    {"kv_store", FAST(kv_store), "kv_store(cache, k, v, pos or plan) -> True or None"},
+    {"kv_rope_store", FAST(kv_rope_store), "kv_rope_store(cache, qkv, cos, sin, pos or plan, heads, type or -1) -> q or None"},
     {"kv_load", FAST(kv_load), "kv_load(cache, start, length, type) -> (k, v) or None"},
-    {"kv_attend", FAST(kv_attend), "kv_attend(cache, q, pos, causal, window, scale) -> out or None"},
+    {"kv_attend", FAST(kv_attend), "kv_attend(cache, q, pos or plan, causal, window, scale, sinks) -> out or None"},
+    {"kv_reserve", FAST(kv_reserve), "kv_reserve(cache, page table, table to start from, length, first or None, sinks) -> (room, free) or None"},
+    {"kv_plan", FAST(kv_plan), "kv_plan(cache, pos, count, tokens, longest, parents or None) -> (handle, tensors ..) or None"},
+    {"kv_keep", FAST(kv_keep), "kv_keep(cache, plan, node) -> pos or None"},
+    {"kv_plan_handle", kv_plan_handle, METH_VARARGS, "kv_plan_handle(address of an xnq_kv_plan, page table, page_size, num_pages, max_seq, device index) -> handle"},
+    {"kv_plan_view", kv_plan_view, METH_O, "kv_plan_view(plan) -> (address, page table, page_size, num_pages, max_seq, device index)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_xnq_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -107,21 +107,11 @@ class KVPlan:
     ``pos``, as it was. For trees ``sees`` (int32 ``[tokens, ceil(longest / 32)]``, bit ``t % 32`` of word ``t // 32``: the token sees token ``t`` of its tree) and
     ``nodes`` (the same for all tokens of a tree ``[batch, ..]``); else None. The tensors are the plan's own and not to be written to."""
 
-    __slots__ = ("tokens", "longest", "batch", "table", "page_size", "num_pages", "max_seq", "start", "offsets", "sequence", "position", "slot", "sees", "nodes", "_view")
+    __slots__ = ("tokens", "longest", "batch", "start", "offsets", "sequence", "position", "slot", "sees", "nodes", "_handle")
 
-    def __init__(self, cache: "QuantizedKVCache", tokens: int, longest: int, tree: bool):
-        dev = cache.device
-        self.tokens, self.longest, self.batch = tokens, longest, cache.batch
-        self.table, self.page_size, self.num_pages, self.max_seq = cache.page_table, cache.page_size, cache.num_pages, cache.max_seq
-        i64 = torch.empty(2 * cache.batch + 1 + 2 * tokens, dtype=torch.int64, device=dev)
-        self.start, self.offsets, self.position, self.slot = i64.split([cache.batch, cache.batch + 1, tokens, tokens])
-        words = -(-longest // 32) if tree else 0
-        i32 = torch.empty(tokens + (tokens + cache.batch) * words, dtype=torch.int32, device=dev)
-        self.sequence, sees, nodes = i32.split([tokens, tokens * words, cache.batch * words])
-        self.sees, self.nodes = (sees.view(tokens, words), nodes.view(cache.batch, words)) if tree else (None, None)
-        p = [t.data_ptr() for t in (self.start, self.offsets, self.sequence, self.position, self.slot)]
-        p = [x or i64.data_ptr() for x in p]   # (of no tokens: an address that is not NULL, which nothing is written to)
-        self._view = _Plan(tokens, cache.batch, longest, *p, (sees.data_ptr() or i32.data_ptr() or 16) if tree else None, nodes.data_ptr() if tree else None)
+    def __init__(self, tokens: int, longest: int, batch: int, made: tuple):
+        self.tokens, self.longest, self.batch = tokens, longest, batch
+        self._handle, self.start, self.offsets, self.sequence, self.position, self.slot, self.sees, self.nodes = made
 
 
 class QuantizedKVCache:
@@ -196,6 +186,9 @@ class QuantizedKVCache:
         order, each up to its first missing page), and ``free`` int64 ``[]``, the pages left."""
         if self.page_table is None:
             raise ValueError("reserve: this cache has no pages")
+        both = self._native.kv_reserve(self._handle, self.page_table, self.page_table if table is None else table, length, first, sinks)
+        if both is not None:
+            return both
         _refuse_derivatives("reserve")
         for what, t in (("length", length), ("first", first)):
             if t is not None and (t.dtype is not torch.int64 or t.device != self.device or t.shape != (self.batch,) or not t.is_contiguous()):
@@ -228,6 +221,9 @@ class QuantizedKVCache:
         if tokens < 0 or (longest is not None and longest < 1):
             raise ValueError(f"plan: {tokens} tokens, up to {longest} a sequence")
         longest = max(1, min(tokens, longest if longest is not None else tokens))
+        made = self._native.kv_plan(self._handle, pos, count, tokens, longest, parents)
+        if made is not None:
+            return KVPlan(tokens, longest, self.batch, made)
         if count.dtype is not torch.int64 or count.device != self.device or count.shape != (self.batch,) or not count.is_contiguous():
             raise ValueError(f"plan: count is contiguous int64 [{self.batch}] on {self.device}")
         if parents is not None:
@@ -236,31 +232,45 @@ class QuantizedKVCache:
             if longest > TREE_MOST:
                 raise ValueError(f"plan: trees of up to {longest} tokens (up to {TREE_MOST} are served)")
         pp, stride = self._positions(pos)
+        b, words = self.batch, -(-longest // 32) if parents is not None else 0
         with torch.cuda.device(self.device):
-            plan = KVPlan(self, tokens, longest, parents is not None)
+            wide = torch.empty(2 * b + 1 + 2 * tokens + 1, dtype=torch.int64, device=self.device)   # (one more than there are: no address is null)
+            narrow = torch.empty(tokens + (tokens + b) * words + 1, dtype=torch.int32, device=self.device)
+            start, offsets, position, slot, _ = wide.split([b, b + 1, tokens, tokens, 1])
+            sequence, sees, nodes, _ = narrow.split([tokens, tokens * words, b * words, 1])
+            w, n = wide.data_ptr(), narrow.data_ptr()
+            tree = parents is not None
+            view = _Plan(tokens, b, longest, w, w + 8 * b, n, w + 8 * (2 * b + 1), w + 8 * (2 * b + 1 + tokens), n + 4 * tokens if tree else None, n + 4 * (tokens + tokens * words) if tree else None)
             _lib.check(_lib.lib().xnq_kv_plan_make(ctypes.byref(self._view), pp, stride, ctypes.c_void_p(count.data_ptr()),
-                                                   None if parents is None else ctypes.c_void_p(parents.data_ptr() or 16), ctypes.byref(plan._view), _stream_ptr(self.device)))
-        return plan
+                                                   ctypes.c_void_p(parents.data_ptr() or n) if tree else None, ctypes.byref(view), _stream_ptr(self.device)))
+        table = self.page_table.data_ptr() if self.page_table is not None else 0
+        handle = self._native.kv_plan_handle(ctypes.addressof(view), table, self.page_size, self.num_pages, self.max_seq, self.device.index)
+        return KVPlan(tokens, longest, b, (handle, start, offsets, sequence, position, slot, sees.view(tokens, words) if tree else None, nodes.view(b, words) if tree else None))
 
-    def _planned(self, who: str, plan: KVPlan) -> None:
-        """Whether the plan's slots are this cache's."""
-        if plan.batch != self.batch or plan.start.device != self.device or plan.max_seq != self.max_seq or plan.page_size != self.page_size or plan.num_pages != self.num_pages or \
-                (plan.table is None) != (self.page_table is None) or (plan.table is not None and plan.table.data_ptr() != self.page_table.data_ptr()):
-            raise ValueError(f"{who}: the plan was made for another cache (its batch, pages and page table have to be this one's)")
+    def _planned(self, who: str, plan: KVPlan) -> ctypes.c_void_p:
+        """The address of the plan's description. Its slots have to be this cache's."""
+        view, *made_for = self._native.kv_plan_view(plan._handle)
+        if plan.batch != self.batch or made_for != [self.page_table.data_ptr() if self.page_table is not None else 0, self.page_size, self.num_pages, self.max_seq, self.device.index]:
+            raise ValueError(f"{who}: the plan was made for another cache (its device, batch, pages and page table have to be this one's)")
+        return ctypes.c_void_p(view)
 
     def keep(self, plan: KVPlan, node: torch.Tensor) -> torch.Tensor:
         """Of each tree of drafted tokens the path to ``node[b]`` (int64 ``[batch]``, the index in its tree; -1: no token) stays: the keys and values of its
         tokens move up to the positions ``pos[b], pos[b] + 1, ..``. Returns where each sequence goes on, int64 ``[batch]``: ``pos`` plus the path's length. What
         the other tokens had stored may lie behind that."""
+        if isinstance(plan, KVPlan):
+            pos = self._native.kv_keep(self._handle, plan._handle, node)
+            if pos is not None:
+                return pos
         _refuse_derivatives("keep")
-        self._planned("keep", plan)
+        view = self._planned("keep", plan)
         if plan.sees is None:
             raise ValueError("keep: the plan is not one of trees (parents)")
         if node.dtype is not torch.int64 or node.device != self.device or node.shape != (self.batch,) or not node.is_contiguous():
             raise ValueError(f"keep: node is contiguous int64 [{self.batch}] on {self.device}")
         with torch.cuda.device(self.device):
             pos = torch.empty(self.batch, dtype=torch.int64, device=self.device)
-            _lib.check(_lib.lib().xnq_kv_keep(ctypes.byref(self._view), ctypes.byref(plan._view), ctypes.c_void_p(node.data_ptr()), ctypes.c_void_p(pos.data_ptr()),
+            _lib.check(_lib.lib().xnq_kv_keep(ctypes.byref(self._view), view, ctypes.c_void_p(node.data_ptr()), ctypes.c_void_p(pos.data_ptr()),
                                               _stream_ptr(self.device)))
         return pos
 
@@ -277,15 +287,16 @@ class QuantizedKVCache:
         """Quantize ``k`` and ``v`` ``[batch, seq, kv_heads, head_dim]`` (f32 / f16 / bf16, any strides) into positions ``pos ..``: the blocks that
         ``BlockQ4_0`` / ``BlockQ8_0::from_float`` make of the f32 values (k_quants.rs:235-270, 636-661), Q8_0's scale being ``max|x| * float32(1 / 127)``.
         With a plan: ``[tokens, kv_heads, head_dim]``, each token into its slot."""
-        if isinstance(pos, KVPlan):
+        plan = pos if isinstance(pos, KVPlan) else None
+        if self._native.kv_store(self._handle, k, v, pos if plan is None else plan._handle):
+            return
+        if plan is not None:
             _refuse_derivatives("store", k, v)
-            self._planned("store", pos)
-            self._packed("k", k, pos, self.kv_heads), self._packed("v", v, pos, self.kv_heads)
+            view = self._planned("store", plan)
+            self._packed("k", k, plan, self.kv_heads), self._packed("v", v, plan, self.kv_heads)
             if k.dtype is not v.dtype:
                 raise ValueError(f"k is {k.dtype}, v {v.dtype}")
-            return self._store_packed(k, v, pos, None)
-        if self._native.kv_store(self._handle, k, v, pos):
-            return
+            return self._store_packed(k, v, plan.tokens, view, None)
         _refuse_derivatives("store", k, v)
         self._tokens("k", k, self.kv_heads), self._tokens("v", v, self.kv_heads)
         if k.shape != v.shape or k.dtype is not v.dtype:
@@ -297,14 +308,13 @@ class QuantizedKVCache:
         2]``) at their positions, k and v stored. Returns q ``[batch, seq, heads, head_dim]`` as ``out_dtype`` (default: ``qkv``'s). With a plan: ``[tokens, ..]``,
         and q ``[tokens, heads, head_dim]``, zeros for rows that are no token."""
         plan = pos if isinstance(pos, KVPlan) else None
-        if plan is None and (out_dtype is None or out_dtype in _TORCH_TO_XNQ):
-            q = self._native.kv_rope_store(self._handle, qkv, cos, sin, pos, heads, -1 if out_dtype is None else _XNQ_IDS[out_dtype])
+        if out_dtype is None or out_dtype in _TORCH_TO_XNQ:
+            q = self._native.kv_rope_store(self._handle, qkv, cos, sin, pos if plan is None else plan._handle, heads, -1 if out_dtype is None else _XNQ_IDS[out_dtype])
             if q is not None:
                 return q
         _refuse_derivatives("rope_store", qkv, cos, sin)
         hd, width = self.head_dim, (heads + 2 * self.kv_heads) * self.head_dim
-        if plan is not None:
-            self._planned("rope_store", plan)
+        view = None if plan is None else self._planned("rope_store", plan)
         if heads < 1 or qkv.dim() != (3 if plan is None else 2) or qkv.shape[-1] != width:
             raise ValueError(f"rope_store: qkv is {tuple(qkv.shape)}; {heads} + 2 * {self.kv_heads} heads of {hd}")
         for t in (cos, sin):
@@ -320,15 +330,15 @@ class QuantizedKVCache:
         out = torch.empty((*q.shape,), dtype=out_dtype or qkv.dtype, device=self.device)
         if out.numel():
             rope = _Rope(cos.data_ptr(), sin.data_ptr(), cos.shape[0], heads, _rows(q), _rows(out))
-            self._store(k, v, pos, rope) if plan is None else self._store_packed(k, v, plan, rope)
+            self._store(k, v, pos, rope) if plan is None else self._store_packed(k, v, plan.tokens, view, rope)
         return out
 
-    def _store_packed(self, k, v, plan, rope) -> None:
-        if plan.tokens == 0:
+    def _store_packed(self, k, v, tokens, view, rope) -> None:
+        if tokens == 0:
             return
         k, v = (t if _served(t) else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
         with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().xnq_kv_store_packed(ctypes.byref(self._view), ctypes.byref(_rows(k)), ctypes.byref(_rows(v)), ctypes.byref(plan._view),
+            _lib.check(_lib.lib().xnq_kv_store_packed(ctypes.byref(self._view), ctypes.byref(_rows(k)), ctypes.byref(_rows(v)), view,
                                                       None if rope is None else ctypes.byref(rope), _stream_ptr(self.device)))
 
     def _store(self, k, v, pos, rope) -> None:
@@ -368,13 +378,14 @@ class QuantizedKVCache:
         least ``plan.longest``) as one at ``p`` = its position does, and its ancestors in the tree, whatever ``causal``. Rows that are no token give zeros; those
         behind the last sequence are left as they are where ``out`` is given."""
         plan = pos if isinstance(pos, KVPlan) else None
-        if out is None and lse is None and plan is None and not (sinks and window):
-            res = self._native.kv_attend(self._handle, q, pos, causal, window, self.head_dim ** -0.5 if scale is None else scale)
+        if out is None and lse is None:
+            res = self._native.kv_attend(self._handle, q, pos if plan is None else plan._handle, causal, window, self.head_dim ** -0.5 if scale is None else scale, sinks)
             if res is not None:
                 return res
         _refuse_derivatives("attend", q, out, lse)
+        view = None
         if plan is not None:
-            self._planned("attend", plan)
+            view = self._planned("attend", plan)
             self._packed("q", q, plan)
         else:
             self._tokens("q", q)
@@ -408,6 +419,6 @@ class QuantizedKVCache:
                 if plan is None and not (sinks and window):
                     rc = L.xnq_kv_attend(*rows, batch, seq, heads, pp, stride, *common, *scratch)
                 else:
-                    rc = L.xnq_kv_attend_packed(*rows, batch, seq, heads, pp, stride, None if plan is None else ctypes.byref(plan._view), int(clear), *common, int(sinks), *scratch)
+                    rc = L.xnq_kv_attend_packed(*rows, batch, seq, heads, pp, stride, view, int(clear), *common, int(sinks), *scratch)
             _lib.check(rc)
         return out
