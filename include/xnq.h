@@ -391,7 +391,7 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
  * (length[b], or where its first missing page begins); *free_pages: pages that no entry names. A page may be named by several rows (a shared beginning): it
  * is free when none does. Rows have ceil(max_seq / page_size) entries. Device memory, up to 2^20 pages. workspace: xnq_kv_reserve_workspace_bytes, 16-byte
  * aligned, of any contents; one call at a time may use it. */
-size_t xnq_kv_reserve_workspace_bytes(int64_t num_pages);
+size_t xnq_kv_reserve_workspace_bytes(int64_t batch, int64_t page_size, int64_t num_pages, int64_t max_seq);
 int xnq_kv_reserve(int32_t *table, int64_t table_stride, const int32_t *from, int64_t from_stride, int64_t batch, int64_t page_size, int64_t num_pages, int64_t max_seq,
                    const long long *length, const long long *first, int64_t sinks, long long *room, long long *free_pages, void *workspace, size_t ws_bytes, void *stream);
 /* Packed tokens: `tokens` rows, those of sequence 0 first, then sequence 1's .., then rows that are no sequence's. Sequence b brings count[b] tokens, for the

@@ -96,7 +96,7 @@ def lib() -> ctypes.CDLL:
     L.xnq_kv_attend_workspace_bytes.argtypes = [i64, i64, ci, ci, ci]
     L.xnq_kv_attend_workspace_bytes.restype = sz
     L.xnq_kv_attend.argtypes = [vp, vp, vp, vp, i64, i64, ci, vp, ci, fp, ci, i64, vp, sz, vp]
-    L.xnq_kv_reserve_workspace_bytes.argtypes = [i64]
+    L.xnq_kv_reserve_workspace_bytes.argtypes = [i64, i64, i64, i64]
     L.xnq_kv_reserve_workspace_bytes.restype = sz
     L.xnq_kv_reserve.argtypes = [vp, i64, vp, i64, i64, i64, i64, i64, vp, vp, i64, vp, vp, vp, sz, vp]
     L.xnq_kv_plan_make.argtypes = [vp, vp, ci, vp, vp, vp, vp]

@@ -392,7 +392,7 @@ PyObject *kv_reserve(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   if (from.scalar_type() != at::kInt || from.sizes() != to.sizes() || !from.is_contiguous() || from.device().index() != c->device) Py_RETURN_NONE;
   at::Tensor out = empty_here({c->batch + 1}, at::kLong);
   long long *const p = static_cast<long long *>(out.mutable_data_ptr());
-  const size_t need = g_reserve_bytes(c->c.num_pages);
+  const size_t need = g_reserve_bytes(c->batch, c->c.page_size, c->c.num_pages, c->c.max_seq);
   const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(std::max<size_t>(need, 16)); // for the current device and stream, where the call launches
   int rc;
   const cudaStream_t stream = stream_of(*c);

@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
   // Where an item's rows go; of an item and the next one: warp 0 writes the next one's while other warps still store this one's rows. Between an item and
   // the one after the next lie barriers that every warp reaches when it is done with the first.
   __shared__ long long s_row[2][R], s_lse_row[2][R];
+  __shared__ bool s_none[2][MORE ? R : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   float *const merge = reinterpret_cast<float *>(smem + SPLIT_WARPS * SPLIT_STAGES * L::BYTES);
   float *const s_m = merge, *const s_l = merge + SPLIT_WARPS * R, *const s_acc = merge + 2 * SPLIT_WARPS * R;
@@ -340,12 +341,24 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
       const long long row = (long long)rt * R + r, s = row / a.group;
       const int h = kvh * a.group + (int)(row - s * a.group);
       if (warp == 0 && t == 0) s_row[turn][r] = out_at + s * a.out.ss + h * a.out.sh, s_lse_row[turn][r] = (lse_row + s) * a.heads + h;
+      int l0 = 0, h0 = INT32_MAX; // no row: its weights are thrown away
+      if constexpr (MORE) { // (a row that is no token likewise: with it, its warp would weigh every tile position by position)
+        sight[n] = Sight{0, INT32_MAX, true};
+        if (r < rows) sight[n] = sight_of(a, sp, s);
+        if (sight[n].none) sight[n].lo = 0, sight[n].hi = INT32_MAX;
+        l0 = sight[n].lo, h0 = sight[n].hi;
+        tree[n] = a.sees && !sight[n].none ? a.sees + (sp.first_row + s) * a.words : nullptr;
+        if (warp == 0 && t == 0) s_none[turn][r] = sight[n].none;
+      } else if (r < rows) {
+        seen_by(a, sp.pos, s, l0, h0);
+        hi_any = max(hi_any, h0), lo_any = min(lo_any, l0);
+      }
       float v[NB][8], top = 0.f;
 #pragma unroll
       for (int bl = 0; bl < NB; bl++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) v[bl][i] = 0.f;
-        if (r < rows) load8_any(a.q.p, a.dtype, q_at + s * a.q.ss + h * a.q.sh + bl * 32 + t * 8, v[bl]);
+        if (r < rows && !(MORE && sight[MORE ? n : 0].none)) load8_any(a.q.p, a.dtype, q_at + s * a.q.ss + h * a.q.sh + bl * 32 + t * 8, v[bl]);
 #pragma unroll
         for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[bl][i]));
       }
@@ -377,17 +390,6 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
           qh[n][bl][i] = pack_half2(hi_v[x] * down, hi_v[y] * down);
           if (SPLIT) ql[n][bl][i] = pack_half2(lo_v[x] * down, lo_v[y] * down);
         }
-      }
-      int l0 = 0, h0 = INT32_MAX; // no row: its weights are thrown away
-      if constexpr (MORE) {
-        sight[n] = Sight{0, INT32_MAX};
-        if (r < rows) {
-          sight[n] = sight_of(a, sp, s), l0 = sight[n].lo, h0 = sight[n].hi;
-          tree[n] = a.sees ? a.sees + (sp.first_row + s) * a.words : nullptr;
-        }
-      } else if (r < rows) {
-        seen_by(a, sp.pos, s, l0, h0);
-        hi_any = max(hi_any, h0), lo_any = min(lo_any, l0);
       }
       lo_all = max(lo_all, l0), hi_all = min(hi_all, h0);
       const float f = fmaxf(ldexpf(fabsf(a.scale) * LOG2E, (SPLIT ? 0 : 24) - e), LEAST_FACTOR);
@@ -443,9 +445,8 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
         if (masked) {
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            const bool real = n * 8 + g < rows;
             const uint32_t m = seen_in_tile(a, sight[n], tree[n], sp.pos, j0);
-            any |= real ? m : 0u;
+            any |= sight[n].none ? 0u : m;
 #pragma unroll
             for (int c = 0; c < 2; c++) col[n][c] = __shfl_sync(0xffffffffu, m, (2 * t + c) * 4);
           }
@@ -760,6 +761,13 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
     constexpr int V = HD / 32;
     const bool whole = ta == 0 && tb == sp.count;
     auto put = [&](int r, float m_all, float l_all, float (&v)[V]) { // a finished row
+      if constexpr (MORE) {
+        if (s_none[turn][r]) {
+          l_all = 0.f;
+#pragma unroll
+          for (int i = 0; i < V; i++) v[i] = 0.f;
+        }
+      }
       const float by = l_all > 0.f ? 1.f / l_all : l_all; // 0: nothing seen, zeros; NaN stays
 #pragma unroll
       for (int i = 0; i < V; i++) v[i] *= by;

@@ -79,12 +79,13 @@ __device__ __forceinline__ Sequence sequence_of(const AttendArgs &a, int b) {
 // What one of a sequence's tokens sees: positions [lo, hi], the first `sinks` up to hi, and tokens of its tree (whose first is at place pos).
 struct Sight {
   int lo, hi;
+  bool none; // no token: sees nothing, and must not be looked at either
 };
 __device__ __forceinline__ Sight sight_of(const AttendArgs &a, const Sequence &x, long long s) {
   const long long p = a.offsets ? a.position[x.first_row + s] : x.pos + s;
   const long long h = p < 0 ? -1 : min(a.sees ? x.pos - 1 : a.causal ? p : x.pos + x.seq - 1, a.c.max_seq - 1);
   const long long l = a.window ? min(max(p - a.window + 1, 0ll), a.c.max_seq) : 0ll;
-  return Sight{(int)l, (int)h};
+  return Sight{(int)l, (int)h, p < 0};
 }
 __device__ __forceinline__ uint32_t bits_between(int from, int to) { // bits [from, to] of 32
   from = max(from, 0), to = min(to, 31);

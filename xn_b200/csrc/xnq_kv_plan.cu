@@ -18,41 +18,94 @@ __device__ unsigned int g_kv_plan_status;
 // The k-th entry (row by row) that is needed and not kept gets the k-th page, in ascending order, that is not used. What pages are free is not state of its
 // own: it follows from the table, so pages that two rows name (a shared beginning) are free when the last of them lets go.
 //
-// One thread-block cluster. Every CTA marks the pages of its run of entries in a bitmap of its own (shared memory); the CTAs add the bitmaps up, a slice each
-// (distributed shared memory), write the list of the first free pages, as many as are missing, and go over their entries again.
-constexpr int RESERVE_THREADS = 1024, RESERVE_WARPS = RESERVE_THREADS / 32, RESERVE_MOST_CTAS = 16;
+// Entries lie in the order of the table, 32 CELLS neighbouring ones to a warp; a lane's are asked for together. Up to RESERVE_SMALL entries: one block, a bitmap of
+// the pages and the list of the free ones in shared memory. More: three kernels over all SMs (clear the bitmap; mark pages and count what is missing; give
+// pages out, every block adding up what is missing before it and, if it misses any itself, reading the bitmap for the free pages of its ranks).
+constexpr int CELLS = 8, RESERVE_THREADS = 256, RESERVE_SMALL_THREADS = 1024, RESERVE_SMALL = RESERVE_SMALL_THREADS * CELLS;
 
+struct Divisor { // n / d for n < 2^31: n m >> (31 + s), s = ceil(log2 d), m = floor(2^(31 + s) / d) + 1, whose error n (m d - 2^(31 + s)) < 2^(31 + s) never carries
+  unsigned m, s;
+  static Divisor of(unsigned d) {
+    unsigned s = 0;
+    while ((1ull << s) < d) s++;
+    return Divisor{(unsigned)((1ull << (31 + s)) / d + 1), 31 + s};
+  }
+  __device__ __forceinline__ unsigned operator()(unsigned n) const { return (unsigned)(((unsigned long long)n * m) >> s); }
+};
 struct ReserveArgs {
   const int *from;
   int *to;
-  long long from_stride, to_stride, num_pages, max_seq, sinks;
+  long long from_stride, to_stride, max_seq;
   const long long *length, *first; // first: null, or [batch]
   long long *room, *free;
-  int *list; // [num_pages]
-  long long cells;
-  int batch, per, page_size; // per: entries of a row
+  uint32_t *bitmap; // many entries: pages that are in use
+  unsigned *missing; // many entries: of a block
+  unsigned num_pages, sinks, cells, per, page_size; // per: entries of a row
+  int batch;
+  Divisor by_per, by_page;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
+struct Cells { // a lane's entries, 32 apart
+  int v[CELLS];                  // their pages; -1: none
+  unsigned row[CELLS], at[CELLS];
+  unsigned in, needed;           // bits: is there such an entry, is it needed
+};
+__device__ __forceinline__ void load_cells(const ReserveArgs &a, unsigned begin, Cells &c) { // begin: the lane's first entry
+  c.in = c.needed = 0u;
+  unsigned n[CELLS], f[CELLS];
+#pragma unroll
+  for (int k = 0; k < CELLS; k++) {
+    const unsigned cell = begin + k * 32;
+    const bool in = cell < a.cells;
+    c.in |= (in ? 1u : 0u) << k;
+    c.row[k] = in ? a.by_per(cell) : 0u, c.at[k] = cell - c.row[k] * a.per;
+    c.v[k] = in ? a.from[c.row[k] * a.from_stride + c.at[k]] : -1;
+    n[k] = in ? (unsigned)min(max(a.length[c.row[k]], 0ll), a.max_seq) : 0u;
+    f[k] = in && a.first ? (unsigned)min(max(a.first[c.row[k]], 0ll), a.max_seq) : 0u;
+  }
+#pragma unroll
+  for (int k = 0; k < CELLS; k++) {
+    bool needed = n[k] && c.at[k] <= a.by_page(n[k] - 1); // entries of positions below the length
+    if (a.first) needed = needed && (c.at[k] >= a.by_page(f[k]) || c.at[k] * (unsigned long long)a.page_size < a.sinks);
+    c.needed |= (needed ? 1u : 0u) << k;
+    if (!needed || (unsigned)c.v[k] >= a.num_pages) c.v[k] = -1;
+  }
 }
-__device__ __forceinline__ void cluster_sync() { // every thread of every CTA; what was written before, shared or global, is seen behind it
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void mark_pages(const Cells &c, uint32_t *bitmap) { // pages of neighbouring entries often share a word: one atomic for the warp
+#pragma unroll
+  for (int k = 0; k < CELLS; k++) {
+    const int v = c.v[k];
+    const unsigned have = __ballot_sync(0xffffffffu, v >= 0);
+    if (!have) continue;
+    const int lead = __ffs(have) - 1, w = __shfl_sync(0xffffffffu, v >> 5, lead);
+    if (__all_sync(0xffffffffu, v < 0 || (v >> 5) == w)) {
+      const unsigned bits = __reduce_or_sync(0xffffffffu, v >= 0 ? 1u << (v & 31) : 0u);
+      if ((threadIdx.x & 31) == 0) atomicOr(bitmap + w, bits);
+    } else if (v >= 0) atomicOr(bitmap + (v >> 5), 1u << (v & 31));
+  }
 }
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
+__device__ __forceinline__ unsigned missing_cells(const Cells &c) { // of the warp
+  unsigned n = 0;
+#pragma unroll
+  for (int k = 0; k < CELLS; k++) n += ((c.needed >> k) & 1u) && c.v[k] < 0;
+  return __reduce_add_sync(0xffffffffu, n);
 }
-__device__ __forceinline__ uint32_t load_remote(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
+// list: the free pages from the rank `base` on; `at`: the rank of the warp's first missing entry; free_all: free pages there are
+__device__ __forceinline__ void give_pages(const ReserveArgs &a, Cells &c, unsigned at, unsigned base, unsigned free_all, const int *list) {
+  const unsigned below = (1u << (threadIdx.x & 31)) - 1u;
+#pragma unroll
+  for (int k = 0; k < CELLS; k++) {
+    const bool none = ((c.needed >> k) & 1u) && c.v[k] < 0;
+    const unsigned who = __ballot_sync(0xffffffffu, none);
+    if (none) {
+      const unsigned r = at + __popc(who & below);
+      if (r < free_all) c.v[k] = list[r - base];
+      else atomicMin(a.room + c.row[k], (long long)c.at[k] * a.page_size);
+    }
+    at += __popc(who);
+    if ((c.in >> k) & 1u) a.to[c.row[k] * a.to_stride + c.at[k]] = c.v[k];
+  }
 }
-__device__ __forceinline__ void store_remote(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-
 // exclusive sums over a block; total: of all
 template <int WARPS>
 __device__ __forceinline__ unsigned block_before(unsigned v, unsigned *s_warp, unsigned &total) {
@@ -65,141 +118,136 @@ __device__ __forceinline__ unsigned block_before(unsigned v, unsigned *s_warp, u
   }
   if (lane == 31) s_warp[warp] = inc;
   __syncthreads();
-  unsigned before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; w++) {
-    const unsigned x = s_warp[w];
-    if (w < warp) before += x;
-    total += x;
-  }
+  const unsigned x = lane < WARPS ? s_warp[lane] : 0u; // (up to 32 warps)
+  const unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0u);
+  total = __reduce_add_sync(0xffffffffu, x);
   __syncthreads();
   return before + inc - v;
 }
-
-__global__ void __launch_bounds__(RESERVE_THREADS, 1) kv_reserve_kernel(const ReserveArgs a, int ctas) {
-  extern __shared__ uint32_t bitmap[];
-  __shared__ unsigned s_warp[RESERVE_WARPS], s_missing[RESERVE_WARPS];
-  __shared__ uint32_t s_cta[2][RESERVE_MOST_CTAS]; // free pages and missing entries of every CTA
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t rank = cluster_rank();
-  const int words = (int)((a.num_pages + 31) / 32);
-  for (int i = threadIdx.x; i < words; i += RESERVE_THREADS) bitmap[i] = 0u;
+// The bitmap in chunks of 256 words, a warp a chunk and a lane 8 neighbouring words of it (words behind the last page's are 0, and no page is free there).
+constexpr unsigned CHUNK = 256, MOST_CHUNKS = (1u << 20) / 32 / CHUNK; // of RESERVE_MOST_PAGES
+__device__ __forceinline__ void load_chunk(const ReserveArgs &a, const uint32_t *bitmap, unsigned chunk, uint32_t (&free)[8]) {
+  const unsigned w = chunk * CHUNK + (threadIdx.x & 31) * 8;
+  const uint4 x = *reinterpret_cast<const uint4 *>(bitmap + w), y = *reinterpret_cast<const uint4 *>(bitmap + w + 4);
+  const uint32_t used[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const long long left = (long long)a.num_pages - (long long)(w + i) * 32; // pages of the word
+    free[i] = ~used[i] & (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u);
+  }
+}
+template <int WARPS>
+__device__ __forceinline__ unsigned count_free(const ReserveArgs &a, const uint32_t *bitmap, unsigned chunks, unsigned *s_chunk, unsigned *s_warp) { // s_chunk: free pages before each chunk
+#pragma unroll 2
+  for (unsigned k = threadIdx.x >> 5; k < chunks; k += WARPS) {
+    uint32_t free[8];
+    load_chunk(a, bitmap, k, free);
+    unsigned n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) n += __popc(free[i]);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) s_chunk[k] = n;
+  }
   __syncthreads();
+  static_assert(MOST_CHUNKS <= 256, "a chunk a thread");
+  unsigned all;
+  const unsigned n = threadIdx.x < chunks ? s_chunk[threadIdx.x] : 0u, before = block_before<WARPS>(n, s_warp, all);
+  if (threadIdx.x < chunks) s_chunk[threadIdx.x] = before;
+  __syncthreads();
+  return all;
+}
+// The free pages of ranks [first, first + n) into list: a word a thread, so that no thread has more than 32 pages to write (with a lane's 8 words as they are
+// loaded above, the pages of a small cache were one lane's: 16 us for 4 rows of 64 entries).
+template <int THREADS>
+__device__ __forceinline__ void list_pages(const ReserveArgs &a, const uint32_t *bitmap, unsigned chunks, unsigned all, const unsigned *s_chunk, unsigned *s_warp, unsigned first, unsigned n, int *list) {
+  constexpr unsigned GROUP = THREADS / CHUNK; // chunks at a time
+  for (unsigned k = 0; k < chunks; k += GROUP) {
+    const unsigned begin = s_chunk[k], end = k + GROUP < chunks ? s_chunk[k + GROUP] : all;
+    if (begin >= first + n || end <= first) continue;
+    const unsigned w = k * CHUNK + threadIdx.x;
+    const long long left = (long long)a.num_pages - (long long)w * 32;
+    uint32_t bits = left > 0 ? ~bitmap[w] & (left >= 32 ? 0xffffffffu : (1u << left) - 1u) : 0u;
+    unsigned sum, rank = begin + block_before<THREADS / 32>(__popc(bits), s_warp, sum);
+    for (; bits; bits &= bits - 1, rank++)
+      if (rank >= first && rank < first + n) list[rank - first] = (int)(w * 32) + __ffs(bits) - 1;
+  }
+}
+
+__global__ void __launch_bounds__(RESERVE_SMALL_THREADS, 1) kv_reserve_small_kernel(const ReserveArgs a) {
+  constexpr int WARPS = RESERVE_SMALL_THREADS / 32;
+  extern __shared__ __align__(16) uint32_t bitmap[];
+  __shared__ int s_list[RESERVE_SMALL];
+  __shared__ unsigned s_warp[WARPS], s_chunk[MOST_CHUNKS];
+  const unsigned chunks = (a.num_pages + 32 * CHUNK - 1) / (32 * CHUNK), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (unsigned i = threadIdx.x; i < chunks * CHUNK; i += RESERVE_SMALL_THREADS) bitmap[i] = 0u;
   pdl_launch_dependents();
   pdl_wait();
-  for (int b = rank * RESERVE_THREADS + threadIdx.x; b < a.batch; b += ctas * RESERVE_THREADS) a.room[b] = min(max(a.length[b], 0ll), a.max_seq);
-
-  // A warp's run of entries, in the order of the table; f(entry, needed, row, place) for each.
-  const long long run = (a.cells + (long long)ctas * RESERVE_WARPS * 32 - 1) / ((long long)ctas * RESERVE_WARPS * 32) * 32;
-  const long long begin = (rank * (long long)RESERVE_WARPS + warp) * run, end = min(begin + run, a.cells);
-  const unsigned ps = (unsigned)a.page_size;
-  auto walk = [&](auto f) {
-    int row = 0, i = 0, known = -1;
-    unsigned last = 0, from = 0, heads = 0; // entries [0, heads) and [from, last) are needed
-    for (long long at = begin; at < end; at += 32) {
-      const long long cell = at + lane;
-      const bool in = cell < end;
-      if (at == begin || a.per < 32) row = in ? (int)(cell / a.per) : 0, i = in ? (int)(cell - (long long)row * a.per) : 0;
-      else {
-        i += 32;
-        if (i >= a.per) i -= a.per, row++;
-      }
-      if (in && row != known) {
-        known = row;
-        const unsigned n = (unsigned)min(max(a.length[row], 0ll), a.max_seq);
-        last = (n + ps - 1) / ps;
-        from = a.first ? min((unsigned)min(max(a.first[row], 0ll), a.max_seq) / ps, last) : 0u;
-        heads = a.first ? min((unsigned)min(a.sinks, a.max_seq + ps) / ps + ((unsigned)min(a.sinks, a.max_seq + ps) % ps != 0), last) : 0u;
-      }
-      const bool needed = in && (unsigned)i < last && ((unsigned)i >= from || (unsigned)i < heads);
-      f(in, needed, row, i);
-    }
-  };
-  auto entry = [&](bool needed, int row, int i) { // -1: no page
-    const int v = needed ? a.from[row * a.from_stride + i] : -1;
-    return v >= 0 && v < a.num_pages ? v : -1;
-  };
-  unsigned missing = 0;
-  walk([&](bool, bool needed, int row, int i) {
-    const int v = entry(needed, row, i);
-    missing += __popc(__ballot_sync(0xffffffffu, needed && v < 0));
-    // Pages of neighbouring entries often share a word: one atomic for the warp.
-    const unsigned have = __ballot_sync(0xffffffffu, v >= 0);
-    if (have) {
-      const int w = __shfl_sync(0xffffffffu, v >> 5, __ffs(have) - 1);
-      if (__all_sync(0xffffffffu, v < 0 || (v >> 5) == w)) {
-        const unsigned bits = __reduce_or_sync(0xffffffffu, v >= 0 ? 1u << (v & 31) : 0u);
-        if (lane == 0) atomicOr(&bitmap[w], bits);
-      } else if (v >= 0) atomicOr(&bitmap[v >> 5], 1u << (v & 31));
-    }
-  });
-  if (lane == 0) s_missing[warp] = missing;
-  if (ctas > 1) cluster_sync();
-  else __syncthreads();
-
-  // ---- this CTA's slice of the pages: all bitmaps together, and how many are free ----
-  const int slice = (words + ctas - 1) / ctas, w0 = min((int)rank * slice, words), w1 = min(w0 + slice, words);
-  const int each = (slice + RESERVE_THREADS - 1) / RESERVE_THREADS, mine0 = min(w0 + (int)threadIdx.x * each, w1), mine1 = min(mine0 + each, w1);
-  const uint32_t map = (uint32_t)__cvta_generic_to_shared(bitmap);
-  if (ctas > 1) {
-    for (int w = w0 + threadIdx.x; w < w1; w += RESERVE_THREADS) { // (in this CTA's own bitmap nobody else looks at this slice)
-      uint32_t x[RESERVE_MOST_CTAS];
-#pragma unroll
-      for (int c = 0; c < RESERVE_MOST_CTAS; c++) x[c] = c < ctas ? load_remote(in_cta(map + w * 4, c)) : 0u;
-      uint32_t all = 0;
-#pragma unroll
-      for (int c = 0; c < RESERVE_MOST_CTAS; c++) all |= x[c];
-      bitmap[w] = all;
-    }
+  Cells c;
+  load_cells(a, warp * (32 * CELLS) + lane, c);
+  for (int b = threadIdx.x; b < a.batch; b += RESERVE_SMALL_THREADS) a.room[b] = min(max(a.length[b], 0ll), a.max_seq);
+  __syncthreads();
+  mark_pages(c, bitmap);
+  unsigned missing_all;
+  const unsigned mine = missing_cells(c), before = block_before<WARPS>(lane == 0 ? mine : 0u, s_warp, missing_all); // (its barriers order the bitmap, too)
+  const unsigned free_all = count_free<WARPS>(a, bitmap, chunks, s_chunk, s_warp);
+  if (missing_all) {
+    list_pages<RESERVE_SMALL_THREADS>(a, bitmap, chunks, free_all, s_chunk, s_warp, 0u, missing_all, s_list);
     __syncthreads();
   }
-  auto free_in = [&](int w) {
-    const long long left = a.num_pages - (long long)w * 32; // pages of the word
-    return ~bitmap[w] & (left >= 32 ? 0xffffffffu : (1u << left) - 1u);
-  };
-  unsigned n_free = 0, free_here, missing_here = 0, missing_before = 0;
-  for (int w = mine0; w < mine1; w++) n_free += __popc(free_in(w));
-  unsigned free_before = block_before<RESERVE_WARPS>(n_free, s_warp, free_here);
-#pragma unroll
-  for (int w = 0; w < RESERVE_WARPS; w++) {
-    if (w < warp) missing_before += s_missing[w];
-    missing_here += s_missing[w];
-  }
-  unsigned free_all = free_here, missing_all = missing_here;
-  if (ctas > 1) {
-    if ((int)threadIdx.x < ctas) {
-      store_remote(in_cta((uint32_t)__cvta_generic_to_shared(&s_cta[0][rank]), threadIdx.x), free_here);
-      store_remote(in_cta((uint32_t)__cvta_generic_to_shared(&s_cta[1][rank]), threadIdx.x), missing_here);
-    }
-    cluster_sync();
-    free_all = missing_all = 0;
-    for (int c = 0; c < ctas; c++) {
-      const unsigned f = s_cta[0][c], m = s_cta[1][c];
-      if (c < (int)rank) free_before += f, missing_before += m;
-      free_all += f, missing_all += m;
-    }
-  }
-  if (missing_all) {
-    for (int w = mine0; w < mine1 && free_before < missing_all; w++)
-      for (uint32_t bits = free_in(w); bits && free_before < missing_all; bits &= bits - 1) a.list[free_before++] = w * 32 + __ffs(bits) - 1;
-    if (ctas > 1) cluster_sync();
-    else __syncthreads();
-  }
+  give_pages(a, c, __shfl_sync(0xffffffffu, before, 0), 0u, free_all, s_list);
+  if (threadIdx.x == 0) *a.free = (long long)free_all - min(free_all, missing_all);
+}
 
-  unsigned at = missing_before; // which of the missing entries the warp is at
-  walk([&](bool in, bool needed, int row, int i) {
-    int v = entry(needed, row, i);
-    const unsigned none = __ballot_sync(0xffffffffu, needed && v < 0);
-    if (needed && v < 0) {
-      const unsigned k = at + __popc(none & ((1u << lane) - 1u));
-      if (k < free_all) v = __ldcg(a.list + k);
-      else atomicMin(a.room + row, (long long)i * a.page_size);
-    }
-    at += __popc(none);
-    if (in) a.to[row * a.to_stride + i] = v;
-  });
-  if (rank == 0 && threadIdx.x == 0) *a.free = (long long)free_all - min(free_all, missing_all);
+__global__ void __launch_bounds__(RESERVE_THREADS) kv_reserve_clear_kernel(const ReserveArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const unsigned words = (a.num_pages + 32 * CHUNK - 1) / (32 * CHUNK) * CHUNK;
+  for (unsigned i = blockIdx.x * RESERVE_THREADS + threadIdx.x; i < words; i += gridDim.x * RESERVE_THREADS) a.bitmap[i] = 0u;
+  for (unsigned b = blockIdx.x * RESERVE_THREADS + threadIdx.x; b < (unsigned)a.batch; b += gridDim.x * RESERVE_THREADS) a.room[b] = min(max(a.length[b], 0ll), a.max_seq);
+}
+__global__ void __launch_bounds__(RESERVE_THREADS) kv_reserve_mark_kernel(const ReserveArgs a) {
+  __shared__ unsigned s_missing[RESERVE_THREADS / 32];
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  Cells c;
+  load_cells(a, blockIdx.x * (RESERVE_THREADS * CELLS) + warp * (32 * CELLS) + lane, c);
+  mark_pages(c, a.bitmap);
+  const unsigned n = missing_cells(c);
+  if (lane == 0) s_missing[warp] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned all = 0;
+#pragma unroll
+    for (int w = 0; w < RESERVE_THREADS / 32; w++) all += s_missing[w];
+    a.missing[blockIdx.x] = all;
+  }
+}
+__global__ void __launch_bounds__(RESERVE_THREADS, 4) kv_reserve_give_kernel(const ReserveArgs a) {
+  constexpr int WARPS = RESERVE_THREADS / 32;
+  __shared__ int s_list[RESERVE_THREADS * CELLS];
+  __shared__ unsigned s_warp[WARPS], s_chunk[MOST_CHUNKS];
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, chunks = (a.num_pages + 32 * CHUNK - 1) / (32 * CHUNK);
+  pdl_launch_dependents();
+  pdl_wait();
+  Cells c;
+  load_cells(a, blockIdx.x * (RESERVE_THREADS * CELLS) + warp * (32 * CELLS) + lane, c);
+  unsigned before = 0, all = 0;
+  for (unsigned x = threadIdx.x; x < gridDim.x; x += RESERVE_THREADS) {
+    const unsigned m = __ldcg(a.missing + x);
+    all += m, before += x < blockIdx.x ? m : 0u;
+  }
+  unsigned here, missing_all, blocks_before, free_all = 0;
+  const unsigned mine = missing_cells(c), at = __shfl_sync(0xffffffffu, block_before<WARPS>(lane == 0 ? mine : 0u, s_warp, here), 0);
+  block_before<WARPS>(before, s_warp, blocks_before);
+  block_before<WARPS>(all, s_warp, missing_all);
+  if (here || blockIdx.x == 0) {
+    free_all = count_free<WARPS>(a, a.bitmap, chunks, s_chunk, s_warp);
+    list_pages<RESERVE_THREADS>(a, a.bitmap, chunks, free_all, s_chunk, s_warp, blocks_before, here, s_list);
+    __syncthreads();
+  }
+  give_pages(a, c, blocks_before + at, blocks_before, free_all, s_list);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.free = (long long)free_all - min(free_all, missing_all);
 }
 
 // ---- where packed tokens go ----
@@ -441,7 +489,7 @@ __global__ void __launch_bounds__(KEEP_WARPS * 32) kv_keep_kernel(KvView c, xnq_
 }
 
 constexpr long long RESERVE_MOST_PAGES = 1ll << 20; // a bitmap of 128 KB
-int reserve_ctas(int64_t cells) { return cells <= 8192 ? 1 : 8; }
+size_t reserve_bitmap_bytes(int64_t num_pages) { return (size_t)((num_pages + 32 * CHUNK - 1) / (32 * CHUNK)) * CHUNK * 4; }
 
 } // namespace
 
@@ -452,7 +500,7 @@ int kv_plan_status(unsigned int *bits) {
 int kv_plan_init() {
   unsigned int zero = 0;
   XNQ_CUDA(cudaMemcpyToSymbol(g_kv_plan_status, &zero, sizeof(zero)));
-  XNQ_CUDA(cudaFuncSetAttribute(kv_reserve_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(RESERVE_MOST_PAGES / 8)));
+  XNQ_CUDA(cudaFuncSetAttribute(kv_reserve_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(RESERVE_MOST_PAGES / 8)));
   XNQ_CUDA(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (PLAN_MOST_BATCH + 1) * 4));
   return XNQ_OK;
 }
@@ -473,7 +521,11 @@ using namespace xnq;
 
 extern "C" {
 
-size_t xnq_kv_reserve_workspace_bytes(int64_t num_pages) { return num_pages < 1 || num_pages > RESERVE_MOST_PAGES ? 0 : (size_t)(num_pages + 3) / 4 * 16; }
+size_t xnq_kv_reserve_workspace_bytes(int64_t batch, int64_t page_size, int64_t num_pages, int64_t max_seq) {
+  if (batch < 0 || page_size < 1 || max_seq < 1 || num_pages < 1 || num_pages > RESERVE_MOST_PAGES) return 0;
+  const int64_t cells = batch * ((max_seq + page_size - 1) / page_size);
+  return cells <= RESERVE_SMALL ? 16 : reserve_bitmap_bytes(num_pages) + (size_t)(cells / (RESERVE_THREADS * CELLS) + 1) * 4;
+}
 
 int xnq_kv_reserve(int32_t *table, int64_t table_stride, const int32_t *from, int64_t from_stride, int64_t batch, int64_t page_size, int64_t num_pages, int64_t max_seq,
                    const long long *length, const long long *first, int64_t sinks, long long *room, long long *free_pages, void *workspace, size_t ws_bytes, void *stream) {
@@ -483,22 +535,28 @@ int xnq_kv_reserve(int32_t *table, int64_t table_stride, const int32_t *from, in
                 (long long)num_pages, (long long)max_seq, (long long)sinks);
   if (num_pages > RESERVE_MOST_PAGES) return fail(XNQ_ERR_UNSUPPORTED, "kv_reserve: %lld pages (up to %lld are served)", (long long)num_pages, RESERVE_MOST_PAGES);
   if (!free_pages || (batch && (!table || !from || !length || !room))) return fail(XNQ_ERR_NULL, "kv_reserve: NULL argument");
-  const int64_t per = (max_seq + page_size - 1) / page_size;
+  const int64_t per = (max_seq + page_size - 1) / page_size, cells = batch * per;
   if (table_stride < per || from_stride < per) return fail(XNQ_ERR_SIZE, "kv_reserve: rows of %lld and %lld entries; %lld positions take %lld", (long long)table_stride, (long long)from_stride, (long long)max_seq, (long long)per);
-  if (batch * per > INT32_MAX - 1024) return fail(XNQ_ERR_SIZE, "kv_reserve: tables of %lld x %lld entries", (long long)batch, (long long)per);
-  if (!workspace || ws_bytes < xnq_kv_reserve_workspace_bytes(num_pages)) return fail(XNQ_ERR_SIZE, "kv_reserve: workspace has %zu bytes, needs %zu", ws_bytes, xnq_kv_reserve_workspace_bytes(num_pages));
+  if (cells > INT32_MAX - RESERVE_SMALL) return fail(XNQ_ERR_SIZE, "kv_reserve: tables of %lld x %lld entries", (long long)batch, (long long)per);
+  const size_t need = xnq_kv_reserve_workspace_bytes(batch, page_size, num_pages, max_seq);
+  if (!workspace || ws_bytes < need) return fail(XNQ_ERR_SIZE, "kv_reserve: workspace has %zu bytes, needs %zu", ws_bytes, need);
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(XNQ_ERR_ALIGN, "kv_reserve: the workspace must be 16-byte aligned");
-  ReserveArgs a{from, table, from_stride, table_stride, num_pages, max_seq, std::min<int64_t>(sinks, INT32_MAX), length, first, room, free_pages, static_cast<int *>(workspace), batch * per, (int)batch, (int)per, (int)page_size};
-  const int ctas = reserve_ctas(a.cells);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas), cfg.blockDim = dim3(RESERVE_THREADS), cfg.dynamicSmemBytes = (size_t)(num_pages + 31) / 32 * 4, cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)ctas, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = 2;
-  XNQ_CUDA(cudaLaunchKernelEx(&cfg, kv_reserve_kernel, a, ctas));
+  uint8_t *const ws = static_cast<uint8_t *>(workspace);
+  const ReserveArgs a{from, table, from_stride, table_stride, max_seq, length, first, room, free_pages, reinterpret_cast<uint32_t *>(ws),
+                      reinterpret_cast<unsigned *>(ws + reserve_bitmap_bytes(num_pages)), (unsigned)num_pages, (unsigned)std::min<int64_t>(sinks, INT32_MAX), (unsigned)cells, (unsigned)per,
+                      (unsigned)page_size, (int)batch, Divisor::of((unsigned)per), Divisor::of((unsigned)page_size)};
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cells <= RESERVE_SMALL) {
+    XNQ_CUDA(launch_pdl(kv_reserve_small_kernel, dim3(1), dim3(RESERVE_SMALL_THREADS), reserve_bitmap_bytes(num_pages), s, a));
+    count_launch();
+    return XNQ_OK;
+  }
+  const dim3 block(RESERVE_THREADS), grid((unsigned)((cells + RESERVE_THREADS * CELLS - 1) / (RESERVE_THREADS * CELLS)));
+  XNQ_CUDA(launch_pdl(kv_reserve_clear_kernel, dim3(32), block, 0, s, a));
+  count_launch();
+  XNQ_CUDA(launch_pdl(kv_reserve_mark_kernel, grid, block, 0, s, a));
+  count_launch();
+  XNQ_CUDA(launch_pdl(kv_reserve_give_kernel, grid, block, 0, s, a));
   count_launch();
   return XNQ_OK;
 }

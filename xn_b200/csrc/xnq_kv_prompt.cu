@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         if (!plain) {
           unsigned bad = 0, most[2] = {0u, 0u};
           uint32_t seen = 0u; // MORE: positions of the tile that some row may see
-          if constexpr (MORE) seen = seen_in_tile(a, Sight{lo, hi}, a.nodes ? a.nodes + (long long)b * a.words : nullptr, pos, j0);
+          if constexpr (MORE) seen = seen_in_tile(a, Sight{lo, hi, false}, a.nodes ? a.nodes + (long long)b * a.words : nullptr, pos, j0);
 #pragma unroll
           for (int k = 0; k < 2 * KW; k++) {
             const bool is_k = k < KW;
@@ -546,11 +546,13 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     const long long at = row0 + row, tok = at / a.group;
     const int h = kvh * a.group + (int)(at - tok * a.group);
     int r_lo = 0, r_hi = INT_MAX;
+    bool live = valid;              // MORE: and a token (one that is none sees nothing, but must not make its warp weigh every tile position by position)
     const uint32_t *tree = nullptr; // MORE: the row's bits
     if constexpr (MORE) {
       if (valid) {
         const Sight v = sight_of(a, sq, tok);
-        r_lo = v.lo, r_hi = v.hi, tree = a.sees ? a.sees + (sq.first_row + tok) * a.words : nullptr;
+        live = !v.none;
+        if (live) r_lo = v.lo, r_hi = v.hi, tree = a.sees ? a.sees + (sq.first_row + tok) * a.words : nullptr;
       }
     } else if (valid) seen_by(a, pos, tok, r_lo, r_hi);
     const int lo_all = __reduce_max_sync(0xffffffffu, valid ? r_lo : 0), hi_all = __reduce_min_sync(0xffffffffu, r_hi);
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       uint4 x[HD / 8];
       const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q.p) + q_at + tok * a.q.ss + h * a.q.sh);
 #pragma unroll
-      for (int c = 0; c < HD / 8; c++) x[c] = valid && n > 0 ? src[c] : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < HD / 8; c++) x[c] = live && n > 0 ? src[c] : make_uint4(0, 0, 0, 0);
       auto value = [&](uint32_t w, int half) {
         if (a.dtype == XNQ_F16) return half ? __high2float(as_half2(w)) : __low2float(as_half2(w));
         return __uint_as_float(half ? w & 0xffff0000u : w << 16);
@@ -665,8 +667,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         bool every, nothing; // row of the warp sees all of them; sees any
         if constexpr (MORE) {
           every = all_seen(a, lo_all, hi_all, i0);
-          if (!every) mine = seen_in_tile(a, Sight{r_lo, r_hi}, tree, pos, i0);
-          nothing = !every && !__any_sync(0xffffffffu, valid && mine);
+          if (!every) mine = seen_in_tile(a, Sight{r_lo, r_hi, false}, tree, pos, i0);
+          nothing = !every && !__any_sync(0xffffffffu, live && mine);
         } else every = i0 >= lo_all && i0 + KV_TILE - 1 <= hi_all, nothing = i0 > hi_any || i0 + KV_TILE - 1 < lo_any;
         if (mt.gone || nothing) { // seen by no row of the warp
 #pragma unroll
@@ -720,6 +722,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     }
     if (alive && n) alive = wait_for(o_done + 8 * q, 0, dead);
     tc_fence_after();
+    if (MORE && !live) l = 0.f, ref = -INFINITY; // zeros
     // ---- the row's result, or its part ----
     if (a.splits == 1) {
       const float by = l > 0.f ? ldexpf(1.f / l, -v_ref) : l; // nothing seen: zeros; NaN stays

@@ -201,7 +201,7 @@ class QuantizedKVCache:
             raise ValueError(f"reserve: table is contiguous int32 {tuple(self.page_table.shape)} on {self.device}")
         out = torch.empty(self.batch + 1, dtype=torch.int64, device=self.device)
         L = _lib.lib()
-        need = int(L.xnq_kv_reserve_workspace_bytes(self.num_pages))
+        need = int(L.xnq_kv_reserve_workspace_bytes(self.batch, self.page_size, self.num_pages, self.max_seq))
         with torch.cuda.device(self.device):
             ws = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
             p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
