@@ -212,6 +212,64 @@ struct Meta { // of a tile
 // In a run of 8 positions, the place of pair i is taken by pair (i + run) & 3: what lies at column n of a tile
 __host__ __device__ constexpr int position_at(int n) { return (n & ~7) | ((((n >> 1) + (n >> 3)) & 3) << 1) | (n & 1); }
 
+// Packed tokens: which sequence's row tile is the unit-th of all that there are, by a whole block (the grid holds as many as there can be). Up to SORTED sequences
+// in the order of what they see, the longest first (the grid's last CTAs end the launch: with the sequences in their own order, 24 trees over 1600 to 8192 positions
+// took 249 us); within a sequence the last row tile first.
+constexpr int SORTED = 64;
+struct UnitScratch {
+  int tiles[SORTED], seen[SORTED]; // row tiles of a sequence, tiles of the cache that it sees
+};
+template <int THREADS>
+__device__ __forceinline__ bool unit_at(const AttendArgs &a, long long unit, int tile_rows, UnitScratch &u, long long *s_at, int &b, long long &rt) {
+  const int batch = (int)a.batch, x = threadIdx.x;
+  const auto tiles_of = [&](const Sequence &q) { return q.here ? (int)(((long long)q.seq * a.group + tile_rows - 1) / tile_rows) : 0; };
+  if (batch == 1) {
+    const Sequence q = sequence_of(a, 0);
+    b = 0, rt = tiles_of(q) - 1 - unit;
+    return rt >= 0;
+  }
+  if (x == 0) s_at[0] = -1;
+  if (batch <= SORTED) {
+    int mine = 0, seen = 0;
+    if (x < batch) {
+      const Sequence q = sequence_of(a, x);
+      u.tiles[x] = mine = tiles_of(q), u.seen[x] = seen = q.count;
+    }
+    __syncthreads();
+    if (x < batch && mine) {
+      long long before = 0;
+      for (int y = 0; y < batch; y++)
+        if (u.seen[y] > seen || (u.seen[y] == seen && y < x)) before += u.tiles[y];
+      if (unit >= before && unit < before + mine) s_at[0] = x, s_at[1] = mine - 1 - (unit - before);
+    }
+    __syncthreads();
+  } else {
+    long long before = 0;
+    const int lane = x & 31, warp = x >> 5;
+    for (int base = 0; base < batch && before <= unit; base += THREADS) {
+      const int mine = base + x < batch ? tiles_of(sequence_of(a, base + x)) : 0;
+      long long inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += up;
+      }
+      __syncthreads(); // (the sums of the round before have been read)
+      if (lane == 31) u.tiles[warp] = (int)inc;
+      __syncthreads();
+      long long first = before + inc - mine;
+      for (int w = 0; w < THREADS / 32; w++) {
+        if (w < warp) first += u.tiles[w];
+        before += u.tiles[w];
+      }
+      if (unit >= first && unit < first + mine) s_at[0] = base + x, s_at[1] = mine - 1 - (unit - first);
+    }
+    __syncthreads();
+  }
+  b = (int)s_at[0], rt = s_at[1];
+  return b >= 0;
+}
+
 // MORE: first positions that stay visible, packed tokens and trees; a CTA's tiles may then be two runs of the cache.
 template <int BITS, int HD, int QT, bool MORE>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(const __grid_constant__ AttendArgs a) {
@@ -228,13 +286,15 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - (uint32_t)__cvta_generic_to_shared(smem_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
+  int unit_b = 0; // MORE, packed
+  long long unit_rt = 0;
   if constexpr (MORE) {
-    if (a.offsets) { // (before this CTA takes anything: most of a ragged batch's grid has no rows)
+    if (a.offsets) { // (before this CTA takes anything: some have no rows)
+      __shared__ long long s_at[2];
+      static_assert(sizeof(UnitScratch) <= sizeof(meta), "what is not in use yet");
       pdl_wait();
-      const int per = (int)a.batch * a.c.kv_heads * a.splits, bk = (int)(blockIdx.x % per) / a.splits, b = bk / a.c.kv_heads;
       if (a.clear) clear_behind(a, HD);
-      const long long all_rows = (a.offsets[b + 1] - a.offsets[b]) * a.group;
-      if (all_rows < a.rows_from || (a.row_tiles - 1 - (int)(blockIdx.x / per)) * (long long)(QT * 128) >= all_rows) return;
+      if (!unit_at<PROMPT_THREADS>(a, blockIdx.x / (a.c.kv_heads * a.splits), QT * 128, *reinterpret_cast<UnitScratch *>(meta), s_at, unit_b, unit_rt)) return;
     }
   }
   const uint32_t raw_full = bar, raw_scanned = bar + 16 * 8, raw_empty = bar + 32 * 8, k_full = bar + 48 * 8, k_empty = k_full + 8 * RING, v_full = k_empty + 8 * RING, v_empty = v_full + 8 * RING,
@@ -262,8 +322,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   pdl_wait();
 
   // ---- which rows, which positions; the row tiles with the most positions first ----
-  const int per = (int)a.batch * a.c.kv_heads * a.splits, rem = (int)(blockIdx.x % per);
-  const int rt = a.row_tiles - 1 - (int)(blockIdx.x / per), split = rem % a.splits, bk = rem / a.splits, kvh = bk % a.c.kv_heads, b = bk / a.c.kv_heads;
+  const bool units = MORE && a.offsets; // (a.row_tiles: of all sequences)
+  const int per = (units ? 1 : (int)a.batch) * a.c.kv_heads * a.splits, rem = (int)(blockIdx.x % per), nth = (int)(blockIdx.x / per);
+  const int rt = units ? (int)unit_rt : a.row_tiles - 1 - nth, split = rem % a.splits, bk = rem / a.splits, kvh = bk % a.c.kv_heads, b = units ? unit_b : bk / a.c.kv_heads;
   Sequence sq; // MORE
   long long all_rows = a.seq * a.group, q_at = b * a.q.sb, out_at = b * a.out.sb, lse_row = (long long)b * a.seq;
   const long long row0 = (long long)rt * (QT * 128);
@@ -752,7 +813,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       }
       if (valid && a.lse) a.lse[(lse_row + tok) * a.heads + h] = l > 0.f ? (ref + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
     } else {
-      float *rec = a.records + (((size_t)(a.row_tiles - 1 - rt) * (per / a.splits) + bk) * a.splits + split) * P::RECORD;
+      float *rec = a.records + (((size_t)nth * (per / a.splits) + bk) * a.splits + split) * P::RECORD;
       if (valid) rec[row] = ref, rec[QT * 128 + row] = l;
       const float by = ldexpf(1.f, -v_ref);
       float *dst = rec + 2 * QT * 128 + (size_t)row * HD;
@@ -783,24 +844,30 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
 template <int HD, bool MORE>
 __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int V = HD / 32, RECORD = 128 * (HD + 2), AHEAD = 8;
-  const int lane = threadIdx.x & 31, units = (int)a.batch * a.c.kv_heads;
+  const bool packed = MORE && a.offsets;
+  const int lane = threadIdx.x & 31, units = (packed ? 1 : (int)a.batch) * a.c.kv_heads;
   const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5);
   long long all_rows = a.seq * a.group;
   pdl_launch_dependents();
   pdl_wait();
-  const int rt = (int)(at / (128ll * units)), bk = (int)(at / 128 % units), row = (int)(at % 128), b = bk / a.c.kv_heads, kvh = bk % a.c.kv_heads;
-  const long long at_row = rt * 128ll + row;
-  if (rt >= a.row_tiles) return;
+  const int nth = (int)(at / (128ll * units)), bk = (int)(at / 128 % units), row = (int)(at % 128); // (a block's rows are of one row tile)
+  int b = bk / a.c.kv_heads;
+  const int kvh = bk % a.c.kv_heads;
+  if (nth >= a.row_tiles) return;
+  long long rt = a.row_tiles - 1 - nth; // (the last row tiles' CTAs come first)
   long long out_at = b * a.out.sb, lse_row = (long long)b * a.seq;
   if constexpr (MORE) {
     if (a.offsets) {
+      __shared__ UnitScratch scratch;
+      __shared__ long long s_at[2];
+      if (!unit_at<256>(a, nth, 128, scratch, s_at, b, rt)) return;
       const long long first = a.offsets[b];
       all_rows = (a.offsets[b + 1] - first) * a.group, out_at = first * a.out.ss, lse_row = first;
-      if (all_rows < a.rows_from) return;
     }
   }
+  const long long at_row = rt * 128ll + row;
   if (at_row >= all_rows) return;
-  const float *const first = a.records + ((size_t)(a.row_tiles - 1 - rt) * units + bk) * a.splits * RECORD; // (the last row tiles' CTAs come first)
+  const float *const first = a.records + ((size_t)nth * units + bk) * a.splits * RECORD;
   float m = -INFINITY, l = 0.f, v[V] = {};
   for (int k = lane; k < a.splits; k += 32) m = fmaxf(m, __ldcg(first + (size_t)k * RECORD + row));
 #pragma unroll
@@ -845,8 +912,16 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_consta
 struct Plan {
   int qt, row_tiles, splits;
 };
-Plan plan_of(int64_t batch, int64_t seq, int group, int kv_heads, int64_t max_seq, int sms) {
-  const int64_t rows = seq * group, heads = batch * kv_heads, two = (rows + 255) / 256, one = (rows + 127) / 128;
+Plan plan_of(int64_t batch, int64_t seq, int group, int kv_heads, int64_t max_seq, int sms, int64_t tokens, int64_t rows_from) {
+  const int64_t rows = seq * group;
+  int64_t heads = batch * kv_heads, two = (rows + 255) / 256, one = (rows + 127) / 128;
+  if (tokens) { // packed: row tiles of all sequences, as many as there can be of these tokens
+    const int64_t all = tokens * group, sequences = std::min<int64_t>(batch, all / std::max<int64_t>(rows_from, 1));
+    const bool single = one == 1;
+    heads = kv_heads, two = std::min(batch * two, all / 256 + sequences), one = std::min(batch * one, all / 128 + sequences);
+    if (!single && heads * one > sms) return Plan{2, (int)std::min<int64_t>(two, INT_MAX), 1};
+    if (heads * one > sms) return Plan{1, (int)std::min<int64_t>(one, INT_MAX), 1};
+  }
   if (one > 1 && heads * one > sms) return Plan{2, (int)two, 1};
   const int64_t steps = (max_seq + BN - 1) / BN;
   return Plan{1, (int)one, (int)std::max<int64_t>(1, std::min<int64_t>(sms / (heads * one), steps / 2))};
@@ -854,12 +929,12 @@ Plan plan_of(int64_t batch, int64_t seq, int group, int kv_heads, int64_t max_se
 
 template <int BITS, int HD, int QT, bool MORE>
 int launch(const AttendArgs &a, cudaStream_t s) {
-  const int64_t grid = (int64_t)a.row_tiles * a.batch * a.c.kv_heads * a.splits;
+  const int64_t heads = (MORE && a.offsets ? 1 : a.batch) * a.c.kv_heads, grid = (int64_t)a.row_tiles * heads * a.splits;
   if (grid > INT_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of query rows are more than one launch takes", (long long)grid);
   XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT, MORE>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
   count_launch();
   if (a.splits == 1) return XNQ_OK;
-  XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD, MORE>, dim3((unsigned)(a.row_tiles * a.batch * a.c.kv_heads * 16)), dim3(256), 0, s, a));
+  XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD, MORE>, dim3((unsigned)(a.row_tiles * heads * 16)), dim3(256), 0, s, a));
   count_launch();
   return XNQ_OK;
 }
@@ -894,7 +969,7 @@ constexpr int MAX_PARTS = 160; // CTAs of a launch that shares positions: no mor
 size_t kv_prompt_parts_bytes(int head_dim) { return (size_t)MAX_PARTS * 128 * (head_dim + 2) * 4; }
 int launch_kv_prompt(const AttendArgs &args, bool more, int bits, int head_dim, int sms, cudaStream_t s) {
   AttendArgs a = args;
-  const Plan p = plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_PARTS));
+  const Plan p = plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_PARTS), a.offsets ? a.tokens : 0, a.rows_from);
   a.row_tiles = p.row_tiles, a.splits = p.splits;
   if (bits == 4) return head_dim == 64 ? launch_hd<4, 64>(a, more, p.qt, s) : launch_hd<4, 128>(a, more, p.qt, s);
   return head_dim == 64 ? launch_hd<8, 64>(a, more, p.qt, s) : launch_hd<8, 128>(a, more, p.qt, s);
