@@ -422,7 +422,9 @@ int xnq_kv_keep(const xnq_kv_cache *cache, const xnq_kv_plan *plan, const long l
  * a window > 0 only j > p - window or j < sinks. plan NULL: q and out [batch, seq, heads, head_dim], p = pos[b] + i. Else q, out [tokens, heads, head_dim] and lse
  * [tokens, heads] (batch, seq, pos and stride_b are not looked at), p the plan's position; with trees a token sees the cache below its tree (p and the window as
  * above; a window of at least `longest`) and the tokens of its tree that it descends from. A token that is none gives zeros; rows behind the last sequence
- * are left as they are, or set to zero (lse -inf) with `clear`. Workspace: xnq_kv_attend_workspace_bytes of (batch, seq), or of (plan->batch, plan->longest). */
+ * are left as they are, or set to zero (lse -inf) with `clear`. Workspace as for xnq_kv_attend: xnq_kv_attend_workspace_bytes, with a plan
+ * xnq_kv_attend_packed_workspace_bytes. */
+size_t xnq_kv_attend_packed_workspace_bytes(const xnq_kv_plan *plan, int heads, int kv_heads, int head_dim);
 int xnq_kv_attend_packed(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
                          int pos_stride, const xnq_kv_plan *plan, int clear, float scale, int causal, int64_t window, int64_t sinks, void *workspace, size_t ws_bytes, void *stream);
 

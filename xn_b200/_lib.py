@@ -102,6 +102,8 @@ def lib() -> ctypes.CDLL:
     L.xnq_kv_plan_make.argtypes = [vp, vp, ci, vp, vp, vp, vp]
     L.xnq_kv_store_packed.argtypes = [vp, vp, vp, vp, vp, vp]
     L.xnq_kv_keep.argtypes = [vp, vp, vp, vp, vp]
+    L.xnq_kv_attend_packed_workspace_bytes.argtypes = [vp, ci, ci, ci]
+    L.xnq_kv_attend_packed_workspace_bytes.restype = sz
     L.xnq_kv_attend_packed.argtypes = [vp, vp, vp, vp, i64, i64, ci, vp, ci, vp, ci, fp, ci, i64, i64, vp, sz, vp]
     L.xnq_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint)]
     L.xnq_device_check_record.argtypes = [ctypes.POINTER(ctypes.c_ulonglong)]
@@ -130,7 +132,7 @@ def native():
         L = lib()
         address = lambda f: ctypes.cast(f, ctypes.c_void_p).value
         m.kv_bind(*(address(f) for f in (L.xnq_kv_store, L.xnq_kv_load, L.xnq_kv_attend, L.xnq_kv_attend_workspace_bytes, L.xnq_kv_reserve, L.xnq_kv_reserve_workspace_bytes,
-                                         L.xnq_kv_plan_make, L.xnq_kv_store_packed, L.xnq_kv_keep, L.xnq_kv_attend_packed)), check)
+                                         L.xnq_kv_plan_make, L.xnq_kv_store_packed, L.xnq_kv_keep, L.xnq_kv_attend_packed, L.xnq_kv_attend_packed_workspace_bytes)), check)
         m.bind(address(L.xnq_matmul_t_bias), address(L.xnq_matvec), address(L.xnq_matmul_workspace_bytes), check)
         _native = m
     return _native

@@ -26,6 +26,7 @@ decltype(&xnq_kv_plan_make) g_plan_make = nullptr;
 decltype(&xnq_kv_store_packed) g_store_packed = nullptr;
 decltype(&xnq_kv_keep) g_keep = nullptr;
 decltype(&xnq_kv_attend_packed) g_attend_packed = nullptr;
+decltype(&xnq_kv_attend_packed_workspace_bytes) g_packed_bytes = nullptr;
 PyObject *g_check = nullptr; // raises the error of a status
 
 struct Cache { // owned by the capsule that the Python object keeps, with its tensors
@@ -65,8 +66,8 @@ struct Block {
   size_t bytes;
   std::mutex lock;
 };
-constexpr size_t BLOCK = 16 << 20; // the parts take 10 MB whatever the call; the rest is tickets
-constexpr int BLOCKS = 16;
+constexpr size_t BLOCK = 16 << 20, LARGE_BLOCK = 36 << 20; // the parts take 10 MB whatever the call, those of many packed tokens 34; the rest is tickets
+constexpr int BLOCKS = 32; // (a stream may have one of each size)
 Block g_blocks[BLOCKS]; // they and the counts: under the interpreter's lock
 int g_num_blocks = 0;
 int64_t g_caches = 0;
@@ -112,7 +113,8 @@ void *graph_block_for(c10::DeviceIndex device, cudaStream_t stream, size_t bytes
 }
 // the stream's block, or null: the call takes and clears one of its own
 Block *block_for(c10::DeviceIndex device, cudaStream_t stream, size_t bytes) {
-  if (bytes > BLOCK) return nullptr;
+  if (bytes > LARGE_BLOCK) return nullptr;
+  const size_t size = bytes > BLOCK ? LARGE_BLOCK : BLOCK;
   cudaStreamCaptureStatus capture;
   if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) {
     (void)cudaGetLastError();
@@ -120,15 +122,15 @@ Block *block_for(c10::DeviceIndex device, cudaStream_t stream, size_t bytes) {
   }
   if (capture != cudaStreamCaptureStatusNone) return nullptr;
   for (int i = 0; i < g_num_blocks; i++)
-    if (g_blocks[i].stream == stream && g_blocks[i].device == device) return &g_blocks[i];
+    if (g_blocks[i].stream == stream && g_blocks[i].device == device && g_blocks[i].bytes >= bytes) return &g_blocks[i];
   if (g_num_blocks == BLOCKS) return nullptr;
   Block &b = g_blocks[g_num_blocks];
   const RelaxedCapture relaxed;
-  if (cudaMalloc(&b.p, BLOCK) != cudaSuccess || cudaMemsetAsync(b.p, 0, BLOCK, stream) != cudaSuccess) {
+  if (cudaMalloc(&b.p, size) != cudaSuccess || cudaMemsetAsync(b.p, 0, XNQ_KV_WORKSPACE_ZEROED, stream) != cudaSuccess) {
     (void)cudaGetLastError();
     return nullptr;
   }
-  b.device = device, b.stream = stream, b.bytes = BLOCK;
+  b.device = device, b.stream = stream, b.bytes = size;
   g_num_blocks++;
   return &b;
 }
@@ -206,12 +208,13 @@ PyObject *kv_cache(PyObject *, PyObject *args) {
 
 // kv_bind(xnq_kv_store, xnq_kv_load, xnq_kv_attend, xnq_kv_attend_workspace_bytes, .., check): the library that ctypes has loaded
 PyObject *kv_bind(PyObject *, PyObject *args) {
-  unsigned long long store, load, attend, ws, reserve, reserve_ws, plan, store_packed, keep, attend_packed;
+  unsigned long long store, load, attend, ws, reserve, reserve_ws, plan, store_packed, keep, attend_packed, packed_ws;
   PyObject *check;
-  if (!PyArg_ParseTuple(args, "KKKKKKKKKKO", &store, &load, &attend, &ws, &reserve, &reserve_ws, &plan, &store_packed, &keep, &attend_packed, &check)) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKO", &store, &load, &attend, &ws, &reserve, &reserve_ws, &plan, &store_packed, &keep, &attend_packed, &packed_ws, &check)) return nullptr;
   g_reserve = reinterpret_cast<decltype(g_reserve)>(reserve), g_reserve_bytes = reinterpret_cast<decltype(g_reserve_bytes)>(reserve_ws);
   g_plan_make = reinterpret_cast<decltype(g_plan_make)>(plan), g_store_packed = reinterpret_cast<decltype(g_store_packed)>(store_packed);
   g_keep = reinterpret_cast<decltype(g_keep)>(keep), g_attend_packed = reinterpret_cast<decltype(g_attend_packed)>(attend_packed);
+  g_packed_bytes = reinterpret_cast<decltype(g_packed_bytes)>(packed_ws);
   g_store = reinterpret_cast<decltype(g_store)>(store), g_load = reinterpret_cast<decltype(g_load)>(load);
   g_attend = reinterpret_cast<decltype(g_attend)>(attend), g_workspace_bytes = reinterpret_cast<decltype(g_workspace_bytes)>(ws);
   Py_INCREF(check);
@@ -352,7 +355,7 @@ PyObject *kv_attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
   at::Tensor out = empty_here(qt.sizes(), qt.scalar_type());
   const xnq_rows o{out.mutable_data_ptr(), q.dtype, plan ? 0 : seq * heads * hd, heads * hd, hd};
   const cudaStream_t stream = stream_of(*c);
-  const size_t need = std::max<size_t>(g_workspace_bytes(c->batch, seq, (int)heads, c->c.kv_heads, c->c.head_dim), 256);
+  const size_t need = std::max<size_t>(plan ? g_packed_bytes(&plan->p, (int)heads, c->c.kv_heads, c->c.head_dim) : g_workspace_bytes(c->batch, seq, (int)heads, c->c.kv_heads, c->c.head_dim), 256);
   Block *const block = block_for(c->device, stream, need);
   c10::DataPtr own;
   void *ws = block ? block->p : graph_block_for(c->device, stream, need);

@@ -878,6 +878,9 @@ int split_nt(int bits, int64_t rows, int64_t heads, int sms) {
 // 129; 64 rows, 36 against 32, 78 against 52, 219 against 131. Q8_0, 16 rows, 29 against 28, 47 against 50, 98 against 135; 64 rows, 46 against 32, 92 against
 // 54, 309 against 136.
 constexpr int64_t PROMPT_ROWS = 64;
+// Packed tokens, where some sequences go there anyway: bf16 rows from here on (a result's rounding to bf16 is 8 times that of the keys to f16). 24 trees, two of
+// them of 48 and 60 rows over some 6000 positions: 230 us with these two here, 52 of it for them.
+constexpr int64_t PACKED_PROMPT_ROWS = 32;
 
 template <int BITS, int HD, int NT, bool SPLIT, bool MORE>
 int run_split(AttendArgs a, int sms, cudaStream_t s) {
@@ -947,9 +950,14 @@ int kv_attend_init(int device) {
 using namespace xnq;
 
 namespace {
+size_t workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim, bool packed) {
+  if (batch <= 0 || seq <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+  // (for the kernel for many rows at its most: a part for every SM)
+  return KV_TICKET_BYTES + std::max(RECORDS_BYTES, seq * (heads / kv_heads) >= PROMPT_ROWS ? kv_prompt_parts_bytes(head_dim, packed) : 0);
+}
 // The checks and arguments of both forms (nothing more where batch or seq is 0).
 int attend_args(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos, int pos_stride, float scale,
-                int causal, int64_t window, void *workspace, size_t ws_bytes, AttendArgs *args, int *sms) {
+                int causal, int64_t window, void *workspace, size_t ws_bytes, bool packed, AttendArgs *args, int *sms) {
   AttendArgs &a = *args;
   int rc = kv_view("kv_attend", cache, batch, &a.c);
   if (rc != XNQ_OK) return rc;
@@ -960,7 +968,7 @@ int attend_args(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *ou
   if (batch == 0 || seq == 0) return XNQ_OK;
   if ((rc = kv_rows("kv_attend", "q", q, &a.q)) != XNQ_OK || (rc = kv_rows("kv_attend", "out", out, &a.out)) != XNQ_OK) return rc;
   if (out->dtype != q->dtype) return fail(XNQ_ERR_DTYPE, "kv_attend: q has type %d, out %d", q->dtype, out->dtype);
-  const size_t need = xnq_kv_attend_workspace_bytes(batch, seq, heads, cache->kv_heads, cache->head_dim);
+  const size_t need = workspace_bytes(batch, seq, heads, cache->kv_heads, cache->head_dim, packed);
   if (!workspace || ws_bytes < need) return fail(XNQ_ERR_SIZE, "kv_attend: workspace has %zu bytes, needs %zu (zero it once after allocating)", ws_bytes, need);
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(XNQ_ERR_ALIGN, "kv_attend: the workspace must be 16-byte aligned");
   int device = 0;
@@ -977,10 +985,9 @@ int attend_args(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *ou
 
 extern "C" {
 
-size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim) {
-  if (batch <= 0 || seq <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
-  // (for the kernel for many rows at its most: a part for every SM)
-  return KV_TICKET_BYTES + std::max(RECORDS_BYTES, seq * (heads / kv_heads) >= PROMPT_ROWS ? kv_prompt_parts_bytes(head_dim) : 0);
+size_t xnq_kv_attend_workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim) { return workspace_bytes(batch, seq, heads, kv_heads, head_dim, false); }
+size_t xnq_kv_attend_packed_workspace_bytes(const xnq_kv_plan *plan, int heads, int kv_heads, int head_dim) {
+  return plan ? workspace_bytes(plan->batch, plan->longest, heads, kv_heads, head_dim, true) : 0;
 }
 
 int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos,
@@ -988,7 +995,7 @@ int xnq_kv_attend(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *
   clear_error();
   AttendArgs a{};
   int sms = 0;
-  const int rc = attend_args(cache, q, out, lse, batch, seq, heads, pos, pos_stride, scale, causal, window, workspace, ws_bytes, &a, &sms);
+  const int rc = attend_args(cache, q, out, lse, batch, seq, heads, pos, pos_stride, scale, causal, window, workspace, ws_bytes, false, &a, &sms);
   if (rc != XNQ_OK || batch == 0 || seq == 0) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int bits = kv_bits(cache->ggml_dtype);
@@ -1009,13 +1016,14 @@ int xnq_kv_attend_packed(const xnq_kv_cache *cache, const xnq_rows *q, const xnq
   }
   AttendArgs a{};
   int sms = 0;
-  const int rc = attend_args(cache, q, out, lse, batch, seq, heads, pos, pos_stride, scale, causal, window, workspace, ws_bytes, &a, &sms);
+  const int rc = attend_args(cache, q, out, lse, batch, seq, heads, pos, pos_stride, scale, causal, window, workspace, ws_bytes, plan != nullptr, &a, &sms);
   if (rc != XNQ_OK || batch == 0 || seq == 0 || (plan && plan->tokens == 0)) return rc;
   a.sinks = window ? std::min<int64_t>(sinks, INT32_MAX) : 0, a.rows_to = INT64_MAX;
   if (plan) {
     a.tokens = plan->tokens, a.offsets = plan->offsets, a.position = plan->position, a.start = plan->start, a.sees = plan->sees, a.nodes = plan->nodes;
     a.words = (int)((plan->longest + 31) / 32), a.clear = clear;
     a.seq = std::min<int64_t>(plan->longest, plan->tokens);
+    if (a.tokens * a.heads > INT32_MAX - 1024) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tokens of %d heads are more than one launch takes", (long long)a.tokens, heads);
   }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int bits = kv_bits(cache->ggml_dtype), hd = cache->head_dim;
@@ -1023,7 +1031,7 @@ int xnq_kv_attend_packed(const xnq_kv_cache *cache, const xnq_rows *q, const xnq
   if (!plan || batch == 1) return launch_kv_prompt(a, true, bits, hd, sms, s);
   // Sequences of their own numbers of tokens: each goes to the kernel for its number of rows.
   AttendArgs few = a;
-  a.rows_from = few.rows_to = PROMPT_ROWS, few.clear = 0;
+  a.rows_from = few.rows_to = q->dtype == XNQ_BF16 ? PACKED_PROMPT_ROWS : PROMPT_ROWS, few.clear = 0;
   const int rc2 = launch_kv_prompt(a, true, bits, hd, sms, s);
   return rc2 != XNQ_OK ? rc2 : run_attend<true>(few, bits, hd, sms, s);
 }

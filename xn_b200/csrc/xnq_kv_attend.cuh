@@ -38,7 +38,7 @@ constexpr unsigned KV_WAIT = 8; // status: a wait of the kernel for many rows ex
 // xnq_kv_prompt.cu: many 16-bit query rows
 int kv_prompt_init(int device);
 int kv_prompt_status(unsigned int *bits);
-size_t kv_prompt_parts_bytes(int head_dim);
+size_t kv_prompt_parts_bytes(int head_dim, bool packed);
 int launch_kv_prompt(const AttendArgs &a, bool more, int bits, int head_dim, int sms, cudaStream_t s);
 
 #ifdef __CUDACC__

@@ -203,6 +203,10 @@ struct PromptShape {
   static constexpr int RECORD = QT * 128 * (HD + 2); // floats of a part: references, sums, rows
 };
 
+struct Work { // of a CTA: rows row0 .. of a sequence and KV head, and which positions: n steps, tiles t0 .. (MORE: of the sequence's two runs of tiles)
+  long long pos, row0, q_at, out_at, lse_row;
+  int rows, seq, lo, hi, head, gap, t0, n, n_tiles, kvh, b, splits;
+};
 struct Meta { // of a tile
   int k_shift, v_shift; // its scales were taken times 2^shift
   unsigned bad;         // positions with a scale that is not finite
@@ -212,62 +216,107 @@ struct Meta { // of a tile
 // In a run of 8 positions, the place of pair i is taken by pair (i + run) & 3: what lies at column n of a tile
 __host__ __device__ constexpr int position_at(int n) { return (n & ~7) | ((((n >> 1) + (n >> 3)) & 3) << 1) | (n & 1); }
 
-// Packed tokens: which sequence's row tile is the unit-th of all that there are, by a whole block (the grid holds as many as there can be). Up to SORTED sequences
-// in the order of what they see, the longest first (the grid's last CTAs end the launch: with the sequences in their own order, 24 trees over 1600 to 8192 positions
-// took 249 us); within a sequence the last row tile first.
-constexpr int SORTED = 64;
-struct UnitScratch {
-  int tiles[SORTED], seen[SORTED]; // row tiles of a sequence, tiles of the cache that it sees
+// Packed tokens: what each CTA does follows from the sequences' lengths, which only the device knows. A unit is a row tile of a sequence and KV head; where one sees
+// more than an SM's share of all steps, `parts` CTAs share its positions. Units lie in the order of what they see, the longest first (24 trees over 1600 to 8192
+// positions: 249 us in the sequences' own order, 230 so, 180 with parts), so those with parts come first and a part's number is its CTA's. Sequences beyond
+// SORTED are taken in their own order, whole.
+constexpr int SORTED = 256;
+struct UnitScratch { // sequences with row tiles
+  int which[SORTED], tiles[SORTED], steps[SORTED], parts[SORTED];
+  int found[4];
 };
+struct Unit {
+  int b, rt, kvh, part, parts;
+  int record; // its first part's
+};
+// By a whole block: the sequences into u, how many there are, and how many CTAs each one's units take. Returns -1: more than SORTED.
 template <int THREADS>
-__device__ __forceinline__ bool unit_at(const AttendArgs &a, long long unit, int tile_rows, UnitScratch &u, long long *s_at, int &b, long long &rt) {
-  const int batch = (int)a.batch, x = threadIdx.x;
-  const auto tiles_of = [&](const Sequence &q) { return q.here ? (int)(((long long)q.seq * a.group + tile_rows - 1) / tile_rows) : 0; };
-  if (batch == 1) {
-    const Sequence q = sequence_of(a, 0);
-    b = 0, rt = tiles_of(q) - 1 - unit;
-    return rt >= 0;
+__device__ __forceinline__ int list_units(const AttendArgs &a, int tile_rows, UnitScratch &u) {
+  const int x = threadIdx.x, lane = x & 31;
+  if (x == 0) u.found[0] = 0;
+  __syncthreads();
+  int n = 0;
+  for (int base = 0; base < a.batch; base += THREADS) { // in the order of the sequences: every block has the same list
+    Sequence q;
+    q.here = false, q.seq = 0;
+    if (base + x < a.batch) q = sequence_of(a, base + x);
+    const bool is = q.here && q.seq > 0;
+    const unsigned vote = __ballot_sync(0xffffffffu, is);
+    if (lane == 0) u.parts[x >> 5] = __popc(vote);
+    __syncthreads();
+    int at = n + __popc(vote & ((1u << lane) - 1u));
+    for (int w = 0; w < THREADS / 32; w++) {
+      if (w < (x >> 5)) at += u.parts[w];
+      n += u.parts[w];
+    }
+    if (is && at < SORTED)
+      u.which[at] = base + x, u.tiles[at] = (int)((unsigned)(q.seq * a.group + tile_rows - 1) / (unsigned)tile_rows), u.steps[at] = (q.count + STEP_TILES - 1) / STEP_TILES;
+    __syncthreads();
   }
-  if (x == 0) s_at[0] = -1;
-  if (batch <= SORTED) {
-    int mine = 0, seen = 0;
-    if (x < batch) {
-      const Sequence q = sequence_of(a, x);
-      u.tiles[x] = mine = tiles_of(q), u.seen[x] = seen = q.count;
+  if (n > SORTED) return -1;
+  if (x < n) {
+    float steps = 0.f; // (the same sums in every CTA)
+    int units = 0;
+    for (int y = 0; y < n; y++) steps += (float)u.tiles[y] * (float)u.steps[y], units += u.tiles[y];
+    // an SM's shares of all steps; units that fill the GPU are cut from 1.25 of them on, others so that all parts run at once
+    const float shares = steps > 0.f ? (float)u.steps[x] * (float)a.splits / (steps * (float)a.c.kv_heads) : 0.f;
+    u.parts[x] = max(1, min((int)(units * a.c.kv_heads > a.splits ? shares + 0.75f : shares * 1.0001f), u.steps[x] / 2));
+  }
+  __syncthreads();
+  return n;
+}
+// the unit of a CTA (of `records` false: the nth unit, all of its parts together); n: list_units'
+template <int THREADS>
+__device__ __forceinline__ bool unit_at(const AttendArgs &a, int nth, int n, int tile_rows, bool whole, UnitScratch &u, Unit &unit) {
+  const int x = threadIdx.x, heads = a.c.kv_heads;
+  if (x == 0) u.found[0] = -1;
+  __syncthreads();
+  if (n >= 0) {
+    if (x < n) {
+      int before = 0, parts = 0; // units before, and their CTAs
+      for (int y = 0; y < n; y++)
+        if (u.steps[y] > u.steps[x] || (u.steps[y] == u.steps[x] && y < x)) before += u.tiles[y], parts += u.tiles[y] * u.parts[y];
+      const int p = u.parts[x], at = nth - (whole ? before : parts) * heads; // of this sequence's
+      if (at >= 0 && at < u.tiles[x] * heads * (whole ? 1 : p)) {
+        const int mine = whole ? at : at / p; // (row tile from the last on, head)
+        u.found[0] = x, u.found[1] = whole ? 0 : at - mine * p, u.found[2] = mine, u.found[3] = parts * heads + mine * p;
+      }
     }
     __syncthreads();
-    if (x < batch && mine) {
-      long long before = 0;
-      for (int y = 0; y < batch; y++)
-        if (u.seen[y] > seen || (u.seen[y] == seen && y < x)) before += u.tiles[y];
-      if (unit >= before && unit < before + mine) s_at[0] = x, s_at[1] = mine - 1 - (unit - before);
+    const int f = u.found[0];
+    if (f < 0) return false;
+    const int mine = u.found[2];
+    unit = Unit{u.which[f], u.tiles[f] - 1 - mine / heads, mine % heads, u.found[1], u.parts[f], u.found[3]};
+    return true;
+  }
+  int before = 0;
+  const int lane = x & 31;
+  for (int base = 0; base < a.batch && before <= nth; base += THREADS) {
+    int mine = 0;
+    if (base + x < a.batch) {
+      const Sequence q = sequence_of(a, base + x);
+      if (q.here) mine = (int)((unsigned)(q.seq * a.group + tile_rows - 1) / (unsigned)tile_rows) * heads;
     }
-    __syncthreads();
-  } else {
-    long long before = 0;
-    const int lane = x & 31, warp = x >> 5;
-    for (int base = 0; base < batch && before <= unit; base += THREADS) {
-      const int mine = base + x < batch ? tiles_of(sequence_of(a, base + x)) : 0;
-      long long inc = mine;
+    int inc = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      __syncthreads(); // (the sums of the round before have been read)
-      if (lane == 31) u.tiles[warp] = (int)inc;
-      __syncthreads();
-      long long first = before + inc - mine;
-      for (int w = 0; w < THREADS / 32; w++) {
-        if (w < warp) first += u.tiles[w];
-        before += u.tiles[w];
-      }
-      if (unit >= first && unit < first + mine) s_at[0] = base + x, s_at[1] = mine - 1 - (unit - first);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
     }
+    __syncthreads(); // (the sums of the round before have been read)
+    if (lane == 31) u.tiles[x >> 5] = inc;
     __syncthreads();
+    int first = before + inc - mine;
+    for (int w = 0; w < THREADS / 32; w++) {
+      if (w < (x >> 5)) first += u.tiles[w];
+      before += u.tiles[w];
+    }
+    if (nth >= first && nth < first + mine) u.found[0] = base + x, u.found[1] = nth - first, u.found[2] = mine / heads;
   }
-  b = (int)s_at[0], rt = s_at[1];
-  return b >= 0;
+  __syncthreads();
+  if (u.found[0] < 0) return false;
+  unit = Unit{u.found[0], u.found[2] - 1 - u.found[1] / heads, u.found[1] % heads, 0, 1, 0};
+  return true;
 }
 
 // MORE: first positions that stay visible, packed tokens and trees; a CTA's tiles may then be two runs of the cache.
@@ -286,15 +335,15 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - (uint32_t)__cvta_generic_to_shared(smem_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
-  int unit_b = 0; // MORE, packed
-  long long unit_rt = 0;
+  Unit unit; // MORE, packed
   if constexpr (MORE) {
-    if (a.offsets) { // (before this CTA takes anything: some have no rows)
-      __shared__ long long s_at[2];
-      static_assert(sizeof(UnitScratch) <= sizeof(meta), "what is not in use yet");
-      pdl_wait();
-      if (a.clear) clear_behind(a, HD);
-      if (!unit_at<PROMPT_THREADS>(a, blockIdx.x / (a.c.kv_heads * a.splits), QT * 128, *reinterpret_cast<UnitScratch *>(meta), s_at, unit_b, unit_rt)) return;
+    if (a.offsets) pdl_wait();
+    if (a.offsets && a.clear) clear_behind(a, HD);
+    if (a.offsets && a.batch > 1) { // (before this CTA takes anything: some have nothing to do; the room is that of the rows of Q, which plain stores fill later)
+      UnitScratch &scratch = *reinterpret_cast<UnitScratch *>(smem);
+      static_assert(sizeof(UnitScratch) <= P::Q_TILE, "its room");
+      const int n = list_units<PROMPT_THREADS>(a, QT * 128, scratch);
+      if (!unit_at<PROMPT_THREADS>(a, blockIdx.x, n, QT * 128, false, scratch, unit)) return;
     }
   }
   const uint32_t raw_full = bar, raw_scanned = bar + 16 * 8, raw_empty = bar + 32 * 8, k_full = bar + 48 * 8, k_empty = k_full + 8 * RING, v_full = k_empty + 8 * RING, v_empty = v_full + 8 * RING,
@@ -322,42 +371,47 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   pdl_wait();
 
   // ---- which rows, which positions; the row tiles with the most positions first ----
-  const bool units = MORE && a.offsets; // (a.row_tiles: of all sequences)
-  const int per = (units ? 1 : (int)a.batch) * a.c.kv_heads * a.splits, rem = (int)(blockIdx.x % per), nth = (int)(blockIdx.x / per);
-  const int rt = units ? (int)unit_rt : a.row_tiles - 1 - nth, split = rem % a.splits, bk = rem / a.splits, kvh = bk % a.c.kv_heads, b = units ? unit_b : bk / a.c.kv_heads;
-  Sequence sq; // MORE
-  long long all_rows = a.seq * a.group, q_at = b * a.q.sb, out_at = b * a.out.sb, lse_row = (long long)b * a.seq;
-  const long long row0 = (long long)rt * (QT * 128);
-  if constexpr (MORE) {
-    sq = sequence_of(a, b);
-    all_rows = (long long)sq.seq * a.group, lse_row = sq.first_row;
-    if (a.offsets) q_at = sq.first_row * a.q.ss, out_at = sq.first_row * a.out.ss;
-  }
-  const int rows = (int)min((long long)(QT * 128), all_rows - row0);
-  const long long s_first = row0 / a.group, s_end = (row0 + rows - 1) / a.group;
-  long long pos;
-  int hi, lo, tiles;
-  if constexpr (MORE) {
-    pos = sq.pos;
-    tiles_seen(a, sq, s_first, s_end);
-    tiles = sq.count;
-    // what the rows see of the cache, but for the first positions and a tree's tokens
-    hi = (int)max(min(a.sees ? pos - 1 : a.causal ? pos + s_end : pos + sq.seq - 1, a.c.max_seq - 1), -1ll);
-    lo = a.window ? (int)min(max(max(a.sees ? pos : pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0;
-  } else {
-    pos = a.pos[(long long)b * a.pos_stride];
-    const long long hi_l = pos + s_end < 0 ? -1 : min(a.causal ? pos + s_end : pos + a.seq - 1, a.c.max_seq - 1);
-    const long long lo_l = a.window ? min(max(max(pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0ll;
-    hi = (int)hi_l, lo = (int)lo_l, tiles = hi < lo ? 0 : hi / KV_TILE - lo / KV_TILE + 1;
-  }
-  const int steps_all = (tiles + STEP_TILES - 1) / STEP_TILES, steps_each = (steps_all + a.splits - 1) / a.splits, step0 = min(split * steps_each, steps_all);
-  const int n = min(steps_all - step0, steps_each); // steps of this CTA
-  const int t0 = (MORE ? 0 : lo / KV_TILE) + step0 * STEP_TILES, n_tiles = min(tiles - step0 * STEP_TILES, n * STEP_TILES);
+  const auto describe = [&](Work &w) {
+    int rt, split;
+    if (MORE && a.offsets && a.batch > 1) rt = unit.rt, split = unit.part, w.splits = unit.parts, w.kvh = unit.kvh, w.b = unit.b;
+    else {
+      const int per = (int)a.batch * a.c.kv_heads * a.splits, rem = (int)(blockIdx.x % per), bk = rem / a.splits;
+      rt = a.row_tiles - 1 - (int)(blockIdx.x / per), split = rem % a.splits, w.splits = a.splits, w.kvh = bk % a.c.kv_heads, w.b = bk / a.c.kv_heads;
+    }
+    w.row0 = (long long)rt * (QT * 128);
+    if constexpr (MORE) {
+      Sequence q = sequence_of(a, w.b);
+      w.rows = (int)min((long long)(QT * 128), (long long)q.seq * a.group - w.row0);
+      if (w.rows <= 0) q.count = 0, q.here = false;
+      const int s_first = (int)((unsigned)w.row0 / (unsigned)a.group), s_end = (int)((unsigned)(w.row0 + w.rows - 1) / (unsigned)a.group);
+      if (q.here) tiles_seen(a, q, s_first, s_end);
+      w.pos = q.pos, w.lse_row = q.first_row, w.seq = q.seq, w.head = q.head, w.gap = q.gap;
+      w.q_at = a.offsets ? q.first_row * a.q.ss : w.b * a.q.sb, w.out_at = a.offsets ? q.first_row * a.out.ss : w.b * a.out.sb;
+      // what the rows see of the cache, but for the first positions and a tree's tokens
+      w.hi = (int)max(min(a.sees ? q.pos - 1 : a.causal ? q.pos + s_end : q.pos + q.seq - 1, a.c.max_seq - 1), -1ll);
+      w.lo = a.window ? (int)min(max(max(a.sees ? q.pos : q.pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0;
+      w.t0 = 0, w.n_tiles = q.count;
+    } else {
+      w.rows = (int)min((long long)(QT * 128), a.seq * a.group - w.row0);
+      w.pos = a.pos[(long long)w.b * a.pos_stride], w.lse_row = w.b * a.seq, w.seq = (int)a.seq, w.q_at = w.b * a.q.sb, w.out_at = w.b * a.out.sb;
+      const long long s_first = w.row0 / a.group, s_end = (w.row0 + w.rows - 1) / a.group;
+      const long long hi_l = w.pos + s_end < 0 ? -1 : min(a.causal ? w.pos + s_end : w.pos + a.seq - 1, a.c.max_seq - 1);
+      const long long lo_l = a.window ? min(max(max(w.pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0ll;
+      w.hi = (int)hi_l, w.lo = (int)lo_l, w.t0 = w.lo / KV_TILE, w.n_tiles = w.hi < w.lo ? 0 : w.hi / KV_TILE - w.t0 + 1;
+    }
+    const int steps_all = (w.n_tiles + STEP_TILES - 1) / STEP_TILES, steps_each = (steps_all + w.splits - 1) / w.splits, step0 = min(split * steps_each, steps_all);
+    w.n = min(steps_all - step0, steps_each);
+    w.t0 += step0 * STEP_TILES, w.n_tiles = min(w.n_tiles - step0 * STEP_TILES, w.n * STEP_TILES);
+  };
+  Work w;
+  describe(w);
+  if (MORE && w.rows < 0) w.rows = 0; // (packed, one sequence: it has fewer tokens than the grid has rows for)
+  const int n = w.n, t0 = w.t0, n_tiles = w.n_tiles;
   const auto tile_of = [&](int i) { // this CTA's i-th tile, in the cache
-    if constexpr (MORE) return sq.tile(t0 + i);
+    if constexpr (MORE) return t0 + i < w.head ? t0 + i : t0 + i + w.gap;
     else return t0 + i;
   };
-  if (threadIdx.x == 0 && !(MORE && a.offsets) && pos + a.seq > a.c.max_seq) atomicOr(&g_kv_prompt_status, KV_PAST_ATTEND);
+  if (threadIdx.x == 0 && !(MORE && a.offsets) && w.pos + a.seq > a.c.max_seq) atomicOr(&g_kv_prompt_status, KV_PAST_ATTEND);
   volatile int *const dead = &s_dead;
 
   if (warp >= LOADER) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
@@ -366,7 +420,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     int i = 0;
     for (; i < n * STEP_TILES; i++) {
       const int slot = i % P::SLOTS, lap = i / P::SLOTS;
-      if ((i & 31) == 0) ahead = i + lane < n_tiles ? kv_tile_at(a.c, b, kvh, tile_of(i + lane), L::BYTES) : nullptr;
+      if ((i & 31) == 0) ahead = i + lane < n_tiles ? kv_tile_at(a.c, w.b, w.kvh, tile_of(i + lane), L::BYTES) : nullptr;
       const uint8_t *src = reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ahead), i & 31));
       if (lap && !wait_for(raw_empty + 8 * slot, (lap - 1) & 1, dead)) break;
       if (lane == 0) {
@@ -416,21 +470,21 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         // Most tiles: all of their positions are seen by some row, every scale is below 4 and the largest keys and values are not below 2^-3, f16's middle:
         // largest scales of 2^-6 (codes up to 8) or 2^-10 (up to 127). (With 2^-6 for 8 bits too, 2048 queries over 8192 positions took 699 us with values
         // of 0.3 and 293 with values of 0.7.)
-        const bool inside = MORE ? all_seen(a, lo, hi, j0) : j0 >= lo && j0 + KV_TILE - 1 <= hi;
+        const bool inside = MORE ? all_seen(a, w.lo, w.hi, j0) : j0 >= w.lo && j0 + KV_TILE - 1 <= w.hi;
         const bool plain = !null[e] && inside && __all_sync(0xffffffffu, max(k_top, v_top) < 0x4400u) && __any_sync(0xffffffffu, k_top >= LEAST_BITS) &&
                            __any_sync(0xffffffffu, v_top >= LEAST_BITS);
         Meta mt{0, 0, 0u, 0};
         if (!plain) {
           unsigned bad = 0, most[2] = {0u, 0u};
           uint32_t seen = 0u; // MORE: positions of the tile that some row may see
-          if constexpr (MORE) seen = seen_in_tile(a, Sight{lo, hi, false}, a.nodes ? a.nodes + (long long)b * a.words : nullptr, pos, j0);
+          if constexpr (MORE) seen = seen_in_tile(a, Sight{w.lo, w.hi, false}, a.nodes ? a.nodes + (long long)w.b * a.words : nullptr, w.pos, j0);
 #pragma unroll
           for (int k = 0; k < 2 * KW; k++) {
             const bool is_k = k < KW;
             const int in = is_k ? lane : lane & ~1, j = j0 + in; // keys: both halves are of position j; values: of j and j + 1
             bool in0, in1;
             if constexpr (MORE) in0 = (seen >> in) & 1u, in1 = is_k ? in0 : (seen >> in) & 2u;
-            else in0 = j >= lo && j <= hi, in1 = is_k ? in0 : j + 1 >= lo && j + 1 <= hi;
+            else in0 = j >= w.lo && j <= w.hi, in1 = is_k ? in0 : j + 1 >= w.lo && j + 1 <= w.hi;
             uint32_t y = null[e] ? 0u : x[e][k] & ((in0 ? 0xffffu : 0u) | (in1 ? 0xffff0000u : 0u));
             if ((y & 0x7c00u) == 0x7c00u) y &= 0xffff0000u, bad |= 1u << in;
             if ((y & 0x7c000000u) == 0x7c000000u) y &= 0xffffu, bad |= (is_k ? 1u : 2u) << in;
@@ -603,25 +657,26 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     const int q = warp >> 2, r = (warp & 3) * 32 + lane; // row tile, row of it
     const uint32_t tm = tmem + ((uint32_t)(warp & 3) << 21), buffers = tm + q * 128, o_acc = tm + 256 + q * HD;
     const int row = q * 128 + r;
-    const bool valid = row < rows;
-    const long long at = row0 + row, tok = at / a.group;
-    const int h = kvh * a.group + (int)(at - tok * a.group);
+    const bool valid = row < w.rows;
+    const long long at = w.row0 + row, tok = MORE ? (long long)((unsigned)at / (unsigned)a.group) : at / a.group;
+    const int h = w.kvh * a.group + (int)(at - tok * a.group);
     int r_lo = 0, r_hi = INT_MAX;
-    bool live = valid;              // MORE: and a token (one that is none sees nothing, but must not make its warp weigh every tile position by position)
-    const uint32_t *tree = nullptr; // MORE: the row's bits
+    bool live = valid; // MORE: and a token (one that is none sees nothing, but must not make its warp weigh every tile position by position)
     if constexpr (MORE) {
       if (valid) {
-        const Sight v = sight_of(a, sq, tok);
+        Sequence q;
+        q.pos = w.pos, q.first_row = w.lse_row, q.seq = w.seq;
+        const Sight v = sight_of(a, q, tok);
         live = !v.none;
-        if (live) r_lo = v.lo, r_hi = v.hi, tree = a.sees ? a.sees + (sq.first_row + tok) * a.words : nullptr;
+        if (live) r_lo = v.lo, r_hi = v.hi;
       }
-    } else if (valid) seen_by(a, pos, tok, r_lo, r_hi);
+    } else if (valid) seen_by(a, w.pos, tok, r_lo, r_hi);
     const int lo_all = __reduce_max_sync(0xffffffffu, valid ? r_lo : 0), hi_all = __reduce_min_sync(0xffffffffu, r_hi);
     const int lo_any = __reduce_min_sync(0xffffffffu, valid ? r_lo : INT_MAX), hi_any = __reduce_max_sync(0xffffffffu, valid ? r_hi : -1);
     float f = 0.f;
     { // the row as an operand
       uint4 x[HD / 8];
-      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q.p) + q_at + tok * a.q.ss + h * a.q.sh);
+      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q.p) + w.q_at + tok * a.q.ss + h * a.q.sh);
 #pragma unroll
       for (int c = 0; c < HD / 8; c++) x[c] = live && n > 0 ? src[c] : make_uint4(0, 0, 0, 0);
       auto value = [&](uint32_t w, int half) {
@@ -719,6 +774,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         tmem_st32(at, pk);
         return;
       }
+      const uint32_t *const tree = MORE && a.sees && live ? a.sees + (w.lse_row + tok) * a.words : nullptr; // the row's bits
       const Meta *mt2 = &meta[(h2 >> 1) % META_STEPS][(h2 & 1) * 2];
 #pragma unroll 1
       for (int c = 0; c < 2; c++) {
@@ -728,7 +784,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         bool every, nothing; // row of the warp sees all of them; sees any
         if constexpr (MORE) {
           every = all_seen(a, lo_all, hi_all, i0);
-          if (!every) mine = seen_in_tile(a, Sight{r_lo, r_hi, false}, tree, pos, i0);
+          if (!every) mine = seen_in_tile(a, Sight{r_lo, r_hi, false}, tree, w.pos, i0);
           nothing = !every && !__any_sync(0xffffffffu, live && mine);
         } else every = i0 >= lo_all && i0 + KV_TILE - 1 <= hi_all, nothing = i0 > hi_any || i0 + KV_TILE - 1 < lo_any;
         if (mt.gone || nothing) { // seen by no row of the warp
@@ -785,9 +841,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     tc_fence_after();
     if (MORE && !live) l = 0.f, ref = -INFINITY; // zeros
     // ---- the row's result, or its part ----
-    if (a.splits == 1) {
+    if (w.splits == 1) {
       const float by = l > 0.f ? ldexpf(1.f / l, -v_ref) : l; // nothing seen: zeros; NaN stays
-      uint16_t *dst = static_cast<uint16_t *>(a.out.p) + out_at + tok * a.out.ss + h * a.out.sh;
+      uint16_t *dst = static_cast<uint16_t *>(a.out.p) + w.out_at + tok * a.out.ss + h * a.out.sh;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 16) {
         uint32_t o[16];
@@ -811,9 +867,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         }
         __syncwarp();
       }
-      if (valid && a.lse) a.lse[(lse_row + tok) * a.heads + h] = l > 0.f ? (ref + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
+      if (valid && a.lse) a.lse[(w.lse_row + tok) * a.heads + h] = l > 0.f ? (ref + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
     } else {
-      float *rec = a.records + (((size_t)nth * (per / a.splits) + bk) * a.splits + split) * P::RECORD;
+      float *rec = a.records + (size_t)blockIdx.x * P::RECORD;
       if (valid) rec[row] = ref, rec[QT * 128 + row] = l;
       const float by = ldexpf(1.f, -v_ref);
       float *dst = rec + 2 * QT * 128 + (size_t)row * HD;
@@ -841,50 +897,28 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
 
 // The parts of rows whose positions `splits` CTAs shared, added in the order of their places: a warp a row, a lane HD / 32 dims. A kernel of its own, because
 // every SM has a share of it: one CTA of the attention adding 18 parts of 128 rows, 1.2 MB, had taken longer than the attention (128 rows of one sequence of 8192 positions: 139 us, now 32).
-template <int HD, bool MORE>
-__global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int V = HD / 32, RECORD = 128 * (HD + 2), AHEAD = 8;
-  const bool packed = MORE && a.offsets;
-  const int lane = threadIdx.x & 31, units = (packed ? 1 : (int)a.batch) * a.c.kv_heads;
-  const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5);
-  long long all_rows = a.seq * a.group;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int nth = (int)(at / (128ll * units)), bk = (int)(at / 128 % units), row = (int)(at % 128); // (a block's rows are of one row tile)
-  int b = bk / a.c.kv_heads;
-  const int kvh = bk % a.c.kv_heads;
-  if (nth >= a.row_tiles) return;
-  long long rt = a.row_tiles - 1 - nth; // (the last row tiles' CTAs come first)
-  long long out_at = b * a.out.sb, lse_row = (long long)b * a.seq;
-  if constexpr (MORE) {
-    if (a.offsets) {
-      __shared__ UnitScratch scratch;
-      __shared__ long long s_at[2];
-      if (!unit_at<256>(a, nth, 128, scratch, s_at, b, rt)) return;
-      const long long first = a.offsets[b];
-      all_rows = (a.offsets[b + 1] - first) * a.group, out_at = first * a.out.ss, lse_row = first;
-    }
-  }
-  const long long at_row = rt * 128ll + row;
-  if (at_row >= all_rows) return;
-  const float *const first = a.records + ((size_t)nth * units + bk) * a.splits * RECORD;
+template <int HD>
+__device__ __forceinline__ void join_row(const AttendArgs &a, const float *first, int tile_rows, int parts, int row, long long out_at, long long lse_at) {
+  constexpr int V = HD / 32, AHEAD = 8;
+  const int lane = threadIdx.x & 31;
+  const size_t record = (size_t)tile_rows * (HD + 2);
   float m = -INFINITY, l = 0.f, v[V] = {};
-  for (int k = lane; k < a.splits; k += 32) m = fmaxf(m, __ldcg(first + (size_t)k * RECORD + row));
+  for (int k = lane; k < parts; k += 32) m = fmaxf(m, __ldcg(first + k * record + row));
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  for (int k0 = 0; k0 < a.splits; k0 += 32) {
-    const int left = min(32, a.splits - k0);
+  for (int k0 = 0; k0 < parts; k0 += 32) {
+    const int left = min(32, parts - k0);
     float mine = 0.f;
     if (lane < left) {
-      const float *p = first + (size_t)(k0 + lane) * RECORD;
+      const float *p = first + (k0 + lane) * record;
       const float mp = __ldcg(p + row);
       mine = mp == -INFINITY ? 0.f : exp2_approx(mp - m);
-      l += mine * __ldcg(p + 128 + row); // (a part of NaN stays one)
+      l += mine * __ldcg(p + tile_rows + row); // (a part of NaN stays one)
     }
     for (int k = 0; k < left; k += AHEAD) {
       float x[AHEAD][V];
 #pragma unroll
-      for (int i = 0; i < AHEAD; i++) load_vec_cg<V>(first + (size_t)(k0 + min(k + i, left - 1)) * RECORD + 256 + (size_t)row * HD + lane * V, x[i]);
+      for (int i = 0; i < AHEAD; i++) load_vec_cg<V>(first + (k0 + min(k + i, left - 1)) * record + 2 * tile_rows + (size_t)row * HD + lane * V, x[i]);
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
         const float by = __shfl_sync(0xffffffffu, mine, (k + i) & 31);
@@ -896,13 +930,47 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_consta
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  const long long tok = at_row / a.group;
-  const int h = kvh * a.group + (int)(at_row - tok * a.group);
   const float by = l > 0.f ? 1.f / l : l; // nothing seen: zeros; NaN stays
 #pragma unroll
   for (int c = 0; c < V; c++) v[c] = l == 0.f ? 0.f : v[c] * by;
-  store_vec<V>(a.out.p, a.dtype, out_at + tok * a.out.ss + h * a.out.sh + lane * V, v);
-  if (a.lse && lane == 0) a.lse[(lse_row + tok) * a.heads + h] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
+  store_vec<V>(a.out.p, a.dtype, out_at + lane * V, v);
+  if (a.lse && lane == 0) a.lse[lse_at] = l > 0.f ? (m + log2f(l)) * LN2 : l == 0.f ? -INFINITY : l;
+}
+template <int HD>
+__global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_constant__ AttendArgs a) {
+  const int units = (int)a.batch * a.c.kv_heads;
+  const long long at = blockIdx.x * 8ll + (threadIdx.x >> 5);
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long first = a.offsets ? a.offsets[0] : 0, all_rows = (a.offsets ? a.offsets[1] - first : a.seq) * a.group; // (packed: one sequence)
+  const int rt = (int)(at / (128ll * units)), bk = (int)(at / 128 % units), row = (int)(at % 128), b = bk / a.c.kv_heads, kvh = bk % a.c.kv_heads;
+  const long long at_row = rt * 128ll + row;
+  if (rt >= a.row_tiles || at_row >= all_rows) return;
+  const long long tok = at_row / a.group;
+  const int h = kvh * a.group + (int)(at_row - tok * a.group);
+  join_row<HD>(a, a.records + ((size_t)(a.row_tiles - 1 - rt) * units + bk) * a.splits * (128 * (HD + 2)), 128, a.splits, row, // (the last row tiles' CTAs come first)
+               b * a.out.sb + (first + tok) * a.out.ss + h * a.out.sh, ((long long)b * a.seq + first + tok) * a.heads + h);
+}
+// Packed tokens: the units that have parts come first; a block goes on from one to the next, 8 rows at a time.
+constexpr int JOIN_BLOCKS = 592;
+template <int HD>
+__global__ void __launch_bounds__(256) kv_attend_join_packed_kernel(const __grid_constant__ AttendArgs a, int tile_rows) {
+  __shared__ UnitScratch u;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int n = list_units<256>(a, tile_rows, u), groups = tile_rows / 8;
+  if (n < 0) return;
+  for (int w = blockIdx.x;; w += gridDim.x) {
+    Unit unit;
+    if (!unit_at<256>(a, w / groups, n, tile_rows, true, u, unit) || unit.parts == 1) return;
+    const long long first = a.offsets[unit.b], all_rows = (a.offsets[unit.b + 1] - first) * a.group;
+    const int row = w % groups * 8 + (threadIdx.x >> 5);
+    const long long at_row = (long long)unit.rt * tile_rows + row, tok = first + at_row / a.group;
+    const int h = unit.kvh * a.group + (int)(at_row % a.group);
+    if (at_row < all_rows)
+      join_row<HD>(a, a.records + (size_t)unit.record * tile_rows * (HD + 2), tile_rows, unit.parts, row, tok * a.out.ss + h * a.out.sh, tok * a.heads + h);
+    __syncthreads(); // (u has been read)
+  }
 }
 
 // Row tiles of 128 rows where an SM each is enough for them, or the rows are no more; CTAs that share a tile's positions where the SMs are more. Else tiles
@@ -912,29 +980,35 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_consta
 struct Plan {
   int qt, row_tiles, splits;
 };
-Plan plan_of(int64_t batch, int64_t seq, int group, int kv_heads, int64_t max_seq, int sms, int64_t tokens, int64_t rows_from) {
-  const int64_t rows = seq * group;
-  int64_t heads = batch * kv_heads, two = (rows + 255) / 256, one = (rows + 127) / 128;
-  if (tokens) { // packed: row tiles of all sequences, as many as there can be of these tokens
-    const int64_t all = tokens * group, sequences = std::min<int64_t>(batch, all / std::max<int64_t>(rows_from, 1));
-    const bool single = one == 1;
-    heads = kv_heads, two = std::min(batch * two, all / 256 + sequences), one = std::min(batch * one, all / 128 + sequences);
-    if (!single && heads * one > sms) return Plan{2, (int)std::min<int64_t>(two, INT_MAX), 1};
-    if (heads * one > sms) return Plan{1, (int)std::min<int64_t>(one, INT_MAX), 1};
-  }
+Plan plan_of(int64_t batch, int64_t seq, int group, int kv_heads, int64_t max_seq, int sms) {
+  const int64_t rows = seq * group, heads = batch * kv_heads, two = (rows + 255) / 256, one = (rows + 127) / 128;
   if (one > 1 && heads * one > sms) return Plan{2, (int)two, 1};
   const int64_t steps = (max_seq + BN - 1) / BN;
   return Plan{1, (int)one, (int)std::max<int64_t>(1, std::min<int64_t>(sms / (heads * one), steps / 2))};
 }
 
+// Packed tokens: row tiles of all sequences, as many as there can be of these tokens (and sequences with `rows_from` rows or more); splits: the SMs, among
+// which the kernel divides the units itself.
+Plan packed_plan_of(const AttendArgs &a, int sms) {
+  const int64_t rows = a.seq * a.group, all = a.tokens * a.group, sequences = std::min<int64_t>(a.batch, all / std::max<int64_t>(a.rows_from, 1));
+  const int64_t two = std::min<int64_t>(a.batch * ((rows + 255) / 256), all / 256 + sequences), one = std::min<int64_t>(a.batch * ((rows + 127) / 128), all / 128 + sequences);
+  const bool pairs = rows > 128 && a.c.kv_heads * one > sms;
+  return Plan{pairs ? 2 : 1, (int)std::min<int64_t>(pairs ? two : one, INT_MAX), sms};
+}
+// CTAs that share units' positions: with U units and s SMs, parts of units that have any are no more than s (U <= s: a unit has as many as its whole shares of an SM)
+// or 1.6 s (else a unit of x >= 1.25 shares has at most x + 0.75), and no more than s beyond the units.
+constexpr int MAX_SMS = 160, MAX_PARTS = MAX_SMS * 8 / 5;
 template <int BITS, int HD, int QT, bool MORE>
 int launch(const AttendArgs &a, cudaStream_t s) {
-  const int64_t heads = (MORE && a.offsets ? 1 : a.batch) * a.c.kv_heads, grid = (int64_t)a.row_tiles * heads * a.splits;
+  const bool packed = MORE && a.offsets && a.batch > 1;
+  const int64_t units = (int64_t)a.row_tiles * a.c.kv_heads; // packed: at most
+  const int64_t grid = packed ? (units <= a.splits ? a.splits : units + a.splits) : (int64_t)a.row_tiles * a.batch * a.c.kv_heads * a.splits;
   if (grid > INT_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of query rows are more than one launch takes", (long long)grid);
   XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT, MORE>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
   count_launch();
-  if (a.splits == 1) return XNQ_OK;
-  XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD, MORE>, dim3((unsigned)(a.row_tiles * heads * 16)), dim3(256), 0, s, a));
+  if (packed) XNQ_CUDA(launch_pdl(kv_attend_join_packed_kernel<HD>, dim3(JOIN_BLOCKS), dim3(256), 0, s, a, QT * 128));
+  else if (a.splits == 1) return XNQ_OK;
+  else XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD>, dim3((unsigned)(a.row_tiles * a.batch * a.c.kv_heads * 16)), dim3(256), 0, s, a));
   count_launch();
   return XNQ_OK;
 }
@@ -965,11 +1039,10 @@ int kv_prompt_init(int) {
     return rc;
   return XNQ_OK;
 }
-constexpr int MAX_PARTS = 160; // CTAs of a launch that shares positions: no more than SMs
-size_t kv_prompt_parts_bytes(int head_dim) { return (size_t)MAX_PARTS * 128 * (head_dim + 2) * 4; }
+size_t kv_prompt_parts_bytes(int head_dim, bool packed) { return (size_t)(packed ? MAX_PARTS * 256 : MAX_SMS * 128) * (head_dim + 2) * 4; }
 int launch_kv_prompt(const AttendArgs &args, bool more, int bits, int head_dim, int sms, cudaStream_t s) {
   AttendArgs a = args;
-  const Plan p = plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_PARTS), a.offsets ? a.tokens : 0, a.rows_from);
+  const Plan p = a.offsets && a.batch > 1 ? packed_plan_of(a, std::min(sms, MAX_SMS)) : plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_SMS));
   a.row_tiles = p.row_tiles, a.splits = p.splits;
   if (bits == 4) return head_dim == 64 ? launch_hd<4, 64>(a, more, p.qt, s) : launch_hd<4, 128>(a, more, p.qt, s);
   return head_dim == 64 ? launch_hd<8, 64>(a, more, p.qt, s) : launch_hd<8, 128>(a, more, p.qt, s);

@@ -413,7 +413,9 @@ class QuantizedKVCache:
         common = (self.head_dim ** -0.5 if scale is None else float(scale), int(causal), int(window))
         rows = (ctypes.byref(self._view), ctypes.byref(_rows(q)), ctypes.byref(_rows(out)), None if lse is None else ctypes.c_void_p(lse.data_ptr()))
         with torch.cuda.device(self.device):
-            ws, lock = _workspace(self.device, max(16, int(L.xnq_kv_attend_workspace_bytes(batch, seq, heads, self.kv_heads, self.head_dim))))
+            need = L.xnq_kv_attend_workspace_bytes(batch, seq, heads, self.kv_heads, self.head_dim) if plan is None else \
+                L.xnq_kv_attend_packed_workspace_bytes(view, heads, self.kv_heads, self.head_dim)
+            ws, lock = _workspace(self.device, max(16, int(need)))
             scratch = (ctypes.c_void_p(ws.data_ptr()), ws.numel(), _stream_ptr(self.device))
             with lock:   # (the interpreter's is free during the call, which may enqueue two kernels)
                 if plan is None and not (sinks and window):
