@@ -917,7 +917,8 @@ int for_each_split(F f) { // f(a launch)
 
 template <int BITS, int HD, bool MORE>
 int run_attend(const AttendArgs &a, int sms, cudaStream_t s) {
-  const int64_t rows = std::min<int64_t>(a.seq * a.group, MORE ? a.rows_to - 1 : INT64_MAX);
+  // (MORE: beside sequences of many rows, those of few are mostly single tokens, if not trees)
+  const int64_t rows = !MORE || a.rows_to == INT64_MAX ? a.seq * a.group : a.sees ? a.rows_to - 1 : std::min<int64_t>(a.group, a.rows_to - 1);
   const bool one = split_nt(BITS, rows, a.batch * a.c.kv_heads, sms) == 1;
   if (a.dtype == XNQ_F32) return one ? run_split<BITS, HD, 1, true, MORE>(a, sms, s) : run_split<BITS, HD, 2, true, MORE>(a, sms, s);
   return one ? run_split<BITS, HD, 1, false, MORE>(a, sms, s) : run_split<BITS, HD, 2, false, MORE>(a, sms, s);

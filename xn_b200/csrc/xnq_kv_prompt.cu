@@ -205,7 +205,7 @@ struct PromptShape {
 
 struct Work { // of a CTA: rows row0 .. of a sequence and KV head, and which positions: n steps, tiles t0 .. (MORE: of the sequence's two runs of tiles)
   long long pos, row0, q_at, out_at, lse_row;
-  int rows, seq, lo, hi, head, gap, t0, n, n_tiles, kvh, b, splits;
+  int rows, seq, lo, hi, head, gap, turn, total, t0, n, n_tiles, kvh, b, splits; // MORE: tiles are taken from the turn-th of `total` on, the ones before it at the end
 };
 struct Meta { // of a tile
   int k_shift, v_shift; // its scales were taken times 2^shift
@@ -390,7 +390,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       // what the rows see of the cache, but for the first positions and a tree's tokens
       w.hi = (int)max(min(a.sees ? q.pos - 1 : a.causal ? q.pos + s_end : q.pos + q.seq - 1, a.c.max_seq - 1), -1ll);
       w.lo = a.window ? (int)min(max(max(a.sees ? q.pos : q.pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0;
-      w.t0 = 0, w.n_tiles = q.count;
+      w.t0 = 0, w.n_tiles = w.total = q.count;
+      // The first tile gives the rows their references: one that all of them see (behind a window's edge, which is another one for each token, rows that have begun with
+      // one or two positions pass their references again and again: 777 tokens that see 2500 positions and the first 7, 89 us instead of 55).
+      const int last_lo = a.window ? (int)min(max((a.sees ? q.pos + q.seq - 1 : q.pos + s_end) - a.window + 1, 0ll), a.c.max_seq) : 0; // (a token's depth is at most its index)
+      const int turn = (last_lo + KV_TILE - 1) / KV_TILE, all_hi = a.sees || !a.causal ? w.hi : (int)min((long long)w.hi, max(q.pos + s_first, -1ll));
+      w.turn = a.window && turn >= q.head + q.gap && turn * KV_TILE + KV_TILE - 1 <= all_hi ? turn - q.gap : 0;
     } else {
       w.rows = (int)min((long long)(QT * 128), a.seq * a.group - w.row0);
       w.pos = a.pos[(long long)w.b * a.pos_stride], w.lse_row = w.b * a.seq, w.seq = (int)a.seq, w.q_at = w.b * a.q.sb, w.out_at = w.b * a.out.sb;
@@ -408,8 +413,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   if (MORE && w.rows < 0) w.rows = 0; // (packed, one sequence: it has fewer tokens than the grid has rows for)
   const int n = w.n, t0 = w.t0, n_tiles = w.n_tiles;
   const auto tile_of = [&](int i) { // this CTA's i-th tile, in the cache
-    if constexpr (MORE) return t0 + i < w.head ? t0 + i : t0 + i + w.gap;
-    else return t0 + i;
+    if constexpr (MORE) {
+      const int at = t0 + i + w.turn, v = at >= w.total ? at - w.total : at;
+      return v < w.head ? v : v + w.gap;
+    } else return t0 + i;
   };
   if (threadIdx.x == 0 && !(MORE && a.offsets) && w.pos + a.seq > a.c.max_seq) atomicOr(&g_kv_prompt_status, KV_PAST_ATTEND);
   volatile int *const dead = &s_dead;
