@@ -163,6 +163,7 @@ struct PackedRows { // of a plan: where each token goes, and the position that i
 
 struct StoreUnits { // warps: [0, kv) store keys and values, the rest rotate queries
   unsigned kv, all, pairs, kv_slices, q_slices;
+  unsigned each; // packed: tokens of a warp that stores keys and values
 };
 
 // PACKED: the tokens of all sequences one after the other (seq: how many). A warp has a token, and the next one with it where the two share a pair.
@@ -182,8 +183,8 @@ __global__ void __launch_bounds__(256, 4) kv_store_kernel(KvView c, KvRows k, Kv
     const long long p = PACKED ? pk.position[s] : pos_p[(long long)b * pos_stride] + s;
     const bool valid = p >= 0 && p < r.rows;
     // A lane takes four dims and their partners half a head on; U rows are on their way at a time. (16-bit types: with eight dims, 252 us instead of 157 for
-    // 8 x 4096 tokens.)
-    constexpr int E = 4, QL = HD / 2 / E, QROWS = 32 / QL, U = sizeof(T) == 2 ? 8 : 4;
+    // 8 x 4096 tokens. PACKED with eight rows: registers spilled, 33000 tokens of 32 sequences 267 us instead of 162.)
+    constexpr int E = 4, QL = HD / 2 / E, QROWS = 32 / QL, U = sizeof(T) == 2 && !PACKED ? 8 : 4;
     using Raw = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
     const int ql = lane % QL, qsub = lane / QL;
     float cs[E], sn[E];
@@ -223,112 +224,120 @@ __global__ void __launch_bounds__(256, 4) kv_store_kernel(KvView c, KvRows k, Kv
     return;
   }
   const unsigned bp = u / un.kv_slices, slice = u - bp * un.kv_slices, b = PACKED ? 0u : bp / un.pairs;
-  long long p0, s0, turn[2]; // the pair's even position (a slot is one, too) and its token; the positions of the two for their rotation
-  bool has[2], past = false;
-  if constexpr (PACKED) {
-    const long long t = bp, at = pk.slot[t];
-    if (at < 0 || ((at & 1) && t > 0 && pk.slot[t - 1] == at - 1)) return; // no token, or the one before has taken it along
-    p0 = at & ~1ll, s0 = t - (at & 1);
-    has[0] = !(at & 1), has[1] = (at & 1) || (t + 1 < seq && pk.slot[t + 1] == at + 1);
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      turn[e] = has[e] ? pk.position[s0 + e] : 0;
-      if (ROPE && has[e] && turn[e] >= r.rows) has[e] = false, past = true;
-    }
-  } else {
-    const long long first = pos_p[(long long)b * pos_stride];
-    p0 = ((first >> 1) + (bp - b * un.pairs)) * 2, s0 = p0 - first;
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const long long p = p0 + e, s = s0 + e;
-      has[e] = s >= 0 && s < seq && p >= 0;
-      if (has[e] && (p >= c.max_seq || (ROPE && p >= r.rows))) has[e] = false, past = true;
-      turn[e] = p;
-    }
-  }
-  if (past && lane == 0) atomicOr(&g_kv_store_status, KV_PAST_STORE);
-  if (!has[0] && !has[1]) return;
-  uint8_t *tile0; // head 0's
-  int row;
-  if constexpr (PACKED) {
-    const long long size = (long long)c.page_tiles * KV_TILE, page = p0 / size;
-    const int in = (int)(p0 - page * size);
-    if (page >= c.num_pages) return; // (the plan is another cache's)
-    tile0 = c.pages + page * c.page_bytes + (long long)(in / KV_TILE) * L::BYTES, row = in % KV_TILE;
-  } else {
-    tile0 = kv_tile_at(c, (int)b, 0, (int)(p0 / KV_TILE), L::BYTES), row = (int)p0 % KV_TILE;
-    if (!tile0) {
-      if (lane == 0) atomicOr(&g_kv_store_status, KV_NO_PAGE);
-      return;
-    }
-  }
-  const int pair = row / 2, blk = l / 4, t = l % 4;
-  float cs[2][8], sn[2][8];
-  if (ROPE) load_tables<HD>(r, turn[0], l, has[0], cs[0], sn[0]), load_tables<HD>(r, turn[1], l, has[1], cs[1], sn[1]);
-  const T *const kp = static_cast<const T *>(k.p) + b * k.sb + s0 * k.ss + l * 8, *const vp = static_cast<const T *>(v.p) + b * v.sb + s0 * v.ss + l * 8;
-  auto row_of = [&](int x, float (&val)[2][8]) { // rows 0 .. KV - 1: keys, the next KV: values
-    const bool is_v = x >= c.kv_heads, in = x < 2 * c.kv_heads;
-    const T *p = is_v ? vp + (x - c.kv_heads) * v.sh : kp + x * k.sh;
-    const long long ss = is_v ? v.ss : k.ss;
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) val[e][i] = 0.f;
-      if (in && has[e]) load8(p + e * ss, val[e]);
-    }
-  };
-  for (int base = slice * ROWS; base < 2 * c.kv_heads; base += un.kv_slices * ROWS) {
-    const int x = base + sub;
-    const bool is_v = x >= c.kv_heads;
-    float val[2][8];
-    row_of(x, val);
-    Codes8 q[2];
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      if (ROPE) { // values keep theirs; the shuffles want every lane
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = val[e][i];
-        rope8<HD>(y, cs[e], sn[e], l >= HD / 16);
-#pragma unroll
-        for (int i = 0; i < 8; i++) val[e][i] = is_v ? val[e][i] : y[i];
-      }
-      q[e] = quantize8<BITS>(val[e]);
-    }
-    if (x >= 2 * c.kv_heads) continue;
-    uint8_t *tile = tile0 + (is_v ? x - c.kv_heads : x) * c.head_bytes;
-    if (!is_v) {
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        if (!has[e]) continue;
-        if (BITS == 4) *reinterpret_cast<uint32_t *>(tile + L::k_word(row + e, t, blk)) = q[e].lo;
-        else *reinterpret_cast<uint2 *>(tile + L::k_word(row + e, t, 2 * blk)) = make_uint2(q[e].lo, q[e].hi);
-        if (t == 0) *reinterpret_cast<__half *>(tile + L::k_scale(row + e, blk)) = q[e].d;
-      }
-      continue;
-    }
-    constexpr int G = BITS / 4; // words a granule of four dims takes
-#pragma unroll
-    for (int half = 0; half < 2; half++) { // dims 8 t + 4 half ..: chunk g = 2 t + half
-#pragma unroll
-      for (int j = 0; j < G; j++) {
-        uint32_t g[2];
+  const auto put = [&](long long token) { // PACKED: of all tokens
+    long long p0, s0; // the pair's even position and its token
+    bool has[2], past = false;
+    uint8_t *tile0; // head 0's
+    int row;
+    float cs[2][8], sn[2][8];
+    if constexpr (PACKED) {
+      const long long at = pk.slot[token], before = token > 0 ? pk.slot[token - 1] : -1, after = token + 1 < seq ? pk.slot[token + 1] : -1;
+      if (at < 0 || ((at & 1) && before == at - 1)) return; // no token, or the one before has taken it along
+      has[0] = !(at & 1), has[1] = (at & 1) || after == at + 1;
+      s0 = token - (at & 1);
+      if (ROPE) {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          const uint32_t w = BITS == 4 ? q[e].lo : (half ? q[e].hi : q[e].lo);
-          g[e] = (BITS == 4 ? w >> (16 * half) : w >> (16 * j)) & 0xffffu;
+          const long long turn = has[e] ? pk.position[s0 + e] : 0;
+          if (has[e] && turn >= r.rows) has[e] = false, past = true;
+          load_tables<HD>(r, turn, l, has[e], cs[e], sn[e]);
         }
-        uint8_t *at = tile + L::v_word(pair, 2 * t + half, G * blk + j);
-        if (has[0] && has[1]) *reinterpret_cast<uint32_t *>(at) = g[0] | (g[1] << 16);
-        else *reinterpret_cast<uint16_t *>(at + (has[0] ? 0 : 2)) = (uint16_t)(has[0] ? g[0] : g[1]);
+      }
+      const long long size = (long long)c.page_tiles * KV_TILE, page = at / size;
+      const int in = (int)(at - page * size);
+      row = in % KV_TILE & ~1;
+      if (page >= c.num_pages) return; // (the plan is another cache's)
+      tile0 = c.pages + page * c.page_bytes + (long long)(in / KV_TILE) * L::BYTES;
+    } else {
+      const long long first = pos_p[(long long)b * pos_stride];
+      p0 = ((first >> 1) + (bp - b * un.pairs)) * 2, s0 = p0 - first;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const long long p = p0 + e, s = s0 + e;
+        has[e] = s >= 0 && s < seq && p >= 0;
+        if (has[e] && (p >= c.max_seq || (ROPE && p >= r.rows))) has[e] = false, past = true;
       }
     }
-    if (t == 0) {
-      __half *at = reinterpret_cast<__half *>(tile + L::v_scale(pair, blk));
-      if (has[0] && has[1]) *reinterpret_cast<__half2 *>(at) = __halves2half2(q[0].d, q[1].d);
-      else at[has[0] ? 0 : 1] = has[0] ? q[0].d : q[1].d;
+    if (past && lane == 0) atomicOr(&g_kv_store_status, KV_PAST_STORE);
+    if (!has[0] && !has[1]) return;
+    if constexpr (!PACKED) {
+      tile0 = kv_tile_at(c, (int)b, 0, (int)(p0 / KV_TILE), L::BYTES);
+      if (!tile0) {
+        if (lane == 0) atomicOr(&g_kv_store_status, KV_NO_PAGE);
+        return;
+      }
+      row = (int)p0 % KV_TILE;
     }
-  }
+    const int pair = row / 2, blk = l / 4, t = l % 4;
+    if (ROPE && !PACKED) load_tables<HD>(r, p0, l, has[0], cs[0], sn[0]), load_tables<HD>(r, p0 + 1, l, has[1], cs[1], sn[1]);
+    const T *const kp = static_cast<const T *>(k.p) + b * k.sb + s0 * k.ss + l * 8, *const vp = static_cast<const T *>(v.p) + b * v.sb + s0 * v.ss + l * 8;
+    auto row_of = [&](int x, float (&val)[2][8]) { // rows 0 .. KV - 1: keys, the next KV: values
+      const bool is_v = x >= c.kv_heads, in = x < 2 * c.kv_heads;
+      const T *p = is_v ? vp + (x - c.kv_heads) * v.sh : kp + x * k.sh;
+      const long long ss = is_v ? v.ss : k.ss;
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) val[e][i] = 0.f;
+        if (in && has[e]) load8(p + e * ss, val[e]);
+      }
+    };
+    for (int base = slice * ROWS; base < 2 * c.kv_heads; base += un.kv_slices * ROWS) {
+      const int x = base + sub;
+      const bool is_v = x >= c.kv_heads;
+      float val[2][8];
+      row_of(x, val);
+      Codes8 q[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        if (ROPE) { // values keep theirs; the shuffles want every lane
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) y[i] = val[e][i];
+          rope8<HD>(y, cs[e], sn[e], l >= HD / 16);
+#pragma unroll
+          for (int i = 0; i < 8; i++) val[e][i] = is_v ? val[e][i] : y[i];
+        }
+        q[e] = quantize8<BITS>(val[e]);
+      }
+      if (x >= 2 * c.kv_heads) continue;
+      uint8_t *tile = tile0 + (is_v ? x - c.kv_heads : x) * c.head_bytes;
+      if (!is_v) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          if (!has[e]) continue;
+          if (BITS == 4) *reinterpret_cast<uint32_t *>(tile + L::k_word(row + e, t, blk)) = q[e].lo;
+          else *reinterpret_cast<uint2 *>(tile + L::k_word(row + e, t, 2 * blk)) = make_uint2(q[e].lo, q[e].hi);
+          if (t == 0) *reinterpret_cast<__half *>(tile + L::k_scale(row + e, blk)) = q[e].d;
+        }
+        continue;
+      }
+      constexpr int G = BITS / 4; // words a granule of four dims takes
+#pragma unroll
+      for (int half = 0; half < 2; half++) { // dims 8 t + 4 half ..: chunk g = 2 t + half
+#pragma unroll
+        for (int j = 0; j < G; j++) {
+          uint32_t g[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const uint32_t w = BITS == 4 ? q[e].lo : (half ? q[e].hi : q[e].lo);
+            g[e] = (BITS == 4 ? w >> (16 * half) : w >> (16 * j)) & 0xffffu;
+          }
+          uint8_t *at = tile + L::v_word(pair, 2 * t + half, G * blk + j);
+          if (has[0] && has[1]) *reinterpret_cast<uint32_t *>(at) = g[0] | (g[1] << 16);
+          else *reinterpret_cast<uint16_t *>(at + (has[0] ? 0 : 2)) = (uint16_t)(has[0] ? g[0] : g[1]);
+        }
+      }
+      if (t == 0) {
+        __half *at = reinterpret_cast<__half *>(tile + L::v_scale(pair, blk));
+        if (has[0] && has[1]) *reinterpret_cast<__half2 *>(at) = __halves2half2(q[0].d, q[1].d);
+        else at[has[0] ? 0 : 1] = has[0] ? q[0].d : q[1].d;
+      }
+    }
+  };
+  if constexpr (PACKED) {
+    for (unsigned k = 0; k < un.each && bp * un.each + k < seq; k++) put(bp * un.each + k);
+  } else put(0);
 }
 
 __device__ __forceinline__ float2 pair_values(uint32_t codes, __half2 d) { // two codes as whole numbers in f16, two scales: the exact products
@@ -428,8 +437,10 @@ unsigned slices_for(int64_t positions, int64_t groups) { return (unsigned)std::m
 template <int BITS, int HD, typename T, bool PACKED>
 int run_store(const KvView &c, const KvRows &k, const KvRows &v, const RopeArgs &r, int64_t batch, int64_t seq, const long long *pos, int pos_stride, const PackedRows &pk, cudaStream_t s) {
   constexpr int ROWS = 32 / (HD / 8);
-  const int64_t pairs = PACKED ? seq : seq / 2 + 1; // that `seq` positions may touch
   StoreUnits un{};
+  // Packed: two tokens a warp where there are enough of them, mostly one pair and a token that the one before has taken along.
+  un.each = PACKED && seq >= 2 * 4736 ? 2 : 1;
+  const int64_t pairs = PACKED ? (seq + un.each - 1) / un.each : seq / 2 + 1; // that `seq` positions may touch
   un.pairs = (unsigned)pairs;
   un.kv_slices = slices_for(batch * pairs, (2 * c.kv_heads + ROWS - 1) / ROWS);
   const int64_t kv = batch * pairs * un.kv_slices;
