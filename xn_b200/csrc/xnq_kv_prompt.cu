@@ -218,13 +218,15 @@ __host__ __device__ constexpr int position_at(int n) { return (n & ~7) | ((((n >
 
 // Packed tokens: what each CTA does follows from the sequences' lengths, which only the device knows. A unit is a row tile of a sequence and KV head; where one sees
 // more than an SM's share of all steps, `parts` CTAs share its positions. Units lie in the order of what they see, the longest first (24 trees over 1600 to 8192
-// positions: 249 us in the sequences' own order, 230 so, 180 with parts), so those with parts come first and a part's number is its CTA's. Sequences beyond
-// SORTED are taken in their own order, whole.
+// positions: 249 us in the sequences' own order, 230 so), so those with parts come first and a part's number is its CTA's. More than SORTED sequences are taken in
+// their own order, whole.
 constexpr int SORTED = 256;
 struct UnitScratch { // sequences with row tiles
-  int which[SORTED], tiles[SORTED], steps[SORTED], parts[SORTED];
+  int which[SORTED], tiles[SORTED], parts[SORTED];
+  float cost[SORTED]; // of a unit: its steps, those of one row tile of 128 rows where there could be two HALF_COST each
   int found[4];
 };
+constexpr float HALF_COST = 0.8f;
 struct Unit {
   int b, rt, kvh, part, parts;
   int record; // its first part's
@@ -250,17 +252,18 @@ __device__ __forceinline__ int list_units(const AttendArgs &a, int tile_rows, Un
       n += u.parts[w];
     }
     if (is && at < SORTED)
-      u.which[at] = base + x, u.tiles[at] = (int)((unsigned)(q.seq * a.group + tile_rows - 1) / (unsigned)tile_rows), u.steps[at] = (q.count + STEP_TILES - 1) / STEP_TILES;
+      u.which[at] = base + x, u.tiles[at] = (int)((unsigned)(q.seq * a.group + tile_rows - 1) / (unsigned)tile_rows), u.cost[at] = (float)((q.count + STEP_TILES - 1) / STEP_TILES) * (tile_rows == 256 && q.seq * a.group <= 128 ? HALF_COST : 1.f);
     __syncthreads();
   }
   if (n > SORTED) return -1;
   if (x < n) {
-    float steps = 0.f; // (the same sums in every CTA)
+    float all = 0.f; // (the same sums in every CTA)
     int units = 0;
-    for (int y = 0; y < n; y++) steps += (float)u.tiles[y] * (float)u.steps[y], units += u.tiles[y];
-    // an SM's shares of all steps; units that fill the GPU are cut from 1.25 of them on, others so that all parts run at once
-    const float shares = steps > 0.f ? (float)u.steps[x] * (float)a.splits / (steps * (float)a.c.kv_heads) : 0.f;
-    u.parts[x] = max(1, min((int)(units * a.c.kv_heads > a.splits ? shares + 0.75f : shares * 1.0001f), u.steps[x] / 2));
+    for (int y = 0; y < n; y++) all += (float)u.tiles[y] * u.cost[y], units += u.tiles[y];
+    // Units that do not fill the GPU are cut into as many parts as they have whole shares of an SM, so that all run at once. Where they do, a part would cost more than it
+    // gains: its start, its end and the joining take as long as some five steps (24 trees, 176 units on 148 SMs: the five longest sequences' in two parts 204 us, whole 178).
+    const float shares = all > 0.f ? u.cost[x] * (float)a.splits / (all * (float)a.c.kv_heads) : 0.f;
+    u.parts[x] = units * a.c.kv_heads > a.splits ? 1 : max(1, min((int)(shares * 1.0001f), (int)(u.cost[x] * 0.5f))); // (no less for a larger cost)
   }
   __syncthreads();
   return n;
@@ -275,7 +278,7 @@ __device__ __forceinline__ bool unit_at(const AttendArgs &a, int nth, int n, int
     if (x < n) {
       int before = 0, parts = 0; // units before, and their CTAs
       for (int y = 0; y < n; y++)
-        if (u.steps[y] > u.steps[x] || (u.steps[y] == u.steps[x] && y < x)) before += u.tiles[y], parts += u.tiles[y] * u.parts[y];
+        if (u.cost[y] > u.cost[x] || (u.cost[y] == u.cost[x] && y < x)) before += u.tiles[y], parts += u.tiles[y] * u.parts[y];
       const int p = u.parts[x], at = nth - (whole ? before : parts) * heads; // of this sequence's
       if (at >= 0 && at < u.tiles[x] * heads * (whole ? 1 : p)) {
         const int mine = whole ? at : at / p; // (row tile from the last on, head)
@@ -348,9 +351,16 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   }
   const uint32_t raw_full = bar, raw_scanned = bar + 16 * 8, raw_empty = bar + 32 * 8, k_full = bar + 48 * 8, k_empty = k_full + 8 * RING, v_full = k_empty + 8 * RING, v_empty = v_full + 8 * RING,
                  s_full = v_empty + 8 * RING, p_full = s_full + 32, pv_done = p_full + 32, o_done = pv_done + 16, q_ready = o_done + 16; // s_full, p_full: [row tile][buffer] (softmax may be two halves ahead of the MMAs)
+  int active = QT; // row tiles that have rows
+  if constexpr (MORE && QT == 2) {
+    const bool by_units = a.offsets && a.batch > 1;
+    const int b = by_units ? unit.b : 0, per = (int)a.batch * a.c.kv_heads * a.splits, rt = by_units ? unit.rt : a.row_tiles - 1 - (int)(blockIdx.x / per);
+    const long long seq = a.offsets ? a.offsets[b + 1] - a.offsets[b] : a.seq;
+    if (seq * a.group - (long long)rt * 256 <= 128) active = 1;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 16; i++) mbar_init(raw_full + 8 * i, 1), mbar_init(raw_scanned + 8 * i, 1), mbar_init(raw_empty + 8 * i, 2);
-    for (int i = 0; i < RING; i++) mbar_init(k_full + 8 * i, 2), mbar_init(v_full + 8 * i, 2), mbar_init(k_empty + 8 * i, QT), mbar_init(v_empty + 8 * i, QT);
+    for (int i = 0; i < RING; i++) mbar_init(k_full + 8 * i, 2), mbar_init(v_full + 8 * i, 2), mbar_init(k_empty + 8 * i, MORE ? active : QT), mbar_init(v_empty + 8 * i, MORE ? active : QT);
     for (int i = 0; i < 2; i++) {
       mbar_init(s_full + 16 * i, 1), mbar_init(s_full + 16 * i + 8, 1), mbar_init(p_full + 16 * i, 4), mbar_init(p_full + 16 * i + 8, 4), mbar_init(pv_done + 8 * i, 1), mbar_init(o_done + 8 * i, 1);
     }
@@ -601,7 +611,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       if (lane == 0) mbar_arrive(full + 8 * stage), mbar_arrive(raw_empty + 8 * slot);
       __syncwarp();
     }
-  } else if (warp >= MMA && warp < MMA + QT) {
+  } else if (warp >= MMA && warp < MMA + QT && (!MORE || warp < MMA + active)) {
     // The loops' course and the descriptors are functions of what the compiler knows to be uniform, so that descriptors stay in uniform registers: moved there
     // one by one they hold an MMA up for longer than it takes. After a wait that gave up nothing more is issued. (One warp for both row tiles was held up by
     // the one while the other was ready: 307 us for 2048 queries at 8192 positions.)
@@ -658,7 +668,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       __syncwarp();
       for (int k = 0; k < 1000 && !mbar_try(o_done + 8 * q, 0); k++) {}
     }
-  } else if (warp < QT * 4) {
+  } else if (warp < QT * 4 && (!MORE || warp < active * 4)) {
     // ---- a row a thread ----
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     const int q = warp >> 2, r = (warp & 3) * 32 + lane; // row tile, row of it
@@ -918,7 +928,9 @@ __device__ __forceinline__ void join_row(const AttendArgs &a, const float *first
   constexpr int V = HD / 32, AHEAD = 8;
   const int lane = threadIdx.x & 31;
   const size_t record = (size_t)tile_rows * (HD + 2);
-  float m = -INFINITY, l = 0.f, v[V] = {};
+  float m = -INFINITY, l = 0.f, v[V] = {}, ahead[AHEAD][V]; // the first parts' values, asked for before their weights are known
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) load_vec_cg<V>(first + min(i, parts - 1) * record + 2 * tile_rows + (size_t)row * HD + lane * V, ahead[i]);
   for (int k = lane; k < parts; k += 32) m = fmaxf(m, __ldcg(first + k * record + row));
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -934,7 +946,12 @@ __device__ __forceinline__ void join_row(const AttendArgs &a, const float *first
     for (int k = 0; k < left; k += AHEAD) {
       float x[AHEAD][V];
 #pragma unroll
-      for (int i = 0; i < AHEAD; i++) load_vec_cg<V>(first + (k0 + min(k + i, left - 1)) * record + 2 * tile_rows + (size_t)row * HD + lane * V, x[i]);
+      for (int i = 0; i < AHEAD; i++) {
+        if (k0 + k == 0) {
+#pragma unroll
+          for (int c = 0; c < V; c++) x[i][c] = ahead[i][c];
+        } else load_vec_cg<V>(first + (k0 + min(k + i, left - 1)) * record + 2 * tile_rows + (size_t)row * HD + lane * V, x[i]);
+      }
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
         const float by = __shfl_sync(0xffffffffu, mine, (k + i) & 31);
@@ -967,7 +984,7 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_consta
   join_row<HD>(a, a.records + ((size_t)(a.row_tiles - 1 - rt) * units + bk) * a.splits * (128 * (HD + 2)), 128, a.splits, row, // (the last row tiles' CTAs come first)
                b * a.out.sb + (first + tok) * a.out.ss + h * a.out.sh, ((long long)b * a.seq + first + tok) * a.heads + h);
 }
-// Packed tokens: the units that have parts come first; a block goes on from one to the next, 8 rows at a time.
+// Packed tokens: the units that have parts come first. A block takes a run of their rows, 8 at a time (of one unit mostly, which is looked up once).
 constexpr int JOIN_BLOCKS = 592;
 template <int HD>
 __global__ void __launch_bounds__(256) kv_attend_join_packed_kernel(const __grid_constant__ AttendArgs a, int tile_rows) {
@@ -975,17 +992,25 @@ __global__ void __launch_bounds__(256) kv_attend_join_packed_kernel(const __grid
   pdl_launch_dependents();
   pdl_wait();
   const int n = list_units<256>(a, tile_rows, u), groups = tile_rows / 8;
-  if (n < 0) return;
-  for (int w = blockIdx.x;; w += gridDim.x) {
-    Unit unit;
-    if (!unit_at<256>(a, w / groups, n, tile_rows, true, u, unit) || unit.parts == 1) return;
+  int units = 0;
+  for (int y = 0; y < n; y++) units += u.parts[y] > 1 ? u.tiles[y] : 0;
+  units *= a.c.kv_heads;
+  const int each = (units * groups + (int)gridDim.x - 1) / (int)gridDim.x, end = min((int)(blockIdx.x + 1) * each, units * groups);
+  Unit unit{};
+  int known = -1;
+  for (int w = blockIdx.x * each; w < end; w++) {
+    const int nth = w / groups;
+    if (nth != known) {
+      __syncthreads(); // (what was found before has been read)
+      if (!unit_at<256>(a, nth, n, tile_rows, true, u, unit)) return;
+      known = nth;
+    }
     const long long first = a.offsets[unit.b], all_rows = (a.offsets[unit.b + 1] - first) * a.group;
-    const int row = w % groups * 8 + (threadIdx.x >> 5);
-    const long long at_row = (long long)unit.rt * tile_rows + row, tok = first + at_row / a.group;
-    const int h = unit.kvh * a.group + (int)(at_row % a.group);
+    const int row = (w - nth * groups) * 8 + (threadIdx.x >> 5);
+    const long long at_row = (long long)unit.rt * tile_rows + row, tok = first + (unsigned)at_row / (unsigned)a.group;
+    const int h = unit.kvh * a.group + (int)((unsigned)at_row % (unsigned)a.group);
     if (at_row < all_rows)
       join_row<HD>(a, a.records + (size_t)unit.record * tile_rows * (HD + 2), tile_rows, unit.parts, row, tok * a.out.ss + h * a.out.sh, tok * a.heads + h);
-    __syncthreads(); // (u has been read)
   }
 }
 
@@ -1011,14 +1036,13 @@ Plan packed_plan_of(const AttendArgs &a, int sms) {
   const bool pairs = rows > 128 && a.c.kv_heads * one > sms;
   return Plan{pairs ? 2 : 1, (int)std::min<int64_t>(pairs ? two : one, INT_MAX), sms};
 }
-// CTAs that share units' positions: with U units and s SMs, parts of units that have any are no more than s (U <= s: a unit has as many as its whole shares of an SM)
-// or 1.6 s (else a unit of x >= 1.25 shares has at most x + 0.75), and no more than s beyond the units.
-constexpr int MAX_SMS = 160, MAX_PARTS = MAX_SMS * 8 / 5;
+// CTAs that share units' positions: a unit has as many as its whole shares of an SM, all of them no more than the SMs.
+constexpr int MAX_PARTS = 160;
 template <int BITS, int HD, int QT, bool MORE>
 int launch(const AttendArgs &a, cudaStream_t s) {
   const bool packed = MORE && a.offsets && a.batch > 1;
   const int64_t units = (int64_t)a.row_tiles * a.c.kv_heads; // packed: at most
-  const int64_t grid = packed ? (units <= a.splits ? a.splits : units + a.splits) : (int64_t)a.row_tiles * a.batch * a.c.kv_heads * a.splits;
+  const int64_t grid = packed ? std::max<int64_t>(units, a.splits) : (int64_t)a.row_tiles * a.batch * a.c.kv_heads * a.splits;
   if (grid > INT_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of query rows are more than one launch takes", (long long)grid);
   XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT, MORE>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
   count_launch();
@@ -1055,10 +1079,10 @@ int kv_prompt_init(int) {
     return rc;
   return XNQ_OK;
 }
-size_t kv_prompt_parts_bytes(int head_dim, bool packed) { return (size_t)(packed ? MAX_PARTS * 256 : MAX_SMS * 128) * (head_dim + 2) * 4; }
+size_t kv_prompt_parts_bytes(int head_dim, bool packed) { return (size_t)MAX_PARTS * (packed ? 256 : 128) * (head_dim + 2) * 4; }
 int launch_kv_prompt(const AttendArgs &args, bool more, int bits, int head_dim, int sms, cudaStream_t s) {
   AttendArgs a = args;
-  const Plan p = a.offsets && a.batch > 1 ? packed_plan_of(a, std::min(sms, MAX_SMS)) : plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_SMS));
+  const Plan p = a.offsets && a.batch > 1 ? packed_plan_of(a, std::min(sms, MAX_PARTS)) : plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_PARTS));
   a.row_tiles = p.row_tiles, a.splits = p.splits;
   if (bits == 4) return head_dim == 64 ? launch_hd<4, 64>(a, more, p.qt, s) : launch_hd<4, 128>(a, more, p.qt, s);
   return head_dim == 64 ? launch_hd<8, 64>(a, more, p.qt, s) : launch_hd<8, 128>(a, more, p.qt, s);
