@@ -205,7 +205,8 @@ struct PromptShape {
 
 struct Work { // of a CTA: rows row0 .. of a sequence and KV head, and which positions: n steps, tiles t0 .. (MORE: of the sequence's two runs of tiles)
   long long pos, row0, q_at, out_at, lse_row;
-  int rows, seq, lo, hi, head, gap, turn, total, t0, n, n_tiles, kvh, b, splits; // MORE: tiles are taken from the turn-th of `total` on, the ones before it at the end
+  int rows, seq, lo, hi, head, gap, turn, total, plain, whole, t0, n, n_tiles, kvh, b, splits; // MORE: tiles are taken from the turn-th of `total` on,
+  // the ones before it at the end; of the first `plain` ones some row sees all positions, of the first `whole` ones every row does
 };
 struct Meta { // of a tile
   int k_shift, v_shift; // its scales were taken times 2^shift
@@ -256,7 +257,9 @@ __device__ __forceinline__ int list_units(const AttendArgs &a, int tile_rows, Un
     __syncthreads();
   }
   if (n > SORTED) return -1;
-  if (x < n) {
+  if (a.splits == 1) { // whole, whatever they are
+    if (x < n) u.parts[x] = 1;
+  } else if (x < n) {
     float all = 0.f; // (the same sums in every CTA)
     int units = 0;
     for (int y = 0; y < n; y++) all += (float)u.tiles[y] * u.cost[y], units += u.tiles[y];
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
 
   // ---- which rows, which positions; the row tiles with the most positions first ----
   const auto describe = [&](Work &w) {
-    int rt, split;
+    int rt, split, all_lo = 0, all_hi = 0; // MORE: every row sees [all_lo, all_hi]
     if (MORE && a.offsets && a.batch > 1) rt = unit.rt, split = unit.part, w.splits = unit.parts, w.kvh = unit.kvh, w.b = unit.b;
     else {
       const int per = (int)a.batch * a.c.kv_heads * a.splits, rem = (int)(blockIdx.x % per), bk = rem / a.splits;
@@ -403,8 +406,9 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       w.t0 = 0, w.n_tiles = w.total = q.count;
       // The first tile gives the rows their references: one that all of them see (behind a window's edge, which is another one for each token, rows that have begun with
       // one or two positions pass their references again and again: 777 tokens that see 2500 positions and the first 7, 89 us instead of 55).
-      const int last_lo = a.window ? (int)min(max((a.sees ? q.pos + q.seq - 1 : q.pos + s_end) - a.window + 1, 0ll), a.c.max_seq) : 0; // (a token's depth is at most its index)
-      const int turn = (last_lo + KV_TILE - 1) / KV_TILE, all_hi = a.sees || !a.causal ? w.hi : (int)min((long long)w.hi, max(q.pos + s_first, -1ll));
+      all_lo = a.window ? (int)min(max((a.sees ? q.pos + q.seq - 1 : q.pos + s_end) - a.window + 1, 0ll), a.c.max_seq) : 0; // (a token's depth is at most its index)
+      all_hi = a.sees || !a.causal ? w.hi : (int)min((long long)w.hi, max(q.pos + s_first, -1ll));
+      const int turn = (all_lo + KV_TILE - 1) / KV_TILE;
       w.turn = a.window && turn >= q.head + q.gap && turn * KV_TILE + KV_TILE - 1 <= all_hi ? turn - q.gap : 0;
     } else {
       w.rows = (int)min((long long)(QT * 128), a.seq * a.group - w.row0);
@@ -417,11 +421,16 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     const int steps_all = (w.n_tiles + STEP_TILES - 1) / STEP_TILES, steps_each = (steps_all + w.splits - 1) / w.splits, step0 = min(split * steps_each, steps_all);
     w.n = min(steps_all - step0, steps_each);
     w.t0 += step0 * STEP_TILES, w.n_tiles = min(w.n_tiles - step0 * STEP_TILES, w.n * STEP_TILES);
+    if constexpr (MORE) { // as long as they lie one behind the other
+      const int v = w.t0 + w.turn, first = v + w.gap, run = v >= w.head && v < w.total ? min(w.n_tiles, w.total - v) : 0;
+      w.plain = first * KV_TILE >= w.lo ? max(min((w.hi + 1) / KV_TILE - first, run), 0) : 0;
+      w.whole = first * KV_TILE >= all_lo ? max(min((all_hi + 1) / KV_TILE - first, run), 0) : 0;
+    }
   };
   Work w;
   describe(w);
   if (MORE && w.rows < 0) w.rows = 0; // (packed, one sequence: it has fewer tokens than the grid has rows for)
-  const int n = w.n, t0 = w.t0, n_tiles = w.n_tiles;
+  const int n = w.n, t0 = w.t0, n_tiles = w.n_tiles, whole = w.whole;
   const auto tile_of = [&](int i) { // this CTA's i-th tile, in the cache
     if constexpr (MORE) {
       const int at = t0 + i + w.turn, v = at >= w.total ? at - w.total : at;
@@ -487,7 +496,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
         // Most tiles: all of their positions are seen by some row, every scale is below 4 and the largest keys and values are not below 2^-3, f16's middle:
         // largest scales of 2^-6 (codes up to 8) or 2^-10 (up to 127). (With 2^-6 for 8 bits too, 2048 queries over 8192 positions took 699 us with values
         // of 0.3 and 293 with values of 0.7.)
-        const bool inside = MORE ? all_seen(a, w.lo, w.hi, j0) : j0 >= w.lo && j0 + KV_TILE - 1 <= w.hi;
+        const bool inside = MORE ? i + e < w.plain : j0 >= w.lo && j0 + KV_TILE - 1 <= w.hi;
         const bool plain = !null[e] && inside && __all_sync(0xffffffffu, max(k_top, v_top) < 0x4400u) && __any_sync(0xffffffffu, k_top >= LEAST_BITS) &&
                            __any_sync(0xffffffffu, v_top >= LEAST_BITS);
         Meta mt{0, 0, 0u, 0};
@@ -770,7 +779,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       const uint32_t at = buffers + (h2 & 1) * HALF; // P takes the place of the first half of the scores
       const int j0 = tile_of(h2 * 2) * KV_TILE;
       const auto edge = [&]() { // a position of the half that some row does not see
-        if constexpr (MORE) return !all_seen(a, lo_all, hi_all, j0) || !all_seen(a, lo_all, hi_all, tile_of(h2 * 2 + 1) * KV_TILE);
+        if constexpr (MORE) return h2 * 2 + 1 >= whole && (!all_seen(a, lo_all, hi_all, j0) || !all_seen(a, lo_all, hi_all, tile_of(h2 * 2 + 1) * KV_TILE));
         else return j0 < lo_all || j0 + HALF - 1 > hi_all;
       };
       bool general = !have_ref || v_ref != 0 || edge() || !s_plain[h2 % (2 * META_STEPS)];
@@ -1029,12 +1038,13 @@ Plan plan_of(int64_t batch, int64_t seq, int group, int kv_heads, int64_t max_se
 }
 
 // Packed tokens: row tiles of all sequences, as many as there can be of these tokens (and sequences with `rows_from` rows or more); splits: the SMs, among
-// which the kernel divides the units itself.
+// which the kernel divides the units itself, or 1 where there can be more units than SMs.
 Plan packed_plan_of(const AttendArgs &a, int sms) {
   const int64_t rows = a.seq * a.group, all = a.tokens * a.group, sequences = std::min<int64_t>(a.batch, all / std::max<int64_t>(a.rows_from, 1));
   const int64_t two = std::min<int64_t>(a.batch * ((rows + 255) / 256), all / 256 + sequences), one = std::min<int64_t>(a.batch * ((rows + 127) / 128), all / 128 + sequences);
   const bool pairs = rows > 128 && a.c.kv_heads * one > sms;
-  return Plan{pairs ? 2 : 1, (int)std::min<int64_t>(pairs ? two : one, INT_MAX), sms};
+  const int64_t tiles = std::min<int64_t>(pairs ? two : one, INT_MAX);
+  return Plan{pairs ? 2 : 1, (int)tiles, tiles * a.c.kv_heads > sms ? 1 : sms};
 }
 // CTAs that share units' positions: a unit has as many as its whole shares of an SM, all of them no more than the SMs.
 constexpr int MAX_PARTS = 160;
@@ -1046,8 +1056,8 @@ int launch(const AttendArgs &a, cudaStream_t s) {
   if (grid > INT_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of query rows are more than one launch takes", (long long)grid);
   XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT, MORE>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
   count_launch();
+  if (a.splits == 1) return XNQ_OK;
   if (packed) XNQ_CUDA(launch_pdl(kv_attend_join_packed_kernel<HD>, dim3(JOIN_BLOCKS), dim3(256), 0, s, a, QT * 128));
-  else if (a.splits == 1) return XNQ_OK;
   else XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD>, dim3((unsigned)(a.row_tiles * a.batch * a.c.kv_heads * 16)), dim3(256), 0, s, a));
   count_launch();
   return XNQ_OK;
