@@ -271,7 +271,16 @@ __device__ __forceinline__ int list_units(const AttendArgs &a, int tile_rows, Un
   __syncthreads();
   return n;
 }
-// the unit of a CTA (of `records` false: the nth unit, all of its parts together); n: list_units'
+// units that have parts, and where the kernel that joins them finds their number
+__device__ __forceinline__ int split_units(const AttendArgs &a, int n, const UnitScratch &u) {
+  int units = 0;
+  for (int y = 0; y < n; y++) units += u.parts[y] > 1 ? u.tiles[y] : 0;
+  return units * a.c.kv_heads;
+}
+constexpr int MAX_PARTS = 160; // CTAs that share units' positions: a unit has as many as its whole shares of an SM, all of them no more than the SMs
+template <int HD>
+__device__ __forceinline__ int *parts_count(const AttendArgs &a) { return reinterpret_cast<int *>(a.records + (size_t)MAX_PARTS * 256 * (HD + 2)); }
+// the unit of a CTA (`whole`: the nth unit, all of its parts together); n: list_units'
 template <int THREADS>
 __device__ __forceinline__ bool unit_at(const AttendArgs &a, int nth, int n, int tile_rows, bool whole, UnitScratch &u, Unit &unit) {
   const int x = threadIdx.x, heads = a.c.kv_heads;
@@ -349,6 +358,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       UnitScratch &scratch = *reinterpret_cast<UnitScratch *>(smem);
       static_assert(sizeof(UnitScratch) <= P::Q_TILE, "its room");
       const int n = list_units<PROMPT_THREADS>(a, QT * 128, scratch);
+      if (blockIdx.x == 0 && a.splits > 1 && threadIdx.x == 0) *parts_count<HD>(a) = split_units(a, n, scratch);
       if (!unit_at<PROMPT_THREADS>(a, blockIdx.x, n, QT * 128, false, scratch, unit)) return;
     }
   }
@@ -1000,10 +1010,9 @@ __global__ void __launch_bounds__(256) kv_attend_join_packed_kernel(const __grid
   __shared__ UnitScratch u;
   pdl_launch_dependents();
   pdl_wait();
-  const int n = list_units<256>(a, tile_rows, u), groups = tile_rows / 8;
-  int units = 0;
-  for (int y = 0; y < n; y++) units += u.parts[y] > 1 ? u.tiles[y] : 0;
-  units *= a.c.kv_heads;
+  const int units = *parts_count<HD>(a), groups = tile_rows / 8;
+  if (units == 0) return;
+  const int n = list_units<256>(a, tile_rows, u);
   const int each = (units * groups + (int)gridDim.x - 1) / (int)gridDim.x, end = min((int)(blockIdx.x + 1) * each, units * groups);
   Unit unit{};
   int known = -1;
@@ -1046,8 +1055,6 @@ Plan packed_plan_of(const AttendArgs &a, int sms) {
   const int64_t tiles = std::min<int64_t>(pairs ? two : one, INT_MAX);
   return Plan{pairs ? 2 : 1, (int)tiles, tiles * a.c.kv_heads > sms ? 1 : sms};
 }
-// CTAs that share units' positions: a unit has as many as its whole shares of an SM, all of them no more than the SMs.
-constexpr int MAX_PARTS = 160;
 template <int BITS, int HD, int QT, bool MORE>
 int launch(const AttendArgs &a, cudaStream_t s) {
   const bool packed = MORE && a.offsets && a.batch > 1;
@@ -1089,7 +1096,7 @@ int kv_prompt_init(int) {
     return rc;
   return XNQ_OK;
 }
-size_t kv_prompt_parts_bytes(int head_dim, bool packed) { return (size_t)MAX_PARTS * (packed ? 256 : 128) * (head_dim + 2) * 4; }
+size_t kv_prompt_parts_bytes(int head_dim, bool packed) { return (size_t)MAX_PARTS * (packed ? 256 : 128) * (head_dim + 2) * 4 + (packed ? 16 : 0); }
 int launch_kv_prompt(const AttendArgs &args, bool more, int bits, int head_dim, int sms, cudaStream_t s) {
   AttendArgs a = args;
   const Plan p = a.offsets && a.batch > 1 ? packed_plan_of(a, std::min(sms, MAX_PARTS)) : plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_PARTS));
