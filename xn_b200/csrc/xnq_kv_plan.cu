@@ -126,15 +126,18 @@ __device__ __forceinline__ unsigned block_before(unsigned v, unsigned *s_warp, u
 }
 // The bitmap in chunks of 256 words, a warp a chunk and a lane 8 neighbouring words of it (words behind the last page's are 0, and no page is free there).
 constexpr unsigned CHUNK = 256, MOST_CHUNKS = (1u << 20) / 32 / CHUNK; // of RESERVE_MOST_PAGES
+__device__ __forceinline__ uint32_t pages_of(const ReserveArgs &a, unsigned w) { // that there are of a word's 32
+  return w * 32 + 32 <= a.num_pages ? 0xffffffffu : w * 32 < a.num_pages ? (1u << (a.num_pages & 31)) - 1u : 0u;
+}
 __device__ __forceinline__ void load_chunk(const ReserveArgs &a, const uint32_t *bitmap, unsigned chunk, uint32_t (&free)[8]) {
   const unsigned w = chunk * CHUNK + (threadIdx.x & 31) * 8;
   const uint4 x = *reinterpret_cast<const uint4 *>(bitmap + w), y = *reinterpret_cast<const uint4 *>(bitmap + w + 4);
   const uint32_t used[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const long long left = (long long)a.num_pages - (long long)(w + i) * 32; // pages of the word
-    free[i] = ~used[i] & (left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u);
-  }
+  for (int i = 0; i < 8; i++) free[i] = ~used[i];
+  if ((chunk + 1) * (CHUNK * 32) > a.num_pages) // (the last one)
+#pragma unroll
+    for (int i = 0; i < 8; i++) free[i] &= pages_of(a, w + i);
 }
 template <int WARPS>
 __device__ __forceinline__ unsigned count_free(const ReserveArgs &a, const uint32_t *bitmap, unsigned chunks, unsigned *s_chunk, unsigned *s_warp) { // s_chunk: free pages before each chunk
@@ -159,15 +162,18 @@ __device__ __forceinline__ unsigned count_free(const ReserveArgs &a, const uint3
 // The free pages of ranks [first, first + n) into list: a word a thread, so that no thread has more than 32 pages to write (with a lane's 8 words as they are
 // loaded above, the pages of a small cache were one lane's: 16 us for 4 rows of 64 entries).
 template <int THREADS>
-__device__ __forceinline__ void list_pages(const ReserveArgs &a, const uint32_t *bitmap, unsigned chunks, unsigned all, const unsigned *s_chunk, unsigned *s_warp, unsigned first, unsigned n, int *list) {
+__device__ __forceinline__ void list_pages(const ReserveArgs &a, const uint32_t *bitmap, unsigned chunks, const unsigned *s_chunk, unsigned *s_warp, unsigned first, unsigned n, int *list) {
   constexpr unsigned GROUP = THREADS / CHUNK; // chunks at a time
-  for (unsigned k = 0; k < chunks; k += GROUP) {
-    const unsigned begin = s_chunk[k], end = k + GROUP < chunks ? s_chunk[k + GROUP] : all;
-    if (begin >= first + n || end <= first) continue;
+  unsigned k = 0; // the chunk of the first one: the last that begins at or before it
+  for (unsigned end = chunks; end - k > 1;) {
+    const unsigned mid = (k + end) / 2;
+    if (s_chunk[mid] <= first) k = mid;
+    else end = mid;
+  }
+  for (k = k / GROUP * GROUP; k < chunks && s_chunk[k] < first + n; k += GROUP) {
     const unsigned w = k * CHUNK + threadIdx.x;
-    const long long left = (long long)a.num_pages - (long long)w * 32;
-    uint32_t bits = left > 0 ? ~bitmap[w] & (left >= 32 ? 0xffffffffu : (1u << left) - 1u) : 0u;
-    unsigned sum, rank = begin + block_before<THREADS / 32>(__popc(bits), s_warp, sum);
+    uint32_t bits = w * 32 < a.num_pages ? ~bitmap[w] & pages_of(a, w) : 0u;
+    unsigned sum, rank = s_chunk[k] + block_before<THREADS / 32>(__popc(bits), s_warp, sum);
     for (; bits; bits &= bits - 1, rank++)
       if (rank >= first && rank < first + n) list[rank - first] = (int)(w * 32) + __ffs(bits) - 1;
   }
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(RESERVE_SMALL_THREADS, 1) kv_reserve_small_ker
   const unsigned mine = missing_cells(c), before = block_before<WARPS>(lane == 0 ? mine : 0u, s_warp, missing_all); // (its barriers order the bitmap, too)
   const unsigned free_all = count_free<WARPS>(a, bitmap, chunks, s_chunk, s_warp);
   if (missing_all) {
-    list_pages<RESERVE_SMALL_THREADS>(a, bitmap, chunks, free_all, s_chunk, s_warp, 0u, missing_all, s_list);
+    list_pages<RESERVE_SMALL_THREADS>(a, bitmap, chunks, s_chunk, s_warp, 0u, missing_all, s_list);
     __syncthreads();
   }
   give_pages(a, c, __shfl_sync(0xffffffffu, before, 0), 0u, free_all, s_list);
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(RESERVE_THREADS, 4) kv_reserve_give_kernel(con
   block_before<WARPS>(all, s_warp, missing_all);
   if (here || blockIdx.x == 0) {
     free_all = count_free<WARPS>(a, a.bitmap, chunks, s_chunk, s_warp);
-    list_pages<RESERVE_THREADS>(a, a.bitmap, chunks, free_all, s_chunk, s_warp, blocks_before, here, s_list);
+    list_pages<RESERVE_THREADS>(a, a.bitmap, chunks, s_chunk, s_warp, blocks_before, here, s_list);
     __syncthreads();
   }
   give_pages(a, c, blocks_before + at, blocks_before, free_all, s_list);
