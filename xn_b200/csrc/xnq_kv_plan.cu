@@ -19,9 +19,11 @@ __device__ unsigned int g_kv_plan_status;
 // own: it follows from the table, so pages that two rows name (a shared beginning) are free when the last of them lets go.
 //
 // Entries lie in the order of the table, 32 CELLS neighbouring ones to a warp; a lane's are asked for together. Up to RESERVE_SMALL entries: one block, a bitmap of
-// the pages and the list of the free ones in shared memory. More: three kernels over all SMs (clear the bitmap; mark pages and count what is missing; give
-// pages out, every block adding up what is missing before it and, if it misses any itself, reading the bitmap for the free pages of its ranks).
-constexpr int CELLS = 8, RESERVE_THREADS = 256, RESERVE_SMALL_THREADS = 1024, RESERVE_SMALL = RESERVE_SMALL_THREADS * CELLS;
+// the pages and the list of the free ones in shared memory (up to 1024 entries and 131072 pages a block of 128 threads: 256 entries 5.2 us, with 512 threads 6.0, with
+// 1024 8.2). More: three kernels over all SMs (clear the bitmap; mark pages and count what is missing; give pages out, every block adding up what is missing
+// before it and, if it misses any itself, reading the bitmap for the free pages of its ranks): 16384 entries 8.9 us, 1024000 22 us, of which the bytes take 1.3.
+// (One cluster of 8 or 16 CTAs with their bitmaps added up in distributed shared memory: 8.6 and 73 us.)
+constexpr int CELLS = 8, RESERVE_THREADS = 256, RESERVE_SMALL_THREADS = 512, RESERVE_SMALL = RESERVE_SMALL_THREADS * CELLS;
 
 struct Divisor { // n / d for n < 2^31: n m >> (31 + s), s = ceil(log2 d), m = floor(2^(31 + s) / d) + 1, whose error n (m d - 2^(31 + s)) < 2^(31 + s) never carries
   unsigned m, s;
@@ -152,7 +154,7 @@ __device__ __forceinline__ unsigned count_free(const ReserveArgs &a, const uint3
     if ((threadIdx.x & 31) == 0) s_chunk[k] = n;
   }
   __syncthreads();
-  static_assert(MOST_CHUNKS <= 256, "a chunk a thread");
+  static_assert(MOST_CHUNKS <= 128 && WARPS >= 4, "a chunk a thread");
   unsigned all;
   const unsigned n = threadIdx.x < chunks ? s_chunk[threadIdx.x] : 0u, before = block_before<WARPS>(n, s_warp, all);
   if (threadIdx.x < chunks) s_chunk[threadIdx.x] = before;
@@ -163,7 +165,7 @@ __device__ __forceinline__ unsigned count_free(const ReserveArgs &a, const uint3
 // loaded above, the pages of a small cache were one lane's: 16 us for 4 rows of 64 entries).
 template <int THREADS>
 __device__ __forceinline__ void list_pages(const ReserveArgs &a, const uint32_t *bitmap, unsigned chunks, const unsigned *s_chunk, unsigned *s_warp, unsigned first, unsigned n, int *list) {
-  constexpr unsigned GROUP = THREADS / CHUNK; // chunks at a time
+  constexpr unsigned GROUP = THREADS > CHUNK ? THREADS / CHUNK : 1, WORDS = THREADS > CHUNK ? 1 : CHUNK / THREADS; // chunks at a time, words of a thread
   unsigned k = 0; // the chunk of the first one: the last that begins at or before it
   for (unsigned end = chunks; end - k > 1;) {
     const unsigned mid = (k + end) / 2;
@@ -171,33 +173,39 @@ __device__ __forceinline__ void list_pages(const ReserveArgs &a, const uint32_t 
     else end = mid;
   }
   for (k = k / GROUP * GROUP; k < chunks && s_chunk[k] < first + n; k += GROUP) {
-    const unsigned w = k * CHUNK + threadIdx.x;
-    uint32_t bits = w * 32 < a.num_pages ? ~bitmap[w] & pages_of(a, w) : 0u;
-    unsigned sum, rank = s_chunk[k] + block_before<THREADS / 32>(__popc(bits), s_warp, sum);
-    for (; bits; bits &= bits - 1, rank++)
-      if (rank >= first && rank < first + n) list[rank - first] = (int)(w * 32) + __ffs(bits) - 1;
+    unsigned before = s_chunk[k];
+#pragma unroll
+    for (unsigned x = 0; x < WORDS; x++) {
+      const unsigned w = k * CHUNK + x * THREADS + threadIdx.x;
+      uint32_t bits = w * 32 < a.num_pages ? ~bitmap[w] & pages_of(a, w) : 0u;
+      unsigned sum, rank = before + block_before<THREADS / 32>(__popc(bits), s_warp, sum);
+      for (; bits; bits &= bits - 1, rank++)
+        if (rank >= first && rank < first + n) list[rank - first] = (int)(w * 32) + __ffs(bits) - 1;
+      before += sum;
+    }
   }
 }
 
-__global__ void __launch_bounds__(RESERVE_SMALL_THREADS, 1) kv_reserve_small_kernel(const ReserveArgs a) {
-  constexpr int WARPS = RESERVE_SMALL_THREADS / 32;
+template <int THREADS> // CELLS entries each
+__global__ void __launch_bounds__(THREADS, 1) kv_reserve_small_kernel(const ReserveArgs a) {
+  constexpr int WARPS = THREADS / 32;
   extern __shared__ __align__(16) uint32_t bitmap[];
-  __shared__ int s_list[RESERVE_SMALL];
+  __shared__ int s_list[THREADS * CELLS];
   __shared__ unsigned s_warp[WARPS], s_chunk[MOST_CHUNKS];
   const unsigned chunks = (a.num_pages + 32 * CHUNK - 1) / (32 * CHUNK), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (unsigned i = threadIdx.x; i < chunks * CHUNK; i += RESERVE_SMALL_THREADS) bitmap[i] = 0u;
+  for (unsigned i = threadIdx.x; i < chunks * CHUNK; i += THREADS) bitmap[i] = 0u;
   pdl_launch_dependents();
   pdl_wait();
   Cells c;
   load_cells(a, warp * (32 * CELLS) + lane, c);
-  for (int b = threadIdx.x; b < a.batch; b += RESERVE_SMALL_THREADS) a.room[b] = min(max(a.length[b], 0ll), a.max_seq);
+  for (int b = threadIdx.x; b < a.batch; b += THREADS) a.room[b] = min(max(a.length[b], 0ll), a.max_seq);
   __syncthreads();
   mark_pages(c, bitmap);
   unsigned missing_all;
   const unsigned mine = missing_cells(c), before = block_before<WARPS>(lane == 0 ? mine : 0u, s_warp, missing_all); // (its barriers order the bitmap, too)
   const unsigned free_all = count_free<WARPS>(a, bitmap, chunks, s_chunk, s_warp);
   if (missing_all) {
-    list_pages<RESERVE_SMALL_THREADS>(a, bitmap, chunks, s_chunk, s_warp, 0u, missing_all, s_list);
+    list_pages<THREADS>(a, bitmap, chunks, s_chunk, s_warp, 0u, missing_all, s_list);
     __syncthreads();
   }
   give_pages(a, c, __shfl_sync(0xffffffffu, before, 0), 0u, free_all, s_list);
@@ -506,7 +514,7 @@ int kv_plan_status(unsigned int *bits) {
 int kv_plan_init() {
   unsigned int zero = 0;
   XNQ_CUDA(cudaMemcpyToSymbol(g_kv_plan_status, &zero, sizeof(zero)));
-  XNQ_CUDA(cudaFuncSetAttribute(kv_reserve_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(RESERVE_MOST_PAGES / 8)));
+  XNQ_CUDA(cudaFuncSetAttribute(kv_reserve_small_kernel<RESERVE_SMALL_THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(RESERVE_MOST_PAGES / 8)));
   XNQ_CUDA(cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (PLAN_MOST_BATCH + 1) * 4));
   return XNQ_OK;
 }
@@ -553,7 +561,9 @@ int xnq_kv_reserve(int32_t *table, int64_t table_stride, const int32_t *from, in
                       (unsigned)page_size, (int)batch, Divisor::of((unsigned)per), Divisor::of((unsigned)page_size)};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (cells <= RESERVE_SMALL) {
-    XNQ_CUDA(launch_pdl(kv_reserve_small_kernel, dim3(1), dim3(RESERVE_SMALL_THREADS), reserve_bitmap_bytes(num_pages), s, a));
+    const size_t smem = reserve_bitmap_bytes(num_pages);
+    if (cells <= 128 * CELLS && smem <= 16384) XNQ_CUDA(launch_pdl(kv_reserve_small_kernel<128>, dim3(1), dim3(128), smem, s, a));
+    else XNQ_CUDA(launch_pdl(kv_reserve_small_kernel<RESERVE_SMALL_THREADS>, dim3(1), dim3(RESERVE_SMALL_THREADS), smem, s, a));
     count_launch();
     return XNQ_OK;
   }

@@ -216,14 +216,16 @@ class QuantizedKVCache:
 
         ``parents`` (int32 ``[tokens]``): the tokens of a sequence are a tree of drafts. Each one's is the index, in its sequence, of the token that it follows (a
         smaller one than its own); -1: it follows what is in the cache; -2: the place is not used. They lie at ``pos, pos + 1, ..`` in the cache, in their
-        order, are rotated at ``pos`` + depth, and see what lies below ``pos`` and their ancestors. Up to 256 tokens a tree."""
-        _refuse_derivatives("plan")
+        order, are rotated at ``pos`` + depth, and see what lies below ``pos`` and their ancestors. Up to 256 tokens a tree.
+
+        The plan holds the slots of the page table as it is when the call runs: after :meth:`reserve`, before the calls that take it."""
         if tokens < 0 or (longest is not None and longest < 1):
             raise ValueError(f"plan: {tokens} tokens, up to {longest} a sequence")
         longest = max(1, min(tokens, longest if longest is not None else tokens))
         made = self._native.kv_plan(self._handle, pos, count, tokens, longest, parents)
         if made is not None:
             return KVPlan(tokens, longest, self.batch, made)
+        _refuse_derivatives("plan")
         if count.dtype is not torch.int64 or count.device != self.device or count.shape != (self.batch,) or not count.is_contiguous():
             raise ValueError(f"plan: count is contiguous int64 [{self.batch}] on {self.device}")
         if parents is not None:
