@@ -734,3 +734,57 @@ def test_refusals():
     empty = c.plan(pos, _pos(0, 0), 0)
     assert c.attend(q[:0], empty).shape == (0, 4, 64) and c.store(x[:0], x[:0], empty) is None and c.rope_store(qkv[:0], cos, cos, empty, 4).shape == (0, 4, 64)
     assert c.keep(c.plan(pos, _pos(0, 0), 0, 1, _i32([])), _pos(-1, 0)).tolist() == [0, 5] and empty.offsets.tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [3, 70])
+def test_rows_that_lie_apart(dt, n):
+    """Queries with heads and tokens apart, one query for all tokens, results between other values."""
+    c = _filled("q4_0", 2, 2, 400, 64, 32)
+    plan = c.plan(_pos(300, 9), _pos(n - 1, 1), n + 2, n)
+    wide = _rand(3, 8, n + 2, 80).to(TYPES[dt]).to(DEV)
+    q = wide[:, :, :64].transpose(0, 1)
+    want = c.attend(q.contiguous(), plan, window=70, sinks=9)
+    assert torch.equal(c.attend(q, plan, window=70, sinks=9), want)
+    assert torch.equal(c.attend(wide[:, :, 3:67].transpose(0, 1), plan), c.attend(wide[:, :, 3:67].transpose(0, 1).contiguous(), plan))   # not 16-byte aligned
+    one = q[:1].expand(n + 2, -1, -1)
+    assert torch.equal(c.attend(one, plan), c.attend(one.contiguous(), plan))
+    room = torch.full((n + 2, 8, 3, 64), 5.0, dtype=TYPES[dt], device=DEV)
+    c.attend(q, plan, window=70, sinks=9, out=room[:, :, 1])
+    assert torch.equal(room[:n, :, 1], want[:n]) and (room[:, :, ::2] == 5.0).all() and (room[n:] == 5.0).all()
+    with pytest.raises(ValueError, match="apart"):
+        c.attend(q, plan, out=room[:1, :, 1].expand(n + 2, -1, -1))
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("H,KV,counts", [(64, 1, [1, 1, 2]), (96, 2, [1, 0, 1]), (5, 5, [1, 2, 1])])
+def test_wide_and_odd_groups(fmt, dt, H, KV, counts):
+    c = _filled(fmt, 3, KV, 500, 128, 64)
+    plan = c.plan(_pos(499 - counts[0], 7, 250), _pos(*counts), sum(counts), max(counts))
+    q = _rand(4, sum(counts), H, 128, gain=1.5).to(TYPES[dt]).to(DEV)
+    for kw in ({}, dict(window=90, sinks=33)):
+        _attends(c, q, plan, (fmt, dt, H, KV, kw), **kw)
+
+
+def test_more_requests_than_pages():
+    batch, pages = 40000, 1000
+    c = _paged(batch, 32, 32, pages)
+    length = torch.arange(batch, device=DEV) % 33   # every 33rd has none
+    room, free = c.reserve(length)
+    need = (length > 0).cumsum(0)
+    there = (length > 0) & (need <= pages)
+    assert torch.equal(room, torch.where(there, length, 0)) and int(free) == 0
+    assert torch.equal(c.page_table[:, 0][there].long(), torch.arange(pages, device=DEV)) and (c.page_table[:, 0][~there] == -1).all()
+
+
+def test_sequences_that_share_their_beginning():
+    """A shared page is read by both, and free when the second lets go."""
+    c = _filled("q8_0", 2, 2, 300, 64, 32)
+    c.page_table[1, :3] = c.page_table[0, :3]
+    q = _rand(1, 2, 4, 64).to(DEV)
+    plan = c.plan(_pos(95, 95), _pos(1, 1), 2, 1)
+    out = c.attend(torch.cat([q[:1], q[:1]]), plan)
+    assert torch.equal(out[0], out[1])
+    free = [int(c.reserve(_pos(*n))[1]) for n in ((96, 96), (0, 96), (0, 0))]
+    assert free == [c.num_pages - 3, c.num_pages - 3, c.num_pages]
