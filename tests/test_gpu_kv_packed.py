@@ -788,3 +788,44 @@ def test_sequences_that_share_their_beginning():
     assert torch.equal(out[0], out[1])
     free = [int(c.reserve(_pos(*n))[1]) for n in ((96, 96), (0, 96), (0, 0))]
     assert free == [c.num_pages - 3, c.num_pages - 3, c.num_pages]
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("others,rows", [(99, 64), (60, 130), (147, 64), (299, 64)])
+def test_parts_of_one_and_units_of_many(dt, others, rows):
+    """One sequence is most of the work and is cut into many parts; the others are a step each: CTAs for all of them."""
+    L, H, KV, hd = 20000, 4, 1, 64
+    B = others + 1
+    c = _cache("q4_0", B, KV, L, hd, 64)
+    c.page_table.fill_(-1)
+    n = rows // H
+    c.reserve(_pos(*([L] + [n] * others)))
+    for at in range(0, L, 2000):
+        pos = torch.full((B,), -10 ** 6, dtype=torch.int64, device=DEV)
+        pos[0] = at
+        x = _rand(at, 1, 2000, KV, hd).to(DEV).expand(B, -1, -1, -1)
+        c.store(x, x, pos)
+    plan = c.plan(_pos(*([L - n] + [0] * others)), _pos(*([n] * B)), B * n, n)
+    x = _rand(5, B * n, KV, hd).to(DEV)
+    c.store(x, x, plan)
+    q = _rand(6, B * n, H, hd).to(TYPES[dt]).to(DEV)
+    out = torch.full_like(q, math.nan)
+    c.attend(q, plan, out=out)
+    one = c.plan(_pos(*([L - n] + [0] * others)), _pos(*([n] + [0] * others)), n, n)   # the long one by itself
+    want, _, tol, _ = _packed_reference_of(c, q, plan, [0, 1, others // 2, others])
+    for b, w in want.items():
+        _check(out[b * n:(b + 1) * n], w, tol, (dt, others, rows, b))
+    assert torch.isfinite(out.float()).all()
+    _check(c.attend(q[:n], one), want[0], tol, (dt, others, rows))
+
+
+def _packed_reference_of(c, q, plan, which):
+    """f64 results of some sequences of a plan without trees (causal, everything seen)."""
+    off, start, out = plan.offsets.tolist(), plan.start.tolist(), {}
+    for b in which:
+        m = off[b + 1] - off[b]
+        k, v = (x[b].double().repeat_interleave(q.shape[1] // c.kv_heads, 0)[:, :start[b] + m] for x in c.load(0, start[b] + m, dtype=torch.float32))
+        score = q[off[b]:off[b + 1]].double().transpose(0, 1) @ k.transpose(-1, -2) * c.head_dim ** -0.5
+        j, p = torch.arange(start[b] + m, device=DEV), (start[b] + torch.arange(m, device=DEV))[:, None]
+        out[b] = (torch.softmax(score.masked_fill(j > p, -math.inf), -1) @ v).transpose(0, 1)
+    return out, None, 0.0, None

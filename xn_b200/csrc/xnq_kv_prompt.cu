@@ -263,8 +263,8 @@ __device__ __forceinline__ int list_units(const AttendArgs &a, int tile_rows, Un
     float all = 0.f; // (the same sums in every CTA)
     int units = 0;
     for (int y = 0; y < n; y++) all += (float)u.tiles[y] * u.cost[y], units += u.tiles[y];
-    // Units that do not fill the GPU are cut into as many parts as they have whole shares of an SM, so that all run at once. Where they do, a part would cost more than it
-    // gains: its start, its end and the joining take as long as some five steps (24 trees, 176 units on 148 SMs: the five longest sequences' in two parts 204 us, whole 178).
+    // Units that do not fill the GPU are cut into as many parts as they have whole shares of an SM, one at least. Where they do, a part would cost more than it gains: its
+    // start, its end and the joining take as long as some five steps (24 trees, 176 units on 148 SMs: the five longest sequences' in two parts 204 us, whole 178).
     const float shares = all > 0.f ? u.cost[x] * (float)a.splits / (all * (float)a.c.kv_heads) : 0.f;
     u.parts[x] = units * a.c.kv_heads > a.splits ? 1 : max(1, min((int)(shares * 1.0001f), (int)(u.cost[x] * 0.5f))); // (no less for a larger cost)
   }
@@ -1058,8 +1058,8 @@ Plan packed_plan_of(const AttendArgs &a, int sms) {
 template <int BITS, int HD, int QT, bool MORE>
 int launch(const AttendArgs &a, cudaStream_t s) {
   const bool packed = MORE && a.offsets && a.batch > 1;
-  const int64_t units = (int64_t)a.row_tiles * a.c.kv_heads; // packed: at most
-  const int64_t grid = packed ? std::max<int64_t>(units, a.splits) : (int64_t)a.row_tiles * a.batch * a.c.kv_heads * a.splits;
+  const int64_t units = (int64_t)a.row_tiles * a.c.kv_heads; // packed: at most; parts: each of its whole shares of the SMs, and one at least
+  const int64_t grid = packed ? (a.splits == 1 ? units : units + a.splits) : (int64_t)a.row_tiles * a.batch * a.c.kv_heads * a.splits;
   if (grid > INT_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of query rows are more than one launch takes", (long long)grid);
   XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT, MORE>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
   count_launch();
