@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
   const uint32_t base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
   uint8_t *const smem = smem_raw + (base - (uint32_t)__cvta_generic_to_shared(smem_raw));
   const uint32_t bar = (uint32_t)__cvta_generic_to_shared(bars);
-  Unit unit; // MORE, packed
+  Unit unit{}; // MORE, packed
   if constexpr (MORE) {
     if (a.offsets) pdl_wait();
     if (a.offsets && a.clear) clear_behind(a, HD);

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(256, 4) kv_store_kernel(KvView c, KvRows k, Kv
       row = (int)p0 % KV_TILE;
     }
     const int pair = row / 2, blk = l / 4, t = l % 4;
-    if (ROPE && !PACKED) load_tables<HD>(r, p0, l, has[0], cs[0], sn[0]), load_tables<HD>(r, p0 + 1, l, has[1], cs[1], sn[1]);
+    if constexpr (ROPE && !PACKED) load_tables<HD>(r, p0, l, has[0], cs[0], sn[0]), load_tables<HD>(r, p0 + 1, l, has[1], cs[1], sn[1]);
     const T *const kp = static_cast<const T *>(k.p) + b * k.sb + s0 * k.ss + l * 8, *const vp = static_cast<const T *>(v.p) + b * v.sb + s0 * v.ss + l * 8;
     auto row_of = [&](int x, float (&val)[2][8]) { // rows 0 .. KV - 1: keys, the next KV: values
       const bool is_v = x >= c.kv_heads, in = x < 2 * c.kv_heads;
