@@ -421,7 +421,8 @@ int xnq_kv_keep(const xnq_kv_cache *cache, const xnq_kv_plan *plan, const long l
 /* xnq_kv_attend with first positions that stay visible and for packed tokens. A query at p sees j <= p (causal) or j < pos + its sequence's new tokens, and with
  * a window > 0 only j > p - window or j < sinks. plan NULL: q and out [batch, seq, heads, head_dim], p = pos[b] + i. Else q, out [tokens, heads, head_dim] and lse
  * [tokens, heads] (batch, seq, pos and stride_b are not looked at), p the plan's position; with trees a token sees the cache below its tree (p and the window as
- * above; a window of at least `longest`) and the tokens of its tree that it descends from. A token that is none gives zeros; rows behind the last sequence
+ * above; a window of at least `longest`) and the tokens of its tree that it descends from. Accuracy as of xnq_kv_attend, but that bf16 sequences of a plan whose longest
+ * may have 64 query rows of a KV head take keys and values in 16 bits from 32 rows on. A token that is none gives zeros; rows behind the last sequence
  * are left as they are, or set to zero (lse -inf) with `clear`. Workspace as for xnq_kv_attend: xnq_kv_attend_workspace_bytes, with a plan
  * xnq_kv_attend_packed_workspace_bytes. */
 size_t xnq_kv_attend_packed_workspace_bytes(const xnq_kv_plan *plan, int heads, int kv_heads, int head_dim);

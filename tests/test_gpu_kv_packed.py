@@ -829,3 +829,57 @@ def _packed_reference_of(c, q, plan, which):
         j, p = torch.arange(start[b] + m, device=DEV), (start[b] + torch.arange(m, device=DEV))[:, None]
         out[b] = (torch.softmax(score.masked_fill(j > p, -math.inf), -1) @ v).transpose(0, 1)
     return out, None, 0.0, None
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_sinks_in_a_graph_at_other_positions(dt):
+    c = _filled("q4_0", 3, 2, 900, 64, 32)
+    for S in (1, 40):
+        q, pos = _rand(1, 3, S, 8, 64).to(TYPES[dt]).to(DEV), _pos(800, 100, -S)
+        s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s):
+            c.attend(q, pos, window=70, sinks=5)
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g, stream=s):
+                out = c.attend(q, pos, window=70, sinks=5)
+        for at in ([800, 100, -S], [3, 859, 500], [0, -1, 31]):
+            pos.copy_(_pos(*at))
+            q.normal_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, c.attend(q, pos, window=70, sinks=5))
+
+
+def test_threads_with_streams_of_their_own():
+    """Plans, packed attention of few and of many rows and page tables from four threads at once: as one after the other."""
+    import threading
+    c = _filled("q8_0", 6, 2, 1200, 64, 32)
+    counts = [[1, 1, 150, 1, 0, 2], [40, 1, 1, 33, 20, 1], [1] * 6, [200, 100, 3, 1, 1, 60]]
+    jobs = []
+    for i, n in enumerate(counts):
+        pos = _pos(*((100 * b + 37 * i) % 900 for b in range(6)))
+        jobs.append((pos, _pos(*n), sum(n), max(n), _rand(i, sum(n), 8, 64).to(torch.bfloat16 if i % 2 else torch.float16).to(DEV)))
+
+    def work(job):
+        pos, n, tokens, longest, q = job
+        plan = c.plan(pos, n, tokens, longest)
+        return c.attend(q, plan, window=300, sinks=9), c.attend(q, plan)
+    want = [[x.clone() for x in work(job)] for job in jobs]
+    torch.cuda.synchronize()
+    wrong, errors = [], []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    got = work(jobs[i])
+                    torch.cuda.current_stream().synchronize()
+                    wrong.extend(i for x, y in zip(got, want[i]) if not torch.equal(x, y))
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(len(jobs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not errors and not wrong and _status() == 0
