@@ -1,7 +1,7 @@
 // Page tables and slot maps of the quantized KV cache, made on the GPU from request lengths; and the accepted path of a tree of drafted tokens kept.
 //
 // All of it is a few hundred kilobytes at most (the largest tables some megabytes) and bound by latency: launches, dependent loads, barriers. So each call is
-// one launch, with nothing read back by the host.
+// one launch (page tables of more than 4096 entries three), with nothing read back by the host.
 #include <algorithm>
 
 #include "xnq_kv_attend.cuh"
@@ -19,8 +19,8 @@ __device__ unsigned int g_kv_plan_status;
 // own: it follows from the table, so pages that two rows name (a shared beginning) are free when the last of them lets go.
 //
 // Entries lie in the order of the table, 32 CELLS neighbouring ones to a warp; a lane's are asked for together. Up to RESERVE_SMALL entries: one block, a bitmap of
-// the pages and the list of the free ones in shared memory (up to 1024 entries and 131072 pages a block of 128 threads: 256 entries 5.2 us, with 512 threads 6.0, with
-// 1024 8.2). More: three kernels over all SMs (clear the bitmap; mark pages and count what is missing; give pages out, every block adding up what is missing
+// the pages and the list of the free ones in shared memory (up to 1024 entries and 131072 pages a block of 128 threads: 256 entries 5.2 us, with 1024
+// threads 8.2; 4096 entries, 512 threads, 6.2). More: three kernels over all SMs (clear the bitmap; mark pages and count what is missing; give pages out, every block adding up what is missing
 // before it and, if it misses any itself, reading the bitmap for the free pages of its ranks): 16384 entries 8.9 us, 1024000 22 us, of which the bytes take 1.3.
 // (One cluster of 8 or 16 CTAs with their bitmaps added up in distributed shared memory: 8.6 and 73 us.)
 constexpr int CELLS = 8, RESERVE_THREADS = 256, RESERVE_SMALL_THREADS = 512, RESERVE_SMALL = RESERVE_SMALL_THREADS * CELLS;
