@@ -66,7 +66,7 @@ struct Block {
   size_t bytes;
   std::mutex lock;
 };
-constexpr size_t BLOCK = 16 << 20, LARGE_BLOCK = 34 << 20; // the parts take 10 MB whatever the call, those of many packed tokens 21 more; the rest is tickets
+constexpr size_t BLOCK = 16 << 20, LARGE_BLOCK = 24 << 20; // the parts take 10 MB whatever the call, those of many packed tokens 21; the rest is tickets
 constexpr int BLOCKS = 32; // (a stream may have one of each size)
 Block g_blocks[BLOCKS]; // they and the counts: under the interpreter's lock
 int g_num_blocks = 0;

@@ -137,7 +137,7 @@ constexpr int split_ctas(int hd, int nt, bool split) { return nt == 1 && !(split
 // has as many row tiles as its own tokens take. Which positions of a tile a row sees is a word of 32 bits, looked at in tiles that some row does not see whole. As
 // fast as the first form: 64 sequences that see 4096 positions and 64 first ones, bf16 over Q4_0, 73 us (3.6 TB/s of cache); one token of 1024, f32, 11.7 us.
 template <int BITS, int HD, int NT, bool SPLIT, bool MORE>
-__device__ __forceinline__ void attend_split(const AttendArgs &a) {
+__global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) kv_attend_split_kernel(const AttendArgs a) {
   using Span = typename std::conditional<MORE, MoreSpan, PlainSpan>::type;
   using L = KvTile<BITS, HD>;
   using P = SplitShape<BITS, HD, NT>;
@@ -158,8 +158,7 @@ __device__ __forceinline__ void attend_split(const AttendArgs &a) {
   uint8_t *const ring = smem + warp * SPLIT_STAGES * L::BYTES;
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
   pdl_launch_dependents();
-  if (!MORE || !a.beside) pdl_wait();
-  else __threadfence(); // (nothing that this SM may still hold of what was there before)
+  pdl_wait();
 
   // ---- this CTA's run of the flattened list: [t0, t1) of `total` tiles ----
   const int per_seq = MORE ? a.c.kv_heads : a.c.kv_heads * a.row_tiles; // items of a sequence (MORE: of a row tile), all of its count of tiles
@@ -852,15 +851,6 @@ __device__ __forceinline__ void attend_split(const AttendArgs &a) {
   }
 }
 
-template <int BITS, int HD, int NT, bool SPLIT, bool MORE>
-__global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) kv_attend_split_kernel(const __grid_constant__ AttendArgs a) {
-  attend_split<BITS, HD, NT, SPLIT, MORE>(a);
-  // `beside`: the kernel before, of the sequences with many rows, lets this one in when all of its CTAs have waited for what came before it, which is what is read
-  // here; this one works on the SMs that it leaves free. Who waits for this one has to find the other's results, too: one CTA ends after it. (Were it all of
-  // them, those that are done would keep the rest of the grid out.)
-  if (MORE && a.beside && blockIdx.x == 0) pdl_wait();
-}
-
 int g_sms[64]; // of the devices that xnq_init has seen
 
 template <int BITS, int HD, int NT, bool SPLIT, bool MORE>
@@ -965,8 +955,7 @@ namespace {
 size_t workspace_bytes(int64_t batch, int64_t seq, int heads, int kv_heads, int head_dim, bool packed) {
   if (batch <= 0 || seq <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
   // (for the kernel for many rows at its most: a part for every SM)
-  const size_t parts = seq * (heads / kv_heads) >= PROMPT_ROWS ? kv_prompt_parts_bytes(head_dim, packed) : 0;
-  return KV_TICKET_BYTES + (packed ? RECORDS_BYTES + parts : std::max(RECORDS_BYTES, parts));
+  return KV_TICKET_BYTES + std::max(RECORDS_BYTES, seq * (heads / kv_heads) >= PROMPT_ROWS ? kv_prompt_parts_bytes(head_dim, packed) : 0);
 }
 // The checks and arguments of both forms (nothing more where batch or seq is 0).
 int attend_args(const xnq_kv_cache *cache, const xnq_rows *q, const xnq_rows *out, float *lse, int64_t batch, int64_t seq, int heads, const long long *pos, int pos_stride, float scale,
@@ -1044,11 +1033,9 @@ int xnq_kv_attend_packed(const xnq_kv_cache *cache, const xnq_rows *q, const xnq
   if (!plan || batch == 1) return launch_kv_prompt(a, true, bits, hd, sms, s);
   // Sequences of their own numbers of tokens: each goes to the kernel for its number of rows.
   AttendArgs few = a;
-  a.rows_from = few.rows_to = q->dtype == XNQ_BF16 ? PACKED_PROMPT_ROWS : PROMPT_ROWS;
-  few.clear = 0, few.beside = 1, few.records += kv_prompt_parts_bytes(hd, true) / 4; // (both are at work at a time)
-  int rc2 = launch_kv_prompt(a, true, bits, hd, sms, s);
-  if (rc2 == XNQ_OK) rc2 = run_attend<true>(few, bits, hd, sms, s);
-  return rc2 != XNQ_OK ? rc2 : launch_kv_join_packed(a, hd, sms, s);
+  a.rows_from = few.rows_to = q->dtype == XNQ_BF16 ? PACKED_PROMPT_ROWS : PROMPT_ROWS, few.clear = 0;
+  const int rc2 = launch_kv_prompt(a, true, bits, hd, sms, s);
+  return rc2 != XNQ_OK ? rc2 : run_attend<true>(few, bits, hd, sms, s);
 }
 
 } // extern "C"

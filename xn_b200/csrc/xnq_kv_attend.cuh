@@ -27,7 +27,6 @@ struct AttendArgs {
   const uint32_t *sees, *nodes; // null: no trees
   int words, clear;             // words of a token's bits; rows behind the last sequence: zeros
   long long rows_from, rows_to; // this launch's sequences: those with that many query rows of a KV head, [from, to)
-  int beside; // few rows: works beside the kernel before it
 };
 
 // Workspace: the tickets, at one place whatever the call, then the parts.
@@ -41,7 +40,6 @@ int kv_prompt_init(int device);
 int kv_prompt_status(unsigned int *bits);
 size_t kv_prompt_parts_bytes(int head_dim, bool packed);
 int launch_kv_prompt(const AttendArgs &a, bool more, int bits, int head_dim, int sms, cudaStream_t s);
-int launch_kv_join_packed(const AttendArgs &a, int head_dim, int sms, cudaStream_t s); // behind the launch above, of more than one packed sequence
 
 #ifdef __CUDACC__
 // positions [lo, hi] that the query at token s of a sequence at `pos` sees

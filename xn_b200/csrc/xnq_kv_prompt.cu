@@ -1065,8 +1065,9 @@ int launch(const AttendArgs &a, cudaStream_t s) {
   if (grid > INT_MAX) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of query rows are more than one launch takes", (long long)grid);
   XNQ_CUDA(launch_pdl(kv_attend_prompt_kernel<BITS, HD, QT, MORE>, dim3((unsigned)grid), dim3(PROMPT_THREADS), (size_t)PromptShape<BITS, HD, QT>::SMEM, s, a));
   count_launch();
-  if (a.splits == 1 || packed) return XNQ_OK;
-  XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD>, dim3((unsigned)(a.row_tiles * a.batch * a.c.kv_heads * 16)), dim3(256), 0, s, a));
+  if (a.splits == 1) return XNQ_OK;
+  if (packed) XNQ_CUDA(launch_pdl(kv_attend_join_packed_kernel<HD>, dim3(JOIN_BLOCKS), dim3(256), 0, s, a, QT * 128));
+  else XNQ_CUDA(launch_pdl(kv_attend_join_kernel<HD>, dim3((unsigned)(a.row_tiles * a.batch * a.c.kv_heads * 16)), dim3(256), 0, s, a));
   count_launch();
   return XNQ_OK;
 }
@@ -1098,16 +1099,6 @@ int kv_prompt_init(int) {
   return XNQ_OK;
 }
 size_t kv_prompt_parts_bytes(int head_dim, bool packed) { return (size_t)MAX_PARTS * (packed ? 256 : 128) * (head_dim + 2) * 4 + (packed ? 16 : 0); }
-int launch_kv_join_packed(const AttendArgs &args, int head_dim, int sms, cudaStream_t s) {
-  AttendArgs a = args;
-  const Plan p = packed_plan_of(a, std::min(sms, MAX_PARTS));
-  a.row_tiles = p.row_tiles, a.splits = p.splits;
-  if (a.splits == 1) return XNQ_OK;
-  if (head_dim == 64) XNQ_CUDA(launch_pdl(kv_attend_join_packed_kernel<64>, dim3(JOIN_BLOCKS), dim3(256), 0, s, a, p.qt * 128));
-  else XNQ_CUDA(launch_pdl(kv_attend_join_packed_kernel<128>, dim3(JOIN_BLOCKS), dim3(256), 0, s, a, p.qt * 128));
-  count_launch();
-  return XNQ_OK;
-}
 int launch_kv_prompt(const AttendArgs &args, bool more, int bits, int head_dim, int sms, cudaStream_t s) {
   AttendArgs a = args;
   const Plan p = a.offsets && a.batch > 1 ? packed_plan_of(a, std::min(sms, MAX_PARTS)) : plan_of(a.batch, a.seq, a.group, a.c.kv_heads, a.c.max_seq, std::min(sms, MAX_PARTS));
