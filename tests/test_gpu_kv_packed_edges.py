@@ -1,0 +1,60 @@
+"""The quantized KV cache between requests: calls that lie at the edge of what is served, and closer looks at results of which test_gpu_kv_packed.py takes one norm."""
+import math
+import random
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_kv_cache import DEV, TYPES, _cache, _check, _filled, _init, _pos, _rand, _status  # noqa: F401 (_init: the module's fixture)
+from test_gpu_kv_packed import CUT, PAST_STORE, _attends, _clean, _i32, _packed_reference, _paged, _tree  # noqa: F401 (_clean: before each test)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("B,L,page", [(6, 500, 32), (40, 4000, 32)])
+def test_steps_without_a_wait_in_between(dt, B, L, page):
+    """A server's steps enqueued one after the other, the page table another one in each: as with a wait behind every call. (40 rows of 125 entries: the table by
+    several kernels.)"""
+    KV, H, hd, n, steps = 2, 8, 64, 200 if B == 6 else 400, 25
+    rng = random.Random(B)
+    c = _cache("q4_0", B, KV, L, hd, page)
+    cos, sin = _rand(4, L, hd // 2).to(DEV), _rand(5, L, hd // 2).to(DEV)
+    at, todo = [0] * B, []
+    for step in range(steps):
+        at = [0 if rng.random() < 0.3 else a for a in at]   # requests end, others begin in their places
+        counts = [min(rng.choice([0, 1, 1, rng.randint(1, 60)]), L - a) for a in at]
+        while sum(counts) > n:
+            counts[counts.index(max(counts))] = 1
+        todo.append((_pos(*at), _pos(*counts), _pos(*(a + m for a, m in zip(at, counts))), (torch.randn(n, (H + 2 * KV) * hd, device=DEV)).to(TYPES[dt])))
+        at = [a + m for a, m in zip(at, counts)]
+    start = torch.randperm(c.num_pages, generator=torch.Generator().manual_seed(1))[:c.page_table.numel()].view(c.page_table.shape).to(torch.int32).to(DEV)
+
+    def run(wait):
+        c.page_table.copy_(start)
+        c.pages.zero_()
+        out = []
+        torch.cuda.synchronize()
+        for pos, count, length, qkv in todo:
+            room, free = c.reserve(length)
+            wait()
+            plan = c.plan(pos, count, n)
+            wait()
+            q = c.rope_store(qkv, cos, sin, plan, H)
+            wait()
+            out += [room, free, plan.slot, plan.position, q, c.attend(q, plan, window=300, sinks=5)]
+            wait()
+            out += [c.attend(q, plan), *c.load(0, 64, dtype=torch.float32), c.page_table.clone()]
+            wait()
+        torch.cuda.synchronize()
+        return out
+    want = run(torch.cuda.synchronize)
+    for _ in range(3):
+        for i, (x, y) in enumerate(zip(run(lambda: None), want)):
+            assert torch.equal(x, y), i
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = run(lambda: None)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

@@ -43,3 +43,11 @@ def test_every_kernel_waits_whatever_its_arguments_are(name, kernel, body):
     assert always, f"{name}: {kernel} does not always wait"
     left = [m.start() for m in re.finditer(r"\breturn\b", body[:always[0]])]
     assert all("pdl_wait();" in body[:at] for at in left), f"{name}: {kernel} ends without having waited"
+
+
+@pytest.mark.parametrize("name", SOURCES)
+def test_nothing_is_read_as_what_never_changes(name):
+    """Page tables, plans and pages are written by kernels that overlap the ones that read them: no load through the read-only path, which is for data that nobody
+    writes while the kernel lives."""
+    found = re.findall(r"__ldg\w*|__restrict__", _text(name)) + re.findall(r"ld\.global[\w.]*\.nc", open(os.path.join(CSRC, name)).read())
+    assert not found, (name, found)

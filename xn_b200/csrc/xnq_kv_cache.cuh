@@ -84,14 +84,15 @@ int kv_plan_check(const char *who, const xnq_kv_plan *p);
 constexpr unsigned KV_PAST_STORE = 1, KV_PAST_ATTEND = 2, KV_NO_PAGE = 4, KV_PLAN_CUT = 16;
 
 #ifdef __CUDACC__
-// The tile of (sequence, head) that holds positions 32 * tile .. ; null where the page table has no page there.
+// The tile of (sequence, head) that holds positions 32 * tile .. ; null where the page table has no page there. (An ordinary load: the kernel that fills the table may be
+// at work when this one begins, so it is not data that stays as it is for the kernel's life, as a load through the read-only path would have it.)
 __device__ __forceinline__ uint8_t *kv_tile_at(const KvView &c, int b, int head, int tile, int tile_bytes) {
   long long page = b;
   int in = tile;
   if (c.table) {
     const int pi = tile / c.page_tiles;
     in = tile - pi * c.page_tiles;
-    page = __ldg(c.table + b * c.table_stride + pi);
+    page = c.table[b * c.table_stride + pi];
     if (page < 0 || page >= c.num_pages) return nullptr;
   }
   return c.pages + page * c.page_bytes + head * c.head_bytes + (long long)in * tile_bytes;

@@ -277,7 +277,7 @@ __device__ __forceinline__ long long tokens_of(const PlanArgs &a, int b) { retur
 __device__ __forceinline__ long long slot_of(const PlanArgs &a, int b, long long place) {
   if (!a.c.table) return (long long)b * a.page_size + place;
   const unsigned pi = (unsigned)place / (unsigned)a.page_size;
-  const int page = __ldg(a.c.table + b * a.c.table_stride + pi);
+  const int page = a.c.table[b * a.c.table_stride + pi];
   if (page < 0 || page >= a.c.num_pages) {
     atomicOr(&g_kv_plan_status, KV_NO_PAGE);
     return -1;
