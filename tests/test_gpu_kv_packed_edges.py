@@ -58,3 +58,17 @@ def test_steps_without_a_wait_in_between(dt, B, L, page):
     with torch.cuda.stream(s):
         got = run(lambda: None)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("B,L,tokens", [(256, 200, 32768), (200, 600, 100000)])
+def test_f32_tokens_of_many_sequences(B, L, tokens):
+    """No more is said of the sequences' lengths than that they are as many tokens as there are: any of them could be as long as all."""
+    KV, H, hd, n = 1, 8, 64, tokens // B
+    c = _filled("q4_0", B, KV, L, hd, 32)
+    counts = [n + (-1) ** b * (b % 37) for b in range(B)]
+    counts[-1] += tokens - sum(counts)
+    starts = [(b * 7) % (L - m) if m < L else 0 for b, m in enumerate(counts)]
+    plan = c.plan(_pos(*starts), _pos(*counts), tokens)
+    assert plan.longest == tokens
+    _attends(c, _rand(2, tokens, H, hd, gain=1.5).to(DEV), plan, (B, tokens))
+    assert _status() == 0

@@ -887,10 +887,14 @@ template <int BITS, int HD, int NT, bool SPLIT, bool MORE>
 int run_split(AttendArgs a, int sms, cudaStream_t s) {
   const int64_t rows = std::min<int64_t>(a.seq * a.group, MORE ? a.rows_to - 1 : INT64_MAX);
   a.row_tiles = (int)((rows + 8 * NT - 1) / (8 * NT));
-  if (MORE && a.batch * a.row_tiles >= 1 << 22) return fail(XNQ_ERR_SIZE, "kv_attend: %lld x %lld query rows are more than one launch takes", (long long)a.batch, (long long)rows);
+  // Row tiles of all sequences: of packed tokens no more than all of the tokens fill, and one begun a sequence. (What a block adds up of them has 22 bits above the
+  // tiles' 40: counted, above.)
+  int64_t row_tiles = a.batch * a.row_tiles;
+  if (MORE && a.offsets) row_tiles = std::min(row_tiles, a.tokens * a.group / (8 * NT) + a.batch);
+  if (MORE && row_tiles >= 1 << 22) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of %d query rows are more than one launch takes", (long long)row_tiles, 8 * NT);
   using Launch = SplitLaunch<BITS, HD, NT, SPLIT, MORE>;
   // no more CTAs than the longest caches could fill
-  const int64_t most = a.batch * a.c.kv_heads * a.row_tiles * ((a.c.max_seq + KV_TILE - 1) / KV_TILE);
+  const int64_t most = a.c.kv_heads * row_tiles * ((a.c.max_seq + KV_TILE - 1) / KV_TILE);
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(std::min(sms * Launch::per_sm, MAX_SPLIT_GRID), std::max<int64_t>(most, a.batch)));
   XNQ_CUDA(launch_pdl(kv_attend_split_kernel<BITS, HD, NT, SPLIT, MORE>, dim3((unsigned)grid), dim3(SPLIT_WARPS * 32), Launch::smem(), s, a));
   count_launch();
