@@ -890,7 +890,7 @@ int run_split(AttendArgs a, int sms, cudaStream_t s) {
   // Row tiles of all sequences: of packed tokens no more than all of the tokens fill, and one begun a sequence. (What a block adds up of them has 22 bits above the
   // tiles' 40: counted, above.)
   int64_t row_tiles = a.batch * a.row_tiles;
-  if (MORE && a.offsets) row_tiles = std::min(row_tiles, a.tokens * a.group / (8 * NT) + a.batch);
+  if (MORE && a.offsets) row_tiles = std::min<int64_t>(row_tiles, a.tokens * a.group / (8 * NT) + a.batch);
   if (MORE && row_tiles >= 1 << 22) return fail(XNQ_ERR_SIZE, "kv_attend: %lld tiles of %d query rows are more than one launch takes", (long long)row_tiles, 8 * NT);
   using Launch = SplitLaunch<BITS, HD, NT, SPLIT, MORE>;
   // no more CTAs than the longest caches could fill
