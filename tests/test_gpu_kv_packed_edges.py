@@ -72,3 +72,52 @@ def test_f32_tokens_of_many_sequences(B, L, tokens):
     assert plan.longest == tokens
     _attends(c, _rand(2, tokens, H, hd, gain=1.5).to(DEV), plan, (B, tokens))
     assert _status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dt,counts", [("f16", [1, 5, 15, 16, 64]), ("bf16", [1, 7, 8, 40])])
+def test_a_plan_of_one_sequence_with_room_for_more(fmt, dt, counts):
+    """Which arithmetic a sequence gets goes by its own rows, not by the room: below 64 rows of a KV head (bf16: 32) keys and weights keep their bits."""
+    L, H, KV, hd = 3000, 8, 2, 128
+    c = _filled(fmt, 1, KV, L, hd, 64)
+    q = _rand(5, 64, H, hd, gain=1.5).to(TYPES[dt]).to(DEV)
+    for n in counts:
+        plan = c.plan(_pos(2900 - n), _pos(n), 64)
+        for kw in ({}, dict(window=700, sinks=40)):
+            lse, out = torch.full((64, H), 7.0, device=DEV), torch.full_like(q, math.nan)
+            c.attend(q, plan, out=out, lse=lse, **kw)
+            want, want_lse, tol, size = _packed_reference(c, q, plan, **kw)
+            _check(out[:n], want[:n], tol, (fmt, dt, n, kw))
+            assert torch.isnan(out[n:]).all() and (lse[n:] == 7.0).all()
+            rows = n * H // KV
+            # as test_gpu_kv_cache.py has it where the scores are products of the codes themselves; else a key's rounding to f16, half a step of 2^-10 at most
+            near = 2e-5 * max(1.0, float(want_lse[:n].abs().max())) + (0.0 if rows < (64 if dt == "f16" else 32) else 2.0 ** -11 * size)
+            assert float((lse[:n] - want_lse[:n]).abs().max()) <= near, (fmt, dt, n, kw)
+            own = c.attend(q, plan, **kw)
+            assert torch.equal(own[:n], out[:n]) and not own[n:].any()
+    assert _status() == 0
+
+
+def test_one_sequence_of_few_and_of_many_tokens_in_a_graph():
+    """One captured step with room for 90 tokens, replayed for a single token, for none and for all of them."""
+    L, H, KV, hd, n = 1200, 8, 1, 64, 90
+    c = _filled("q4_0", 1, KV, L, hd, 32)
+    pos, count, q = _pos(100), _pos(n), _rand(1, n, H, hd).to(torch.float16).to(DEV)
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        c.attend(q, c.plan(pos, count, n))
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            plan = c.plan(pos, count, n)
+            out = c.attend(q, plan)
+    torch.cuda.synchronize()
+    for at, m in ((1199, 1), (3, 90), (0, 0), (800, 7), (1000, 8), (7, 1), (1110, 90)):
+        pos.fill_(at), count.fill_(m), q.normal_()
+        g.replay()
+        torch.cuda.synchronize()
+        mine = c.plan(pos, count, n)
+        assert torch.equal(out, c.attend(q, mine)) and not out[m:].any()
+        if m:
+            want, _, tol, _ = _packed_reference(c, q, mine)
+            _check(out[:m], want[:m], tol, (at, m))
+    assert _status() == 0

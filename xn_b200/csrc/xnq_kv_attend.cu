@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(SPLIT_WARPS * 32, split_ctas(HD, NT, SPLIT)) k
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
   pdl_launch_dependents();
   pdl_wait();
+  if (MORE && a.offsets && a.batch == 1 && (a.offsets[1] - a.offsets[0]) * a.group >= a.rows_to) return; // one sequence, of many rows: the other kernel's
 
   // ---- this CTA's run of the flattened list: [t0, t1) of `total` tiles ----
   const int per_seq = MORE ? a.c.kv_heads : a.c.kv_heads * a.row_tiles; // items of a sequence (MORE: of a row tile), all of its count of tiles
@@ -1034,8 +1035,10 @@ int xnq_kv_attend_packed(const xnq_kv_cache *cache, const xnq_rows *q, const xnq
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int bits = kv_bits(cache->ggml_dtype), hd = cache->head_dim;
   if (q->dtype == XNQ_F32 || a.seq * a.group < PROMPT_ROWS) return run_attend<true>(a, bits, hd, sms, s);
-  if (!plan || batch == 1) return launch_kv_prompt(a, true, bits, hd, sms, s);
-  // Sequences of their own numbers of tokens: each goes to the kernel for its number of rows.
+  if (!plan) return launch_kv_prompt(a, true, bits, hd, sms, s);
+  // Sequences of their own numbers of tokens, which the device alone knows: each goes to the kernel for its number of rows, a single one too (a step with room for more
+  // tokens than it has: of few rows it has nothing to see in the first kernel, whose zeros the second one's results take the place of; of many, the second ends at once.
+  // A tree of 26 over 4096 positions takes 25.5 us, without the second launch 22.6).
   AttendArgs few = a;
   a.rows_from = few.rows_to = q->dtype == XNQ_BF16 ? PACKED_PROMPT_ROWS : PROMPT_ROWS, few.clear = 0;
   const int rc2 = launch_kv_prompt(a, true, bits, hd, sms, s);

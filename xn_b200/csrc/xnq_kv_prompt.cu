@@ -999,7 +999,7 @@ __global__ void __launch_bounds__(256) kv_attend_join_kernel(const __grid_consta
   const long long first = a.offsets ? a.offsets[0] : 0, all_rows = (a.offsets ? a.offsets[1] - first : a.seq) * a.group; // (packed: one sequence)
   const int rt = (int)(at / (128ll * units)), bk = (int)(at / 128 % units), row = (int)(at % 128), b = bk / a.c.kv_heads, kvh = bk % a.c.kv_heads;
   const long long at_row = rt * 128ll + row;
-  if (rt >= a.row_tiles || at_row >= all_rows) return;
+  if (rt >= a.row_tiles || at_row >= all_rows || all_rows < a.rows_from) return;
   const long long tok = at_row / a.group;
   const int h = kvh * a.group + (int)(at_row - tok * a.group);
   join_row<HD>(a, a.records + ((size_t)(a.row_tiles - 1 - rt) * units + bk) * a.splits * (128 * (HD + 2)), 128, a.splits, row, // (the last row tiles' CTAs come first)
