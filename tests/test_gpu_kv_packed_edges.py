@@ -121,3 +121,38 @@ def test_one_sequence_of_few_and_of_many_tokens_in_a_graph():
             want, _, tol, _ = _packed_reference(c, q, mine)
             _check(out[:m], want[:m], tol, (at, m))
     assert _status() == 0
+
+
+@pytest.mark.parametrize("page", [None, 32])
+@pytest.mark.parametrize("at", [2 ** 63 - 1, 2 ** 63 - 3, 2 ** 62, 2 ** 31, 2 ** 32 + 5, -2 ** 63, -2 ** 63 + 2])
+def test_positions_far_outside_the_cache(page, at):
+    """A sequence at a position that no cache reaches (a server's mark of an unused place) brings tokens that are none: no sum of positions wraps round into the cache."""
+    B, KV, H, hd, L, n = 3, 1, 4, 64, 100, 7
+    c = _filled("q4_0", B, KV, L, hd, page)
+    before = c.pages.clone()
+    x, q = _rand(1, 3 * n, KV, hd).to(DEV), _rand(2, 3 * n, H, hd).to(DEV)
+    for parents in (None, _i32([i - 1 for i in range(n)] * 3), _i32([-1] + [0] * (n - 1) + [-1] * n + [-1] + [0] * (n - 1))):
+        plan = c.plan(_pos(5, at, 60), _pos(n, n, n), 3 * n, n, parents)
+        assert plan.position[n:2 * n].tolist() == [-1] * n and plan.slot[n:2 * n].tolist() == [-1] * n and plan.start.tolist() == [5, at, 60]
+        assert (plan.position[:n] >= 0).all() and (plan.position[2 * n:] >= 0).all()
+        if parents is not None:
+            assert not plan.sees[n:2 * n].any() and plan.nodes[:, 0].tolist() == [127, 0, 127]
+        c.store(x, x, plan)
+        for dt in ("f32", "bf16"):
+            for kw in ({}, dict(window=20, sinks=5)):
+                out = c.attend(q.to(TYPES[dt]), plan, **kw)
+                assert not out[n:2 * n].any() and out[:n].any(-1).all() and out[2 * n:].any(-1).all()
+        if parents is not None:
+            assert c.keep(plan, _pos(2, 3, -1))[1:].tolist() == [at, 60]
+        assert torch.equal(c.load(0, L)[0][1], _restored(c, before, 1))
+    assert _status() & ~PAST_STORE == 0 and bool(_status() & PAST_STORE) == (at > 0)
+
+
+def _restored(c, pages, b):
+    """Sequence b's keys as another state of the memory has them."""
+    now = c.pages.clone()
+    c.pages.copy_(pages)
+    k = c.load(0, c.max_seq)[0][b]
+    c.pages.copy_(now)
+    return k
+

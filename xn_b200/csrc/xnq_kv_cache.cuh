@@ -84,6 +84,9 @@ int kv_plan_check(const char *who, const xnq_kv_plan *p);
 constexpr unsigned KV_PAST_STORE = 1, KV_PAST_ATTEND = 2, KV_NO_PAGE = 4, KV_PLAN_CUT = 16;
 
 #ifdef __CUDACC__
+// A sequence's first place, such that numbers of tokens and windows can be added and taken off: one far outside every cache (a caller's mark of an unused place, 2^63 - 1
+// say) must not wrap round into it.
+__device__ __forceinline__ long long first_place(const long long *pos, long long i) { return max(min(pos[i], 1ll << 62), -(1ll << 62)); }
 // The tile of (sequence, head) that holds positions 32 * tile .. ; null where the page table has no page there. (An ordinary load: the kernel that fills the table may be
 // at work when this one begins, so it is not data that stays as it is for the kernel's life, as a load through the read-only path would have it.)
 __device__ __forceinline__ uint8_t *kv_tile_at(const KvView &c, int b, int head, int tile, int tile_bytes) {

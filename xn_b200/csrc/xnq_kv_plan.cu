@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) kv_plan_kernel(const PlanArgs a)
         else hi = mid;
       }
       seq = lo;
-      place = a.pos[(long long)seq * a.pos_stride] + (t - s_off[seq]);
+      place = first_place(a.pos, (long long)seq * a.pos_stride) + (t - s_off[seq]);
       if (place >= a.c.max_seq) {
         atomicOr(&g_kv_plan_status, KV_PAST_STORE);
         place = -1;
@@ -380,9 +380,9 @@ __global__ void __launch_bounds__(XNQ_KV_TREE_MOST) kv_plan_trees_kernel(const P
 #pragma unroll
   for (int w = 0; w < W; w++) before += s_sum[0][w], all += s_sum[1][w];
   const long long tokens = a.p.tokens, off = min(before, tokens), here = min(before + tokens_of(a, b), tokens) - off; // of this sequence
-  const long long pos = a.pos[(long long)b * a.pos_stride];
+  const long long pos = first_place(a.pos, (long long)b * a.pos_stride);
   if (i == 0) {
-    a.p.offsets[b] = off, a.p.start[b] = pos;
+    a.p.offsets[b] = off, a.p.start[b] = a.pos[(long long)b * a.pos_stride];
     if (b == batch - 1) a.p.offsets[batch] = off + here;
   }
   if (b == 0 && (cut || all > tokens)) atomicOr(&g_kv_plan_status, KV_PLAN_CUT);
