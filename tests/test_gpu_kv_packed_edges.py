@@ -156,3 +156,19 @@ def _restored(c, pages, b):
     c.pages.copy_(now)
     return k
 
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("S,H", [(1, 4), (3, 4), (40, 256)])
+def test_rectangles_far_outside_the_cache(dt, S, H):
+    """The calls with a position a sequence, next to one that is served; a query past the cache sees all of it, or what its window leaves."""
+    c = _filled("q4_0", 2, 1, 37, 64)
+    q = _rand(3, 2, S, H, 64).to(TYPES[dt]).to(DEV)
+    end = c.attend(q, _pos(20, 37 + 40))
+    for at in (2 ** 62, 2 ** 63 - 1, 2 ** 63 - 2):
+        for kw in ({}, dict(causal=False)):
+            out = c.attend(q, _pos(20, at), **kw)
+            assert torch.equal(out[1], end[1]) and out[0].any(-1).all(), (at, kw)
+        for kw in (dict(window=9), dict(window=9, causal=False)):
+            assert not c.attend(q, _pos(20, at), **kw)[1].any()
+        assert torch.equal(c.attend(q, _pos(20, at), window=9, sinks=37)[1], c.attend(q, _pos(20, 37 + 40), window=9, sinks=37)[1])

@@ -58,7 +58,7 @@ __device__ __forceinline__ void span_of(const AttendArgs &a, int b, MoreSpan &s)
 }
 template <int R>
 __device__ __forceinline__ void span_of(const AttendArgs &a, int b, PlainSpan &s) {
-  s.pos = a.pos[(long long)b * a.pos_stride];
+  s.pos = first_place(a.pos, (long long)b * a.pos_stride);
   const long long hi = min(s.pos + a.seq - 1, a.c.max_seq - 1), p0 = max(s.pos, 0ll), lo = a.window ? max(p0 - a.window + 1, 0ll) : 0ll;
   s.first = (int)(min(lo, a.c.max_seq) / KV_TILE);
   s.count = hi < lo ? 0 : (int)(hi / KV_TILE) - s.first + 1;

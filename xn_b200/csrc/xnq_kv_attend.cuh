@@ -68,10 +68,10 @@ __device__ __forceinline__ void tiles_seen(const AttendArgs &a, Sequence &x, lon
 __device__ __forceinline__ Sequence sequence_of(const AttendArgs &a, int b) {
   Sequence x;
   if (a.offsets) {
-    x.pos = a.start[b], x.first_row = a.offsets[b], x.seq = (int)(a.offsets[b + 1] - x.first_row);
+    x.pos = first_place(a.start, b), x.first_row = a.offsets[b], x.seq = (int)(a.offsets[b + 1] - x.first_row);
     const long long rows = (long long)x.seq * a.group;
     x.here = rows >= a.rows_from && rows < a.rows_to;
-  } else x.pos = a.pos[(long long)b * a.pos_stride], x.first_row = b * a.seq, x.seq = (int)a.seq, x.here = true;
+  } else x.pos = first_place(a.pos, (long long)b * a.pos_stride), x.first_row = b * a.seq, x.seq = (int)a.seq, x.here = true;
   x.head = x.gap = x.count = 0;
   if (x.here && x.seq > 0) tiles_seen(a, x, 0, x.seq - 1);
   return x;

@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
       w.turn = a.window && turn >= q.head + q.gap && turn * KV_TILE + KV_TILE - 1 <= all_hi ? turn - q.gap : 0;
     } else {
       w.rows = (int)min((long long)(QT * 128), a.seq * a.group - w.row0);
-      w.pos = a.pos[(long long)w.b * a.pos_stride], w.lse_row = w.b * a.seq, w.seq = (int)a.seq, w.q_at = w.b * a.q.sb, w.out_at = w.b * a.out.sb;
+      w.pos = first_place(a.pos, (long long)w.b * a.pos_stride), w.lse_row = w.b * a.seq, w.seq = (int)a.seq, w.q_at = w.b * a.q.sb, w.out_at = w.b * a.out.sb;
       const long long s_first = w.row0 / a.group, s_end = (w.row0 + w.rows - 1) / a.group;
       const long long hi_l = w.pos + s_end < 0 ? -1 : min(a.causal ? w.pos + s_end : w.pos + a.seq - 1, a.c.max_seq - 1);
       const long long lo_l = a.window ? min(max(max(w.pos + s_first, 0ll) - a.window + 1, 0ll), a.c.max_seq) : 0ll;
