@@ -172,3 +172,20 @@ def test_rectangles_far_outside_the_cache(dt, S, H):
         for kw in (dict(window=9), dict(window=9, causal=False)):
             assert not c.attend(q, _pos(20, at), **kw)[1].any()
         assert torch.equal(c.attend(q, _pos(20, at), window=9, sinks=37)[1], c.attend(q, _pos(20, 37 + 40), window=9, sinks=37)[1])
+
+
+@pytest.mark.parametrize("batch", [2, 4000])
+def test_a_page_that_ends_behind_the_last_position_is_given_back(batch):
+    """Rows of one page and a bit: `first` is compared with where the last page ends, which is past max_seq."""
+    c = _paged(batch, 100, 64, 2 * batch)
+    length = torch.full((batch,), 100, dtype=torch.int64, device=DEV)
+    room, free = c.reserve(length)
+    assert int(free) == 0 and (room == 100).all()
+    before = c.page_table.clone()
+    for first, needed in ((63, [True, True]), (64, [False, True]), (100, [False, True]), (127, [False, True]), (128, [False, False]), (2 ** 62, [False, False]), (2 ** 63 - 1, [False, False])):
+        for sinks in (0, 64, 65):
+            keep = torch.tensor([needed[0] or sinks > 0, needed[1] or sinks > 64], device=DEV)
+            room, free = c.reserve(length, first=torch.full_like(length, first), sinks=sinks, table=before)
+            assert torch.equal(c.page_table, torch.where(keep, before, -1)), (first, sinks)
+            assert (room == 100).all() and int(free) == batch * (2 - int(keep.sum()))
+    assert _status() == 0

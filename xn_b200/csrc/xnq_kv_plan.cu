@@ -37,7 +37,7 @@ struct Divisor { // n / d for n < 2^31: n m >> (31 + s), s = ceil(log2 d), m = f
 struct ReserveArgs {
   const int *from;
   int *to;
-  long long from_stride, to_stride, max_seq;
+  long long from_stride, to_stride, max_seq, end; // end: of a row's last page, max_seq or behind it
   const long long *length, *first; // first: null, or [batch]
   long long *room, *free;
   uint32_t *bitmap; // many entries: pages that are in use
@@ -54,7 +54,7 @@ struct Cells { // a lane's entries, 32 apart
 };
 __device__ __forceinline__ void load_cells(const ReserveArgs &a, unsigned begin, Cells &c) { // begin: the lane's first entry
   c.in = c.needed = 0u;
-  unsigned n[CELLS], f[CELLS];
+  unsigned n[CELLS], f[CELLS], past = 0u; // past: bits, `first` lies behind the last page
 #pragma unroll
   for (int k = 0; k < CELLS; k++) {
     const unsigned cell = begin + k * 32;
@@ -63,12 +63,14 @@ __device__ __forceinline__ void load_cells(const ReserveArgs &a, unsigned begin,
     c.row[k] = in ? a.by_per(cell) : 0u, c.at[k] = cell - c.row[k] * a.per;
     c.v[k] = in ? a.from[c.row[k] * a.from_stride + c.at[k]] : -1;
     n[k] = in ? (unsigned)min(max(a.length[c.row[k]], 0ll), a.max_seq) : 0u;
-    f[k] = in && a.first ? (unsigned)min(max(a.first[c.row[k]], 0ll), a.max_seq) : 0u;
+    const long long first = in && a.first ? a.first[c.row[k]] : 0ll;
+    f[k] = (unsigned)min(max(first, 0ll), a.max_seq); // (from max_seq to `end`: the same page)
+    past |= (first >= a.end ? 1u : 0u) << k;
   }
 #pragma unroll
   for (int k = 0; k < CELLS; k++) {
     bool needed = n[k] && c.at[k] <= a.by_page(n[k] - 1); // entries of positions below the length
-    if (a.first) needed = needed && (c.at[k] >= a.by_page(f[k]) || c.at[k] * (unsigned long long)a.page_size < a.sinks);
+    if (a.first) needed = needed && ((!((past >> k) & 1u) && c.at[k] >= a.by_page(f[k])) || c.at[k] * (unsigned long long)a.page_size < a.sinks);
     c.needed |= (needed ? 1u : 0u) << k;
     if (!needed || (unsigned)c.v[k] >= a.num_pages) c.v[k] = -1;
   }
@@ -559,7 +561,7 @@ int xnq_kv_reserve(int32_t *table, int64_t table_stride, const int32_t *from, in
   if (!workspace || ws_bytes < need) return fail(XNQ_ERR_SIZE, "kv_reserve: workspace has %zu bytes, needs %zu", ws_bytes, need);
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(XNQ_ERR_ALIGN, "kv_reserve: the workspace must be 16-byte aligned");
   uint8_t *const ws = static_cast<uint8_t *>(workspace);
-  const ReserveArgs a{from, table, from_stride, table_stride, max_seq, length, first, room, free_pages, reinterpret_cast<uint32_t *>(ws),
+  const ReserveArgs a{from, table, from_stride, table_stride, max_seq, per * page_size, length, first, room, free_pages, reinterpret_cast<uint32_t *>(ws),
                       reinterpret_cast<unsigned *>(ws + reserve_bitmap_bytes(num_pages)), (unsigned)num_pages, (unsigned)std::min<int64_t>(sinks, INT32_MAX), (unsigned)cells, (unsigned)per,
                       (unsigned)page_size, (int)batch, Divisor::of((unsigned)per), Divisor::of((unsigned)page_size)};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
