@@ -436,13 +436,14 @@ __global__ void __launch_bounds__(XNQ_KV_TREE_MOST) kv_plan_trees_kernel(const P
 // ---- the accepted path kept ----
 // The tokens that `node` sees, r = 0, 1, .. in their order, move from place pos + index to pos + r; index >= r, and both ascend. A warp takes the keys or the
 // values of a head, KEEP_ROWS tokens at a time: all of them are read before one is written, and what a later batch reads lies behind what this one writes. Bound
-// by the chain offsets, bits, pages, codes: 24 trees of up to 40 tokens, 8 heads of 128 in Q4_0, 5.4 us.
+// by the chain offsets, bits, pages, codes: 24 trees of up to 40 tokens, 8 heads of 128 in Q4_0, 5.1 us, in Q8_0 5.5.
 constexpr int KEEP_WARPS = 4, KEEP_ROWS = 8;
 template <int BITS, int HD>
 __global__ void __launch_bounds__(KEEP_WARPS * 32) kv_keep_kernel(KvView c, xnq_kv_plan p, const long long *node, long long *pos_out) {
   using L = KvTile<BITS, HD>;
   constexpr int W = L::W, NB = L::NB;
-  constexpr int K_ITEMS = 4 * W + NB / 2, V_ITEMS = 16 * W + NB, EACH = (V_ITEMS + 31) / 32; // 32-bit words of a key, 16-bit halves of a value; with scales
+  constexpr int K_ITEMS = 4 * W + NB / 2, V_ITEMS = 8 * W + NB, EACH = ((K_ITEMS > V_ITEMS ? K_ITEMS : V_ITEMS) + 31) / 32; // 32-bit words of a key, 16-bit halves of a value; with scales
+  static_assert(K_ITEMS * 4 == L::RB + NB * 2 && V_ITEMS * 2 == L::RB + NB * 2, "a position's bytes");
   __shared__ uint16_t s_path[KEEP_WARPS][XNQ_KV_TREE_MOST];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, words = ((int)p.longest + 31) / 32;
   const long long unit = (long long)blockIdx.x * KEEP_WARPS + warp; // (sequence, head, keys or values)
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(KEEP_WARPS * 32) kv_keep_kernel(KvView c, xnq_
     if (x < 8 * W) return tile + L::v_word(row / 2, x / W, x % W) + (row & 1) * 2;
     return tile + L::v_scale(row / 2, x - 8 * W) + (row & 1) * 2;
   };
-  const int items = is_v ? 8 * W + NB : K_ITEMS;
+  const int items = is_v ? V_ITEMS : K_ITEMS;
   for (int r0 = 0; r0 < n; r0 += KEEP_ROWS) {
     // lanes 0 .. 7 look up where the batch's tokens are, lanes 8 .. 15 where they go
     const int r = r0 + (lane & (KEEP_ROWS - 1));
