@@ -104,6 +104,7 @@ def test_one_sequence_of_few_and_of_many_tokens_in_a_graph():
     c = _filled("q4_0", 1, KV, L, hd, 32)
     pos, count, q = _pos(100), _pos(n), _rand(1, n, H, hd).to(torch.float16).to(DEV)
     s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
         c.attend(q, c.plan(pos, count, n))
         torch.cuda.synchronize()
@@ -189,3 +190,65 @@ def test_a_page_that_ends_behind_the_last_position_is_given_back(batch):
             assert torch.equal(c.page_table, torch.where(keep, before, -1)), (first, sinks)
             assert (room == 100).all() and int(free) == batch * (2 - int(keep.sum()))
     assert _status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["q4_0", "q8_0"])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_each_sequence_by_itself(fmt, dt):
+    """A norm and a logarithm's bound a sequence, by the kernel that serves its rows: of a long sequence among short ones no part is lost or taken twice, whose share of
+    one norm over all rows is small."""
+    L, H, KV, hd = 20000, 8, 2, 64
+    c = _filled(fmt, 4, KV, L, hd, 128)
+    for counts, starts in (([64, 70, 1, 64], [19900, 300, 5000, 0]), ([20, 100, 3, 0], [19980, 100, 9000, 4]), ([130, 0, 0, 0], [19870, 0, 0, 0]), ([6, 7, 1, 2], [19000, 12000, 19999, 6])):
+        n = sum(counts)
+        q = _rand(9, n, H, hd, gain=1.5).to(TYPES[dt]).to(DEV)
+        plan = c.plan(_pos(*starts), _pos(*counts), n, 130)
+        for kw in ({}, dict(window=7000, sinks=50)):
+            lse, out = torch.full((n, H), 7.0, device=DEV), torch.full_like(q, math.nan)
+            c.attend(q, plan, out=out, lse=lse, **kw)
+            want, want_lse, tol, size = _packed_reference(c, q, plan, **kw)
+            off = plan.offsets.tolist()
+            for b, m in enumerate(counts):
+                if m == 0:
+                    continue
+                r = slice(off[b], off[b + 1])
+                _check(out[r], want[r], tol, (fmt, dt, counts, b, kw))
+                # few rows: scores of the codes' own products, as test_gpu_kv_cache.py has it; many: a key's rounding to f16 is half a step, 2^-11 of it at most
+                few = m * H // KV < (64 if dt == "f16" else 32)
+                near = 2e-5 * max(1.0, float(want_lse[r].abs().max())) + (0.0 if few else 2.0 ** -11 * size)
+                assert float((lse[r] - want_lse[r]).abs().max()) <= near, (fmt, dt, counts, b, kw)
+    assert _status() == 0
+
+
+def test_every_thread_has_compared_its_results():
+    """Plans, packed attention of few and of many rows and page tables from four threads with streams of their own: all of them come to their end."""
+    tables = [_paged(9, 700, 32, 100 + i) for i in range(4)]
+    c = _filled("q4_0", 5, 2, 1000, 64, 32)
+    counts = [[1, 1, 120, 0, 2], [30, 1, 17, 33, 1], [1] * 5, [150, 90, 3, 1, 40]]
+    jobs = [(_pos(*((100 * b + 31 * i) % 800 for b in range(5))), _pos(*n), sum(n) + 2, _rand(i, sum(n) + 2, 8, 64).to(torch.float16 if i % 2 else torch.bfloat16).to(DEV),
+             _pos(*((70 * b + 211 * i) % 700 for b in range(9)))) for i, n in enumerate(counts)]
+
+    def work(i):
+        pos, n, tokens, q, length = jobs[i]
+        tables[i].page_table.fill_(-1)
+        plan = c.plan(pos, n, tokens)
+        return [c.attend(q, plan, window=200, sinks=9), c.attend(q, plan), plan.slot, *tables[i].reserve(length), tables[i].page_table.clone()]
+    want = [[x.clone() for x in work(i)] for i in range(4)]
+    torch.cuda.synchronize()
+    compared, errors = [0] * 4, []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    got = work(i)
+                    torch.cuda.current_stream().synchronize()
+                    compared[i] += all(torch.equal(x, y) for x, y in zip(got, want[i]))
+        except Exception as e:   # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not errors and not any(t.is_alive() for t in threads) and compared == [60] * 4 and _status() == 0
