@@ -252,3 +252,20 @@ def test_every_thread_has_compared_its_results():
     for t in threads:
         t.join(120)
     assert not errors and not any(t.is_alive() for t in threads) and compared == [60] * 4 and _status() == 0
+
+
+@pytest.mark.parametrize("L", [120, 1000])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("starts,counts,room", [([900], [1], 1), ([900], [3], 80), ([10], [80], 80), ([700], [90], 300), ([0], [0], 70), ([900, 3], [1, 70], 90), ([5, 800, 60, 400], [1, 90, 8, 9], 200),
+                                                ([-4], [3], 64), ([-70, 20], [70, 2], 80)])
+def test_results_in_the_place_of_the_queries(L, dt, starts, counts, room):
+    """Every row's query is read before its result is written, by whichever kernel has it."""
+    c, starts = _filled("q4_0", len(starts), 2, L, 64, 32), [min(s, L - n) for s, n in zip(starts, counts)]
+    q = _rand(3, room, 8, 64).to(TYPES[dt]).to(DEV)
+    plan = c.plan(_pos(*starts), _pos(*counts), room)
+    for kw in ({}, dict(window=200, sinks=9)):
+        want, lse, mine = c.attend(q, plan, **kw), torch.full((room, 8), 7.0, device=DEV), q.clone()
+        c.attend(mine, plan, out=mine, lse=lse, **kw)
+        n = sum(counts)
+        assert torch.equal(mine[:n], want[:n]) and torch.equal(mine[n:], q[n:]) and (lse[n:] == 7.0).all()
+        assert torch.equal(torch.isfinite(lse[:n]), (plan.position[:n] >= 0)[:, None].expand(-1, 8))

@@ -1037,8 +1037,8 @@ int xnq_kv_attend_packed(const xnq_kv_cache *cache, const xnq_rows *q, const xnq
   if (q->dtype == XNQ_F32 || a.seq * a.group < PROMPT_ROWS) return run_attend<true>(a, bits, hd, sms, s);
   if (!plan) return launch_kv_prompt(a, true, bits, hd, sms, s);
   // Sequences of their own numbers of tokens, which the device alone knows: each goes to the kernel for its number of rows, a single one too (a step with room for more
-  // tokens than it has: of few rows it has nothing to see in the first kernel, whose zeros the second one's results take the place of; of many, the second ends at once.
-  // A tree of 26 over 4096 positions takes 25.8 us, without the second launch 22.6).
+  // tokens than it has). The other kernel touches none of its rows, so that results may take the place of queries. A tree of 26 over 4096 positions takes 25.8 us, without
+  // the second launch, which finds nothing, 22.6.
   AttendArgs few = a;
   a.rows_from = few.rows_to = q->dtype == XNQ_BF16 ? PACKED_PROMPT_ROWS : PROMPT_ROWS, few.clear = 0;
   const int rc2 = launch_kv_prompt(a, true, bits, hd, sms, s);

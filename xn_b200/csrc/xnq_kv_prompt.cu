@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(con
     w.row0 = (long long)rt * (QT * 128);
     if constexpr (MORE) {
       Sequence q = sequence_of(a, w.b);
-      w.rows = (int)min((long long)(QT * 128), (long long)q.seq * a.group - w.row0);
+      w.rows = (int)min((long long)(QT * 128), (q.here ? (long long)q.seq * a.group : 0ll) - w.row0); // (not here: one sequence, of few rows, which are the other kernel's)
       if (w.rows <= 0) q.count = 0, q.here = false;
       const int s_first = (int)((unsigned)w.row0 / (unsigned)a.group), s_end = (int)((unsigned)(w.row0 + w.rows - 1) / (unsigned)a.group);
       if (q.here) tiles_seen(a, q, s_first, s_end);
