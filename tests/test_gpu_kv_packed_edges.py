@@ -269,3 +269,27 @@ def test_results_in_the_place_of_the_queries(L, dt, starts, counts, room):
         n = sum(counts)
         assert torch.equal(mine[:n], want[:n]) and torch.equal(mine[n:], q[n:]) and (lse[n:] == 7.0).all()
         assert torch.equal(torch.isfinite(lse[:n]), (plan.position[:n] >= 0)[:, None].expand(-1, 8))
+
+
+def test_a_table_of_one_row_whatever_its_stride():
+    """Of a dimension of one entry a stride means nothing, in the ordinary call as under a mode that looks at torch's operators."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from xn_b200.dtypes import GgmlDType
+    from xn_b200.kv_cache import QuantizedKVCache
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    own = torch.full((4,), -1, dtype=torch.int32, device=DEV).as_strided((1, 4), (0, 1))
+    c = QuantizedKVCache(GgmlDType.Q4_0, 1, 1, 128, 64, DEV, page_size=32, num_pages=9, page_table=own)
+    table = _i32([5, 7, -1, 3]).as_strided((1, 4), (0, 1))
+    assert table.stride(0) == 0 and table.is_contiguous()
+    x = _rand(0, 3, 1, 64).to(DEV)
+    for mode in (None, Watch()):
+        c.page_table.fill_(-1)
+        with mode if mode is not None else torch.no_grad():
+            room, free = c.reserve(_pos(128), table=table)
+            plan = c.plan(_pos(60), _pos(3), 3)
+            c.store(x, x, plan)
+        assert c.page_table.tolist() == [[5, 7, 0, 3]] and room.tolist() == [128] and int(free) == 5 and plan.slot.tolist() == [7 * 32 + 28 + i for i in range(3)]
+    assert float((c.load(60, 3, torch.float32)[0][0, 0] - x[:, 0]).abs().max()) <= float(x.abs().max()) / 8 and _status() == 0

@@ -152,7 +152,7 @@ class QuantizedKVCache:
             raise ValueError(f"QuantizedKVCache: page_table is contiguous int32 {shape} on {self.device}, of a cache by pages")
         self.page_table = page_table if page_table is not None else torch.full(shape, -1, dtype=torch.int32, device=self.device) if paged else None
         self._view = _Cache(int(self.dtype), kv_heads, head_dim, self.page_size, self.num_pages, self.pages.data_ptr(),
-                            self.page_table.data_ptr() if paged else None, self.page_table.stride(0) if paged else 0, max_seq)
+                            self.page_table.data_ptr() if paged else None, shape[1] if paged else 0, max_seq)
 
         self._native = _lib.native()   # the ordinary call, in C++ (csrc/torch_kv_cache.cpp); what it hands back as None is taken here
         self._handle = self._native.kv_cache(ctypes.addressof(self._view), batch, self.device.index)
@@ -205,7 +205,7 @@ class QuantizedKVCache:
         with torch.cuda.device(self.device):
             ws = torch.empty(max(need, 16), dtype=torch.uint8, device=self.device)
             p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())
-            _lib.check(L.xnq_kv_reserve(p(self.page_table), self.page_table.stride(0), p(table), table.stride(0), self.batch, self.page_size, self.num_pages, self.max_seq,
+            _lib.check(L.xnq_kv_reserve(p(self.page_table), table.shape[1], p(table), table.shape[1], self.batch, self.page_size, self.num_pages, self.max_seq,
                                         p(length), p(first), sinks, p(out), ctypes.c_void_p(out.data_ptr() + 8 * self.batch), p(ws), need, _stream_ptr(self.device)))
         return out[:-1], out[-1]
 
