@@ -336,7 +336,7 @@ __device__ __forceinline__ bool unit_at(const AttendArgs &a, int nth, int n, int
 
 // MORE: first positions that stay visible, packed tokens and trees; a CTA's tiles may then be two runs of the cache. Bound as the first form is, by the chain of its roles
 // (instructions come from further away, the code being larger): 2048 tokens that see 4096 positions and 128 first ones 210 us (Q8_0), 777 that see 2500 and 7
-// of 64 dims 57 us, 24 trees of 12 to 63 tokens over 1600 to 8192 positions 167 us, one of 26 over 4096 22.6 us with the joining of its parts.
+// of 64 dims 57 us, 24 trees of 12 to 63 tokens over 1600 to 8192 positions 170 us, one of 26 over 4096 22.6 us with the joining of its parts.
 template <int BITS, int HD, int QT, bool MORE>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1) kv_attend_prompt_kernel(const __grid_constant__ AttendArgs a) {
   using P = PromptShape<BITS, HD, QT>;
