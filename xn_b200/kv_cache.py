@@ -218,7 +218,8 @@ class QuantizedKVCache:
         smaller one than its own); -1: it follows what is in the cache; -2: the place is not used. They lie at ``pos, pos + 1, ..`` in the cache, in their
         order, are rotated at ``pos`` + depth, and see what lies below ``pos`` and their ancestors. Up to 256 tokens a tree.
 
-        The plan holds the slots of the page table as it is when the call runs: after :meth:`reserve`, before the calls that take it."""
+        The plan holds the slots of the page table as it is when the call runs: after :meth:`reserve`, before the calls that take it. It is made on the current
+        stream; another stream that takes it waits for this one first, or reads what is not there yet."""
         if tokens < 0 or (longest is not None and longest < 1):
             raise ValueError(f"plan: {tokens} tokens, up to {longest} a sequence")
         longest = max(1, min(tokens, longest if longest is not None else tokens))
